@@ -15,6 +15,7 @@
 #include "../host/hy_gguf.hpp"
 #include "hy_device.hpp"
 #include "hy_launch.hpp"
+#include "hy_paged.hpp"
 #include "hy_rules.hpp"
 
 namespace hy {
@@ -211,6 +212,67 @@ int run(hy_attn_ctx* c, const AttnLayer& W, const float* x, int T, int mode, con
     return HY_OK;
 }
 
+// what hy_attn_forward_paged and the paged decoder layer take besides x and out
+struct PagedStep {
+    hy::PagedView cache;  // of the layer
+    const hy_paged_batch* batch;
+    const float* cos_t;
+    const float* sin_t;
+    uint32_t n_pos;
+    void* ws;
+    size_t ws_bytes;
+};
+
+int check_paged(const hy_attn_ctx* c, uint32_t layer, const hy_paged_cache* cache, const hy_paged_batch* b,
+                PagedStep* st) {
+    HY_TRY(check_layer(c, layer, true));
+    HY_TRY(hy::paged_cache_check(cache, (uint32_t)c->nh, &st->cache));
+    if (st->cache.nkv != c->nkv || st->cache.hd != c->hd)
+        return fail(HY_ERR_INVALID, "the cache has %d heads of %d, the context %d of %d", st->cache.nkv, st->cache.hd,
+                    c->nkv, c->hd);
+    HY_TRY(hy::paged_batch_check(b, st->cache, true));
+    if (b->n_rows > (uint32_t)c->Tm)
+        return fail(HY_ERR_INVALID, "n_rows=%u exceeds max_tokens=%d", b->n_rows, c->Tm);
+    const uint64_t el = st->cache.type == HY_TYPE_F32 ? 4 : 2;
+    if (cache->layer_stride * el % 16 || cache->layer_stride >> 44)
+        return fail(HY_ERR_INVALID, "layer_stride=%llu must be a multiple of 16 bytes below 2^44 elements",
+                    (unsigned long long)cache->layer_stride);
+    st->cache.k = static_cast<uint8_t*>(st->cache.k) + layer * cache->layer_stride * el;
+    st->cache.v = static_cast<uint8_t*>(st->cache.v) + layer * cache->layer_stride * el;
+    st->batch = b;
+    const size_t need = hy::paged_attn_ws_bytes(c->nh, c->nkv, c->hd);
+    if (!st->ws || st->ws_bytes < need)
+        return fail(HY_ERR_INVALID, "workspace of %zu bytes at %p: %zu bytes needed", st->ws_bytes, st->ws, need);
+    return HY_OK;
+}
+
+// run() over a paged cache
+int run_paged(hy_attn_ctx* c, const AttnLayer& W, const float* x, const PagedStep& st, float* out, hipStream_t s,
+              const float* resid = nullptr) {
+    const int T = (int)st.batch->n_rows;
+    HY_TRY(timed(c, AK_QKV, s,
+                 [&] { return hy::launch_gemm_nt_f32(x, W.qkv_w, nullptr, c->qkv, T, c->nqkv, c->H, s, c->gemm_ws); }));
+    int rc = HY_OK;  // the paged calls set their own errors
+    const auto call = [&](int r) {
+        rc = r;
+        return hipSuccess;
+    };
+    HY_TRY(timed(c, AK_ROPE, s, [&] {
+        return call(hy::paged_append(c->qkv, st.batch->n_rows, (uint32_t)c->nh, st.cache, st.batch->positions_dev,
+                                     st.batch->slots_dev, c->cfg.rope_theta, st.cos_t, st.sin_t, st.n_pos, W.q_norm,
+                                     W.k_norm, c->cfg.rms_norm_eps, c->q, s));
+    }));
+    HY_TRY(rc);
+    HY_TRY(timed(c, AK_ATTN, s, [&] {
+        return call(hy::paged_attention(c->q, (uint32_t)c->nh, st.cache, st.batch, 1.0f / sqrtf((float)c->hd),
+                                        c->merged, st.ws, st.ws_bytes, s));
+    }));
+    HY_TRY(rc);
+    return timed(c, AK_OPROJ, s, [&] {
+        return hy::launch_gemm_nt_f32(c->merged, W.o_w, resid, out, T, c->H, c->nh * c->hd, s, c->gemm_ws);
+    });
+}
+
 // GGUF tensor -> f32 host copy (row-major as stored: ne0 innermost): F32, F16, BF16,
 // Q8_0 or Q4_0, as the reference loader's read_tensor_data takes every tensor
 // (src/hunyuan_gguf_loader.cpp:167-222)
@@ -400,6 +462,15 @@ int hy_attn_forward_cached(hy_attn_ctx* c, uint32_t layer, const float* x, uint3
                pos0, pos0 + (int)T, 0, out, s));
     L.cache_len += T;
     return HY_OK;
+}
+
+int hy_attn_forward_paged(hy_attn_ctx* c, uint32_t layer, const float* x, const hy_paged_cache* cache,
+                          const hy_paged_batch* batch, const float* cos_t, const float* sin_t, uint32_t n_pos,
+                          float* out, void* ws, size_t ws_bytes, void* stream) {
+    if (!x || !out) return fail(HY_ERR_INVALID, "null x/out");
+    PagedStep st{{}, nullptr, cos_t, sin_t, n_pos, ws, ws_bytes};
+    HY_TRY(check_paged(c, layer, cache, batch, &st));
+    return run_paged(c, c->layers[layer], x, st, out, static_cast<hipStream_t>(stream));
 }
 
 int hy_attn_cache_reset(hy_attn_ctx* c) {
@@ -687,6 +758,36 @@ int hy_model_forward(hy_model_ctx* m, const int32_t* ids, uint32_t T, const int3
     HY_TRY(run_layers(m, m->hb, T, positions, (uint32_t)m->L, s, &h));
     HIP_TRY(hy::launch_rms_norm_w(h, m->fnorm, (int)T, m->H, m->cfg.attn.rms_norm_eps, m->normed, s));
     HIP_TRY(hy::launch_gemm_nt_f32(m->normed, m->lm_head, nullptr, logits, (int)T, m->V, m->H, s, m->attn->gemm_ws));
+    return HY_OK;
+}
+
+int hy_model_forward_paged(hy_model_ctx* m, const int32_t* ids, const hy_paged_cache* cache,
+                           const hy_paged_batch* batch, float* logits, void* ws, size_t ws_bytes, void* stream) {
+    if (!m) return fail(HY_ERR_INVALID, "null ctx");
+    if (!ids || !logits) return fail(HY_ERR_INVALID, "null ids/logits");
+    hy_attn_ctx* c = m->attn;
+    for (uint32_t l = 0; l < (uint32_t)m->L; l++) {  // every layer, before anything is launched
+        PagedStep st{{}, nullptr, nullptr, nullptr, 0, ws, ws_bytes};
+        HY_TRY(check_paged(c, l, cache, batch, &st));
+    }
+    const int T = (int)batch->n_rows;
+    const float eps = m->cfg.attn.rms_norm_eps;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    HIP_TRY(hy::launch_embed(ids, m->embed, T, m->H, m->V, m->hb, s));
+    const float* cur = m->hb;
+    for (uint32_t l = 0; l < (uint32_t)m->L; l++) {  // as hy_decoder_layer_forward
+        const AttnLayer& W = c->layers[l];
+        PagedStep st{{}, nullptr, nullptr, nullptr, 0, ws, ws_bytes};
+        HY_TRY(check_paged(c, l, cache, batch, &st));
+        float* dst = cur == m->ha ? m->hb : m->ha;
+        HIP_TRY(W.has_in_norm ? hy::launch_rms_norm_w(cur, W.in_norm, T, m->H, eps, c->xn, s)
+                              : hy::launch_rms_norm(cur, T, m->H, eps, c->xn, s));
+        HY_TRY(run_paged(c, W, c->xn, st, c->hres, s, cur));
+        HY_TRY(hy_moe_stack_forward(m->moe, l, 1, c->hres, (uint32_t)T, eps, dst, stream));
+        cur = dst;
+    }
+    HIP_TRY(hy::launch_rms_norm_w(cur, m->fnorm, T, m->H, eps, m->normed, s));
+    HIP_TRY(hy::launch_gemm_nt_f32(m->normed, m->lm_head, nullptr, logits, T, m->V, m->H, s, c->gemm_ws));
     return HY_OK;
 }
 

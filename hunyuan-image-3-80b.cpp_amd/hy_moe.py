@@ -17,8 +17,10 @@ LIB_PATH = os.path.join(HERE, "libhy_moe.so")
 ROOT = os.path.dirname(HERE)
 HEADER = os.path.join(ROOT, "include", "hy_moe.h")
 ATTN_HEADER = os.path.join(ROOT, "include", "hy_attn.h")
+PAGED_HEADER = os.path.join(ROOT, "include", "hy_paged.h")
 
 F32, Q4_0, Q8_0 = 0, 2, 8
+F16, BF16 = 1, 30  # cache types besides F32
 PATH_AUTO, PATH_VALU, PATH_MFMA = 0, 1, 2
 TENSOR_X, TENSOR_ROUTER, TENSOR_GU, TENSOR_DN = 0, 1, 2, 3
 
@@ -49,6 +51,36 @@ class AttnConfig(C.Structure):
 
 class ModelConfig(C.Structure):
     _fields_ = [("moe", Config), ("attn", AttnConfig), ("vocab", C.c_uint32)]
+
+
+class PagedCache(C.Structure):
+    """hy_paged_cache: a pool of pages (k, v: objects with .ptr), dense unless strides
+    (page, head, token; in elements) are given.  The object keeps k and v alive."""
+    _fields_ = [
+        ("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("type", C.c_int32), ("n_pages", C.c_uint32),
+        ("page_size", C.c_uint32), ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+        ("page_stride", C.c_uint64), ("head_stride", C.c_uint64), ("token_stride", C.c_uint64),
+        ("layer_stride", C.c_uint64),
+    ]
+
+    def __init__(self, k, v, wtype, n_pages, page_size, nkv, hd, strides=(0, 0, 0), layer_stride=0):
+        super().__init__(k.ptr, v.ptr, wtype, n_pages, page_size, nkv, hd, *strides, layer_stride)
+        self.keep = (k, v)
+
+
+class PagedBatch(C.Structure):
+    """hy_paged_batch: the requests of one step (arrays: objects with .ptr, kept alive)."""
+    _fields_ = [
+        ("n_req", C.c_uint32), ("n_rows", C.c_uint32), ("max_pages", C.c_uint32), ("max_new", C.c_uint32),
+        ("q_start_dev", C.c_void_p), ("kv_len_dev", C.c_void_p), ("table_dev", C.c_void_p),
+        ("positions_dev", C.c_void_p), ("slots_dev", C.c_void_p), ("seen_dev", C.c_void_p),
+    ]
+
+    def __init__(self, n_req, n_rows, max_pages, max_new, q_start, kv_len, table, positions=None, slots=None,
+                 seen=None):
+        arrays = (q_start, kv_len, table, positions, slots, seen)
+        super().__init__(n_req, n_rows, max_pages, max_new, *[None if a is None else a.ptr for a in arrays])
+        self.keep = arrays
 
 
 _vp = C.c_void_p
@@ -138,6 +170,19 @@ _SIGS = {
     "hy_moe_prof_name": (C.c_char_p, [_i32]),
     "hy_moe_prof_count": (_i32, []),
     "hy_moe_last_routing": (C.c_int, [_vp, C.POINTER(_u32), _vp]),
+    "hy_paged_plan": (C.c_int, [_vp, _vp, _u32, _u32, _u32, _u32, _u32] + [_vp] * 12),
+    "hy_rope_qknorm_paged": (C.c_int, [_vp, _u32, _u32, C.POINTER(PagedCache), _vp, _vp, _f, _vp, _vp, _u32, _vp, _vp,
+                                       _f, _vp, _vp]),
+    "hy_paged_attention_ws": (C.c_size_t, [_u32, C.POINTER(PagedCache), C.POINTER(PagedBatch)]),
+    "hy_paged_attention": (C.c_int, [_vp, _u32, C.POINTER(PagedCache), C.POINTER(PagedBatch), _f, _vp, _vp,
+                                     C.c_size_t, _vp]),
+    "hy_verify_drafts_ws": (C.c_size_t, [_u32, _u32, _u32]),
+    "hy_verify_drafts": (C.c_int, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp,
+                                   C.c_size_t, _vp]),
+    "hy_attn_forward_paged": (C.c_int, [_vp, _u32, _vp, C.POINTER(PagedCache), C.POINTER(PagedBatch), _vp, _vp, _u32,
+                                        _vp, _vp, C.c_size_t, _vp]),
+    "hy_model_forward_paged": (C.c_int, [_vp, _vp, C.POINTER(PagedCache), C.POINTER(PagedBatch), _vp, _vp,
+                                         C.c_size_t, _vp]),
 }
 
 _lib = None
@@ -591,6 +636,13 @@ class Attn:
         check(lib().hy_attn_forward_cached(self.h, layer, x.ptr, T, cos.ptr if cos is not None else None,
                                            sin.ptr if sin is not None else None, out.ptr, stream))
 
+    def forward_paged(self, x: Buf, cache, batch, out: Buf, ws: Buf, ws_bytes, cos=None, sin=None, n_pos=0,
+                      stream=None, layer=0):
+        """forward over a paged cache (PagedCache, PagedBatch with positions and slots)."""
+        check(lib().hy_attn_forward_paged(self.h, layer, x.ptr, cache, batch, cos.ptr if cos is not None else None,
+                                          sin.ptr if sin is not None else None, n_pos, out.ptr, ws.ptr, ws_bytes,
+                                          stream))
+
     def set_input_norm(self, w=None, layer=0):
         """input_layernorm weight [H] (None: unit) for decoder_layer_forward."""
         if w is None:
@@ -684,6 +736,9 @@ class Model:
         check(lib().hy_model_forward(self.h, ids.ptr, T, positions.ptr if positions is not None else None,
                                      logits.ptr, stream))
 
+    def forward_paged(self, ids: Buf, cache, batch, logits: Buf, ws: Buf, ws_bytes, stream=None):
+        check(lib().hy_model_forward_paged(self.h, ids.ptr, cache, batch, logits.ptr, ws.ptr, ws_bytes, stream))
+
     def forward_hidden(self, embeds: Buf, T, hidden: Buf, n_layers=0, positions=None, stream=None):
         check(lib().hy_model_forward_hidden(self.h, embeds.ptr, T, positions.ptr if positions is not None else None,
                                             n_layers, hidden.ptr, stream))
@@ -705,3 +760,52 @@ def lm_head_f32(x, w, resid=None):
     rb = Buf.from_array(np.ascontiguousarray(resid, dtype=np.float32)) if resid is not None else None
     check(lib().hy_lm_head_f32(xb.ptr, wb.ptr, rb.ptr if rb is not None else None, T, Hd, V, ob.ptr, None))
     return ob.numpy()
+
+
+# ------------------------------------------------------------------ paged serving
+
+def paged_plan(cached, new, n_req, n_rows, page_size, max_pages, n_pages, table, held, held_out, free, n_free,
+               n_free_out, q_start, kv_len, positions, slots, status, stream=None):
+    """Tables, row offsets, positions and slots of a step from its lengths (hy_paged_plan)."""
+    check(lib().hy_paged_plan(cached.ptr, new.ptr, n_req, n_rows, page_size, max_pages, n_pages, table.ptr, held.ptr,
+                              held_out.ptr, free.ptr, n_free.ptr, n_free_out.ptr, q_start.ptr, kv_len.ptr,
+                              positions.ptr, slots.ptr, status.ptr, stream))
+
+
+def rope_qknorm_paged(qkv, n_rows, nh, cache, positions, slots, theta, cos, sin, n_pos, q_norm, k_norm, eps, q,
+                      stream=None):
+    """Rotary embedding, QK-norm and the write of the cache (hy_rope_qknorm_paged)."""
+    check(lib().hy_rope_qknorm_paged(qkv.ptr, n_rows, nh, cache, positions.ptr, slots.ptr, theta,
+                                     cos.ptr if cos is not None else None, sin.ptr if sin is not None else None, n_pos,
+                                     q_norm.ptr if q_norm is not None else None,
+                                     k_norm.ptr if k_norm is not None else None, eps, q.ptr, stream))
+
+
+def paged_attention_ws(nh, cache, batch):
+    """Workspace bytes of paged_attention."""
+    n = lib().hy_paged_attention_ws(nh, cache, batch)
+    if n == 0:
+        check(-1)
+    return n
+
+
+def paged_attention(q, nh, cache, batch, scale, out, ws, ws_bytes, stream=None):
+    """Attention of the batch's rows over the cache (hy_paged_attention)."""
+    check(lib().hy_paged_attention(q.ptr, nh, cache, batch, scale, out.ptr, ws.ptr, ws_bytes, stream))
+
+
+def verify_drafts_ws(n_req, n_rows, vocab):
+    """Workspace bytes of verify_drafts."""
+    n = lib().hy_verify_drafts_ws(n_req, n_rows, vocab)
+    if n == 0:
+        check(-1)
+    return n
+
+
+def verify_drafts(logits, draft_probs, ids, q_start, n_req, n_rows, max_new, vocab, temperature, u_accept, u_sample,
+                  accepted, tokens, ws, ws_bytes, stream=None):
+    """Accepted drafts and next tokens of every request (hy_verify_drafts)."""
+    check(lib().hy_verify_drafts(logits.ptr, draft_probs.ptr if draft_probs is not None else None, ids.ptr,
+                                 q_start.ptr, n_req, n_rows, max_new, vocab,
+                                 temperature.ptr if temperature is not None else None, u_accept.ptr, u_sample.ptr,
+                                 accepted.ptr, tokens.ptr, ws.ptr, ws_bytes, stream))
