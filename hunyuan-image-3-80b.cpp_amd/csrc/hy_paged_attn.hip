@@ -1,73 +1,505 @@
 // hy_paged_attn.hip -- attention of ragged batches of new tokens over a paged cache
 // (hy_paged_attention): out = sum_j softmax_j(scale q . k_j) v_j over the keys a row sees.
+//
+// paged_few_kernel: requests of few rows (single tokens, drafts).  A stream over K and V: one
+// wave works for itself on 16 NT rows (token x query head of a kv head) and goes over its keys
+// 32 (f32: 16) at a time, straight from memory into the operands of 16 x 16 MFMAs, without LDS
+// and barriers:
+//  * S^T = K Q^T: lane l = 16 g + i holds key i's dims, 16 bytes at a time;
+//  * the result has keys 4 g + v and row i in lane l, which is the B operand of
+//    O^T = V^T P^T as it stands: V's lane holds the 4 keys 4 g .. 4 g + 3 of its dims, so for
+//    16-bit types the pairs of keys are put together by byte permutes;
+//  * softmax statistics: one query row per lane, joined over the four g.
+// f32 accuracy from 16-bit operands: q and the probabilities are split into pieces that the
+// matrix cores multiply exactly -- a f16 cache: two f16 pieces (22 bits, q scaled per row by a
+// power of two, p by 2^14); a bf16 cache: three bf16 pieces (24 bits) -- while K and V go in as
+// they are.  f32 caches use the fp32 MFMAs.
+// Keys that a row does not see get weight 0; 0 times an infinity or NaN in their V would
+// still be felt, so where some rows do not see a key, V is looked at, and if it is not
+// finite these products are done key by key (slow_values).
 #include "hy_device.hpp"
+#include "hy_lds.hpp"
 #include "hy_paged.hpp"
+#include "hy_paged_part.hpp"
+#include "hy_split.hpp"
 
 namespace hy {
 
-// request of a row: the last r with q_start[r] <= t (requests without rows in between have
-// equal starts); -1 behind the last
-__device__ __forceinline__ int row_request(const int* __restrict__ q_start, int n_req, int t) {
-    int lo = 0, hi = n_req;  // q_start[lo] <= t < q_start[hi]
-    if (t < q_start[0] || t >= q_start[n_req]) return -1;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (q_start[mid] <= t)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    return lo;
-}
+typedef _Float16 v8h16_t __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h16_t __attribute__((ext_vector_type(2)));
 
-// One wave per (row, head), one key at a time, lane l two dims (or one) of it.
+// the operand kinds of a cache type
 template <class E>
-__global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnArgs a) {
-    const int64_t wid = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
-    if (wid >= (int64_t)a.n_rows * a.nh) return;
-    const int t = (int)(wid / a.nh), h = (int)(wid % a.nh), l = threadIdx.x % WAVE, hd = a.c.hd;
-    const int r = row_request(a.q_start, a.n_req, t);
-    if (r < 0) return;
-    const int g = h / (a.nh / a.c.nkv);
-    const int cap = a.max_pages << a.c.shift;
-    const int kv = min(max(a.kv_len[r], 0), cap);
-    const int end = min(a.seen ? a.seen[t] : kv - (a.q_start[r + 1] - t) + 1, kv);
-    const bool two = hd == 128;
-    const float* const q = a.q + ((int64_t)t * a.nh + h) * hd;
-    const float q0 = q[l] * a.scale, q1 = two ? q[64 + l] * a.scale : 0.0f;
-    const E* const kb = static_cast<const E*>(a.c.k) + g * a.c.head_stride + l;
-    const E* const vb = static_cast<const E*>(a.c.v) + g * a.c.head_stride + l;
-    float m = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int j = 0; j < end; j++) {
-        const int page = a.table[(int64_t)r * a.max_pages + (j >> a.c.shift)];
-        if (page < 0 || page >= a.c.n_pages) continue;
-        const int64_t at = page * a.c.page_stride + (j & ((1 << a.c.shift) - 1)) * a.c.token_stride;
-        float s = q0 * (float)kb[at] + (two ? q1 * (float)kb[at + 64] : 0.0f);
-        s = wave_sum(s);
-        const float mn = fmaxf(m, s);
-        const float old = m == mn ? 1.0f : hy_expf(m - mn), p = s == mn ? 1.0f : hy_expf(s - mn);
-        m = mn;
-        sum = sum * old + p;
-        o0 = o0 * old + p * (float)vb[at];
-        if (two) o1 = o1 * old + p * (float)vb[at + 64];
+struct PaType;
+template <>
+struct PaType<_Float16> {
+    static constexpr int PIECES = 2;
+    static __device__ __forceinline__ v4f_t mfma(v4i_t a, v4i_t b, v4f_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h16_t, a), __builtin_bit_cast(v8h16_t, b), c,
+                                                      0, 0, 0);
     }
-    float* const out = a.out + ((int64_t)t * a.nh + h) * hd + l;
-    const float inv = m == -INFINITY ? 0.0f : 1.0f / sum;
-    out[0] = o0 * inv;
-    if (two) out[64] = o1 * inv;
+    // two floats -> their pieces, packed
+    static __device__ __forceinline__ void split(float a, float b, uint32_t (&p)[2]) {
+        const v2h16_t h = __builtin_convertvector((v2f_t){a, b}, v2h16_t);
+        const v2f_t r = (v2f_t){a, b} - __builtin_convertvector(h, v2f_t);
+        p[0] = __builtin_bit_cast(uint32_t, h);
+        p[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2h16_t));
+    }
+    static __device__ __forceinline__ bool odd(uint32_t w) {  // an infinity or NaN among the two
+        return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
+    }
+};
+template <>
+struct PaType<__bf16> {
+    static constexpr int PIECES = 3;
+    static __device__ __forceinline__ v4f_t mfma(v4i_t a, v4i_t b, v4f_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf_t, a), __builtin_bit_cast(v8bf_t, b), c,
+                                                       0, 0, 0);
+    }
+    static __device__ __forceinline__ void split(float a, float b, uint32_t (&p)[3]) {
+        uint32_t lost = 0;
+        const Split2 s = split2(a, b, lost);
+#pragma unroll
+        for (int i = 0; i < 3; i++) p[i] = s.p[i];
+    }
+    static __device__ __forceinline__ bool odd(uint32_t w) {
+        return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+    }
+};
+template <>
+struct PaType<float> {
+    static constexpr int PIECES = 1;
+    static __device__ __forceinline__ bool odd(uint32_t w) { return (w & 0x7F800000u) == 0x7F800000u; }
+};
+
+__device__ __forceinline__ float group_max(float v) {  // over lanes i, 16 + i, 32 + i, 48 + i
+    v = fmaxf(v, shfl_xor(v, 16));
+    return fmaxf(v, shfl_xor(v, 32));
+}
+__device__ __forceinline__ float group_sum(float v) {
+    v += shfl_xor(v, 16);
+    return v + shfl_xor(v, 32);
 }
 
-size_t paged_attn_ws_bytes(int, int, int) { return 16; }
+constexpr int PF_WAVES = 4;
+constexpr float PF_PSCALE = 16384.0f;  // of the probabilities' f16 pieces
 
-hipError_t launch_paged_attn(const PagedAttnArgs& a, int, hipStream_t s) {
-    const dim3 grid((unsigned)(((int64_t)a.n_rows * a.nh + 3) / 4));
-    if (a.c.type == HY_TYPE_F32)
-        hipLaunchKernelGGL(paged_attn_kernel<float>, grid, dim3(256), 0, s, a);
-    else if (a.c.type == HY_TYPE_F16)
-        hipLaunchKernelGGL(paged_attn_kernel<_Float16>, grid, dim3(256), 0, s, a);
+template <class E, int HD, int NT>
+__global__ __launch_bounds__(WAVE * PF_WAVES, NT == 1 ? 2 : 1) void paged_few_kernel(PagedAttnArgs a, PartShape ps) {
+    using P = PaType<E>;
+    constexpr bool F32T = sizeof(E) == 4, F16T = std::is_same<E, _Float16>::value;
+    constexpr int KB = F32T ? 16 : 32;       // keys per turn
+    constexpr int KT = KB / 16;              // 16-key tiles of scores
+    constexpr int NQ = F32T ? HD / 16 : HD / 32;   // 16-byte loads of a key per lane
+    constexpr int VL = F32T ? HD / 64 : 1;         // loads of a value row per lane
+    constexpr int VD = F32T ? 4 : HD / 16;         // dims of each
+    constexpr int ND = HD / 16;              // 16-dim tiles of the output
+    constexpr int PC = P::PIECES;
+    constexpr int VW = VD * (int)sizeof(E) / 4;    // dwords of a V load
+    __shared__ int64_t pre[WAVE * PF_WAVES + 1];
+    __shared__ float p_s[PF_WAVES][KB][16 * NT];
+    const int lane = threadIdx.x % WAVE, i = lane % 16, g4 = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    const int64_t total = part_sums<WAVE * PF_WAVES>(a, ps, pre);
+    const int64_t stretch = part_stretch(ps, total);
+    const int worker = blockIdx.x * PF_WAVES + wave;
+    int64_t x = worker * stretch;
+    const int64_t x_end = min(x + stretch, total);
+    const int G = a.nh / a.c.nkv, pmask = (1 << a.c.shift) - 1;
+    const float qscale = a.scale * 1.4426950408889634f;
+
+    while (x < x_end) {
+        const PartItem it = part_find<WAVE * PF_WAVES>(a, ps, pre, x);
+        const int64_t p0 = x - it.at, p1 = min(x_end - it.at, it.len);  // this piece
+        x = it.at + p1;
+
+        // rows of this lane's columns; rows past the last repeat it and are not stored
+        const int n_live = min(it.q.n * G - it.tile * ps.M, ps.M);
+        int row[NT], head[NT], end[NT], last = 0, first = 0x7fffffff;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const int rho = it.tile * ps.M + min(16 * t + i, n_live - 1), tok = rho / G;
+            row[t] = it.q.start + tok;
+            head[t] = it.g * G + rho - tok * G;
+            end[t] = a.seen ? min(a.seen[row[t]], it.q.kv) : it.q.kv - it.q.n + tok + 1;
+            last = max(last, end[t]);
+            first = min(first, end[t]);
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) {
+            last = max(last, shfl_xor(last, d));
+            first = min(first, shfl_xor(first, d));
+        }
+        last = __builtin_amdgcn_readfirstlane(last);
+        first = __builtin_amdgcn_readfirstlane(first);
+        const int64_t blocks = ((int64_t)last + 31) / 32;
+        const int t0 = (int)(p0 * blocks / it.len) * (32 / KB), t1 = (int)(p1 * blocks / it.len) * (32 / KB);
+
+        // q: scaled by scale * log2(e) (scores in the base-2 domain); f16: by a power of two that
+        // brings the row's largest to [2^13, 2^14), undone on the scores
+        float qx[F32T ? NT : 1][F32T ? HD / 4 : 1];
+        v4i_t qf[F32T ? 1 : NT][F32T ? 1 : NQ][PC];
+        float unscale[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const float* const qp = a.q + ((int64_t)row[t] * a.nh + head[t]) * HD;
+            unscale[t] = 1.0f;
+            if constexpr (F32T) {
+#pragma unroll
+                for (int s = 0; s < NQ; s++) {
+                    const v4f_t q = *reinterpret_cast<const v4f_t*>(qp + 16 * s + 4 * g4);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) qx[t][4 * s + j] = q[j] * qscale;
+                }
+            } else {
+                v4f_t q[NQ][2];
+                float big = 0.0f;
+#pragma unroll
+                for (int s = 0; s < NQ; s++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        q[s][u] = *reinterpret_cast<const v4f_t*>(qp + 32 * s + 8 * g4 + 4 * u) * qscale;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) big = fmaxf(big, fabsf(q[s][u][j]));
+                    }
+                float up = 1.0f;
+                if constexpr (F16T) {
+                    big = group_max(big);
+                    const int e = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -100), 100);
+                    up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
+                    unscale[t] = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
+                }
+#pragma unroll
+                for (int s = 0; s < NQ; s++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        uint32_t w[PC];
+                        P::split(q[s][j / 2][2 * (j % 2)] * up, q[s][j / 2][2 * (j % 2) + 1] * up, w);
+#pragma unroll
+                        for (int c = 0; c < PC; c++) qf[t][s][c][j] = (int)w[c];
+                    }
+            }
+        }
+
+        // block table: 64 entries in the lanes, the next 64 on their way
+        const int* const trow = a.table + (int64_t)it.r * a.max_pages;
+        const int n_tab = (it.q.kv + pmask) >> a.c.shift;
+        auto entries = [&](int seg) {
+            const int p = seg * 64 + lane;
+            const int e = p < n_tab ? trow[p] : -1;
+            return e >= 0 && e < a.c.n_pages ? e : -1;
+        };
+        int seg = (t0 * KB) >> (a.c.shift + 6);
+        int tab = entries(seg), tab2 = entries(seg + 1);
+        const E* const kbase = static_cast<const E*>(a.c.k) + it.g * a.c.head_stride;
+        const E* const vbase = static_cast<const E*>(a.c.v) + it.g * a.c.head_stride;
+
+        v4i_t kx[2][KT][NQ];
+        int vx[2][KT][4][VL * VW];
+        int vpage[2][KT];  // the page of this lane's value keys, -1: none
+        // loads of turn t into buffer b; keys without a page read page 0
+        auto load = [&](int t, auto bc) {
+            constexpr int b = decltype(bc)::value;
+            const int s = (t * KB) >> (a.c.shift + 6);
+            if (s != seg) {  // wave-uniform; turns come in order
+                seg = s;
+                tab = tab2;
+                tab2 = entries(seg + 1);
+            }
+#pragma unroll
+            for (int u = 0; u < KT; u++) {
+                const int key = t * KB + 16 * u + i;
+                const int pg = max(__shfl(tab, (key >> a.c.shift) & 63, WAVE), 0);
+                const E* const kp = kbase + pg * a.c.page_stride + (key & pmask) * a.c.token_stride + 16 / sizeof(E) * g4;
+#pragma unroll
+                for (int n = 0; n < NQ; n++)
+                    kx[b][u][n] = *reinterpret_cast<const v4i_t*>(kp + 64 / sizeof(E) * n);
+            }
+#pragma unroll
+            for (int u = 0; u < KT; u++) {
+                const int key = t * KB + 16 * u + 4 * g4;
+                vpage[b][u] = __shfl(tab, (key >> a.c.shift) & 63, WAVE);
+                const E* const vp = vbase + max(vpage[b][u], 0) * a.c.page_stride + (key & pmask) * a.c.token_stride + VD * i;
+#pragma unroll
+                for (int v = 0; v < 4; v++)
+#pragma unroll
+                    for (int n = 0; n < VL; n++) {
+                        const E* const src = vp + v * a.c.token_stride + 64 * n;
+                        if constexpr (VW == 4) {
+                            const v4i_t w = *reinterpret_cast<const v4i_t*>(src);
+#pragma unroll
+                            for (int j = 0; j < 4; j++) vx[b][u][v][4 * n + j] = w[j];
+                        } else {
+                            const uint2 w = *reinterpret_cast<const uint2*>(src);
+                            vx[b][u][v][0] = (int)w.x;
+                            vx[b][u][v][1] = (int)w.y;
+                        }
+                    }
+            }
+        };
+
+        v4f_t o[NT][ND];
+        float m_run[NT], l_run[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            m_run[t] = -INFINITY;
+            l_run[t] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[t][d] = v4f_t{};
+        }
+
+        auto turn = [&](int t, auto bc) {
+            constexpr int b = decltype(bc)::value;
+            v4f_t s[NT][KT];
+#pragma unroll
+            for (int c = 0; c < NT; c++)
+#pragma unroll
+                for (int u = 0; u < KT; u++) {
+                    v4f_t acc = v4f_t{};
+#pragma unroll
+                    for (int n = 0; n < NQ; n++) {
+                        if constexpr (F32T) {
+                            const v4f_t k = __builtin_bit_cast(v4f_t, kx[b][u][n]);
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                acc = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j], qx[c][4 * n + j], acc, 0, 0, 0);
+                        } else {
+#pragma unroll
+                            for (int q = PC - 1; q >= 0; q--) acc = P::mfma(kx[b][u][n], qf[c][n][q], acc);
+                        }
+                    }
+                    s[c][u] = acc;
+                }
+            bool none = false;
+#pragma unroll
+            for (int u = 0; u < KT; u++) none |= vpage[b][u] < 0;
+            const bool edge = (t + 1) * KB > first || __any(none);
+#pragma unroll
+            for (int c = 0; c < NT; c++) {
+                float big = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < KT; u++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        if constexpr (F16T) s[c][u][v] *= unscale[c];
+                        if (edge) {
+                            const int key = t * KB + 16 * u + 4 * g4 + v;
+                            if (key >= end[c] || vpage[b][u] < 0) s[c][u][v] = -INFINITY;
+                        }
+                        big = fmaxf(big, s[c][u][v]);
+                    }
+                const float m = fmaxf(m_run[c], group_max(big));
+                const float ref = m == -INFINITY ? 0.0f : m;
+                const float alpha = __builtin_amdgcn_exp2f(m_run[c] - ref);
+                float sum = 0.0f;
+#pragma unroll
+                for (int u = 0; u < KT; u++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        s[c][u][v] = __builtin_amdgcn_exp2f(s[c][u][v] - ref);
+                        sum += s[c][u][v];
+                    }
+                l_run[c] = l_run[c] * alpha + group_sum(sum);
+                m_run[c] = m;
+                if (__any(alpha != 1.0f)) {
+#pragma unroll
+                    for (int d = 0; d < ND; d++) o[c][d] *= alpha;
+                }
+            }
+            bool odd = false;
+            if (edge) {
+#pragma unroll
+                for (int u = 0; u < KT; u++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++)
+#pragma unroll
+                        for (int w = 0; w < VL * VW; w++) odd |= P::odd((uint32_t)vx[b][u][v][w]);
+            }
+            if (__any(odd)) {
+                // slow values: key by key, rows of weight 0 untouched.  The wave's own p_s.
+#pragma unroll
+                for (int c = 0; c < NT; c++)
+#pragma unroll
+                    for (int u = 0; u < KT; u++)
+#pragma unroll
+                        for (int v = 0; v < 4; v++) p_s[wave][16 * u + 4 * g4 + v][16 * c + i] = s[c][u][v];
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                for (int k = 0; k < KB; k++) {
+                    const int key = t * KB + k;
+                    const int pg = (key >> a.c.shift) < n_tab ? trow[key >> a.c.shift] : -1;
+                    if (pg < 0 || pg >= a.c.n_pages) continue;
+                    const E* const vp = vbase + pg * a.c.page_stride + (key & pmask) * a.c.token_stride;
+#pragma unroll
+                    for (int c = 0; c < NT; c++) {
+                        const float p = p_s[wave][k][16 * c + i] * (F16T ? PF_PSCALE : 1.0f);
+#pragma unroll
+                        for (int d = 0; d < ND; d++)
+#pragma unroll
+                            for (int v = 0; v < 4; v++) {
+                                const int dim = F32T ? 64 * (d / 4) + 4 * (4 * g4 + v) + d % 4 : VD * (4 * g4 + v) + d;
+                                const float w = p * (float)vp[dim];
+                                if (p != 0.0f) o[c][d][v] += w;
+                            }
+                    }
+                }
+                __builtin_amdgcn_wave_barrier();
+                return;
+            }
+            if constexpr (F32T) {
+#pragma unroll
+                for (int v = 0; v < 4; v++)
+#pragma unroll
+                    for (int d = 0; d < ND; d++)
+#pragma unroll
+                        for (int c = 0; c < NT; c++)
+                            o[c][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vx[b][0][v][d]),
+                                                                          s[c][0][v], o[c][d], 0, 0, 0);
+            } else {
+                v4i_t pf[NT][PC];
+#pragma unroll
+                for (int c = 0; c < NT; c++)
+#pragma unroll
+                    for (int u = 0; u < KT; u++)
+#pragma unroll
+                        for (int v = 0; v < 2; v++) {
+                            uint32_t w[PC];
+                            const float f = F16T ? PF_PSCALE : 1.0f;
+                            P::split(s[c][u][2 * v] * f, s[c][u][2 * v + 1] * f, w);
+#pragma unroll
+                            for (int q = 0; q < PC; q++) pf[c][q][2 * u + v] = (int)w[q];
+                        }
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    v4i_t vf;  // dims VD i + d of keys 4 g4 .. + 3 of both tiles
+#pragma unroll
+                    for (int u = 0; u < KT; u++)
+#pragma unroll
+                        for (int v = 0; v < 2; v++)
+                            vf[2 * u + v] = (int)__builtin_amdgcn_perm(
+                                (uint32_t)vx[b][u][2 * v + 1][d / 2], (uint32_t)vx[b][u][2 * v][d / 2],
+                                d % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                    for (int c = 0; c < NT; c++)
+#pragma unroll
+                        for (int q = PC - 1; q >= 0; q--) o[c][d] = P::mfma(vf, pf[c][q], o[c][d]);
+                }
+            }
+        };
+
+        using std::integral_constant;
+        if (t0 < t1) load(t0, integral_constant<int, 0>{});
+        for (int t = t0; t < t1; t += 2) {
+            if (t + 1 < t1) load(t + 1, integral_constant<int, 1>{});
+            turn(t, integral_constant<int, 0>{});
+            if (t + 1 >= t1) break;
+            if (t + 2 < t1) load(t + 2, integral_constant<int, 0>{});
+            turn(t + 1, integral_constant<int, 1>{});
+        }
+
+        const float down = F16T ? 1.0f / PF_PSCALE : 1.0f;
+        const bool whole = p0 == 0 && p1 == it.len;
+        float* const slot = a.ws + (size_t)(2 * worker + (p0 == 0 ? 1 : 0)) * part_slot_floats(ps.M, HD);
+#pragma unroll
+        for (int c = 0; c < NT; c++) {
+            if (16 * c + i >= n_live) continue;
+            float* dst;
+            float f = down;
+            if (whole) {
+                dst = a.out + ((int64_t)row[c] * a.nh + head[c]) * HD;
+                f = l_run[c] == 0.0f ? 0.0f : down / l_run[c];
+            } else {
+                dst = slot + (16 * c + i) * HD;
+                if (g4 == 0) {
+                    slot[ps.M * HD + 16 * c + i] = m_run[c];
+                    slot[ps.M * (HD + 1) + 16 * c + i] = l_run[c];
+                }
+            }
+            // dims VD (4 g4 + v) + d are in a row for d = 0 .. VD - 1
+#pragma unroll
+            for (int n = 0; n < VL; n++)
+#pragma unroll
+                for (int v = 0; v < 4; v++)
+#pragma unroll
+                    for (int j = 0; j < VD; j += 4) {
+                        const int d = VD * n + j;
+                        *reinterpret_cast<v4f_t*>(dst + 64 * n + VD * (4 * g4 + v) + j) =
+                            (v4f_t){o[c][d][v], o[c][d + 1][v], o[c][d + 2][v], o[c][d + 3][v]} * f;
+                    }
+        }
+    }
+}
+
+// Joins the pieces of every cut item: work group w the item that worker w begins and another
+// ends, a thread 4 dims of a row at a time.
+template <int HD>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartShape ps) {
+    __shared__ int64_t pre[257];
+    const int64_t total = part_sums<256>(a, ps, pre);
+    const int64_t stretch = part_stretch(ps, total);
+    const int64_t cut = ((int64_t)blockIdx.x + 1) * stretch;  // the end of worker w's stretch
+    if (cut >= total) return;
+    const PartItem it = part_find<256>(a, ps, pre, cut);
+    if (it.at >= cut || it.at < cut - stretch) return;  // begins here, or was begun by another
+    const int w0 = blockIdx.x, w1 = (int)((it.at + it.len - 1) / stretch);
+    const int G = a.nh / a.c.nkv;
+    const int n_live = min(it.q.n * G - it.tile * ps.M, ps.M);
+    const size_t sf = part_slot_floats(ps.M, HD);
+    const float* const first = a.ws + (size_t)(2 * w0 + 1) * sf;
+    auto slot = [&](int w) { return w == w0 ? first : a.ws + (size_t)(2 * w) * sf; };
+    constexpr int TR = HD / 4, RPB = 256 / TR;  // threads per row, rows at a time
+    const int d = threadIdx.x % TR * 4;
+    for (int i = blockIdx.y * RPB + threadIdx.x / TR; i < n_live; i += RPB * gridDim.y) {
+        float m = -INFINITY;
+        bool nan = false;
+        for (int w = w0; w <= w1; w++) {
+            const float x = slot(w)[ps.M * HD + i];
+            nan |= x != x;
+            m = fmaxf(m, x);
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        v4f_t o = v4f_t{};
+        float l = nan ? __builtin_nanf("") : 0.0f;
+        for (int w = w0; w <= w1; w++) {
+            const float* const s = slot(w);
+            const float f = __builtin_amdgcn_exp2f(s[ps.M * HD + i] - ref);
+            l += f * s[ps.M * (HD + 1) + i];
+            o += f * *reinterpret_cast<const v4f_t*>(s + i * HD + d);
+        }
+        const int rho = it.tile * ps.M + i, tok = rho / G;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        *reinterpret_cast<v4f_t*>(a.out + ((int64_t)(it.q.start + tok) * a.nh + it.g * G + rho - tok * G) * HD + d) =
+            o * inv;
+    }
+}
+
+constexpr int PF_GROUPS = 512;  // two per CU
+constexpr int PF_WORKERS = PF_GROUPS * PF_WAVES;
+constexpr int PF_MAX_M = 32;
+
+size_t paged_attn_ws_bytes(int, int, int hd) { return 2 * PF_WORKERS * part_slot_floats(PF_MAX_M, hd) * 4; }
+
+template <class E, int HD>
+static hipError_t launch_few(const PagedAttnArgs& a, int max_rows, hipStream_t s) {
+    const bool two = max_rows > 16;
+    const PartShape ps{two ? 32 : 16, 0, (int64_t)1 << 62, PF_WORKERS, 64};
+    if (two)
+        hipLaunchKernelGGL((paged_few_kernel<E, HD, 2>), dim3(PF_GROUPS), dim3(WAVE * PF_WAVES), 0, s, a, ps);
     else
-        hipLaunchKernelGGL(paged_attn_kernel<__bf16>, grid, dim3(256), 0, s, a);
+        hipLaunchKernelGGL((paged_few_kernel<E, HD, 1>), dim3(PF_GROUPS), dim3(WAVE * PF_WAVES), 0, s, a, ps);
+    hipLaunchKernelGGL(paged_join_kernel<HD>, dim3(PF_WORKERS, 1), dim3(256), 0, s, a, ps);
     return hipGetLastError();
+}
+
+hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s) {
+    const int64_t rows = (int64_t)max_new * (a.nh / a.c.nkv);
+    const int max_rows = (int)min(rows, (int64_t)1 << 30);
+    const bool big = a.c.hd == 128;
+    if (a.c.type == HY_TYPE_F32) return big ? launch_few<float, 128>(a, max_rows, s) : launch_few<float, 64>(a, max_rows, s);
+    if (a.c.type == HY_TYPE_F16)
+        return big ? launch_few<_Float16, 128>(a, max_rows, s) : launch_few<_Float16, 64>(a, max_rows, s);
+    return big ? launch_few<__bf16, 128>(a, max_rows, s) : launch_few<__bf16, 64>(a, max_rows, s);
 }
 
 }  // namespace hy
