@@ -16,7 +16,7 @@
 // they are.  f32 caches use the fp32 MFMAs.
 // Keys that a row does not see get weight 0; 0 times an infinity or NaN in their V would
 // still be felt, so where some rows do not see a key, V is looked at, and if it is not
-// finite these products are done key by key (slow_values).
+// finite the piece is computed again key by key (slow_rows).
 #include "hy_device.hpp"
 #include "hy_lds.hpp"
 #include "hy_paged.hpp"
@@ -85,7 +85,7 @@ constexpr int PF_WAVES = 4;
 constexpr float PF_PSCALE = 16384.0f;  // of the probabilities' f16 pieces
 
 template <class E, int HD, int NT>
-__global__ __launch_bounds__(WAVE * PF_WAVES, NT == 1 ? 2 : 1) void paged_few_kernel(PagedAttnArgs a, PartShape ps) {
+__global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttnArgs a, PartShape ps) {
     using P = PaType<E>;
     constexpr bool F32T = sizeof(E) == 4, F16T = std::is_same<E, _Float16>::value;
     constexpr int KB = F32T ? 16 : 32;       // keys per turn
@@ -97,7 +97,6 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, NT == 1 ? 2 : 1) void paged_few_ke
     constexpr int PC = P::PIECES;
     constexpr int VW = VD * (int)sizeof(E) / 4;    // dwords of a V load
     __shared__ int64_t pre[WAVE * PF_WAVES + 1];
-    __shared__ float p_s[PF_WAVES][KB][16 * NT];
     const int lane = threadIdx.x % WAVE, i = lane % 16, g4 = lane / 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int64_t total = part_sums<WAVE * PF_WAVES>(a, ps, pre);
@@ -194,12 +193,12 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, NT == 1 ? 2 : 1) void paged_few_ke
         const E* const kbase = static_cast<const E*>(a.c.k) + it.g * a.c.head_stride;
         const E* const vbase = static_cast<const E*>(a.c.v) + it.g * a.c.head_stride;
 
-        v4i_t kx[2][KT][NQ];
-        int vx[2][KT][4][VL * VW];
-        int vpage[2][KT];  // the page of this lane's value keys, -1: none
-        // loads of turn t into buffer b; keys without a page read page 0
-        auto load = [&](int t, auto bc) {
-            constexpr int b = decltype(bc)::value;
+        v4i_t kx[KT][NQ];
+        int vx[KT][4][VL * VW];
+        int vpage[KT];  // the page of this lane's value keys, -1: none
+        auto page_of = [&](int key) { return __shfl(tab, (key >> a.c.shift) & 63, WAVE); };
+        // loads of a turn; keys without a page read page 0
+        auto load_k = [&](int t) {
             const int s = (t * KB) >> (a.c.shift + 6);
             if (s != seg) {  // wave-uniform; turns come in order
                 seg = s;
@@ -209,17 +208,18 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, NT == 1 ? 2 : 1) void paged_few_ke
 #pragma unroll
             for (int u = 0; u < KT; u++) {
                 const int key = t * KB + 16 * u + i;
-                const int pg = max(__shfl(tab, (key >> a.c.shift) & 63, WAVE), 0);
-                const E* const kp = kbase + pg * a.c.page_stride + (key & pmask) * a.c.token_stride + 16 / sizeof(E) * g4;
+                const E* const kp = kbase + max(page_of(key), 0) * a.c.page_stride + (key & pmask) * a.c.token_stride +
+                                    16 / sizeof(E) * g4;
 #pragma unroll
-                for (int n = 0; n < NQ; n++)
-                    kx[b][u][n] = *reinterpret_cast<const v4i_t*>(kp + 64 / sizeof(E) * n);
+                for (int n = 0; n < NQ; n++) kx[u][n] = *reinterpret_cast<const v4i_t*>(kp + 64 / sizeof(E) * n);
             }
+        };
+        auto load_v = [&](int t) {
 #pragma unroll
             for (int u = 0; u < KT; u++) {
                 const int key = t * KB + 16 * u + 4 * g4;
-                vpage[b][u] = __shfl(tab, (key >> a.c.shift) & 63, WAVE);
-                const E* const vp = vbase + max(vpage[b][u], 0) * a.c.page_stride + (key & pmask) * a.c.token_stride + VD * i;
+                vpage[u] = page_of(key);
+                const E* const vp = vbase + max(vpage[u], 0) * a.c.page_stride + (key & pmask) * a.c.token_stride + VD * i;
 #pragma unroll
                 for (int v = 0; v < 4; v++)
 #pragma unroll
@@ -228,17 +228,18 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, NT == 1 ? 2 : 1) void paged_few_ke
                         if constexpr (VW == 4) {
                             const v4i_t w = *reinterpret_cast<const v4i_t*>(src);
 #pragma unroll
-                            for (int j = 0; j < 4; j++) vx[b][u][v][4 * n + j] = w[j];
+                            for (int j = 0; j < 4; j++) vx[u][v][4 * n + j] = w[j];
                         } else {
                             const uint2 w = *reinterpret_cast<const uint2*>(src);
-                            vx[b][u][v][0] = (int)w.x;
-                            vx[b][u][v][1] = (int)w.y;
+                            vx[u][v][0] = (int)w.x;
+                            vx[u][v][1] = (int)w.y;
                         }
                     }
             }
         };
 
         v4f_t o[NT][ND];
+        bool odd = false;  // an infinity or NaN in V where some rows do not see a key
         float m_run[NT], l_run[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -248,8 +249,13 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, NT == 1 ? 2 : 1) void paged_few_ke
             for (int d = 0; d < ND; d++) o[t][d] = v4f_t{};
         }
 
-        auto turn = [&](int t, auto bc) {
-            constexpr int b = decltype(bc)::value;
+        if (t0 < t1) {
+            load_k(t0);
+            load_v(t0);
+        }
+        for (int t = t0; t < t1; t++) {
+            // K's registers are free after the scores, V's after its products: the next turn's
+            // loads go out there and run under the rest, and under the other wave of the SIMD
             v4f_t s[NT][KT];
 #pragma unroll
             for (int c = 0; c < NT; c++)
@@ -259,20 +265,23 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, NT == 1 ? 2 : 1) void paged_few_ke
 #pragma unroll
                     for (int n = 0; n < NQ; n++) {
                         if constexpr (F32T) {
-                            const v4f_t k = __builtin_bit_cast(v4f_t, kx[b][u][n]);
+                            const v4f_t k = __builtin_bit_cast(v4f_t, kx[u][n]);
 #pragma unroll
                             for (int j = 0; j < 4; j++)
                                 acc = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j], qx[c][4 * n + j], acc, 0, 0, 0);
                         } else {
 #pragma unroll
-                            for (int q = PC - 1; q >= 0; q--) acc = P::mfma(kx[b][u][n], qf[c][n][q], acc);
+                            for (int q = PC - 1; q >= 0; q--) acc = P::mfma(kx[u][n], qf[c][n][q], acc);
                         }
                     }
                     s[c][u] = acc;
                 }
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + 1 < t1) load_k(t + 1);
+            __builtin_amdgcn_sched_barrier(0);
             bool none = false;
 #pragma unroll
-            for (int u = 0; u < KT; u++) none |= vpage[b][u] < 0;
+            for (int u = 0; u < KT; u++) none |= vpage[u] < 0;
             const bool edge = (t + 1) * KB > first || __any(none);
 #pragma unroll
             for (int c = 0; c < NT; c++) {
@@ -284,7 +293,7 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, NT == 1 ? 2 : 1) void paged_few_ke
                         if constexpr (F16T) s[c][u][v] *= unscale[c];
                         if (edge) {
                             const int key = t * KB + 16 * u + 4 * g4 + v;
-                            if (key >= end[c] || vpage[b][u] < 0) s[c][u][v] = -INFINITY;
+                            if (key >= end[c] || vpage[u] < 0) s[c][u][v] = -INFINITY;
                         }
                         big = fmaxf(big, s[c][u][v]);
                     }
@@ -306,46 +315,13 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, NT == 1 ? 2 : 1) void paged_few_ke
                     for (int d = 0; d < ND; d++) o[c][d] *= alpha;
                 }
             }
-            bool odd = false;
             if (edge) {
 #pragma unroll
                 for (int u = 0; u < KT; u++)
 #pragma unroll
                     for (int v = 0; v < 4; v++)
 #pragma unroll
-                        for (int w = 0; w < VL * VW; w++) odd |= P::odd((uint32_t)vx[b][u][v][w]);
-            }
-            if (__any(odd)) {
-                // slow values: key by key, rows of weight 0 untouched.  The wave's own p_s.
-#pragma unroll
-                for (int c = 0; c < NT; c++)
-#pragma unroll
-                    for (int u = 0; u < KT; u++)
-#pragma unroll
-                        for (int v = 0; v < 4; v++) p_s[wave][16 * u + 4 * g4 + v][16 * c + i] = s[c][u][v];
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-                for (int k = 0; k < KB; k++) {
-                    const int key = t * KB + k;
-                    const int pg = (key >> a.c.shift) < n_tab ? trow[key >> a.c.shift] : -1;
-                    if (pg < 0 || pg >= a.c.n_pages) continue;
-                    const E* const vp = vbase + pg * a.c.page_stride + (key & pmask) * a.c.token_stride;
-#pragma unroll
-                    for (int c = 0; c < NT; c++) {
-                        const float p = p_s[wave][k][16 * c + i] * (F16T ? PF_PSCALE : 1.0f);
-#pragma unroll
-                        for (int d = 0; d < ND; d++)
-#pragma unroll
-                            for (int v = 0; v < 4; v++) {
-                                const int dim = F32T ? 64 * (d / 4) + 4 * (4 * g4 + v) + d % 4 : VD * (4 * g4 + v) + d;
-                                const float w = p * (float)vp[dim];
-                                if (p != 0.0f) o[c][d][v] += w;
-                            }
-                    }
-                }
-                __builtin_amdgcn_wave_barrier();
-                return;
+                        for (int w = 0; w < VL * VW; w++) odd |= P::odd((uint32_t)vx[u][v][w]);
             }
             if constexpr (F32T) {
 #pragma unroll
@@ -354,7 +330,7 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, NT == 1 ? 2 : 1) void paged_few_ke
                     for (int d = 0; d < ND; d++)
 #pragma unroll
                         for (int c = 0; c < NT; c++)
-                            o[c][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vx[b][0][v][d]),
+                            o[c][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vx[0][v][d]),
                                                                           s[c][0][v], o[c][d], 0, 0, 0);
             } else {
                 v4i_t pf[NT][PC];
@@ -378,7 +354,7 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, NT == 1 ? 2 : 1) void paged_few_ke
 #pragma unroll
                         for (int v = 0; v < 2; v++)
                             vf[2 * u + v] = (int)__builtin_amdgcn_perm(
-                                (uint32_t)vx[b][u][2 * v + 1][d / 2], (uint32_t)vx[b][u][2 * v][d / 2],
+                                (uint32_t)vx[u][2 * v + 1][d / 2], (uint32_t)vx[u][2 * v][d / 2],
                                 d % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
                     for (int c = 0; c < NT; c++)
@@ -386,19 +362,21 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, NT == 1 ? 2 : 1) void paged_few_ke
                         for (int q = PC - 1; q >= 0; q--) o[c][d] = P::mfma(vf, pf[c][q], o[c][d]);
                 }
             }
-        };
-
-        using std::integral_constant;
-        if (t0 < t1) load(t0, integral_constant<int, 0>{});
-        for (int t = t0; t < t1; t += 2) {
-            if (t + 1 < t1) load(t + 1, integral_constant<int, 1>{});
-            turn(t, integral_constant<int, 0>{});
-            if (t + 1 >= t1) break;
-            if (t + 2 < t1) load(t + 2, integral_constant<int, 0>{});
-            turn(t + 1, integral_constant<int, 1>{});
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + 1 < t1) load_v(t + 1);
         }
 
-        const float down = F16T ? 1.0f / PF_PSCALE : 1.0f;
+        float down = F16T ? 1.0f / PF_PSCALE : 1.0f;
+        if (__any(odd)) {  // again, key by key
+            down = 1.0f;
+#pragma unroll
+            for (int c = 0; c < NT; c++)
+                slow_rows<E, HD, 4>(
+                    a, trow, it.q.kv, t0 * KB, t1 * KB, end[c], a.q + ((int64_t)row[c] * a.nh + head[c]) * HD, kbase, vbase,
+                    [&](int n) { return F32T ? 64 * (n / 16) + 4 * (4 * g4 + n % 4) + n / 4 % 4 : VD * (4 * g4 + n % 4) + n / 4; },
+                    [&](int n, float v) { o[c][n / 4][n % 4] = v; }, [&](int n) { return o[c][n / 4][n % 4]; }, m_run[c],
+                    l_run[c]);
+        }
         const bool whole = p0 == 0 && p1 == it.len;
         float* const slot = a.ws + (size_t)(2 * worker + (p0 == 0 ? 1 : 0)) * part_slot_floats(ps.M, HD);
 #pragma unroll
@@ -478,28 +456,50 @@ constexpr int PF_GROUPS = 512;  // two per CU
 constexpr int PF_WORKERS = PF_GROUPS * PF_WAVES;
 constexpr int PF_MAX_M = 32;
 
-size_t paged_attn_ws_bytes(int, int, int hd) { return 2 * PF_WORKERS * part_slot_floats(PF_MAX_M, hd) * 4; }
+// rows of a request up to which the stream takes it
+constexpr int PF_MAX_ROWS = PF_MAX_M;
+
+size_t paged_attn_ws_bytes(int, int, int hd) {
+    return max(2 * PF_WORKERS * part_slot_floats(PF_MAX_M, hd), 2 * PM_WORKERS * part_slot_floats(PM_TILE, hd)) * 4;
+}
+
+static void launch_join(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
+    const dim3 grid(ps.workers, ps.M > PF_MAX_M ? 8 : 1);
+    if (a.c.hd == 128)
+        hipLaunchKernelGGL(paged_join_kernel<128>, grid, dim3(256), 0, s, a, ps);
+    else
+        hipLaunchKernelGGL(paged_join_kernel<64>, grid, dim3(256), 0, s, a, ps);
+}
 
 template <class E, int HD>
-static hipError_t launch_few(const PagedAttnArgs& a, int max_rows, hipStream_t s) {
-    const bool two = max_rows > 16;
-    const PartShape ps{two ? 32 : 16, 0, (int64_t)1 << 62, PF_WORKERS, 64};
-    if (two)
+static void launch_few(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
+    if (ps.M == 32)
         hipLaunchKernelGGL((paged_few_kernel<E, HD, 2>), dim3(PF_GROUPS), dim3(WAVE * PF_WAVES), 0, s, a, ps);
     else
         hipLaunchKernelGGL((paged_few_kernel<E, HD, 1>), dim3(PF_GROUPS), dim3(WAVE * PF_WAVES), 0, s, a, ps);
-    hipLaunchKernelGGL(paged_join_kernel<HD>, dim3(PF_WORKERS, 1), dim3(256), 0, s, a, ps);
-    return hipGetLastError();
 }
 
 hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s) {
-    const int64_t rows = (int64_t)max_new * (a.nh / a.c.nkv);
-    const int max_rows = (int)min(rows, (int64_t)1 << 30);
-    const bool big = a.c.hd == 128;
-    if (a.c.type == HY_TYPE_F32) return big ? launch_few<float, 128>(a, max_rows, s) : launch_few<float, 64>(a, max_rows, s);
-    if (a.c.type == HY_TYPE_F16)
-        return big ? launch_few<_Float16, 128>(a, max_rows, s) : launch_few<_Float16, 64>(a, max_rows, s);
-    return big ? launch_few<__bf16, 128>(a, max_rows, s) : launch_few<__bf16, 64>(a, max_rows, s);
+    const int64_t rows = (int64_t)max_new * (a.nh / a.c.nkv);  // of one request, at most
+    constexpr int64_t ALL = (int64_t)1 << 62;
+    const bool many = rows > PF_MAX_ROWS;
+    if (!many || a.n_req > 1) {
+        const PartShape ps{rows > 16 ? 32 : 16, 0, many ? PF_MAX_ROWS : ALL, PF_WORKERS, 64};
+        const bool big = a.c.hd == 128;
+        if (a.c.type == HY_TYPE_F32)
+            big ? launch_few<float, 128>(a, ps, s) : launch_few<float, 64>(a, ps, s);
+        else if (a.c.type == HY_TYPE_F16)
+            big ? launch_few<_Float16, 128>(a, ps, s) : launch_few<_Float16, 64>(a, ps, s);
+        else
+            big ? launch_few<__bf16, 128>(a, ps, s) : launch_few<__bf16, 64>(a, ps, s);
+        launch_join(a, ps, s);
+    }
+    if (many) {
+        const PartShape ps{PM_TILE, a.n_req > 1 ? PF_MAX_ROWS : 0, ALL, PM_WORKERS, 64};
+        (void)launch_paged_many(a, ps, s);
+        launch_join(a, ps, s);
+    }
+    return hipGetLastError();
 }
 
 }  // namespace hy

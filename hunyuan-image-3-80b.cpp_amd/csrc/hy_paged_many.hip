@@ -1,0 +1,515 @@
+// hy_paged_many.hip -- the paged attention of requests with many rows (chunks of a prompt): a
+// work group of eight waves per tile of 256 rows (token x query head of a kv head, 32 per
+// wave) and stretch of keys (hy_paged_part.hpp), both products on the f16 matrix cores with f32
+// accuracy.
+//
+// Splits.  q and the weights go in as two f16 pieces, hi + lo (11 + 11 bits, each rounded to
+// nearest: 2^-24 of the value), an f32 cache's K and V too, 16-bit caches as one (exact).  A
+// product is hi hi + hi lo + lo hi; the missing lo lo is below 2^-24 of it.  f16 has few
+// exponents, so every vector is scaled by a power of two that brings its largest element to
+// the top of its range: q per row, and for f32 and bf16 caches K and V per key (elements down to
+// 2^-27 of their vector's largest keep all bits of a piece, none is off by more than 2^-38 of it).  K's
+// factor is undone on the scores.  V's, 2^e_j, joins the weights: with R the running
+// maximum of s_j + e_j the accumulators sum w_j v_j 2^-e_j, w_j = 2^(s_j + e_j - R) <= 1,
+// and w_j 2^-e_j = 2^(s_j - R), which leaves out = O / l in any reference R.
+//
+// Blocks of 32 keys: every thread loads its share of a block of K and V one block ahead,
+// splits it and stores the pieces to LDS, K as it is and V transposed, both in MFMA operand
+// order.  Scores are computed transposed, S^T = K Q^T, so a query's statistics stay in its
+// lane pair and its weights are the operand of O^T += V^T W^T as they lie.  The two waves of
+// a SIMD run half a block apart: one multiplies the last block's weights with V while the other
+// is at this block's scores, so one's softmax runs under the other's products.
+//
+// Keys that no row sees are stored as zeros and masked; where V holds an infinity or NaN, which 0
+// times a weight would not keep out, the piece is computed again key by key (slow_rows).
+#include "hy_device.hpp"
+#include "hy_lds.hpp"
+#include "hy_paged.hpp"
+#include "hy_paged_part.hpp"
+#include "hy_split.hpp"
+
+namespace hy {
+
+typedef _Float16 v8h16_t __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h16_t __attribute__((ext_vector_type(2)));
+
+constexpr int PM_WAVES = 8, PM_THREADS = WAVE * PM_WAVES, PM_M = PM_TILE;
+static_assert(PM_M == 32 * PM_WAVES && PM_WORKERS % 8 == 0, "32 rows per wave, whole XCDs");
+constexpr int PM_UP = 14;   // q's and K's largest elements go to [2^14, 2^15), weights to 2^14
+constexpr int PM_VUP = 13;  // V's to [2^13, 2^14): 2^-e of an e up to 126 is a normal number
+
+__device__ __forceinline__ v16f_t mfma_f16(v4i_t a, v4i_t b, v16f_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h16_t, a), __builtin_bit_cast(v8h16_t, b), c, 0,
+                                                  0, 0);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126..127
+// two floats -> f16 pieces, packed
+__device__ __forceinline__ uint32_t pk_f16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f_t){a, b}, v2h16_t));
+}
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = pk_f16(a, b);
+    const v2f_t r = (v2f_t){a, b} - __builtin_convertvector(__builtin_bit_cast(v2h16_t, hi), v2f_t);
+    lo = pk_f16(r[0], r[1]);
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+}
+// exponent of the power of two at or below a magnitude (as f32 bits), not below lo
+__device__ __forceinline__ int exponent(uint32_t magnitude, int lo) {
+    return min(max((int)(magnitude >> 23) - 127, lo), 127);
+}
+
+template <class E, int HD>
+struct PmLds {
+    static constexpr int KP = sizeof(E) == 4 ? 2 : 1;  // pieces of K and V
+    // K: per piece HD / 8 chunks (8 dims) of 32 keys x 16 bytes; 32 bytes between chunks put the
+    // chunks that a wave stores at once on different banks
+    static constexpr int CHUNK_K = 32 * 16 + 32, PIECE_K = HD / 8 * CHUNK_K, BUF_K = KP * PIECE_K;
+    // V: per piece 4 chunks (2 c + h: keys 16 c + 4 h .. + 3 and 16 c + 8 + 4 h .. + 3) of HD dims
+    // x 16 bytes, even dims before odd ones
+    static constexpr int CHUNK_V = HD * 16, PIECE_V = 4 * CHUNK_V, BUF_V = KP * PIECE_V;
+    static constexpr int OFF_V = 2 * BUF_K, BYTES = OFF_V + 3 * BUF_V;
+};
+
+template <class E, int HD>
+__global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs a, PartShape ps) {
+    using L = PmLds<E, HD>;
+    constexpr bool SCALED = !std::is_same<E, _Float16>::value;
+    constexpr int KP = L::KP;
+    constexpr int NC = HD / 16, ND = HD / 32;
+    constexpr int KL = HD / 8;  // threads per key of K
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[L::BYTES];
+    __shared__ __attribute__((aligned(16))) float k_fac[3][32], v_exp[3][32], v_inv[3][32];
+    __shared__ __attribute__((aligned(8))) uint8_t there_s[3][PM_WAVES];  // 4 keys: 1, or 0 (no page)
+    __shared__ int odd_s;  // an infinity or NaN in this piece's V
+    __shared__ int last_s[PM_WAVES];
+    __shared__ int64_t pre[PM_THREADS + 1];
+    const int tid = threadIdx.x, lane = tid % WAVE, lr = lane % 32, h = lane / 32;
+    const int wv = __builtin_amdgcn_readfirstlane(tid / WAVE), lag = wv / 4;
+    const int64_t total = part_sums<PM_THREADS>(a, ps, pre);
+    const int64_t stretch = part_stretch(ps, total);
+    // neighbouring stretches, which share kv heads, on one XCD (work groups go round the XCDs)
+    const int per_xcd = ps.workers / 8, worker = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
+    int64_t x = worker * stretch;
+    const int64_t x_end = min(x + stretch, total);
+    const int G = a.nh / a.c.nkv, pmask = (1 << a.c.shift) - 1;
+
+    while (x < x_end) {
+        const PartItem it = part_find<PM_THREADS>(a, ps, pre, x);
+        const int64_t p0 = x - it.at, p1 = min(x_end - it.at, it.len);
+        x = it.at + p1;
+        const int kv = it.q.kv;
+        const int n_live = min(it.q.n * G - it.tile * PM_M, PM_M);
+        // this lane's row (the last one again past the end) and the keys it sees
+        const int my = 32 * wv + lr, rho = it.tile * PM_M + min(my, n_live - 1), tok = rho / G;
+        const int row = it.q.start + tok, head = it.g * G + rho - tok * G;
+        const int end = a.seen ? min(a.seen[row], kv) : kv - it.q.n + tok + 1;
+        int last = end, first = end;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            last = max(last, shfl_xor(last, d));
+            first = min(first, shfl_xor(first, d));
+        }
+        last = 32 * wv < n_live ? max(__builtin_amdgcn_readfirstlane(last), 0) : 0;
+        first = __builtin_amdgcn_readfirstlane(first);
+        if (lane == 0) last_s[wv] = last;
+        if (tid == 0) odd_s = 0;
+        __syncthreads();
+        int tile_last = 0;
+#pragma unroll
+        for (int w = 0; w < PM_WAVES; w++) tile_last = max(tile_last, last_s[w]);
+        tile_last = __builtin_amdgcn_readfirstlane(tile_last);
+        const int64_t blocks = ((int64_t)tile_last + 31) / 32;
+        const int kb0 = (int)(p0 * blocks / it.len), kb1 = (int)(p1 * blocks / it.len);
+        const int my_kb1 = min((last + 31) / 32, kb1);
+
+        // ---- loads and stores of blocks
+        const int* const trow = a.table + (int64_t)it.r * a.max_pages;
+        auto entry = [&](int key) {  // wave-uniform
+            if (key >= kv) return -1;
+            const int e = trow[key >> a.c.shift];
+            return e >= 0 && e < a.c.n_pages ? e : -1;
+        };
+        const E* const kg = static_cast<const E*>(a.c.k) + it.g * a.c.head_stride;
+        const E* const vg = static_cast<const E*>(a.c.v) + it.g * a.c.head_stride;
+        constexpr int KPW = WAVE / KL;  // keys of K per wave
+        const bool k_mine = tid < 32 * KL, v_mine = lane < HD / 2;
+        const int k_key = tid / KL, k_ch = tid % KL;
+        uint8_t* const k_dst = lds + k_ch * L::CHUNK_K + k_key * 16;
+        uint8_t* const v_dst = lds + L::OFF_V + (2 * (wv / 4) + wv % 2) * L::CHUNK_V + lane * 16 + 8 * (wv / 2 % 2);
+        v4i_t kx[KP];
+        typedef typename std::conditional<KP == 2, uint2, uint32_t>::type vrow_t;
+        vrow_t vx[4];
+        bool v_there = false;
+        int ek = -1, ev = -1;  // page of the block loaded next
+        auto next_k = [&](int kb) { ek = wv * KPW < 32 ? entry(kb * 32 + wv * KPW) : -1; };
+        auto next_v = [&](int kb) { ev = entry(kb * 32 + 4 * wv); };
+        auto load_k = [&](int kb) {
+            const int off = (kb * 32 + k_key) & pmask;
+            const E* const p = kg + max(ek, 0) * a.c.page_stride + off * a.c.token_stride + 8 * k_ch;
+            if (k_mine) {
+#pragma unroll
+                for (int u = 0; u < KP; u++) kx[u] = *reinterpret_cast<const v4i_t*>(p + 4 * u);
+            }
+            next_k(kb + 1);
+        };
+        auto load_v = [&](int kb) {
+            const int off = (kb * 32 + 4 * wv) & pmask;
+            const E* const p = vg + max(ev, 0) * a.c.page_stride + off * a.c.token_stride + 2 * lane;
+            if (v_mine) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) vx[j] = *reinterpret_cast<const vrow_t*>(p + j * a.c.token_stride);
+            }
+            v_there = ev >= 0;
+            next_v(kb + 1);
+        };
+        auto put_k = [&](int kb) {
+            uint8_t* const d = k_dst + (kb & 1) * L::BUF_K;
+            if constexpr (!SCALED) {
+                if (k_mine) *reinterpret_cast<v4i_t*>(d) = kx[0];
+            } else {
+                float f[8];
+                uint32_t big = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    uint32_t w;
+                    if constexpr (KP == 2)
+                        w = (uint32_t)kx[j / 4][j % 4];
+                    else
+                        w = j % 2 ? (uint32_t)kx[0][j / 2] & 0xffff0000u : (uint32_t)kx[0][j / 2] << 16;
+                    f[j] = __uint_as_float(w);
+                    big = max(big, w & 0x7fffffffu);
+                }
+                big = dpp_umax<0xB1>(big);   // the key's KL neighbouring lanes
+                big = dpp_umax<0x4E>(big);
+                big = dpp_umax<0x141>(big);
+                if constexpr (KL == 16) big = dpp_umax<0x140>(big);
+                const int e = exponent(big, -100);
+                const float up = pow2(PM_UP - e);
+                v4i_t hi, lo;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t w0, w1;
+                    if constexpr (KP == 2) {
+                        split_f16(f[2 * j] * up, f[2 * j + 1] * up, w0, w1);
+                        lo[j] = (int)w1;
+                    } else {
+                        w0 = pk_f16(f[2 * j] * up, f[2 * j + 1] * up);
+                    }
+                    hi[j] = (int)w0;
+                }
+                if (k_mine) {
+                    *reinterpret_cast<v4i_t*>(d) = hi;
+                    if constexpr (KP == 2) *reinterpret_cast<v4i_t*>(d + L::PIECE_K) = lo;
+                    if (k_ch == 0) k_fac[kb % 3][k_key] = pow2(e - PM_UP);
+                }
+            }
+        };
+        auto put_v = [&](int kb) {
+            uint8_t* const d = v_dst + (kb % 3) * L::BUF_V;
+            const int key0 = kb * 32 + 4 * wv;
+            bool odd = false;
+            float f[4][2];
+            uint32_t w2[4][2], big[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const bool there = v_there && key0 + j < kv && v_mine;
+                if constexpr (KP == 2) {
+                    w2[j][0] = there ? vx[j].x : 0;
+                    w2[j][1] = there ? vx[j].y : 0;
+                } else {
+                    w2[j][0] = there ? vx[j] : 0;
+                }
+                if constexpr (SCALED) {
+                    if constexpr (KP == 1) {
+                        w2[j][1] = w2[j][0] & 0xffff0000u;
+                        w2[j][0] <<= 16;
+                    }
+                    big[j] = max(w2[j][0] & 0x7fffffffu, w2[j][1] & 0x7fffffffu);
+                    f[j][0] = __uint_as_float(w2[j][0]);
+                    f[j][1] = __uint_as_float(w2[j][1]);
+                }
+            }
+            if constexpr (SCALED) {
+                // row j's largest: lanes of equal l % 4 share one row from the second step on
+                uint32_t b0 = lane & 1 ? big[1] : big[0], g0 = lane & 1 ? big[0] : big[1];
+                uint32_t b1 = lane & 1 ? big[3] : big[2], g1 = lane & 1 ? big[2] : big[3];
+                b0 = max(b0, dpp_u<0xB1>(g0));
+                b1 = max(b1, dpp_u<0xB1>(g1));
+                uint32_t b = lane & 2 ? b1 : b0;
+                const uint32_t g = lane & 2 ? b0 : b1;
+                b = max(b, dpp_u<0x4E>(g));   // lane l: row l % 4 of its quad
+                b = dpp_umax<0x124>(b);       // rotations by 4 and 8 in 16 lanes
+                b = dpp_umax<0x128>(b);
+                b = max(b, (uint32_t)shfl_xor((int)b, 16));
+                b = max(b, (uint32_t)shfl_xor((int)b, 32));
+                odd = __any(b >= 0x7f800000u);
+                // (no exponent of its own for a row of zeros: it has to share the sum's range)
+                const int e = b >= 0x7f800000u || b == 0 ? 0 : min(exponent(b, -60), 126);
+                if (lane < 4) {
+                    v_exp[kb % 3][4 * wv + lane] = (float)e;
+                    v_inv[kb % 3][4 * wv + lane] = pow2(-e);
+                }
+                const uint32_t up = __float_as_uint(pow2(PM_VUP - e));
+                const float u0 = __uint_as_float(dpp_u<0x00>(up)), u1 = __uint_as_float(dpp_u<0x55>(up));
+                const float u2 = __uint_as_float(dpp_u<0xAA>(up)), u3 = __uint_as_float(dpp_u<0xFF>(up));
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    uint2 hi, lo;
+                    if constexpr (KP == 2) {
+                        split_f16(f[0][n] * u0, f[1][n] * u1, hi.x, lo.x);
+                        split_f16(f[2][n] * u2, f[3][n] * u3, hi.y, lo.y);
+                    } else {
+                        hi.x = pk_f16(f[0][n] * u0, f[1][n] * u1);
+                        hi.y = pk_f16(f[2][n] * u2, f[3][n] * u3);
+                    }
+                    if (v_mine) {
+                        *reinterpret_cast<uint2*>(d + n * (HD / 2) * 16) = hi;
+                        if constexpr (KP == 2) *reinterpret_cast<uint2*>(d + n * (HD / 2) * 16 + L::PIECE_V) = lo;
+                    }
+                }
+            } else {
+                bool o = false;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    o |= (w2[j][0] & 0x7C00u) == 0x7C00u || (w2[j][0] & 0x7C000000u) == 0x7C000000u;
+                odd = __any(o);
+                if (v_mine) {
+#pragma unroll
+                    for (int n = 0; n < 2; n++)
+                        *reinterpret_cast<uint2*>(d + n * (HD / 2) * 16) =
+                            make_uint2(__builtin_amdgcn_perm(w2[1][0], w2[0][0], n ? 0x07060302u : 0x05040100u),
+                                       __builtin_amdgcn_perm(w2[3][0], w2[2][0], n ? 0x07060302u : 0x05040100u));
+                }
+            }
+            if (lane == 0) {
+                there_s[kb % 3][wv] = v_there ? 1 : 0;
+                if (odd) odd_s = 1;
+            }
+        };
+
+        v16f_t o[ND];
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[d] = v16f_t{};
+        float m_run = -INFINITY, l_run = 0.0f;
+        if (kb0 < kb1) {
+            next_k(kb0);
+            next_v(kb0);
+            load_k(kb0);
+            load_v(kb0);
+        }
+
+        // ---- q: pieces of dims 16 c + 8 h .. + 7, times scale * log2(e) (scores in the base-2
+        // domain) and the row's power of two
+        v4i_t qf[NC][2];
+        float unscale;
+        {
+            const float qscale = a.scale * 1.4426950408889634f;
+            const float* const qp = a.q + ((int64_t)row * a.nh + head) * HD + 8 * h;
+            v4f_t q[NC][2];
+            uint32_t big = 0;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    q[c][u] = *reinterpret_cast<const v4f_t*>(qp + 16 * c + 4 * u) * qscale;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) big = max(big, __float_as_uint(q[c][u][j]) & 0x7fffffffu);
+                }
+            big = max(big, (uint32_t)shfl_xor((int)big, 32));
+            const int e = exponent(big, -100);
+            const float up = pow2(PM_UP - e);
+            unscale = pow2(e - PM_UP);
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t w0, w1;
+                    split_f16(q[c][j / 2][2 * (j % 2)] * up, q[c][j / 2][2 * (j % 2) + 1] * up, w0, w1);
+                    qf[c][0][j] = (int)w0;
+                    qf[c][1][j] = (int)w1;
+                }
+        }
+
+        v4i_t pf[2][2];  // the weights' pieces, keys 16 c .. in step c
+        // scores of block kb and its weights' pieces; returns the factor of o
+        auto scores = [&](int kb) {
+            const uint8_t* const kb_ = lds + (kb & 1) * L::BUF_K + h * L::CHUNK_K + lr * 16;
+            v4i_t kf[2][KP];
+            auto read = [&](int c) {
+#pragma unroll
+                for (int q = 0; q < KP; q++)
+                    kf[c & 1][q] = *reinterpret_cast<const v4i_t*>(kb_ + q * L::PIECE_K + 2 * c * L::CHUNK_K);
+            };
+            v16f_t s = v16f_t{};
+            read(0);
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                if (c + 1 < NC) read(c + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (KP == 2) s = mfma_f16(kf[c & 1][1], qf[c][0], s);
+                s = mfma_f16(kf[c & 1][0], qf[c][1], s);
+                s = mfma_f16(kf[c & 1][0], qf[c][0], s);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const uint64_t there = *reinterpret_cast<const uint64_t*>(there_s[kb % 3]);
+            const bool all = there == 0x0101010101010101ull;
+            v4f_t inv[4];
+            float big = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                v4f_t fac, ex;
+                if constexpr (SCALED) {
+                    fac = *reinterpret_cast<const v4f_t*>(&k_fac[kb % 3][8 * u + 4 * h]);
+                    ex = *reinterpret_cast<const v4f_t*>(&v_exp[kb % 3][8 * u + 4 * h]);
+                    inv[u] = *reinterpret_cast<const v4f_t*>(&v_inv[kb % 3][8 * u + 4 * h]);
+                }
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    float t = s[4 * u + v] * unscale;
+                    if constexpr (SCALED) t = fmaf(t, fac[v], ex[v]);
+                    if (!all || kb * 32 + 32 > first) {  // wave-uniform
+                        if (!((there >> (8 * (2 * u + h))) & 1) || kb * 32 + 8 * u + 4 * h + v >= end) t = -INFINITY;
+                    }
+                    s[4 * u + v] = t;
+                    big = fmaxf(big, t);
+                }
+            }
+            big = fmaxf(big, shfl_xor(big, 32));
+            const float m = fmaxf(m_run, big);
+            const float ref = m == -INFINITY ? 0.0f : m;
+            const float alpha = __builtin_amdgcn_exp2f(m_run - ref);
+            float sum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                s[v] = __builtin_amdgcn_exp2f(s[v] - (ref - (float)PM_UP));
+                if constexpr (SCALED)
+                    sum = fmaf(s[v], inv[v / 4][v % 4], sum);
+                else
+                    sum += s[v];
+            }
+            sum += shfl_xor(sum, 32);
+            l_run = l_run * alpha + sum;
+            m_run = m;
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t w0, w1;
+                    split_f16(s[8 * c + 2 * j], s[8 * c + 2 * j + 1], w0, w1);
+                    pf[c][0][j] = (int)w0;
+                    pf[c][1][j] = (int)w1;
+                }
+            return alpha;
+        };
+        auto values = [&](int kb, float alpha) {
+            if (__any(alpha != 1.0f)) {
+#pragma unroll
+                for (int d = 0; d < ND; d++) o[d] *= alpha;
+            }
+            const uint8_t* const vb = lds + L::OFF_V + (kb % 3) * L::BUF_V + h * L::CHUNK_V + lr * 16;
+            v4i_t vf[2][KP];
+            auto read = [&](int i) {  // slots 32 (i % ND) .. of step i / ND
+#pragma unroll
+                for (int q = 0; q < KP; q++)
+                    vf[i & 1][q] = *reinterpret_cast<const v4i_t*>(vb + q * L::PIECE_V + 2 * (i / ND) * L::CHUNK_V +
+                                                                   512 * (i % ND));
+            };
+            read(0);
+#pragma unroll
+            for (int i = 0; i < 2 * ND; i++) {
+                if (i + 1 < 2 * ND) read(i + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                v16f_t& t = o[i % ND];
+                if constexpr (KP == 2) t = mfma_f16(vf[i & 1][1], pf[i / ND][0], t);
+                t = mfma_f16(vf[i & 1][0], pf[i / ND][1], t);
+                t = mfma_f16(vf[i & 1][0], pf[i / ND][0], t);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+
+        if (kb0 < kb1) {
+            put_k(kb0);
+            load_k(kb0 + 1);
+        }
+        float alpha = 1.0f;
+        for (int kb = kb0; kb < kb1; kb++) {
+            put_v(kb);
+            load_v(kb + 1);
+            __syncthreads();  // block kb is in LDS; K of block kb - 1 and V of kb - 2 are read out
+            if (lag == 1 && kb > kb0 && kb - 1 < my_kb1) values(kb - 1, alpha);
+            if (kb < my_kb1) alpha = scores(kb);
+            if (kb + 1 < kb1) put_k(kb + 1);
+            load_k(kb + 2);
+            if (lag == 0 && kb < my_kb1) values(kb, alpha);
+        }
+        if (lag == 1 && my_kb1 == kb1 && kb0 < kb1) values(kb1 - 1, alpha);
+
+        // l carries the weights' factor too, scaled values have one of their own
+        float down = SCALED ? pow2(-PM_VUP) : 1.0f;
+        __syncthreads();
+        if (odd_s) {  // again, key by key
+            slow_rows<E, HD, 2>(
+                a, trow, kv, kb0 * 32, my_kb1 * 32, end, a.q + ((int64_t)row * a.nh + head) * HD, kg, vg,
+                [&](int i) { return 2 * (32 * (i / 16 % (ND / 2)) + 8 * (i % 16 / 4) + 4 * h + i % 4) + i / (8 * ND); },
+                [&](int i, float v) { o[i / 16][i % 16] = v; }, [&](int i) { return o[i / 16][i % 16]; }, m_run, l_run);
+            down = pow2(PM_UP);  // as the other pieces of its item
+            l_run *= down;
+        }
+        if (my < n_live) {
+            const bool whole = p0 == 0 && p1 == it.len;
+            float* dst;
+            float f = down;
+            if (whole) {
+                dst = a.out + ((int64_t)row * a.nh + head) * HD;
+                f = l_run == 0.0f ? 0.0f : down / l_run;
+            } else {
+                float* const slot = a.ws + (size_t)(2 * worker + (p0 == 0 ? 1 : 0)) * part_slot_floats(PM_M, HD);
+                dst = slot + my * HD;
+                if (h == 0) {
+                    slot[PM_M * HD + my] = m_run;
+                    slot[PM_M * (HD + 1) + my] = l_run;
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < ND / 2; d++)
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    float* const p = dst + 2 * (32 * d + 8 * u + 4 * h);
+#pragma unroll
+                    for (int v = 0; v < 2; v++)
+                        *reinterpret_cast<v4f_t*>(p + 4 * v) =
+                            (v4f_t){o[d][4 * u + 2 * v], o[d + ND / 2][4 * u + 2 * v], o[d][4 * u + 2 * v + 1],
+                                    o[d + ND / 2][4 * u + 2 * v + 1]} *
+                            f;
+                }
+        }
+        __syncthreads();  // last_s and the buffers are free
+    }
+}
+
+template <class E>
+static void launch(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
+    if (a.c.hd == 128)
+        hipLaunchKernelGGL((paged_many_kernel<E, 128>), dim3(ps.workers), dim3(PM_THREADS), 0, s, a, ps);
+    else
+        hipLaunchKernelGGL((paged_many_kernel<E, 64>), dim3(ps.workers), dim3(PM_THREADS), 0, s, a, ps);
+}
+
+hipError_t launch_paged_many(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
+    if (a.c.type == HY_TYPE_F32)
+        launch<float>(a, ps, s);
+    else if (a.c.type == HY_TYPE_F16)
+        launch<_Float16>(a, ps, s);
+    else
+        launch<__bf16>(a, ps, s);
+    return hipGetLastError();
+}
+
+}  // namespace hy

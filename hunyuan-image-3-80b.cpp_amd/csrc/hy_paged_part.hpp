@@ -75,6 +75,12 @@ __device__ __forceinline__ int64_t part_sums(const PagedAttnArgs& a, const PartS
     return total;
 }
 
+// a value that all lanes share, in scalar registers
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    return (int64_t)(((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v));
+}
+
 __device__ __forceinline__ int64_t part_stretch(const PartShape& p, int64_t total) {
     return max((total + p.workers - 1) / p.workers, (int64_t)p.min_keys);
 }
@@ -90,18 +96,19 @@ struct PartItem {
 template <int THREADS>
 __device__ __forceinline__ PartItem part_find(const PagedAttnArgs& a, const PartShape& p, const int64_t* pre,
                                               int64_t x) {
+    x = uniform(x);
     int lo = 0, hi = THREADS;  // pre[lo] <= x < pre[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (pre[mid] <= x)
+        if (uniform(pre[mid]) <= x)
             lo = mid;
         else
             hi = mid;
     }
     const int per = (a.n_req + THREADS - 1) / THREADS;
     PartItem it;
-    it.r = lo * per;
-    it.at = pre[lo];
+    it.r = uniform(lo * per);
+    it.at = uniform(pre[uniform(lo)]);
     it.q = part_req(a, p, it.r);
     while (x - it.at >= it.q.head * a.c.nkv) {
         it.at += it.q.head * a.c.nkv;
@@ -124,9 +131,52 @@ __device__ __forceinline__ PartItem part_find(const PagedAttnArgs& a, const Part
     return it;
 }
 
+// Attention of this lane's row over keys k0 .. k1 - 1, key by key in f32: what the kernels do
+// again where their V holds infinities or NaNs.  A key of weight 0 does not touch the row.
+// LPR lanes (l, l + 64 / LPR, ...) share a row, the i-th of a lane's HD / LPR dims is dim(i);
+// set and get access the sums, m and l get the running maximum (base 2) and sum.
+template <class E, int HD, int LPR, class Dim, class Set, class Get>
+__device__ __forceinline__ void slow_rows(const PagedAttnArgs& a, const int* trow, int kv, int k0, int k1, int end,
+                                          const float* q, const E* kg, const E* vg, Dim dim, Set set, Get get,
+                                          float& m, float& l) {
+    constexpr int N = HD / LPR;
+    const float qscale = a.scale * 1.4426950408889634f;
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) set(i, 0.0f);
+#pragma unroll 1
+    for (int key = k0; key < min(k1, kv); key++) {
+        const int e = trow[key >> a.c.shift];
+        if (e < 0 || e >= a.c.n_pages) continue;
+        const int64_t at = e * a.c.page_stride + (key & ((1 << a.c.shift) - 1)) * a.c.token_stride;
+        const float* qk = q;
+        asm volatile("" : "+v"(qk));  // read again for every key, not kept in registers
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; i++) s = fmaf(qk[dim(i)] * qscale, (float)kg[at + dim(i)], s);
+#pragma unroll
+        for (int d = 32; d >= 64 / LPR; d >>= 1) s += shfl_xor(s, d);
+        if (key >= end) s = -INFINITY;
+        const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
+        const float alpha = __builtin_amdgcn_exp2f(m - ref), p = __builtin_amdgcn_exp2f(s - ref);
+        m = mn;
+        l = l * alpha + p;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float v = p * (float)vg[at + dim(i)];
+            set(i, get(i) * alpha + (p != 0.0f ? v : 0.0f));
+        }
+    }
+}
+
 // Partial results: worker w's first piece, of an item begun before it, in slot 2 w, its last,
 // of an item it begins and another ends, in 2 w + 1.  A slot: [M][hd] unnormalised output,
 // [M] running maximum, [M] sum.
 __host__ __device__ __forceinline__ size_t part_slot_floats(int M, int hd) { return (size_t)M * (hd + 2); }
+
+// requests of many rows: tiles of PM_TILE rows, PM_WORKERS work groups (hy_paged_many.hip)
+constexpr int PM_TILE = 256, PM_WORKERS = 256;
+hipError_t launch_paged_many(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s);
 
 }  // namespace hy
