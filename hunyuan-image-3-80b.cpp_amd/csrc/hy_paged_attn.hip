@@ -21,12 +21,9 @@
 #include "hy_lds.hpp"
 #include "hy_paged.hpp"
 #include "hy_paged_part.hpp"
-#include "hy_split.hpp"
+#include "hy_paged_split.hpp"
 
 namespace hy {
-
-typedef _Float16 v8h16_t __attribute__((ext_vector_type(8)));
-typedef _Float16 v2h16_t __attribute__((ext_vector_type(2)));
 
 // the operand kinds of a cache type
 template <class E>
@@ -40,10 +37,7 @@ struct PaType<_Float16> {
     }
     // two floats -> their pieces, packed
     static __device__ __forceinline__ void split(float a, float b, uint32_t (&p)[2]) {
-        const v2h16_t h = __builtin_convertvector((v2f_t){a, b}, v2h16_t);
-        const v2f_t r = (v2f_t){a, b} - __builtin_convertvector(h, v2f_t);
-        p[0] = __builtin_bit_cast(uint32_t, h);
-        p[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2h16_t));
+        split_f16(a, b, p[0], p[1]);
     }
     static __device__ __forceinline__ bool odd(uint32_t w) {  // an infinity or NaN among the two
         return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
@@ -72,20 +66,19 @@ struct PaType<float> {
     static __device__ __forceinline__ bool odd(uint32_t w) { return (w & 0x7F800000u) == 0x7F800000u; }
 };
 
-__device__ __forceinline__ float group_max(float v) {  // over lanes i, 16 + i, 32 + i, 48 + i
-    v = fmaxf(v, shfl_xor(v, 16));
-    return fmaxf(v, shfl_xor(v, 32));
-}
-__device__ __forceinline__ float group_sum(float v) {
-    v += shfl_xor(v, 16);
-    return v + shfl_xor(v, 32);
-}
+// over lanes i, 16 + i, 32 + i, 48 + i
+__device__ __forceinline__ float group_max(float v) { return fmax_half(fmax_row(v)); }
+__device__ __forceinline__ float group_sum(float v) { return fadd_half(fadd_row(v)); }
 
 constexpr int PF_WAVES = 4;
-constexpr float PF_PSCALE = 16384.0f;  // of the probabilities' f16 pieces
+// The running maximum that weights are relative to is left behind while a block's scores do not
+// pass it by more than PA_LAG (base 2): weights are up to 2^PA_LAG, and the sums are rescaled
+// once or twice per row instead of at every new maximum.
+constexpr float PA_LAG = 8.0f;
+constexpr float PF_PSCALE = 64.0f;  // of the weights' f16 pieces: below 2^14 with PA_LAG
 
 template <class E, int HD, int NT>
-__global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttnArgs a, PartShape ps) {
+__global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && NT == 2 && HD == 128 ? 1 : 2) void paged_few_kernel(PagedAttnArgs a, PartShape ps) {
     using P = PaType<E>;
     constexpr bool F32T = sizeof(E) == 4, F16T = std::is_same<E, _Float16>::value;
     constexpr int KB = F32T ? 16 : 32;       // keys per turn
@@ -96,43 +89,56 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
     constexpr int ND = HD / 16;              // 16-dim tiles of the output
     constexpr int PC = P::PIECES;
     constexpr int VW = VD * (int)sizeof(E) / 4;    // dwords of a V load
-    __shared__ int64_t pre[WAVE * PF_WAVES + 1];
+    __shared__ PartSums<WAVE * PF_WAVES> sums;
     const int lane = threadIdx.x % WAVE, i = lane % 16, g4 = lane / 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    const int64_t total = part_sums<WAVE * PF_WAVES>(a, ps, pre);
+    const int64_t total = part_sums(a, ps, sums);
     const int64_t stretch = part_stretch(ps, total);
     const int worker = blockIdx.x * PF_WAVES + wave;
     int64_t x = worker * stretch;
     const int64_t x_end = min(x + stretch, total);
-    const int G = a.nh / a.c.nkv, pmask = (1 << a.c.shift) - 1;
+    const int G = ps.G, pmask = (1 << a.c.shift) - 1;
     const float qscale = a.scale * 1.4426950408889634f;
 
     while (x < x_end) {
-        const PartItem it = part_find<WAVE * PF_WAVES>(a, ps, pre, x);
+        const PartItem it = part_find(a, ps, sums, x);
         const int64_t p0 = x - it.at, p1 = min(x_end - it.at, it.len);  // this piece
         x = it.at + p1;
 
         // rows of this lane's columns; rows past the last repeat it and are not stored
         const int n_live = min(it.q.n * G - it.tile * ps.M, ps.M);
-        int row[NT], head[NT], end[NT], last = 0, first = 0x7fffffff;
+        int row[NT], head[NT], end[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const int rho = it.tile * ps.M + min(16 * t + i, n_live - 1), tok = rho / G;
             row[t] = it.q.start + tok;
             head[t] = it.g * G + rho - tok * G;
             end[t] = a.seen ? min(a.seen[row[t]], it.q.kv) : it.q.kv - it.q.n + tok + 1;
-            last = max(last, end[t]);
-            first = min(first, end[t]);
         }
+        int last, first;  // the most and the fewest keys that a row sees
+        if (a.seen) {
+            last = max(end[0], 0);
+            first = end[0];
+            if constexpr (NT == 2) {
+                last = max(last, end[1]);
+                first = min(first, end[1]);
+            }
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) {
-            last = max(last, shfl_xor(last, d));
-            first = min(first, shfl_xor(first, d));
+            for (int d = 1; d < 16; d <<= 1) {
+                last = max(last, shfl_xor(last, d));
+                first = min(first, shfl_xor(first, d));
+            }
+        } else {
+            const int rho = it.tile * ps.M;
+            first = it.q.kv - it.q.n + rho / G + 1;
+            last = max(it.q.kv - it.q.n + (rho + n_live - 1) / G + 1, 0);
         }
-        last = __builtin_amdgcn_readfirstlane(last);
-        first = __builtin_amdgcn_readfirstlane(first);
-        const int64_t blocks = ((int64_t)last + 31) / 32;
-        const int t0 = (int)(p0 * blocks / it.len) * (32 / KB), t1 = (int)(p1 * blocks / it.len) * (32 / KB);
+        last = uniform(last);
+        first = uniform(first);
+        const int blocks = (last + 31) / 32;
+        const int t0 = part_block(p0, it.len, blocks) * (32 / KB), t1 = part_block(p1, it.len, blocks) * (32 / KB);
+
+        const int slot_id = p0 == 0 && p1 == it.len ? -1 : 2 * worker + (p0 == 0 ? 1 : 0);  // -1: all of it is here
 
         // q: scaled by scale * log2(e) (scores in the base-2 domain); f16: by a power of two that
         // brings the row's largest to [2^13, 2^14), undone on the scores
@@ -144,12 +150,14 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
             const float* const qp = a.q + ((int64_t)row[t] * a.nh + head[t]) * HD;
             unscale[t] = 1.0f;
             if constexpr (F32T) {
+                v4f_t q[NQ];
 #pragma unroll
-                for (int s = 0; s < NQ; s++) {
-                    const v4f_t q = *reinterpret_cast<const v4f_t*>(qp + 16 * s + 4 * g4);
+                for (int s = 0; s < NQ; s++) q[s] = *reinterpret_cast<const v4f_t*>(qp + 16 * s + 4 * g4);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) qx[t][4 * s + j] = q[j] * qscale;
-                }
+                for (int s = 0; s < NQ; s++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) qx[t][4 * s + j] = q[s][j] * qscale;
             } else {
                 v4f_t q[NQ][2];
                 float big = 0.0f;
@@ -157,7 +165,14 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
                 for (int s = 0; s < NQ; s++)
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
-                        q[s][u] = *reinterpret_cast<const v4f_t*>(qp + 32 * s + 8 * g4 + 4 * u) * qscale;
+                        q[s][u] = *reinterpret_cast<const v4f_t*>(qp + 32 * s + 8 * g4 + 4 * u);
+                    }
+                __builtin_amdgcn_sched_barrier(0);  // all of them in flight
+#pragma unroll
+                for (int s = 0; s < NQ; s++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        q[s][u] *= qscale;
 #pragma unroll
                         for (int j = 0; j < 4; j++) big = fmaxf(big, fabsf(q[s][u][j]));
                     }
@@ -285,35 +300,39 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
             const bool edge = (t + 1) * KB > first || __any(none);
 #pragma unroll
             for (int c = 0; c < NT; c++) {
+                if (edge) {  // wave-uniform
+                    asm volatile("");
+#pragma unroll
+                    for (int u = 0; u < KT; u++)
+#pragma unroll
+                        for (int v = 0; v < 4; v++)
+                            if (t * KB + 16 * u + 4 * g4 + v >= end[c] || vpage[u] < 0) s[c][u][v] = -INFINITY;
+                }
                 float big = -INFINITY;
 #pragma unroll
                 for (int u = 0; u < KT; u++)
 #pragma unroll
                     for (int v = 0; v < 4; v++) {
                         if constexpr (F16T) s[c][u][v] *= unscale[c];
-                        if (edge) {
-                            const int key = t * KB + 16 * u + 4 * g4 + v;
-                            if (key >= end[c] || vpage[u] < 0) s[c][u][v] = -INFINITY;
-                        }
                         big = fmaxf(big, s[c][u][v]);
                     }
-                const float m = fmaxf(m_run[c], group_max(big));
-                const float ref = m == -INFINITY ? 0.0f : m;
-                const float alpha = __builtin_amdgcn_exp2f(m_run[c] - ref);
-                float sum = 0.0f;
+                if (__any(big > m_run[c] + PA_LAG)) {
+                    big = group_max(big);
+                    const float m = big > m_run[c] + PA_LAG ? big : m_run[c];
+                    const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[c] - m);
+                    m_run[c] = m;
+                    l_run[c] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < ND; d++) o[c][d] *= alpha;
+                }
+                const float ref = m_run[c] == -INFINITY ? 0.0f : m_run[c];
 #pragma unroll
                 for (int u = 0; u < KT; u++)
 #pragma unroll
                     for (int v = 0; v < 4; v++) {
                         s[c][u][v] = __builtin_amdgcn_exp2f(s[c][u][v] - ref);
-                        sum += s[c][u][v];
+                        l_run[c] += s[c][u][v];  // of this lane's keys; joined behind the loop
                     }
-                l_run[c] = l_run[c] * alpha + group_sum(sum);
-                m_run[c] = m;
-                if (__any(alpha != 1.0f)) {
-#pragma unroll
-                    for (int d = 0; d < ND; d++) o[c][d] *= alpha;
-                }
             }
             if (edge) {
 #pragma unroll
@@ -366,6 +385,8 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
             if (t + 1 < t1) load_v(t + 1);
         }
 
+#pragma unroll
+        for (int c = 0; c < NT; c++) l_run[c] = group_sum(l_run[c]);
         float down = F16T ? 1.0f / PF_PSCALE : 1.0f;
         if (__any(odd)) {  // again, key by key
             down = 1.0f;
@@ -377,14 +398,13 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
                     [&](int n, float v) { o[c][n / 4][n % 4] = v; }, [&](int n) { return o[c][n / 4][n % 4]; }, m_run[c],
                     l_run[c]);
         }
-        const bool whole = p0 == 0 && p1 == it.len;
-        float* const slot = a.ws + (size_t)(2 * worker + (p0 == 0 ? 1 : 0)) * part_slot_floats(ps.M, HD);
+        float* const slot = a.ws + (size_t)max(slot_id, 0) * part_slot_floats(ps.M, HD);
 #pragma unroll
         for (int c = 0; c < NT; c++) {
             if (16 * c + i >= n_live) continue;
             float* dst;
             float f = down;
-            if (whole) {
+            if (slot_id < 0) {
                 dst = a.out + ((int64_t)row[c] * a.nh + head[c]) * HD;
                 f = l_run[c] == 0.0f ? 0.0f : down / l_run[c];
             } else {
@@ -409,52 +429,73 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
     }
 }
 
-// Joins the pieces of every cut item: work group w the item that worker w begins and another
-// ends, a thread 4 dims of a row at a time.
-template <int HD>
+// Joins the pieces of every cut item: a team of THREADS / JOBS threads per worker w takes the
+// item that w begins and another ends, HD / 4 threads a row, 4 dims each.  The pieces' statistics
+// and sums are fetched PJ at a time, which is what a join of few rows waits for.
+constexpr int PJ = 8;
+template <int HD, int JOBS>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartShape ps) {
-    __shared__ int64_t pre[257];
-    const int64_t total = part_sums<256>(a, ps, pre);
+    __shared__ PartSums<256> sums;
+    const int64_t total = part_sums(a, ps, sums);
     const int64_t stretch = part_stretch(ps, total);
-    const int64_t cut = ((int64_t)blockIdx.x + 1) * stretch;  // the end of worker w's stretch
+    constexpr int TEAM = 256 / JOBS;  // a wave at least
+    const int w0 = uniform((int)(blockIdx.x * JOBS + threadIdx.x / TEAM)), tt = threadIdx.x % TEAM;
+    const int64_t cut = ((int64_t)w0 + 1) * stretch;  // the end of worker w0's stretch
     if (cut >= total) return;
-    const PartItem it = part_find<256>(a, ps, pre, cut);
+    const PartItem it = part_find(a, ps, sums, cut);
     if (it.at >= cut || it.at < cut - stretch) return;  // begins here, or was begun by another
-    const int w0 = blockIdx.x, w1 = (int)((it.at + it.len - 1) / stretch);
-    const int G = a.nh / a.c.nkv;
-    const int n_live = min(it.q.n * G - it.tile * ps.M, ps.M);
+    const int64_t past = it.at + it.len - cut;           // beyond w0's stretch
+    int n_piece = 1 + uniform((int)((float)past * __builtin_amdgcn_rcpf((float)stretch)));
+    while ((int64_t)(n_piece - 1) * stretch >= past) n_piece--;
+    while ((int64_t)(n_piece - 1) * stretch < past) n_piece++;
+    const int n_live = min(it.q.n * ps.G - it.tile * ps.M, ps.M);
     const size_t sf = part_slot_floats(ps.M, HD);
     const float* const first = a.ws + (size_t)(2 * w0 + 1) * sf;
-    auto slot = [&](int w) { return w == w0 ? first : a.ws + (size_t)(2 * w) * sf; };
-    constexpr int TR = HD / 4, RPB = 256 / TR;  // threads per row, rows at a time
-    const int d = threadIdx.x % TR * 4;
-    for (int i = blockIdx.y * RPB + threadIdx.x / TR; i < n_live; i += RPB * gridDim.y) {
-        float m = -INFINITY;
-        bool nan = false;
-        for (int w = w0; w <= w1; w++) {
-            const float x = slot(w)[ps.M * HD + i];
-            nan |= x != x;
-            m = fmaxf(m, x);
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
+    const float* const rest = a.ws + (size_t)(2 * w0) * sf;  // piece k > 0: + 2 k slots
+    constexpr int TR = HD / 4, RPB = TEAM / TR;  // threads per row, rows at a time
+    const int d = tt % TR * 4;
+    for (int i = blockIdx.y * RPB + tt / TR; i < n_live; i += RPB * gridDim.y) {
+        float m = -INFINITY, l = 0.0f;
         v4f_t o = v4f_t{};
-        float l = nan ? __builtin_nanf("") : 0.0f;
-        for (int w = w0; w <= w1; w++) {
-            const float* const s = slot(w);
-            const float f = __builtin_amdgcn_exp2f(s[ps.M * HD + i] - ref);
-            l += f * s[ps.M * (HD + 1) + i];
-            o += f * *reinterpret_cast<const v4f_t*>(s + i * HD + d);
+        for (int k0 = 0; k0 < n_piece; k0 += PJ) {
+            float mk[PJ], lk[PJ];
+            v4f_t ok[PJ];
+#pragma unroll
+            for (int j = 0; j < PJ; j++) {
+                const int k = min(k0 + j, n_piece - 1);
+                const float* const s = k == 0 ? first : rest + (size_t)(2 * k) * sf;
+                mk[j] = s[ps.M * HD + i];
+                lk[j] = s[ps.M * (HD + 1) + i];
+                ok[j] = *reinterpret_cast<const v4f_t*>(s + i * HD + d);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            float mn = m;
+#pragma unroll
+            for (int j = 0; j < PJ; j++) mn = fmaxf(mn, mk[j]);
+            const float ref = mn == -INFINITY ? 0.0f : mn, alpha = __builtin_amdgcn_exp2f(m - ref);
+            m = mn;
+            l *= alpha;
+            o *= alpha;
+#pragma unroll
+            for (int j = 0; j < PJ; j++) {
+                const float f = __builtin_amdgcn_exp2f(mk[j] - ref);
+                if (k0 + j < n_piece) {
+                    l += f * lk[j];
+                    o += f * ok[j];
+                }
+            }
         }
-        const int rho = it.tile * ps.M + i, tok = rho / G;
+        const int rho = it.tile * ps.M + i, tok = rho / ps.G;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        *reinterpret_cast<v4f_t*>(a.out + ((int64_t)(it.q.start + tok) * a.nh + it.g * G + rho - tok * G) * HD + d) =
-            o * inv;
+        *reinterpret_cast<v4f_t*>(a.out + ((int64_t)(it.q.start + tok) * a.nh + it.g * ps.G + rho - tok * ps.G) * HD +
+                                  d) = o * inv;
     }
 }
 
 constexpr int PF_GROUPS = 512;  // two per CU
 constexpr int PF_WORKERS = PF_GROUPS * PF_WAVES;
 constexpr int PF_MAX_M = 32;
+constexpr int PF_MIN_KEYS = 64, PM_MIN_KEYS = 128;
 
 // rows of a request up to which the stream takes it
 constexpr int PF_MAX_ROWS = PF_MAX_M;
@@ -463,12 +504,18 @@ size_t paged_attn_ws_bytes(int, int, int hd) {
     return max(2 * PF_WORKERS * part_slot_floats(PF_MAX_M, hd), 2 * PM_WORKERS * part_slot_floats(PM_TILE, hd)) * 4;
 }
 
+template <int HD>
 static void launch_join(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
-    const dim3 grid(ps.workers, ps.M > PF_MAX_M ? 8 : 1);
-    if (a.c.hd == 128)
-        hipLaunchKernelGGL(paged_join_kernel<128>, grid, dim3(256), 0, s, a, ps);
+    if (ps.M <= PF_MAX_M)  // few rows: a wave each
+        hipLaunchKernelGGL((paged_join_kernel<HD, 4>), dim3(ps.workers / 4), dim3(256), 0, s, a, ps);
     else
-        hipLaunchKernelGGL(paged_join_kernel<64>, grid, dim3(256), 0, s, a, ps);
+        hipLaunchKernelGGL((paged_join_kernel<HD, 1>), dim3(ps.workers, 8), dim3(256), 0, s, a, ps);
+}
+static void launch_join(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
+    if (a.c.hd == 128)
+        launch_join<128>(a, ps, s);
+    else
+        launch_join<64>(a, ps, s);
 }
 
 template <class E, int HD>
@@ -480,11 +527,12 @@ static void launch_few(const PagedAttnArgs& a, const PartShape& ps, hipStream_t 
 }
 
 hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s) {
-    const int64_t rows = (int64_t)max_new * (a.nh / a.c.nkv);  // of one request, at most
+    const int G = a.nh / a.c.nkv;
+    const int64_t rows = (int64_t)max_new * G;  // of one request, at most
     constexpr int64_t ALL = (int64_t)1 << 62;
     const bool many = rows > PF_MAX_ROWS;
     if (!many || a.n_req > 1) {
-        const PartShape ps{rows > 16 ? 32 : 16, 0, many ? PF_MAX_ROWS : ALL, PF_WORKERS, 64};
+        const PartShape ps = part_shape(rows > 16 ? 5 : 4, G, 0, many ? PF_MAX_ROWS : ALL, PF_WORKERS, PF_MIN_KEYS);
         const bool big = a.c.hd == 128;
         if (a.c.type == HY_TYPE_F32)
             big ? launch_few<float, 128>(a, ps, s) : launch_few<float, 64>(a, ps, s);
@@ -495,7 +543,7 @@ hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s)
         launch_join(a, ps, s);
     }
     if (many) {
-        const PartShape ps{PM_TILE, a.n_req > 1 ? PF_MAX_ROWS : 0, ALL, PM_WORKERS, 64};
+        const PartShape ps = part_shape(PM_TILE_SHIFT, G, a.n_req > 1 ? PF_MAX_ROWS : 0, ALL, PM_WORKERS, PM_MIN_KEYS);
         (void)launch_paged_many(a, ps, s);
         launch_join(a, ps, s);
     }

@@ -10,7 +10,7 @@
 // the top of its range: q per row, and for f32 and bf16 caches K and V per key (elements down to
 // 2^-27 of their vector's largest keep all bits of a piece, none is off by more than 2^-38 of it).  K's
 // factor is undone on the scores.  V's, 2^e_j, joins the weights: with R the running
-// maximum of s_j + e_j the accumulators sum w_j v_j 2^-e_j, w_j = 2^(s_j + e_j - R) <= 1,
+// maximum of s_j + e_j the accumulators sum w_j v_j 2^-e_j, w_j = 2^(s_j + e_j - R),
 // and w_j 2^-e_j = 2^(s_j - R), which leaves out = O / l in any reference R.
 //
 // Blocks of 32 keys: every thread loads its share of a block of K and V one block ahead,
@@ -26,32 +26,25 @@
 #include "hy_lds.hpp"
 #include "hy_paged.hpp"
 #include "hy_paged_part.hpp"
-#include "hy_split.hpp"
+#include "hy_paged_split.hpp"
 
 namespace hy {
 
-typedef _Float16 v8h16_t __attribute__((ext_vector_type(8)));
-typedef _Float16 v2h16_t __attribute__((ext_vector_type(2)));
-
 constexpr int PM_WAVES = 8, PM_THREADS = WAVE * PM_WAVES, PM_M = PM_TILE;
 static_assert(PM_M == 32 * PM_WAVES && PM_WORKERS % 8 == 0, "32 rows per wave, whole XCDs");
-constexpr int PM_UP = 14;   // q's and K's largest elements go to [2^14, 2^15), weights to 2^14
+constexpr int PM_UP = 14;   // q's and K's largest elements go to [2^14, 2^15)
 constexpr int PM_VUP = 13;  // V's to [2^13, 2^14): 2^-e of an e up to 126 is a normal number
+// The running maximum R that weights are relative to is left behind while a block does not pass
+// it by more than PM_LAG: weights are up to 2^PM_LAG, and the sums are rescaled once or twice
+// per row instead of at every new maximum.  Weights carry a factor 2^PM_WUP.
+constexpr float PM_LAG = 8.0f;
+constexpr int PM_WUP = 6;
 
 __device__ __forceinline__ v16f_t mfma_f16(v4i_t a, v4i_t b, v16f_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h16_t, a), __builtin_bit_cast(v8h16_t, b), c, 0,
                                                   0, 0);
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126..127
-// two floats -> f16 pieces, packed
-__device__ __forceinline__ uint32_t pk_f16(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f_t){a, b}, v2h16_t));
-}
-__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
-    hi = pk_f16(a, b);
-    const v2f_t r = (v2f_t){a, b} - __builtin_convertvector(__builtin_bit_cast(v2h16_t, hi), v2f_t);
-    lo = pk_f16(r[0], r[1]);
-}
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
@@ -84,24 +77,25 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
     constexpr int KP = L::KP;
     constexpr int NC = HD / 16, ND = HD / 32;
     constexpr int KL = HD / 8;  // threads per key of K
+    constexpr int RING = KP == 2 ? 2 : 3;  // operands read ahead of the products (registers allowing)
     __shared__ __attribute__((aligned(1024))) uint8_t lds[L::BYTES];
     __shared__ __attribute__((aligned(16))) float k_fac[3][32], v_exp[3][32], v_inv[3][32];
     __shared__ __attribute__((aligned(8))) uint8_t there_s[3][PM_WAVES];  // 4 keys: 1, or 0 (no page)
     __shared__ int odd_s;  // an infinity or NaN in this piece's V
     __shared__ int last_s[PM_WAVES];
-    __shared__ int64_t pre[PM_THREADS + 1];
+    __shared__ PartSums<PM_THREADS> sums;
     const int tid = threadIdx.x, lane = tid % WAVE, lr = lane % 32, h = lane / 32;
     const int wv = __builtin_amdgcn_readfirstlane(tid / WAVE), lag = wv / 4;
-    const int64_t total = part_sums<PM_THREADS>(a, ps, pre);
+    const int64_t total = part_sums(a, ps, sums);
     const int64_t stretch = part_stretch(ps, total);
     // neighbouring stretches, which share kv heads, on one XCD (work groups go round the XCDs)
     const int per_xcd = ps.workers / 8, worker = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
     int64_t x = worker * stretch;
     const int64_t x_end = min(x + stretch, total);
-    const int G = a.nh / a.c.nkv, pmask = (1 << a.c.shift) - 1;
+    const int G = ps.G, pmask = (1 << a.c.shift) - 1;
 
     while (x < x_end) {
-        const PartItem it = part_find<PM_THREADS>(a, ps, pre, x);
+        const PartItem it = part_find(a, ps, sums, x);
         const int64_t p0 = x - it.at, p1 = min(x_end - it.at, it.len);
         x = it.at + p1;
         const int kv = it.q.kv;
@@ -110,14 +104,18 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         const int my = 32 * wv + lr, rho = it.tile * PM_M + min(my, n_live - 1), tok = rho / G;
         const int row = it.q.start + tok, head = it.g * G + rho - tok * G;
         const int end = a.seen ? min(a.seen[row], kv) : kv - it.q.n + tok + 1;
-        int last = end, first = end;
+        int last = end, first = end;  // the most and the fewest keys that a row of the wave sees
+        if (a.seen) {
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            last = max(last, shfl_xor(last, d));
-            first = min(first, shfl_xor(first, d));
+            for (int d = 1; d < 32; d <<= 1) {
+                last = max(last, shfl_xor(last, d));
+                first = min(first, shfl_xor(first, d));
+            }
+        } else {  // the last row's (in all rows order), the first row's
+            last = __builtin_amdgcn_readlane(end, 31);
         }
-        last = 32 * wv < n_live ? max(__builtin_amdgcn_readfirstlane(last), 0) : 0;
-        first = __builtin_amdgcn_readfirstlane(first);
+        last = 32 * wv < n_live ? max(uniform(last), 0) : 0;
+        first = uniform(first);
         if (lane == 0) last_s[wv] = last;
         if (tid == 0) odd_s = 0;
         __syncthreads();
@@ -125,49 +123,57 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
 #pragma unroll
         for (int w = 0; w < PM_WAVES; w++) tile_last = max(tile_last, last_s[w]);
         tile_last = __builtin_amdgcn_readfirstlane(tile_last);
-        const int64_t blocks = ((int64_t)tile_last + 31) / 32;
-        const int kb0 = (int)(p0 * blocks / it.len), kb1 = (int)(p1 * blocks / it.len);
+        const int blocks = (tile_last + 31) / 32;
+        const int kb0 = part_block(p0, it.len, blocks), kb1 = part_block(p1, it.len, blocks);
         const int my_kb1 = min((last + 31) / 32, kb1);
+        const int slot_id = p0 == 0 && p1 == it.len ? -1 : 2 * worker + (p0 == 0 ? 1 : 0);  // -1: all of it is here
 
         // ---- loads and stores of blocks
         const int* const trow = a.table + (int64_t)it.r * a.max_pages;
-        auto entry = [&](int key) {  // wave-uniform
-            if (key >= kv) return -1;
-            const int e = trow[key >> a.c.shift];
-            return e >= 0 && e < a.c.n_pages ? e : -1;
+        // 64 entries in the lanes, and the next 64: a block's page is a lane read away (an entry
+        // fetched per block was waited for with all loads before it: 2.3 us a block)
+        const int n_tab = (kv + pmask) >> a.c.shift;
+        auto entries = [&](int seg) {
+            const int p = seg * 64 + lane;
+            const int e = p < n_tab ? trow[p] : -1;
+            return e < a.c.n_pages ? e : -1;
+        };
+        int seg = (kb0 * 32) >> (a.c.shift + 6), tab = entries(seg), tab2 = entries(seg + 1);
+        auto page_of = [&](int key) {  // wave-uniform; keys up to 64 pages past those of load_v
+            const int p = (key >> a.c.shift) - seg * 64;
+            return p < 64 ? __builtin_amdgcn_readlane(tab, p) : __builtin_amdgcn_readlane(tab2, p - 64);
         };
         const E* const kg = static_cast<const E*>(a.c.k) + it.g * a.c.head_stride;
         const E* const vg = static_cast<const E*>(a.c.v) + it.g * a.c.head_stride;
         constexpr int KPW = WAVE / KL;  // keys of K per wave
-        const bool k_mine = tid < 32 * KL, v_mine = lane < HD / 2;
-        const int k_key = tid / KL, k_ch = tid % KL;
+        // head_dim 64: every vector is loaded twice (loads under a condition could not be counted, and
+        // every wait would wait for all of them), and stored once
+        const bool k_mine = HD == 128 || tid < 32 * KL, v_mine = HD == 128 || lane < HD / 2;
+        const int k_key = tid / KL % 32, k_ch = tid % KL;
         uint8_t* const k_dst = lds + k_ch * L::CHUNK_K + k_key * 16;
         uint8_t* const v_dst = lds + L::OFF_V + (2 * (wv / 4) + wv % 2) * L::CHUNK_V + lane * 16 + 8 * (wv / 2 % 2);
         v4i_t kx[KP];
         typedef typename std::conditional<KP == 2, uint2, uint32_t>::type vrow_t;
         vrow_t vx[4];
         bool v_there = false;
-        int ek = -1, ev = -1;  // page of the block loaded next
-        auto next_k = [&](int kb) { ek = wv * KPW < 32 ? entry(kb * 32 + wv * KPW) : -1; };
-        auto next_v = [&](int kb) { ev = entry(kb * 32 + 4 * wv); };
         auto load_k = [&](int kb) {
-            const int off = (kb * 32 + k_key) & pmask;
-            const E* const p = kg + max(ek, 0) * a.c.page_stride + off * a.c.token_stride + 8 * k_ch;
-            if (k_mine) {
+            const int off = (kb * 32 + k_key) & pmask, e = page_of(kb * 32 + (wv * KPW) % 32);
+            const E* const p = kg + max(e, 0) * a.c.page_stride + off * a.c.token_stride + 8 * k_ch;
 #pragma unroll
-                for (int u = 0; u < KP; u++) kx[u] = *reinterpret_cast<const v4i_t*>(p + 4 * u);
-            }
-            next_k(kb + 1);
+            for (int u = 0; u < KP; u++) kx[u] = *reinterpret_cast<const v4i_t*>(p + 4 * u);
         };
         auto load_v = [&](int kb) {
-            const int off = (kb * 32 + 4 * wv) & pmask;
-            const E* const p = vg + max(ev, 0) * a.c.page_stride + off * a.c.token_stride + 2 * lane;
-            if (v_mine) {
+            const int off = (kb * 32 + 4 * wv) & pmask, e = page_of(kb * 32 + 4 * wv);
+            const E* const p = vg + max(e, 0) * a.c.page_stride + off * a.c.token_stride + 2 * (lane % (HD / 2));
 #pragma unroll
-                for (int j = 0; j < 4; j++) vx[j] = *reinterpret_cast<const vrow_t*>(p + j * a.c.token_stride);
+            for (int j = 0; j < 4; j++) vx[j] = *reinterpret_cast<const vrow_t*>(p + j * a.c.token_stride);
+            v_there = e >= 0;
+            const int s = ((kb + 1) * 32) >> (a.c.shift + 6);  // the next call's
+            if (s != seg) {
+                seg = s;
+                tab = tab2;
+                tab2 = entries(seg + 1);
             }
-            v_there = ev >= 0;
-            next_v(kb + 1);
         };
         auto put_k = [&](int kb) {
             uint8_t* const d = k_dst + (kb & 1) * L::BUF_K;
@@ -247,8 +253,8 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 b = max(b, dpp_u<0x4E>(g));   // lane l: row l % 4 of its quad
                 b = dpp_umax<0x124>(b);       // rotations by 4 and 8 in 16 lanes
                 b = dpp_umax<0x128>(b);
-                b = max(b, (uint32_t)shfl_xor((int)b, 16));
-                b = max(b, (uint32_t)shfl_xor((int)b, 32));
+                const auto umax = [](uint32_t p, uint32_t q) { return max(p, q); };
+                b = with_half(with_row(b, umax), umax);
                 odd = __any(b >= 0x7f800000u);
                 // (no exponent of its own for a row of zeros: it has to share the sum's range)
                 const int e = b >= 0x7f800000u || b == 0 ? 0 : min(exponent(b, -60), 126);
@@ -299,8 +305,6 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         for (int d = 0; d < ND; d++) o[d] = v16f_t{};
         float m_run = -INFINITY, l_run = 0.0f;
         if (kb0 < kb1) {
-            next_k(kb0);
-            next_v(kb0);
             load_k(kb0);
             load_v(kb0);
         }
@@ -318,11 +322,18 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             for (int c = 0; c < NC; c++)
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    q[c][u] = *reinterpret_cast<const v4f_t*>(qp + 16 * c + 4 * u) * qscale;
+                    q[c][u] = *reinterpret_cast<const v4f_t*>(qp + 16 * c + 4 * u);
+                }
+            __builtin_amdgcn_sched_barrier(0);  // all of them in flight
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    q[c][u] *= qscale;
 #pragma unroll
                     for (int j = 0; j < 4; j++) big = max(big, __float_as_uint(q[c][u][j]) & 0x7fffffffu);
                 }
-            big = max(big, (uint32_t)shfl_xor((int)big, 32));
+            big = with_half(big, [](uint32_t p, uint32_t q) { return max(p, q); });
             const int e = exponent(big, -100);
             const float up = pow2(PM_UP - e);
             unscale = pow2(e - PM_UP);
@@ -338,30 +349,30 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         }
 
         v4i_t pf[2][2];  // the weights' pieces, keys 16 c .. in step c
-        // scores of block kb and its weights' pieces; returns the factor of o
+        // scores of block kb and its weights' pieces
         auto scores = [&](int kb) {
             const uint8_t* const kb_ = lds + (kb & 1) * L::BUF_K + h * L::CHUNK_K + lr * 16;
-            v4i_t kf[2][KP];
+            v4i_t kf[RING][KP];
             auto read = [&](int c) {
 #pragma unroll
                 for (int q = 0; q < KP; q++)
-                    kf[c & 1][q] = *reinterpret_cast<const v4i_t*>(kb_ + q * L::PIECE_K + 2 * c * L::CHUNK_K);
+                    kf[c % RING][q] = *reinterpret_cast<const v4i_t*>(kb_ + q * L::PIECE_K + 2 * c * L::CHUNK_K);
             };
             v16f_t s = v16f_t{};
-            read(0);
+#pragma unroll
+            for (int c = 0; c < RING - 1; c++) read(c);
 #pragma unroll
             for (int c = 0; c < NC; c++) {
-                if (c + 1 < NC) read(c + 1);
+                if (c + RING - 1 < NC) read(c + RING - 1);
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (KP == 2) s = mfma_f16(kf[c & 1][1], qf[c][0], s);
-                s = mfma_f16(kf[c & 1][0], qf[c][1], s);
-                s = mfma_f16(kf[c & 1][0], qf[c][0], s);
+                if constexpr (KP == 2) s = mfma_f16(kf[c % RING][1], qf[c][0], s);
+                s = mfma_f16(kf[c % RING][0], qf[c][1], s);
+                s = mfma_f16(kf[c % RING][0], qf[c][0], s);
                 __builtin_amdgcn_sched_barrier(0);
             }
             const uint64_t there = *reinterpret_cast<const uint64_t*>(there_s[kb % 3]);
             const bool all = there == 0x0101010101010101ull;
             v4f_t inv[4];
-            float big = -INFINITY;
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 v4f_t fac, ex;
@@ -372,31 +383,43 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 }
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
-                    float t = s[4 * u + v] * unscale;
-                    if constexpr (SCALED) t = fmaf(t, fac[v], ex[v]);
-                    if (!all || kb * 32 + 32 > first) {  // wave-uniform
-                        if (!((there >> (8 * (2 * u + h))) & 1) || kb * 32 + 8 * u + 4 * h + v >= end) t = -INFINITY;
-                    }
+                    float t = s[4 * u + v];
+                    if constexpr (SCALED) t = fmaf(t, fac[v] * unscale, ex[v]);
                     s[4 * u + v] = t;
-                    big = fmaxf(big, t);
                 }
             }
-            big = fmaxf(big, shfl_xor(big, 32));
-            const float m = fmaxf(m_run, big);
-            const float ref = m == -INFINITY ? 0.0f : m;
-            const float alpha = __builtin_amdgcn_exp2f(m_run - ref);
-            float sum = 0.0f;
+            if (!all || kb * 32 + 32 > first) {  // wave-uniform
+                asm volatile("");                // a branch, not 80 operations more in every block
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                s[v] = __builtin_amdgcn_exp2f(s[v] - (ref - (float)PM_UP));
-                if constexpr (SCALED)
-                    sum = fmaf(s[v], inv[v / 4][v % 4], sum);
-                else
-                    sum += s[v];
+                for (int v = 0; v < 16; v++)
+                    if (!((there >> (8 * (2 * (v / 4) + h))) & 1) || kb * 32 + 8 * (v / 4) + 4 * h + v % 4 >= end)
+                        s[v] = -INFINITY;
             }
-            sum += shfl_xor(sum, 32);
-            l_run = l_run * alpha + sum;
-            m_run = m;
+            float big = s[0];
+#pragma unroll
+            for (int v = 1; v < 16; v++) big = fmaxf(big, s[v]);
+            if constexpr (!SCALED) big *= unscale;
+            if (__any(big > m_run + PM_LAG)) {
+                big = fmax_half(big);
+                const float m = big > m_run + PM_LAG ? big : m_run;
+                const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - m);
+                m_run = m;
+                l_run *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; d++) o[d] *= alpha;  // all blocks before kb are in it
+            }
+            const float ref = m_run == -INFINITY ? 0.0f : m_run;
+            const float up = ref - (float)PM_WUP;
+#pragma unroll
+            for (int v = 0; v < 16; v++) {  // l_run: of this lane's keys; joined behind the loop
+                if constexpr (SCALED) {
+                    s[v] = __builtin_amdgcn_exp2f(s[v] - up);
+                    l_run = fmaf(s[v], inv[v / 4][v % 4], l_run);
+                } else {
+                    s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], unscale, -up));
+                    l_run += s[v];
+                }
+            }
 #pragma unroll
             for (int c = 0; c < 2; c++)
 #pragma unroll
@@ -406,30 +429,26 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                     pf[c][0][j] = (int)w0;
                     pf[c][1][j] = (int)w1;
                 }
-            return alpha;
         };
-        auto values = [&](int kb, float alpha) {
-            if (__any(alpha != 1.0f)) {
-#pragma unroll
-                for (int d = 0; d < ND; d++) o[d] *= alpha;
-            }
+        auto values = [&](int kb) {
             const uint8_t* const vb = lds + L::OFF_V + (kb % 3) * L::BUF_V + h * L::CHUNK_V + lr * 16;
-            v4i_t vf[2][KP];
+            v4i_t vf[RING][KP];
             auto read = [&](int i) {  // slots 32 (i % ND) .. of step i / ND
 #pragma unroll
                 for (int q = 0; q < KP; q++)
-                    vf[i & 1][q] = *reinterpret_cast<const v4i_t*>(vb + q * L::PIECE_V + 2 * (i / ND) * L::CHUNK_V +
+                    vf[i % RING][q] = *reinterpret_cast<const v4i_t*>(vb + q * L::PIECE_V + 2 * (i / ND) * L::CHUNK_V +
                                                                    512 * (i % ND));
             };
-            read(0);
+#pragma unroll
+            for (int i = 0; i < RING - 1; i++) read(i);
 #pragma unroll
             for (int i = 0; i < 2 * ND; i++) {
-                if (i + 1 < 2 * ND) read(i + 1);
+                if (i + RING - 1 < 2 * ND) read(i + RING - 1);
                 __builtin_amdgcn_sched_barrier(0);
                 v16f_t& t = o[i % ND];
-                if constexpr (KP == 2) t = mfma_f16(vf[i & 1][1], pf[i / ND][0], t);
-                t = mfma_f16(vf[i & 1][0], pf[i / ND][1], t);
-                t = mfma_f16(vf[i & 1][0], pf[i / ND][0], t);
+                if constexpr (KP == 2) t = mfma_f16(vf[i % RING][1], pf[i / ND][0], t);
+                t = mfma_f16(vf[i % RING][0], pf[i / ND][1], t);
+                t = mfma_f16(vf[i % RING][0], pf[i / ND][0], t);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
@@ -438,18 +457,18 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             put_k(kb0);
             load_k(kb0 + 1);
         }
-        float alpha = 1.0f;
         for (int kb = kb0; kb < kb1; kb++) {
             put_v(kb);
             load_v(kb + 1);
             __syncthreads();  // block kb is in LDS; K of block kb - 1 and V of kb - 2 are read out
-            if (lag == 1 && kb > kb0 && kb - 1 < my_kb1) values(kb - 1, alpha);
-            if (kb < my_kb1) alpha = scores(kb);
+            if (lag == 1 && kb > kb0 && kb - 1 < my_kb1) values(kb - 1);
+            if (kb < my_kb1) scores(kb);
             if (kb + 1 < kb1) put_k(kb + 1);
             load_k(kb + 2);
-            if (lag == 0 && kb < my_kb1) values(kb, alpha);
+            if (lag == 0 && kb < my_kb1) values(kb);
         }
-        if (lag == 1 && my_kb1 == kb1 && kb0 < kb1) values(kb1 - 1, alpha);
+        if (lag == 1 && my_kb1 == kb1 && kb0 < kb1) values(kb1 - 1);
+        l_run = fadd_half(l_run);
 
         // l carries the weights' factor too, scaled values have one of their own
         float down = SCALED ? pow2(-PM_VUP) : 1.0f;
@@ -459,18 +478,17 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 a, trow, kv, kb0 * 32, my_kb1 * 32, end, a.q + ((int64_t)row * a.nh + head) * HD, kg, vg,
                 [&](int i) { return 2 * (32 * (i / 16 % (ND / 2)) + 8 * (i % 16 / 4) + 4 * h + i % 4) + i / (8 * ND); },
                 [&](int i, float v) { o[i / 16][i % 16] = v; }, [&](int i) { return o[i / 16][i % 16]; }, m_run, l_run);
-            down = pow2(PM_UP);  // as the other pieces of its item
+            down = pow2(PM_WUP);  // as the other pieces of its item
             l_run *= down;
         }
         if (my < n_live) {
-            const bool whole = p0 == 0 && p1 == it.len;
             float* dst;
             float f = down;
-            if (whole) {
+            if (slot_id < 0) {
                 dst = a.out + ((int64_t)row * a.nh + head) * HD;
                 f = l_run == 0.0f ? 0.0f : down / l_run;
             } else {
-                float* const slot = a.ws + (size_t)(2 * worker + (p0 == 0 ? 1 : 0)) * part_slot_floats(PM_M, HD);
+                float* const slot = a.ws + (size_t)slot_id * part_slot_floats(PM_M, HD);
                 dst = slot + my * HD;
                 if (h == 0) {
                     slot[PM_M * HD + my] = m_run;

@@ -6,8 +6,8 @@
 // equal stretches, one per worker: however ragged the lengths, every worker has the same share.
 // Lengths are in device memory, so every work group sums them itself (part_sums).  An item
 // inside one worker's stretch is written by it; one that is cut leaves a partial result per
-// piece, joined afterwards.  A piece [x0, x1) of nominal length W takes the key blocks
-// floor(x0 B / W) .. floor(x1 B / W) - 1 of the item's real B.
+// piece, joined afterwards.  A piece [x0, x1) of an item of nominal length W takes the
+// key blocks from x0 B / W to x1 B / W (part_block) of the item's real B.
 #pragma once
 #include "hy_device.hpp"
 #include "hy_paged.hpp"
@@ -15,64 +15,15 @@
 namespace hy {
 
 struct PartShape {
-    int M;          // rows of a tile
+    int M, m_shift;            // rows of a tile: 1 << m_shift
+    int G, tau;                // query heads of a kv head; nominal tokens per tile, max(M / G, 1)
     int64_t rows_lo, rows_hi;  // requests with rows_lo < rows <= rows_hi belong to this launch
     int workers;
-    int min_keys;   // of a stretch
+    int min_keys;              // of a stretch
 };
-
-struct PartReq {
-    int start, n, kv;   // first row, rows (tokens), keys
-    int tiles, tau;     // tiles of its rows, nominal tokens per tile
-    int64_t base, head; // keys before its first token; nominal length of a head's tiles
-    // nominal length of tiles 0 .. k - 1
-    __device__ __forceinline__ int64_t upto(int64_t k) const {
-        const int64_t f = min(k, (int64_t)(n / tau));
-        return k * base + (int64_t)tau * (f * (f + 1) / 2) + (k - f) * n;
-    }
-};
-
-__device__ __forceinline__ PartReq part_req(const PagedAttnArgs& a, const PartShape& p, int r) {
-    PartReq q;
-    const int G = a.nh / a.c.nkv;
-    const int s0 = min(max(a.q_start[r], 0), a.n_rows), s1 = min(max(a.q_start[r + 1], 0), a.n_rows);
-    q.start = s0;
-    q.n = max(s1 - s0, 0);
-    q.kv = min(max(a.kv_len[r], 0), a.max_pages << a.c.shift);
-    const int64_t rows = (int64_t)q.n * G;
-    q.tiles = rows > p.rows_lo && rows <= p.rows_hi ? (int)((rows + p.M - 1) / p.M) : 0;
-    q.tau = max(p.M / G, 1);
-    q.base = max(q.kv - q.n, 0);
-    q.head = q.upto(q.tiles);
-    return q;
-}
-
-// Sums of the requests' nominal lengths: thread i of the THREADS holds the sum before its
-// per = ceil(n_req / THREADS) consecutive ones in pre[i], the whole in pre[THREADS].
-template <int THREADS>
-__device__ __forceinline__ int64_t part_sums(const PagedAttnArgs& a, const PartShape& p, int64_t* pre) {
-    const int tid = threadIdx.x, per = (a.n_req + THREADS - 1) / THREADS;
-    int64_t s = 0;
-    for (int r = tid * per; r < min((tid + 1) * per, a.n_req); r++) s += part_req(a, p, r).head * a.c.nkv;
-    int64_t v = s;
-#pragma unroll
-    for (int d = 1; d < WAVE; d <<= 1) {
-        const int64_t o = __shfl_up(v, d, WAVE);
-        if (tid % WAVE >= d) v += o;
-    }
-    __shared__ int64_t wave_sum_s[THREADS / WAVE];
-    if (tid % WAVE == WAVE - 1) wave_sum_s[tid / WAVE] = v;
-    __syncthreads();
-    int64_t before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / WAVE; w++) {
-        if (w < tid / WAVE) before += wave_sum_s[w];
-        total += wave_sum_s[w];
-    }
-    pre[tid] = before + v - s;
-    if (tid == 0) pre[THREADS] = total;
-    __syncthreads();
-    return total;
+inline PartShape part_shape(int m_shift, int G, int64_t rows_lo, int64_t rows_hi, int workers, int min_keys) {
+    const int M = 1 << m_shift;
+    return {M, m_shift, G, M / G > 1 ? M / G : 1, rows_lo, rows_hi, workers, min_keys};
 }
 
 // a value that all lanes share, in scalar registers
@@ -81,8 +32,80 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
     return (int64_t)(((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v));
 }
 
+struct PartReq {
+    int start, n, kv;   // first row, rows (tokens), keys
+    int tiles, full;    // tiles of its rows; those whose nominal tokens do not reach past the last
+    int64_t base, head; // keys before its first token; nominal length of a head's tiles
+    // nominal length of tiles 0 .. k - 1
+    __device__ __forceinline__ int64_t upto(int tau, int64_t k) const {
+        const int64_t f = min(k, (int64_t)full);
+        return k * base + (int64_t)tau * (f * (f + 1) / 2) + (k - f) * n;
+    }
+};
+
+__device__ __forceinline__ PartReq part_req(const PartShape& p, int start, int n, int kv) {
+    PartReq q{start, n, kv, 0, n / p.tau, max(kv - n, 0), 0};
+    const int64_t rows = (int64_t)n * p.G;
+    if (rows > p.rows_lo && rows <= p.rows_hi) q.tiles = (int)((rows + p.M - 1) >> p.m_shift);
+    q.head = q.upto(p.tau, q.tiles);
+    return q;
+}
+
+// What a work group of THREADS keeps of the batch in LDS: thread i has the per = ceil(n_req /
+// THREADS) requests from i * per on; the sum of nominal lengths before them, and, of the
+// first THREADS requests, row start, rows and keys.
+template <int THREADS>
+struct PartSums {
+    int64_t pre[THREADS + 1];
+    int64_t wave[THREADS / WAVE];
+    int start[THREADS], n[THREADS], kv[THREADS];
+};
+
+__device__ __forceinline__ void part_load(const PagedAttnArgs& a, int r, int& start, int& n, int& kv) {
+    const int s0 = a.q_start[r], s1 = a.q_start[r + 1], k = a.kv_len[r];
+    start = min(max(s0, 0), a.n_rows);
+    n = max(min(max(s1, 0), a.n_rows) - start, 0);
+    kv = min(max(k, 0), a.max_pages << a.c.shift);
+}
+
+// fills s; returns the sum of all nominal lengths
+template <int THREADS>
+__device__ __forceinline__ int64_t part_sums(const PagedAttnArgs& a, const PartShape& p, PartSums<THREADS>& s) {
+    const int tid = threadIdx.x, per = (a.n_req + THREADS - 1) / THREADS;
+    int64_t mine = 0;
+    for (int r = tid * per; r < min((tid + 1) * per, a.n_req); r++) {
+        int start, n, kv;
+        part_load(a, r, start, n, kv);
+        mine += part_req(p, start, n, kv).head * a.c.nkv;
+        if (r < THREADS) {
+            s.start[r] = start;
+            s.n[r] = n;
+            s.kv[r] = kv;
+        }
+    }
+    int64_t v = mine;
+#pragma unroll
+    for (int d = 1; d < WAVE; d <<= 1) {
+        const int64_t o = __shfl_up(v, d, WAVE);
+        if (tid % WAVE >= d) v += o;
+    }
+    if (tid % WAVE == WAVE - 1) s.wave[tid / WAVE] = v;
+    __syncthreads();
+    int64_t before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / WAVE; w++) {
+        if (w < tid / WAVE) before += s.wave[w];
+        total += s.wave[w];
+    }
+    s.pre[tid] = before + v - mine;
+    if (tid == 0) s.pre[THREADS] = total;
+    __syncthreads();
+    return uniform(total);
+}
+
 __device__ __forceinline__ int64_t part_stretch(const PartShape& p, int64_t total) {
-    return max((total + p.workers - 1) / p.workers, (int64_t)p.min_keys);
+    // workers is a power of two
+    return max((total + p.workers - 1) >> (31 - __builtin_clz(p.workers)), (int64_t)p.min_keys);
 }
 
 struct PartItem {
@@ -92,43 +115,58 @@ struct PartItem {
     int64_t len;  // its nominal length
 };
 
-// the item at place x (0 <= x < total); uniform over the wave
+// the item at place x (0 <= x < total), the same for the whole wave
 template <int THREADS>
-__device__ __forceinline__ PartItem part_find(const PagedAttnArgs& a, const PartShape& p, const int64_t* pre,
+__device__ __forceinline__ PartItem part_find(const PagedAttnArgs& a, const PartShape& p, const PartSums<THREADS>& s,
                                               int64_t x) {
-    x = uniform(x);
-    int lo = 0, hi = THREADS;  // pre[lo] <= x < pre[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (uniform(pre[mid]) <= x)
-            lo = mid;
-        else
-            hi = mid;
-    }
+    // pre[lo] <= x < pre[lo + 1] (ties: the last): 64 of pre at once, then those between two
+    constexpr int STEP = THREADS / WAVE;
+    const int lane = threadIdx.x % WAVE;
+    const int b = (__builtin_popcountll(__ballot(s.pre[lane * STEP] <= x)) - 1) * STEP;
+    const int lo = b + __builtin_popcountll(__ballot(s.pre[b + lane % STEP] <= x && lane < STEP)) - 1;
     const int per = (a.n_req + THREADS - 1) / THREADS;
     PartItem it;
-    it.r = uniform(lo * per);
-    it.at = uniform(pre[uniform(lo)]);
-    it.q = part_req(a, p, it.r);
-    while (x - it.at >= it.q.head * a.c.nkv) {
+    it.r = lo * per;
+    it.at = uniform(s.pre[lo]);
+    for (;; it.r++) {
+        int start, n, kv;
+        if (it.r < THREADS) {
+            start = s.start[it.r];
+            n = s.n[it.r];
+            kv = s.kv[it.r];
+        } else {
+            part_load(a, it.r, start, n, kv);
+        }
+        it.q = part_req(p, uniform(start), uniform(n), uniform(kv));
+        if (x - it.at < it.q.head * a.c.nkv) break;
         it.at += it.q.head * a.c.nkv;
-        it.r++;
-        it.q = part_req(a, p, it.r);
     }
-    it.g = (int)((x - it.at) / it.q.head);
+    // estimates in f32, then a step either way
+    it.g = uniform((int)((float)(x - it.at) * __builtin_amdgcn_rcpf((float)it.q.head)));
+    while (it.q.head * it.g > x - it.at) it.g--;
+    while (it.q.head * (it.g + 1) <= x - it.at) it.g++;
     it.at += it.q.head * it.g;
-    int t0 = 0, t1 = it.q.tiles;  // upto(t0) <= x - at < upto(t1)
-    while (t1 - t0 > 1) {
-        const int mid = (t0 + t1) / 2;
-        if (it.q.upto(mid) <= x - it.at)
-            t0 = mid;
-        else
-            t1 = mid;
+    const int64_t y = x - it.at;  // upto(tile) <= y < upto(tile + 1)
+    int t = 0;
+    if (it.q.tiles > 1) {
+        // tiles of full size: t base + tau t (t + 1) / 2 = y
+        const float b = (float)it.q.base + 0.5f * p.tau, yf = (float)y;
+        t = min(uniform((int)(2.0f * yf * __builtin_amdgcn_rcpf(b + __builtin_amdgcn_sqrtf(b * b + 2.0f * p.tau * yf)))),
+                it.q.tiles - 1);
+        while (t > 0 && it.q.upto(p.tau, t) > y) t--;
+        while (t + 1 < it.q.tiles && it.q.upto(p.tau, t + 1) <= y) t++;
     }
-    it.tile = t0;
-    it.at += it.q.upto(t0);
-    it.len = it.q.upto(t0 + 1) - it.q.upto(t0);
+    it.tile = t;
+    const int64_t t0 = it.q.upto(p.tau, t);
+    it.at += t0;
+    it.len = it.q.upto(p.tau, t + 1) - t0;
     return it;
+}
+
+// the block where a piece ending at place y of an item of nominal length len ends: rounded, but
+// growing with y and the same for both who share the cut
+__device__ __forceinline__ int part_block(int64_t y, int64_t len, int blocks) {
+    return y >= len ? blocks : min(uniform((int)((float)y * ((float)blocks / (float)len))), blocks);
 }
 
 // Attention of this lane's row over keys k0 .. k1 - 1, key by key in f32: what the kernels do
@@ -176,7 +214,7 @@ __device__ __forceinline__ void slow_rows(const PagedAttnArgs& a, const int* tro
 __host__ __device__ __forceinline__ size_t part_slot_floats(int M, int hd) { return (size_t)M * (hd + 2); }
 
 // requests of many rows: tiles of PM_TILE rows, PM_WORKERS work groups (hy_paged_many.hip)
-constexpr int PM_TILE = 256, PM_WORKERS = 256;
+constexpr int PM_TILE_SHIFT = 8, PM_TILE = 1 << PM_TILE_SHIFT, PM_WORKERS = 256;
 hipError_t launch_paged_many(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s);
 
 }  // namespace hy
