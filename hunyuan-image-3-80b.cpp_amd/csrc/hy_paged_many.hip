@@ -80,7 +80,6 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
     constexpr int RING = KP == 2 ? 2 : 3;  // operands read ahead of the products (registers allowing)
     __shared__ __attribute__((aligned(1024))) uint8_t lds[L::BYTES];
     __shared__ __attribute__((aligned(16))) float k_fac[3][32], v_exp[3][32], v_inv[3][32];
-    __shared__ __attribute__((aligned(8))) uint8_t there_s[3][PM_WAVES];  // 4 keys: 1, or 0 (no page)
     __shared__ int odd_s;  // an infinity or NaN in this piece's V
     __shared__ int last_s[PM_WAVES];
     __shared__ PartSums<PM_THREADS> sums;
@@ -129,19 +128,35 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         const int slot_id = p0 == 0 && p1 == it.len ? -1 : 2 * worker + (p0 == 0 ? 1 : 0);  // -1: all of it is here
 
         // ---- loads and stores of blocks
+        // Block table: where the pages of 64 entries start, in the lanes, and of the next 64: a
+        // block's page is a lane read away (an entry fetched per block was waited for with all
+        // loads before it: 2 us a block).  Addresses are a scalar base and a 32-bit lane offset.
         const int* const trow = a.table + (int64_t)it.r * a.max_pages;
-        // 64 entries in the lanes, and the next 64: a block's page is a lane read away (an entry
-        // fetched per block was waited for with all loads before it: 2.3 us a block)
         const int n_tab = (kv + pmask) >> a.c.shift;
+        bool bad = false;  // an entry that names no page; its keys are read from page 0 and masked
+        auto page_ok = [&](int key) {
+            const int p = key >> a.c.shift;
+            if (p >= n_tab) return false;
+            const int e = trow[p];
+            return e >= 0 && e < a.c.n_pages;
+        };
         auto entries = [&](int seg) {
             const int p = seg * 64 + lane;
-            const int e = p < n_tab ? trow[p] : -1;
-            return e < a.c.n_pages ? e : -1;
+            const int e = p < n_tab ? trow[p] : 0;
+            const bool ok = e >= 0 && e < a.c.n_pages;
+            bad |= (bool)__any(!ok);
+            return ok ? e * a.c.page_stride : 0;
         };
-        int seg = (kb0 * 32) >> (a.c.shift + 6), tab = entries(seg), tab2 = entries(seg + 1);
-        auto page_of = [&](int key) {  // wave-uniform; keys up to 64 pages past those of load_v
+        int seg = (kb0 * 32) >> (a.c.shift + 6);
+        int64_t tab = entries(seg), tab2 = entries(seg + 1);
+        auto lane64 = [](int64_t v, int l) {
+            return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) |
+                             (uint32_t)__builtin_amdgcn_readlane((int)v, l));
+        };
+        auto cell_of = [&](int key) {  // wave-uniform; keys up to 64 pages past those of load_v
             const int p = (key >> a.c.shift) - seg * 64;
-            return p < 64 ? __builtin_amdgcn_readlane(tab, p) : __builtin_amdgcn_readlane(tab2, p - 64);
+            const int64_t page = p < 64 ? lane64(tab, p) : lane64(tab2, p - 64);
+            return page + ((key & ~31) & pmask) * a.c.token_stride;
         };
         const E* const kg = static_cast<const E*>(a.c.k) + it.g * a.c.head_stride;
         const E* const vg = static_cast<const E*>(a.c.v) + it.g * a.c.head_stride;
@@ -150,24 +165,24 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         // every wait would wait for all of them), and stored once
         const bool k_mine = HD == 128 || tid < 32 * KL, v_mine = HD == 128 || lane < HD / 2;
         const int k_key = tid / KL % 32, k_ch = tid % KL;
+        const uint32_t in_page = min(pmask, 31), ts = (uint32_t)a.c.token_stride;
+        const uint32_t k_off = ((k_key & in_page) * ts + 8 * k_ch) * sizeof(E);
+        const uint32_t v_off = (((4 * wv) & in_page) * ts + 2 * (lane % (HD / 2))) * sizeof(E);
         uint8_t* const k_dst = lds + k_ch * L::CHUNK_K + k_key * 16;
         uint8_t* const v_dst = lds + L::OFF_V + (2 * (wv / 4) + wv % 2) * L::CHUNK_V + lane * 16 + 8 * (wv / 2 % 2);
         v4i_t kx[KP];
         typedef typename std::conditional<KP == 2, uint2, uint32_t>::type vrow_t;
         vrow_t vx[4];
-        bool v_there = false;
+        uint32_t v_big = 0;  // the largest magnitude of V's: whether one was infinite or no number
         auto load_k = [&](int kb) {
-            const int off = (kb * 32 + k_key) & pmask, e = page_of(kb * 32 + (wv * KPW) % 32);
-            const E* const p = kg + max(e, 0) * a.c.page_stride + off * a.c.token_stride + 8 * k_ch;
+            const char* const p = reinterpret_cast<const char*>(kg + cell_of(kb * 32 + (wv * KPW) % 32));
 #pragma unroll
-            for (int u = 0; u < KP; u++) kx[u] = *reinterpret_cast<const v4i_t*>(p + 4 * u);
+            for (int u = 0; u < KP; u++) kx[u] = *reinterpret_cast<const v4i_t*>(p + k_off + 16 * u);
         };
         auto load_v = [&](int kb) {
-            const int off = (kb * 32 + 4 * wv) & pmask, e = page_of(kb * 32 + 4 * wv);
-            const E* const p = vg + max(e, 0) * a.c.page_stride + off * a.c.token_stride + 2 * (lane % (HD / 2));
+            const char* const p = reinterpret_cast<const char*>(vg + cell_of(kb * 32 + 4 * wv));
 #pragma unroll
-            for (int j = 0; j < 4; j++) vx[j] = *reinterpret_cast<const vrow_t*>(p + j * a.c.token_stride);
-            v_there = e >= 0;
+            for (int j = 0; j < 4; j++) vx[j] = *reinterpret_cast<const vrow_t*>(p + (v_off + j * ts * sizeof(E)));
             const int s = ((kb + 1) * 32) >> (a.c.shift + 6);  // the next call's
             if (s != seg) {
                 seg = s;
@@ -175,7 +190,8 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 tab2 = entries(seg + 1);
             }
         };
-        auto put_k = [&](int kb) {
+        // block kb, r = kb % 3
+        auto put_k = [&](int kb, int r) {
             uint8_t* const d = k_dst + (kb & 1) * L::BUF_K;
             if constexpr (!SCALED) {
                 if (k_mine) *reinterpret_cast<v4i_t*>(d) = kx[0];
@@ -213,33 +229,35 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 if (k_mine) {
                     *reinterpret_cast<v4i_t*>(d) = hi;
                     if constexpr (KP == 2) *reinterpret_cast<v4i_t*>(d + L::PIECE_K) = lo;
-                    if (k_ch == 0) k_fac[kb % 3][k_key] = pow2(e - PM_UP);
+                    if (k_ch == 0) k_fac[r][k_key] = pow2(e - PM_UP);
                 }
             }
         };
-        auto put_v = [&](int kb) {
-            uint8_t* const d = v_dst + (kb % 3) * L::BUF_V;
+        auto put_v = [&](int kb, int r) {
+            uint8_t* const d = v_dst + r * L::BUF_V;
             const int key0 = kb * 32 + 4 * wv;
-            bool odd = false;
-            float f[4][2];
-            uint32_t w2[4][2], big[4];
+            if (bad || key0 + 4 > kv) {  // wave-uniform: keys that are not there are zeros
+                const bool ok = page_ok(key0);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const bool there = v_there && key0 + j < kv && v_mine;
-                if constexpr (KP == 2) {
-                    w2[j][0] = there ? vx[j].x : 0;
-                    w2[j][1] = there ? vx[j].y : 0;
-                } else {
-                    w2[j][0] = there ? vx[j] : 0;
-                }
-                if constexpr (SCALED) {
-                    if constexpr (KP == 1) {
-                        w2[j][1] = w2[j][0] & 0xffff0000u;
-                        w2[j][0] <<= 16;
+                for (int j = 0; j < 4; j++)
+                    if (!ok || key0 + j >= kv) vx[j] = vrow_t{};
+            }
+            float f[4][2];
+            uint32_t big[4];
+            if constexpr (SCALED) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t w0, w1;
+                    if constexpr (KP == 2) {
+                        w0 = vx[j].x;
+                        w1 = vx[j].y;
+                    } else {
+                        w0 = vx[j] << 16;
+                        w1 = vx[j] & 0xffff0000u;
                     }
-                    big[j] = max(w2[j][0] & 0x7fffffffu, w2[j][1] & 0x7fffffffu);
-                    f[j][0] = __uint_as_float(w2[j][0]);
-                    f[j][1] = __uint_as_float(w2[j][1]);
+                    big[j] = v_mine ? max(w0 & 0x7fffffffu, w1 & 0x7fffffffu) : 0;
+                    f[j][0] = __uint_as_float(w0);
+                    f[j][1] = __uint_as_float(w1);
                 }
             }
             if constexpr (SCALED) {
@@ -255,12 +273,12 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 b = dpp_umax<0x128>(b);
                 const auto umax = [](uint32_t p, uint32_t q) { return max(p, q); };
                 b = with_half(with_row(b, umax), umax);
-                odd = __any(b >= 0x7f800000u);
+                v_big = max(v_big, b);
                 // (no exponent of its own for a row of zeros: it has to share the sum's range)
                 const int e = b >= 0x7f800000u || b == 0 ? 0 : min(exponent(b, -60), 126);
                 if (lane < 4) {
-                    v_exp[kb % 3][4 * wv + lane] = (float)e;
-                    v_inv[kb % 3][4 * wv + lane] = pow2(-e);
+                    v_exp[r][4 * wv + lane] = (float)e;
+                    v_inv[r][4 * wv + lane] = pow2(-e);
                 }
                 const uint32_t up = __float_as_uint(pow2(PM_VUP - e));
                 const float u0 = __uint_as_float(dpp_u<0x00>(up)), u1 = __uint_as_float(dpp_u<0x55>(up));
@@ -281,22 +299,19 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                     }
                 }
             } else {
-                bool o = false;
+                typedef unsigned short v2u16_t __attribute__((ext_vector_type(2)));
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    o |= (w2[j][0] & 0x7C00u) == 0x7C00u || (w2[j][0] & 0x7C000000u) == 0x7C000000u;
-                odd = __any(o);
+                    v_big = __builtin_bit_cast(
+                        uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u16_t, v_big),
+                                                            __builtin_bit_cast(v2u16_t, vx[j] & 0x7fff7fffu)));
                 if (v_mine) {
 #pragma unroll
                     for (int n = 0; n < 2; n++)
                         *reinterpret_cast<uint2*>(d + n * (HD / 2) * 16) =
-                            make_uint2(__builtin_amdgcn_perm(w2[1][0], w2[0][0], n ? 0x07060302u : 0x05040100u),
-                                       __builtin_amdgcn_perm(w2[3][0], w2[2][0], n ? 0x07060302u : 0x05040100u));
+                            make_uint2(__builtin_amdgcn_perm(vx[1], vx[0], n ? 0x07060302u : 0x05040100u),
+                                       __builtin_amdgcn_perm(vx[3], vx[2], n ? 0x07060302u : 0x05040100u));
                 }
-            }
-            if (lane == 0) {
-                there_s[kb % 3][wv] = v_there ? 1 : 0;
-                if (odd) odd_s = 1;
             }
         };
 
@@ -350,7 +365,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
 
         v4i_t pf[2][2];  // the weights' pieces, keys 16 c .. in step c
         // scores of block kb and its weights' pieces
-        auto scores = [&](int kb) {
+        auto scores = [&](int kb, int r) {
             const uint8_t* const kb_ = lds + (kb & 1) * L::BUF_K + h * L::CHUNK_K + lr * 16;
             v4i_t kf[RING][KP];
             auto read = [&](int c) {
@@ -370,16 +385,14 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 s = mfma_f16(kf[c % RING][0], qf[c][0], s);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            const uint64_t there = *reinterpret_cast<const uint64_t*>(there_s[kb % 3]);
-            const bool all = there == 0x0101010101010101ull;
             v4f_t inv[4];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 v4f_t fac, ex;
                 if constexpr (SCALED) {
-                    fac = *reinterpret_cast<const v4f_t*>(&k_fac[kb % 3][8 * u + 4 * h]);
-                    ex = *reinterpret_cast<const v4f_t*>(&v_exp[kb % 3][8 * u + 4 * h]);
-                    inv[u] = *reinterpret_cast<const v4f_t*>(&v_inv[kb % 3][8 * u + 4 * h]);
+                    fac = *reinterpret_cast<const v4f_t*>(&k_fac[r][8 * u + 4 * h]);
+                    ex = *reinterpret_cast<const v4f_t*>(&v_exp[r][8 * u + 4 * h]);
+                    inv[u] = *reinterpret_cast<const v4f_t*>(&v_inv[r][8 * u + 4 * h]);
                 }
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
@@ -388,12 +401,16 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                     s[4 * u + v] = t;
                 }
             }
-            if (!all || kb * 32 + 32 > first) {  // wave-uniform
-                asm volatile("");                // a branch, not 80 operations more in every block
+            if (bad || kb * 32 + 32 > first) {  // wave-uniform
+                asm volatile("");               // a branch, not 80 operations more in every block
 #pragma unroll
-                for (int v = 0; v < 16; v++)
-                    if (!((there >> (8 * (2 * (v / 4) + h))) & 1) || kb * 32 + 8 * (v / 4) + 4 * h + v % 4 >= end)
-                        s[v] = -INFINITY;
+                for (int u = 0; u < 4; u++) {
+                    const int key = kb * 32 + 8 * u + 4 * h;
+                    const bool ok = !bad || page_ok(key);
+#pragma unroll
+                    for (int v = 0; v < 4; v++)
+                        if (!ok || key + v >= end) s[4 * u + v] = -INFINITY;
+                }
             }
             float big = s[0];
 #pragma unroll
@@ -430,8 +447,8 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                     pf[c][1][j] = (int)w1;
                 }
         };
-        auto values = [&](int kb) {
-            const uint8_t* const vb = lds + L::OFF_V + (kb % 3) * L::BUF_V + h * L::CHUNK_V + lr * 16;
+        auto values = [&](int r) {
+            const uint8_t* const vb = lds + L::OFF_V + r * L::BUF_V + h * L::CHUNK_V + lr * 16;
             v4i_t vf[RING][KP];
             auto read = [&](int i) {  // slots 32 (i % ND) .. of step i / ND
 #pragma unroll
@@ -453,25 +470,34 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             }
         };
 
+        int r = kb0 % 3, before = 0;  // kb % 3, (kb - 1) % 3
         if (kb0 < kb1) {
-            put_k(kb0);
+            put_k(kb0, r);
             load_k(kb0 + 1);
         }
         for (int kb = kb0; kb < kb1; kb++) {
-            put_v(kb);
+            const int next = r == 2 ? 0 : r + 1;
+            put_v(kb, r);
             load_v(kb + 1);
             __syncthreads();  // block kb is in LDS; K of block kb - 1 and V of kb - 2 are read out
-            if (lag == 1 && kb > kb0 && kb - 1 < my_kb1) values(kb - 1);
-            if (kb < my_kb1) scores(kb);
-            if (kb + 1 < kb1) put_k(kb + 1);
+            if (lag == 1 && kb > kb0 && kb - 1 < my_kb1) values(before);
+            if (kb < my_kb1) scores(kb, r);
+            if (kb + 1 < kb1) put_k(kb + 1, next);
             load_k(kb + 2);
-            if (lag == 0 && kb < my_kb1) values(kb);
+            if (lag == 0 && kb < my_kb1) values(r);
+            before = r;
+            r = next;
         }
-        if (lag == 1 && my_kb1 == kb1 && kb0 < kb1) values(kb1 - 1);
+        if (lag == 1 && my_kb1 == kb1 && kb0 < kb1) values(before);
         l_run = fadd_half(l_run);
 
         // l carries the weights' factor too, scaled values have one of their own
         float down = SCALED ? pow2(-PM_VUP) : 1.0f;
+        if constexpr (SCALED)
+            v_big = v_big >= 0x7f800000u;
+        else
+            v_big = (v_big & 0xffffu) >= 0x7c00u || v_big >= 0x7c000000u;
+        if (__any(v_big != 0)) odd_s = 1;
         __syncthreads();
         if (odd_s) {  // again, key by key
             slow_rows<E, HD, 2>(

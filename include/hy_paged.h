@@ -47,7 +47,7 @@ typedef struct {
     uint32_t head_dim;     /* 64 or 128 */
     uint64_t page_stride;  /* elements */
     uint64_t head_stride;
-    uint64_t token_stride;
+    uint64_t token_stride; /* 2^24 at most */
     uint64_t layer_stride; /* elements from one layer's pool to the next (calls with a layer) */
 } hy_paged_cache;
 

@@ -71,6 +71,7 @@ BAD_CACHE = [
     (dict(page_stride=1 << 14, head_stride=2048, token_stride=132), INVALID),           # not 16 bytes
     (dict(page_stride=1 << 14, head_stride=2048, token_stride=64), INVALID),            # below head_dim
     (dict(page_stride=1 << 41, head_stride=2048, token_stride=128), INVALID),
+    (dict(page_stride=1 << 14, head_stride=2048, token_stride=(1 << 24) + 128), UNSUPPORTED),
 ]
 
 
