@@ -432,13 +432,13 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && NT == 2 
 // Joins the pieces of every cut item: a team of THREADS / JOBS threads per worker w takes the
 // item that w begins and another ends, HD / 4 threads a row, 4 dims each.  The pieces' statistics
 // and sums are fetched PJ at a time, which is what a join of few rows waits for.
-constexpr int PJ = 8;
 template <int HD, int JOBS>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartShape ps) {
     __shared__ PartSums<256> sums;
     const int64_t total = part_sums(a, ps, sums);
     const int64_t stretch = part_stretch(ps, total);
     constexpr int TEAM = 256 / JOBS;  // a wave at least
+    constexpr int PJ = JOBS > 1 ? 8 : 2;  // items of many rows rarely have more than 2 pieces
     const int w0 = uniform((int)(blockIdx.x * JOBS + threadIdx.x / TEAM)), tt = threadIdx.x % TEAM;
     const int64_t cut = ((int64_t)w0 + 1) * stretch;  // the end of worker w0's stretch
     if (cut >= total) return;
@@ -506,10 +506,12 @@ size_t paged_attn_ws_bytes(int, int, int hd) {
 
 template <int HD>
 static void launch_join(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
-    if (ps.M <= PF_MAX_M)  // few rows: a wave each
-        hipLaunchKernelGGL((paged_join_kernel<HD, 4>), dim3(ps.workers / 4), dim3(256), 0, s, a, ps);
+    // a wave takes 2 rows (head_dim 128) at a time, each round a trip to memory: rows over work
+    // groups until a round or two are left (24 rows of 8 pieces: 24 us in one, 10 us in four)
+    if (ps.M <= PF_MAX_M)
+        hipLaunchKernelGGL((paged_join_kernel<HD, 4>), dim3(ps.workers / 4, ps.M / 8), dim3(256), 0, s, a, ps);
     else
-        hipLaunchKernelGGL((paged_join_kernel<HD, 1>), dim3(ps.workers, 8), dim3(256), 0, s, a, ps);
+        hipLaunchKernelGGL((paged_join_kernel<HD, 1>), dim3(ps.workers, 4), dim3(256), 0, s, a, ps);
 }
 static void launch_join(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
     if (a.c.hd == 128)
