@@ -9,126 +9,177 @@
 namespace hy {
 
 // ---------------------------------------------------------------- tables and slots
-// One work group: every thread owns PL_PER consecutive requests, and the three sums over
-// requests (rows, pages given back, pages taken) are scans over the threads' totals.
-constexpr int PL_THREADS = 1024, PL_PER = PG_MAX_REQ / PL_THREADS;
+// One work group, a request (or PER consecutive ones) per thread: sums over requests (rows, pages
+// given back, pages taken) by scans, then the pages and the rows one per thread, whose request a
+// search in LDS finds.  All of it is latency: 8 requests 6 us, 1024 requests 11.  Rows beyond
+// PL_ROWS go to a second launch over the whole chip (16 000 rows in one work group: 40 us).
+// Sums saturate at PL_CAP, which is past every bound that they are compared with.
+constexpr int PL_CAP = (1 << 30) - 1, PL_ROWS = 4096;
 
+__device__ __forceinline__ int sat_add(int a, int b) { return min(a + b, PL_CAP); }  // of two up to PL_CAP
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int sat_step(int v) {
+    return sat_add(v, __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false));
+}
+// inclusive sum over the lanes of a wave: shifts inside 16-lane rows, then the rows' last lanes
+__device__ __forceinline__ int wave_scan(int v) {
+    v = sat_step<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+    v = sat_step<0x112, 0xF>(v);
+    v = sat_step<0x114, 0xF>(v);
+    v = sat_step<0x118, 0xF>(v);
+    v = sat_step<0x142, 0xA>(v);  // lane 15 to row 1, lane 47 to row 3
+    return sat_step<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
+}
 // exclusive sum over the work group's threads; total: of all of them
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* part, int64_t& total) {
-    const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
-    int64_t s = v;
-#pragma unroll
-    for (int d = 1; d < WAVE; d <<= 1) {
-        const int64_t o = __shfl_up(s, d, WAVE);
-        if (lane >= d) s += o;
-    }
-    __syncthreads();  // part may still be read
+template <int THREADS>
+__device__ __forceinline__ int block_scan(int v, int* part, int& total) {
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+    const int s = wave_scan(v);
     if (lane == WAVE - 1) part[wave] = s;
     __syncthreads();
-    int64_t before = 0;
+    int before = 0;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < PL_THREADS / WAVE; w++) {
-        if (w < wave) before += part[w];
-        total += part[w];
+    for (int w = 0; w < THREADS / WAVE; w++) {
+        const int p = part[w];
+        before = w < wave ? sat_add(before, p) : before;
+        total = sat_add(total, p);
     }
-    return before + s - v;
+    // exclusive: the lane before's inclusive sum (a saturated one cannot be taken back by v)
+    const int prev = __shfl_up(s, 1, WAVE);
+    return sat_add(before, lane ? prev : 0);
 }
 
-__global__ __launch_bounds__(PL_THREADS) void paged_plan_kernel(PagedPlanArgs a) {
-    __shared__ int64_t part[PL_THREADS / WAVE];
-    const int tid = threadIdx.x;
-    const int r0 = tid * PL_PER;
-    const int page = 1 << a.shift;
-    int cached[PL_PER], held[PL_PER], rows[PL_PER], status[PL_PER];
-    int64_t add[PL_PER];
-    int64_t sum = 0, total;
-#pragma unroll
-    for (int i = 0; i < PL_PER; i++) {
-        const int r = r0 + i;
-        const bool live = r < a.n_req;
-        cached[i] = live ? a.cached[r] : 0;
-        add[i] = live ? a.add[r] : 0;
-        held[i] = live ? a.held[r] : 0;
-        rows[i] = add[i] >= 0 && add[i] <= a.n_rows ? (int)add[i] : 0;
-        sum += rows[i];
+// the last r < n with at[r] <= x (at ascending, at[0] <= x)
+__device__ __forceinline__ int find_last(const int* at, int n, int x) {
+    int lo = 0;
+    for (int step = 1 << (31 - __builtin_clz(n)); step; step >>= 1)
+        if (lo + step < n && at[lo + step] <= x) lo += step;
+    return lo;
+}
+
+// position and slot of row t, of a request served with `cached` tokens (negative: not served)
+__device__ __forceinline__ void plan_row(const PagedPlanArgs& a, int t, int r, int start, int cached) {
+    int pos = 0, slot = -1;
+    if (cached >= 0) {
+        pos = cached + t - start;
+        const int p = a.table[(int64_t)r * a.max_pages + (pos >> a.shift)];
+        if (p >= 0 && p < a.n_pages) slot = (p << a.shift) + (pos & ((1 << a.shift) - 1));
     }
-    const int64_t n_free_in = a.n_free[0];
-    // every read of held and n_free is done before any write (they may be the outputs)
-    int64_t at = block_scan(sum, part, total);
-    int want[PL_PER], start[PL_PER];
-    int64_t give_sum = 0, take_sum = 0;
+    a.positions[t] = pos;
+    a.slots[t] = slot;
+}
+
+template <int THREADS, int PER>
+__global__ __launch_bounds__(THREADS) void paged_plan_kernel(PagedPlanArgs a, int rows_here) {
+    constexpr int N = THREADS * PER;
+    __shared__ int part[3][THREADS / WAVE];
+    __shared__ int start_s[N], give_s[N], take_s[N], held_s[N], want_s[N], cached_s[N];
+    __shared__ int used_s;
+    const int tid = threadIdx.x, r0 = tid * PER, page = 1 << a.shift;
+    int cached[PER], held[PER], add[PER], rows[PER], want[PER], status[PER];
+    int sum = 0, total;
 #pragma unroll
-    for (int i = 0; i < PL_PER; i++) {
+    for (int i = 0; i < PER; i++) {
+        const int r = min(r0 + i, a.n_req - 1);
+        cached[i] = a.cached[r];
+        add[i] = a.add[r];
+        held[i] = a.held[r];
+    }
+    const int n_free = min(max(a.n_free[0], 0), a.n_pages);
+    // every read of held and n_free is done before any write (they may be the outputs): the first scan
+    // has a barrier
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        rows[i] = r0 + i < a.n_req && add[i] >= 0 && add[i] <= a.n_rows ? add[i] : 0;
+        sum = sat_add(sum, rows[i]);
+    }
+    if (tid == 0) used_s = 0;
+    int at = block_scan<THREADS>(sum, part[0], total);
+    const int n_used = min(total, a.n_rows);
+    int give_sum = 0, take_sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
         const int r = r0 + i;
         const int64_t len = (int64_t)cached[i] + add[i], w = (len + page - 1) >> a.shift;
-        const bool bad = cached[i] < 0 || add[i] < 0 || at + add[i] > a.n_rows || held[i] < 0 ||
+        const bool bad = cached[i] < 0 || add[i] < 0 || (int64_t)at + add[i] > a.n_rows || held[i] < 0 ||
                          held[i] > a.max_pages;
         status[i] = bad ? 3 : w > a.max_pages ? 2 : 0;
-        want[i] = status[i] ? held[i] : (int)w;  // refused requests keep what they have
-        start[i] = (int)min(at, (int64_t)a.n_rows);
-        if (r < a.n_req) a.q_start[r] = start[i];
-        at += rows[i];
-        give_sum += max(held[i] - want[i], 0);
-        take_sum += max(want[i] - held[i], 0);
+        want[i] = status[i] || r >= a.n_req ? held[i] : (int)w;  // refused requests keep what they have
+        start_s[r] = min(at, a.n_rows);
+        held_s[r] = held[i];
+        want_s[r] = want[i];
+        if (r < a.n_req) a.q_start[r] = min(at, a.n_rows);
+        at = sat_add(at, rows[i]);
+        give_sum = sat_add(give_sum, max(held[i] - want[i], 0));
+        take_sum = sat_add(take_sum, max(want[i] - held[i], 0));
     }
-    if (tid == 0) a.q_start[a.n_req] = (int)min(total, (int64_t)a.n_rows);
-    const int n_rows_used = (int)min(total, (int64_t)a.n_rows);
-    int64_t given, taken;
-    int64_t push = min(max(n_free_in, (int64_t)0), (int64_t)a.n_pages) + block_scan(give_sum, part, given);
-    int64_t upto = block_scan(take_sum, part, taken);
-    const int64_t avail = min(min(max(n_free_in, (int64_t)0), (int64_t)a.n_pages) + given, (int64_t)a.n_pages);
+    if (tid == 0) a.q_start[a.n_req] = n_used;
+    int given, taken;
+    int give = block_scan<THREADS>(give_sum, part[1], given), take = block_scan<THREADS>(take_sum, part[2], taken);
+    const int avail = min(sat_add(n_free, given), a.n_pages);
 #pragma unroll
-    for (int i = 0; i < PL_PER; i++) {
-        int* row = a.table + (int64_t)(r0 + i) * a.max_pages;
-        for (int k = want[i]; k < held[i]; k++, push++)
-            if (push < a.n_pages) a.free_[push] = row[k];
-    }
-    __syncthreads();  // the stack is whole
-    int64_t used = 0;
-#pragma unroll
-    for (int i = 0; i < PL_PER; i++) {
-        const int r = r0 + i;
-        if (r >= a.n_req) continue;
-        const int need = max(want[i] - held[i], 0);
-        upto += need;
-        if (need && upto > avail) {
+    for (int i = 0; i < PER; i++) {
+        const int r = r0 + i, need = max(want[i] - held[i], 0);
+        give_s[r] = give;
+        take_s[r] = take;
+        give = sat_add(give, max(held[i] - want[i], 0));
+        take = sat_add(take, need);
+        if (need && take > avail) {
             status[i] = 1;
-            want[i] = held[i];
-        } else {
-            used += need;
-            int* row = a.table + (int64_t)r * a.max_pages;
-            for (int k = 0; k < need; k++) row[held[i] + k] = a.free_[avail - 1 - (upto - need) - k];
+        } else if (need) {
+            atomicMax(&used_s, take);  // those that are served come before those that are not
         }
-        a.status[r] = status[i];
-        a.held_out[r] = status[i] == 0 ? want[i] : held[i];
-        a.kv_len[r] = status[i] == 0 ? cached[i] + (int)add[i] : 0;
-    }
-    (void)block_scan(used, part, total);  // and a barrier: the tables are whole
-    if (tid == 0) a.n_free_out[0] = (int)(avail - total);
-#pragma unroll
-    for (int i = 0; i < PL_PER; i++) {
-        const int r = r0 + i;
-        const int* row = a.table + (int64_t)r * a.max_pages;
-        for (int k = 0; k < rows[i] && start[i] + k < n_rows_used; k++) {
-            int pos = 0, slot = -1;
-            if (status[i] == 0) {
-                pos = cached[i] + k;
-                const int p = row[pos >> a.shift];
-                if (p >= 0 && p < a.n_pages) slot = (p << a.shift) + (pos & (page - 1));
-            }
-            a.positions[start[i] + k] = pos;
-            a.slots[start[i] + k] = slot;
+        cached_s[r] = status[i] == 0 ? cached[i] : -1;
+        if (r < a.n_req) {
+            a.status[r] = status[i];
+            a.held_out[r] = status[i] == 0 ? want[i] : held[i];
+            a.kv_len[r] = status[i] == 0 ? cached[i] + add[i] : 0;
         }
     }
-    for (int t = n_rows_used + tid; t < a.n_rows; t += PL_THREADS) {
-        a.positions[t] = 0;
-        a.slots[t] = -1;
+    __syncthreads();
+    const int used = used_s;
+    if (tid == 0) a.n_free_out[0] = avail - used;
+    if (given) {  // the same for all
+        for (int e = tid; e < min(given, a.n_pages - n_free); e += THREADS) {
+            const int r = find_last(give_s, a.n_req, e);
+            a.free_[n_free + e] = a.table[(int64_t)r * a.max_pages + want_s[r] + e - give_s[r]];
+        }
+        __syncthreads();  // the stack is whole
     }
+    for (int e = tid; e < used; e += THREADS) {
+        const int r = find_last(take_s, a.n_req, e);
+        a.table[(int64_t)r * a.max_pages + held_s[r] + e - take_s[r]] = a.free_[avail - 1 - e];
+    }
+    if (!rows_here) return;
+    __syncthreads();  // the tables are whole
+    for (int t = tid; t < a.n_rows; t += THREADS) {
+        const int r = t < n_used ? find_last(start_s, a.n_req, t) : 0;
+        plan_row(a, t, r, start_s[r], t < n_used ? cached_s[r] : -1);
+    }
+}
+
+// the rows' positions and slots, from what the first launch wrote
+__global__ __launch_bounds__(256) void paged_plan_rows_kernel(PagedPlanArgs a) {
+    __shared__ int start_s[PG_MAX_REQ];
+    for (int r = threadIdx.x; r < a.n_req; r += 256) start_s[r] = a.q_start[r];
+    const int n_used = a.q_start[a.n_req], t = blockIdx.x * 256 + threadIdx.x;
+    __syncthreads();
+    if (t >= a.n_rows) return;
+    const int r = t < n_used ? find_last(start_s, a.n_req, t) : 0;
+    plan_row(a, t, r, start_s[r], t < n_used && a.status[r] == 0 ? a.cached[r] : -1);
 }
 
 hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(PL_THREADS), 0, s, a);
+    const int here = a.n_rows <= PL_ROWS;
+    if (a.n_req <= 256 && a.n_rows <= 1024)
+        hipLaunchKernelGGL((paged_plan_kernel<256, 1>), dim3(1), dim3(256), 0, s, a, here);
+    else if (a.n_req <= 1024)
+        hipLaunchKernelGGL((paged_plan_kernel<1024, 1>), dim3(1), dim3(1024), 0, s, a, here);
+    else
+        hipLaunchKernelGGL((paged_plan_kernel<1024, PG_MAX_REQ / 1024>), dim3(1), dim3(1024), 0, s, a, here);
+    if (!here) hipLaunchKernelGGL(paged_plan_rows_kernel, dim3((a.n_rows + 255) / 256), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

@@ -17,26 +17,29 @@
 
 namespace hy {
 
-// 2^y to 1e-14: whole part by ldexp, the rest |r| <= 1/2 by the series of e^(r ln 2) to
-// degree 11 (remainder (0.347)^12 / 12! = 6e-15).  2^-inf = 0,
-// and so is the masked logit of an infinite temperature, -inf times 0.
+// 2^y: whole part n by ldexp, the rest |r| <= 1/2 by the series of e^(r ln 2) to degree 11, its
+// powers of ln 2 in the coefficients (remainder (0.347)^12 / 12! = 6e-15).  y below -1100 and
+// no number (the masked logit of an infinite temperature, -inf times 0): 0.
 __device__ __forceinline__ double exp2_f64(double y) {
-    if (!(y >= -1100.0)) return 0.0;
-    const double n = rint(y), r = (y - n) * 0.6931471805599453;
-    double p = 1.0 / 39916800;
-    p = fma(p, r, 1.0 / 3628800);
-    p = fma(p, r, 1.0 / 362880);
-    p = fma(p, r, 1.0 / 40320);
-    p = fma(p, r, 1.0 / 5040);
-    p = fma(p, r, 1.0 / 720);
-    p = fma(p, r, 1.0 / 120);
-    p = fma(p, r, 1.0 / 24);
-    p = fma(p, r, 1.0 / 6);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
+    y = fmax(y, -1100.0);
+    const double n = rint(y), r = y - n;
+    constexpr double L = 0.6931471805599453094, L2 = L * L, L4 = L2 * L2, L8 = L4 * L4;
+    double p = L8 * L2 * L / 39916800;
+    p = fma(p, r, L8 * L2 / 3628800);
+    p = fma(p, r, L8 * L / 362880);
+    p = fma(p, r, L8 / 40320);
+    p = fma(p, r, L4 * L2 * L / 5040);
+    p = fma(p, r, L4 * L2 / 720);
+    p = fma(p, r, L4 * L / 120);
+    p = fma(p, r, L4 / 24);
+    p = fma(p, r, L2 * L / 6);
+    p = fma(p, r, L2 / 2);
+    p = fma(p, r, L);
     p = fma(p, r, 1.0);
     return __builtin_ldexp(p, (int)n);
 }
+// weight of a logit, 2^((l - m) c): the difference first, it is exact for logits near m of any size
+__device__ __forceinline__ double weight(float l, double c, double m) { return exp2_f64(((double)l - m) * c); }
 
 constexpr int VF_THREADS = 256, VF_VEC = 8, VF_SLICE = VF_THREADS * VF_VEC * 4;
 
@@ -133,21 +136,22 @@ __global__ __launch_bounds__(VF_THREADS) void verify_rows_kernel(VerifyArgs a, V
             m = fmaxf(m, x[j][n]);
         }
     m = block_fold(m, pf, [](float p, float q) { return fmaxf(p, q); });
-    int arg = V;
-#pragma unroll
-    for (int j = VF_VEC - 1; j >= 0; j--)
-#pragma unroll
-        for (int n = 3; n >= 0; n--)
-            if (x[j][n] == m) arg = min(arg, s * VF_SLICE + 4 * ((int)threadIdx.x + VF_THREADS * j) + n);
-    arg = block_fold(arg, pi, [](int p, int q) { return min(p, q); });
     bad = __syncthreads_or(bad);
+    int arg = V;
     double z = 0.0;
-    if (temp > 0.0f && m > -INFINITY && !bad) {  // the same for the work group
+    if (!(temp > 0.0f)) {  // the same for the work group, as all conditions here
+#pragma unroll
+        for (int j = VF_VEC - 1; j >= 0; j--)
+#pragma unroll
+            for (int n = 3; n >= 0; n--)
+                if (x[j][n] == m) arg = s * VF_SLICE + 4 * ((int)threadIdx.x + VF_THREADS * j) + n;
+        arg = block_fold(arg, pi, [](int p, int q) { return min(p, q); });
+    } else if (m > -INFINITY && !bad) {
         const double c = 1.4426950408889634 / (double)temp;
 #pragma unroll
         for (int j = 0; j < VF_VEC; j++)
 #pragma unroll
-            for (int n = 0; n < 4; n++) z += exp2_f64(((double)x[j][n] - (double)m) * c);
+            for (int n = 0; n < 4; n++) z += weight(x[j][n], c, (double)m);
         z = block_fold(z, pd, [](double p, double q) { return p + q; });
     }
     if (threadIdx.x == 0) out[(int64_t)row * S + s] = {z, m, arg, bad, 0};
@@ -204,7 +208,7 @@ __global__ __launch_bounds__(VF_THREADS) void verify_rest_kernel(VerifyArgs a, c
             bool take = false;
             if (!last && x >= 0 && x < V) {
                 const double q = a.draft ? (double)a.draft[(int64_t)row * V + x] : 1.0;
-                const double w = exp2_f64(((double)a.logits[(int64_t)row * V + x] - (double)mm) * c);
+                const double w = weight(a.logits[(int64_t)row * V + x], c, (double)mm);
                 take = (double)a.u_accept[row] * q < w / z;
             }
             end = !take;
@@ -233,12 +237,13 @@ __global__ __launch_bounds__(VF_THREADS) void verify_rest_kernel(VerifyArgs a, c
     f4_any_t x[VF_VEC], q[VF_VEC];
     load_slice(l, V, s, -INFINITY, x);
     if (a.draft && refused) load_slice(a.draft + (int64_t)p.row * V, V, s, 0.0f, q);
+    const double m = (double)p.m, inv = 1.0 / p.z;
     double left = 0.0, all = 0.0;
 #pragma unroll
     for (int j = 0; j < VF_VEC; j++)
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const double v = exp2_f64(((double)x[j][k] - (double)p.m) * c) / p.z;
+            const double v = weight(x[j][k], c, m) * inv;
             all += v;
             if (refused) {
                 const int i = s * VF_SLICE + 4 * ((int)threadIdx.x + VF_THREADS * j) + k;
@@ -255,16 +260,17 @@ __global__ __launch_bounds__(VF_THREADS) void verify_rest_kernel(VerifyArgs a, c
 
 __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, const VfRest* __restrict__ rest,
                                                                 const VfPick* __restrict__ pick) {
-    constexpr int WAVES = VF_THREADS / WAVE, PER = VF_SLICE / VF_THREADS;
-    __shared__ double pd[WAVES];
+    constexpr int WAVES = VF_THREADS / WAVE;
+    __shared__ double runs[VF_VEC * WAVES];
+    static_assert(VF_VEC * WAVES <= WAVE, "a run per lane");
     __shared__ int pi[WAVES];
     const int V = a.vocab, S = vf_slices(V), r = blockIdx.x, tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
     const VfPick p = pick[r];
-    const int lo = max(a.q_start[r], 0);
+    const int lo = max(a.q_start[r], 0), hi = min(a.q_start[r + 1], a.n_rows);
+    const float temp = a.temp ? a.temp[r] : 1.0f, u_sample = a.u_sample[r];
     int tok = p.tok;
     if (p.row >= 0) {
-        const bool refused = p.row < min(a.q_start[r + 1], a.n_rows) - 1;
-        const float temp = a.temp ? a.temp[r] : 1.0f;
+        const bool refused = p.row < hi - 1;
         const double c = 1.4426950408889634 / (double)temp;
         const VfRest* const rs = rest + (int64_t)r * S;
         // sums over the slices, in order; every wave for itself
@@ -276,7 +282,7 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, c
         left = wave_fold(left, [](double u, double v) { return u + v; });
         all = wave_fold(all, [](double u, double v) { return u + v; });
         const bool whole = !(left > 0.0);  // nothing is left: from p
-        const double thr = (double)a.u_sample[r] * (whole ? all : left);
+        const double thr = (double)u_sample * (whole ? all : left);
         double before = 0.0;
         int s = -1, s_any = -1;  // the first slice whose running sum exceeds thr; the last one with any weight
         double s_before = 0.0, any_before = 0.0;
@@ -307,50 +313,84 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, c
             s = s_any;
             s_before = any_before;
         }
-        // in the slice, thread i has PER consecutive tokens
-        const float* const l = a.logits + (int64_t)p.row * V;
+        // in the slice: VF_VEC x WAVES runs of 4 x 64 tokens (load_slice's order), their sums, then
+        // the lanes of the run that u falls into
         const float* const dr = a.draft && refused && !whole ? a.draft + (int64_t)p.row * V : nullptr;
-        const int i0 = s * VF_SLICE + tid * PER;
-        float x[PER], q[PER];
+        f4_any_t x[VF_VEC], q[VF_VEC];
+        load_slice(a.logits + (int64_t)p.row * V, V, s, -INFINITY, x);
+        if (dr) load_slice(dr, V, s, 0.0f, q);
+        const double m = (double)p.m, inv = 1.0 / p.z;
+        double sum[VF_VEC];
+        auto left_of = [&](int j, int k) {
+            const double v = weight(x[j][k], c, m) * inv;
+            if (dr) return v > (double)q[j][k] ? v - (double)q[j][k] : 0.0;
+            return refused && !whole && s * VF_SLICE + 4 * (tid + VF_THREADS * j) + k == p.x ? 0.0 : v;
+        };
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            x[k] = i0 + k < V ? l[i0 + k] : -INFINITY;
-            q[k] = dr && i0 + k < V ? dr[i0 + k] : 0.0f;
+        for (int j = 0; j < VF_VEC; j++) {
+            double u = 0.0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) u += left_of(j, k);
+            sum[j] = u;
         }
-        double v[PER], sum = 0.0;
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            v[k] = exp2_f64(((double)x[k] - (double)p.m) * c) / p.z;
-            if (dr)
-                v[k] = v[k] > (double)q[k] ? v[k] - (double)q[k] : 0.0;
-            else if (refused && !whole && i0 + k == p.x)
-                v[k] = 0.0;
-            sum += v[k];
+        for (int j = 0; j < VF_VEC; j++) {
+            const double u = wave_fold(sum[j], [](double u, double v) { return u + v; });
+            if (lane == 0) runs[j * WAVES + wave] = u;
         }
-        double run = sum;
+        __syncthreads();
+        const double mine_run = lane < VF_VEC * WAVES ? runs[lane] : 0.0;  // a run per lane
+        double run = mine_run;
 #pragma unroll
-        for (int d = 1; d < WAVE; d <<= 1) {
+        for (int d = 1; d < VF_VEC * WAVES; d <<= 1) {
             const double o = __shfl_up(run, d, WAVE);
             if (lane >= d) run += o;
         }
-        if (lane == WAVE - 1) pd[wave] = run;
-        __syncthreads();
-        double at = s_before + run - sum;
+        const unsigned long long over = __ballot(mine_run > 0.0 && s_before + run > thr), some = __ballot(mine_run > 0.0);
+        // no run: the sums of the slice and of its runs may round apart
+        const int at = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
+        const double at_before = s_before + __shfl(run - mine_run, max(at, 0), WAVE);
+        tok = -1;
+        if (at >= 0 && at % WAVES == wave) {
+            const int j = at / WAVES;
+            f4_any_t xj = x[0], qj = q[0];
+            double mine = sum[0];
 #pragma unroll
-        for (int w = 0; w < WAVES; w++)
-            if (w < wave) at += pd[w];
-        int found = V, any = -1;
+            for (int k = 1; k < VF_VEC; k++)
+                if (k == j) {
+                    xj = x[k];
+                    qj = q[k];
+                    mine = sum[k];
+                }
+            x[0] = xj;
+            q[0] = qj;
+            double upto = mine;
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            at += v[k];
-            if (v[k] > 0.0) {
-                any = i0 + k;
-                if (found == V && at > thr) found = i0 + k;
+            for (int d = 1; d < WAVE; d <<= 1) {
+                const double o = __shfl_up(upto, d, WAVE);
+                if (lane >= d) upto += o;
             }
+            double here = at_before + upto - mine;
+            const int i0 = s * VF_SLICE + 4 * (tid + VF_THREADS * j);
+            int found = V, any = -1;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                double v = weight(x[0][k], c, m) * inv;
+                if (dr)
+                    v = v > (double)q[0][k] ? v - (double)q[0][k] : 0.0;
+                else if (refused && !whole && i0 + k == p.x)
+                    v = 0.0;
+                here += v;
+                if (v > 0.0) {
+                    any = i0 + k;
+                    if (found == V && here > thr) found = i0 + k;
+                }
+            }
+            found = wave_fold(found, [](int u, int v) { return min(u, v); });
+            any = wave_fold(any, [](int u, int v) { return max(u, v); });
+            tok = found < V ? found : any;
         }
-        found = block_fold(found, pi, [](int u, int w) { return min(u, w); });
-        any = block_fold(any, pi, [](int u, int w) { return max(u, w); });
-        tok = found < V ? found : any;  // the sums of the slice and of its tokens may round apart
+        tok = block_fold(tok, pi, [](int u, int v) { return max(u, v); });
     }
     int* const out = a.tokens + (int64_t)r * a.max_new;
     for (int i = tid; i < a.max_new; i += VF_THREADS) out[i] = i < p.accepted ? a.ids[lo + i + 1] : i == p.accepted ? tok : -1;
