@@ -240,7 +240,7 @@ int check_paged(const hy_attn_ctx* c, uint32_t layer, const hy_paged_cache* cach
     st->cache.k = static_cast<uint8_t*>(st->cache.k) + layer * cache->layer_stride * el;
     st->cache.v = static_cast<uint8_t*>(st->cache.v) + layer * cache->layer_stride * el;
     st->batch = b;
-    const size_t need = hy::paged_attn_ws_bytes(c->nh, c->nkv, c->hd);
+    const size_t need = hy::paged_batch_ws(b, (uint32_t)c->nh, st->cache);
     if (!st->ws || st->ws_bytes < need)
         return fail(HY_ERR_INVALID, "workspace of %zu bytes at %p: %zu bytes needed", st->ws_bytes, st->ws, need);
     return HY_OK;

@@ -69,7 +69,7 @@ struct PagedAttnArgs {
     float* ws;
 };
 hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s);
-size_t paged_attn_ws_bytes(int nh, int nkv, int hd);
+size_t paged_attn_ws_bytes(int n_req, int max_new, int G, int hd);
 
 struct VerifyArgs {
     const float* logits;
@@ -93,6 +93,7 @@ int paged_batch_check(const hy_paged_batch* b, const PagedView& c, bool writes);
 int paged_append(const float* qkv, uint32_t n_rows, uint32_t n_heads, const PagedView& c, const int32_t* positions,
                  const int32_t* slots, float theta, const float* cos_t, const float* sin_t, uint32_t n_pos,
                  const float* q_norm, const float* k_norm, float eps, float* q, hipStream_t s);
+size_t paged_batch_ws(const hy_paged_batch* b, uint32_t n_heads, const PagedView& c);
 int paged_attention(const float* q, uint32_t n_heads, const PagedView& c, const hy_paged_batch* b, float scale,
                     float* out, void* ws, size_t ws_bytes, hipStream_t s);
 

@@ -398,7 +398,7 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && NT == 2 
                     [&](int n, float v) { o[c][n / 4][n % 4] = v; }, [&](int n) { return o[c][n / 4][n % 4]; }, m_run[c],
                     l_run[c]);
         }
-        float* const slot = a.ws + (size_t)max(slot_id, 0) * part_slot_floats(ps.M, HD);
+        float* const slot = a.ws + ps.ws + (size_t)max(slot_id, 0) * part_slot_floats(ps.M, HD);
 #pragma unroll
         for (int c = 0; c < NT; c++) {
             if (16 * c + i >= n_live) continue;
@@ -433,13 +433,13 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && NT == 2 
 // item that w begins and another ends, HD / 4 threads a row, 4 dims each.  The pieces' statistics
 // and sums are fetched PJ at a time, which is what a join of few rows waits for.
 template <int HD, int JOBS>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartShape ps) {
-    __shared__ PartSums<256> sums;
+__device__ __forceinline__ void join(const PagedAttnArgs& a, const PartShape& ps, PartSums<256>& sums, int group,
+                                     int split, int splits) {
     const int64_t total = part_sums(a, ps, sums);
     const int64_t stretch = part_stretch(ps, total);
     constexpr int TEAM = 256 / JOBS;  // a wave at least
     constexpr int PJ = JOBS > 1 ? 8 : 2;  // items of many rows rarely have more than 2 pieces
-    const int w0 = uniform((int)(blockIdx.x * JOBS + threadIdx.x / TEAM)), tt = threadIdx.x % TEAM;
+    const int w0 = uniform(group * JOBS + (int)threadIdx.x / TEAM), tt = threadIdx.x % TEAM;
     const int64_t cut = ((int64_t)w0 + 1) * stretch;  // the end of worker w0's stretch
     if (cut >= total) return;
     const PartItem it = part_find(a, ps, sums, cut);
@@ -450,11 +450,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartSh
     while ((int64_t)(n_piece - 1) * stretch < past) n_piece++;
     const int n_live = min(it.q.n * ps.G - it.tile * ps.M, ps.M);
     const size_t sf = part_slot_floats(ps.M, HD);
-    const float* const first = a.ws + (size_t)(2 * w0 + 1) * sf;
-    const float* const rest = a.ws + (size_t)(2 * w0) * sf;  // piece k > 0: + 2 k slots
+    const float* const first = a.ws + ps.ws + (size_t)(2 * w0 + 1) * sf;
+    const float* const rest = a.ws + ps.ws + (size_t)(2 * w0) * sf;  // piece k > 0: + 2 k slots
     constexpr int TR = HD / 4, RPB = TEAM / TR;  // threads per row, rows at a time
     const int d = tt % TR * 4;
-    for (int i = blockIdx.y * RPB + tt / TR; i < n_live; i += RPB * gridDim.y) {
+    for (int i = split * RPB + tt / TR; i < n_live; i += RPB * splits) {
         float m = -INFINITY, l = 0.0f;
         v4f_t o = v4f_t{};
         for (int k0 = 0; k0 < n_piece; k0 += PJ) {
@@ -495,29 +495,43 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartSh
 constexpr int PF_GROUPS = 512;  // two per CU
 constexpr int PF_WORKERS = PF_GROUPS * PF_WAVES;
 constexpr int PF_MAX_M = 32;
-constexpr int PF_MIN_KEYS = 64, PM_MIN_KEYS = 128;
+constexpr int PF_MAX_ROWS = PF_MAX_M;  // rows of a request up to which the stream takes it
+// Rows over work groups until a round or two are left, as each round is a trip to memory (24 rows
+// of 8 pieces: 24 us in one work group, 15 in four).
+constexpr int PJ_FEW_ROWS = 8, PJ_MANY_SPLITS = 4;
 
-// rows of a request up to which the stream takes it
-constexpr int PF_MAX_ROWS = PF_MAX_M;
-
-size_t paged_attn_ws_bytes(int, int, int hd) {
-    return max(2 * PF_WORKERS * part_slot_floats(PF_MAX_M, hd), 2 * PM_WORKERS * part_slot_floats(PM_TILE, hd)) * 4;
-}
-
+// first few.workers / 4 x few.M / 8 work groups for the stream's items, then many.workers x
+// PJ_MANY_SPLITS for the others'
 template <int HD>
-static void launch_join(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
-    // a wave takes 2 rows (head_dim 128) at a time, each round a trip to memory: rows over work
-    // groups until a round or two are left (24 rows of 8 pieces: 24 us in one, 10 us in four)
-    if (ps.M <= PF_MAX_M)
-        hipLaunchKernelGGL((paged_join_kernel<HD, 4>), dim3(ps.workers / 4, ps.M / 8), dim3(256), 0, s, a, ps);
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartShape few, PartShape many) {
+    __shared__ PartSums<256> sums;
+    const int splits = few.M / PJ_FEW_ROWS, few_groups = few.workers / 4 * splits, b = (int)blockIdx.x - few_groups;
+    if (b < 0)
+        join<HD, 4>(a, few, sums, (int)blockIdx.x / splits, (int)blockIdx.x % splits, splits);
     else
-        hipLaunchKernelGGL((paged_join_kernel<HD, 1>), dim3(ps.workers, 4), dim3(256), 0, s, a, ps);
+        join<HD, 1>(a, many, sums, b / PJ_MANY_SPLITS, b % PJ_MANY_SPLITS, PJ_MANY_SPLITS);
 }
-static void launch_join(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
-    if (a.c.hd == 128)
-        launch_join<128>(a, ps, s);
-    else
-        launch_join<64>(a, ps, s);
+
+// which launches a batch takes: workers 0: not that one
+struct PaPlan {
+    PartShape few, many;
+};
+static PaPlan pa_plan(int n_req, int max_new, int G, int hd) {
+    const int64_t rows = (int64_t)max_new * G;  // of one request, at most
+    constexpr int64_t ALL = (int64_t)1 << 62;
+    const bool many = rows > PF_MAX_ROWS, few = !many || n_req > 1;
+    PaPlan p;
+    // Starting an item is worth 16 keys of a full stream, 256 of a many-row tile (20 000 of its 3500
+    // to 6500 cycles per 32 keys); a stretch is 64 keys at least, 128.
+    p.few = part_shape(rows > 16 ? 5 : 4, G, 0, many ? PF_MAX_ROWS : ALL, few ? PF_WORKERS : 0, 16, 64, 0);
+    const size_t few_ws = few ? 2 * (size_t)PF_WORKERS * part_slot_floats(p.few.M, hd) : 0;
+    p.many = part_shape(PM_TILE_SHIFT, G, few ? PF_MAX_ROWS : 0, ALL, many ? PM_WORKERS : 0, 256, 128, few_ws);
+    return p;
+}
+
+size_t paged_attn_ws_bytes(int n_req, int max_new, int G, int hd) {
+    const PaPlan p = pa_plan(n_req, max_new, G, hd);
+    return 4 * (p.many.ws + 2 * (size_t)p.many.workers * part_slot_floats(PM_TILE, hd));
 }
 
 template <class E, int HD>
@@ -529,26 +543,22 @@ static void launch_few(const PagedAttnArgs& a, const PartShape& ps, hipStream_t 
 }
 
 hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s) {
-    const int G = a.nh / a.c.nkv;
-    const int64_t rows = (int64_t)max_new * G;  // of one request, at most
-    constexpr int64_t ALL = (int64_t)1 << 62;
-    const bool many = rows > PF_MAX_ROWS;
-    if (!many || a.n_req > 1) {
-        const PartShape ps = part_shape(rows > 16 ? 5 : 4, G, 0, many ? PF_MAX_ROWS : ALL, PF_WORKERS, PF_MIN_KEYS);
-        const bool big = a.c.hd == 128;
+    const PaPlan p = pa_plan(a.n_req, max_new, a.nh / a.c.nkv, a.c.hd);
+    const bool big = a.c.hd == 128;
+    if (p.few.workers) {
         if (a.c.type == HY_TYPE_F32)
-            big ? launch_few<float, 128>(a, ps, s) : launch_few<float, 64>(a, ps, s);
+            big ? launch_few<float, 128>(a, p.few, s) : launch_few<float, 64>(a, p.few, s);
         else if (a.c.type == HY_TYPE_F16)
-            big ? launch_few<_Float16, 128>(a, ps, s) : launch_few<_Float16, 64>(a, ps, s);
+            big ? launch_few<_Float16, 128>(a, p.few, s) : launch_few<_Float16, 64>(a, p.few, s);
         else
-            big ? launch_few<__bf16, 128>(a, ps, s) : launch_few<__bf16, 64>(a, ps, s);
-        launch_join(a, ps, s);
+            big ? launch_few<__bf16, 128>(a, p.few, s) : launch_few<__bf16, 64>(a, p.few, s);
     }
-    if (many) {
-        const PartShape ps = part_shape(PM_TILE_SHIFT, G, a.n_req > 1 ? PF_MAX_ROWS : 0, ALL, PM_WORKERS, PM_MIN_KEYS);
-        (void)launch_paged_many(a, ps, s);
-        launch_join(a, ps, s);
-    }
+    if (p.many.workers) (void)launch_paged_many(a, p.many, s);
+    const dim3 grid(p.few.workers / 4 * (p.few.M / PJ_FEW_ROWS) + p.many.workers * PJ_MANY_SPLITS);
+    if (big)
+        hipLaunchKernelGGL(paged_join_kernel<128>, grid, dim3(256), 0, s, a, p.few, p.many);
+    else
+        hipLaunchKernelGGL(paged_join_kernel<64>, grid, dim3(256), 0, s, a, p.few, p.many);
     return hipGetLastError();
 }
 

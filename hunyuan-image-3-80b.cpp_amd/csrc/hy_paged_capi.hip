@@ -126,12 +126,17 @@ int paged_append(const float* qkv, uint32_t n_rows, uint32_t n_heads, const Page
     return HY_OK;
 }
 
+size_t paged_batch_ws(const hy_paged_batch* b, uint32_t n_heads, const PagedView& c) {
+    return paged_attn_ws_bytes((int)b->n_req, (int)(b->max_new < b->n_rows ? b->max_new : b->n_rows),
+                               (int)n_heads / c.nkv, c.hd);
+}
+
 int paged_attention(const float* q, uint32_t n_heads, const PagedView& c, const hy_paged_batch* b, float scale,
                     float* out, void* ws, size_t ws_bytes, hipStream_t s) {
     if (!q || !out) return fail(HY_ERR_INVALID, "null q/out");
     if (!std::isfinite(scale)) return fail(HY_ERR_INVALID, "scale is not finite");
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(HY_ERR_INVALID, "q and out must be aligned to 16 bytes");
-    const size_t need = paged_attn_ws_bytes((int)n_heads, c.nkv, c.hd);
+    const size_t need = paged_batch_ws(b, n_heads, c);
     if (!ws || ws_bytes < need || !aligned(ws, 16))
         return fail(HY_ERR_INVALID, "workspace of %zu bytes at %p: %zu bytes aligned to 16 needed", ws_bytes, ws, need);
     const PagedAttnArgs a{q, out, c, (int)n_heads, (int)b->n_req, (int)b->n_rows, (int)b->max_pages, b->q_start_dev,
@@ -173,7 +178,7 @@ int hy_rope_qknorm_paged(const float* qkv, uint32_t n_rows, uint32_t n_heads, co
 size_t hy_paged_attention_ws(uint32_t n_heads, const hy_paged_cache* cache, const hy_paged_batch* batch) {
     hy::PagedView c;
     if (hy::paged_cache_check(cache, n_heads, &c) != HY_OK || hy::paged_batch_check(batch, c, false) != HY_OK) return 0;
-    return hy::paged_attn_ws_bytes((int)n_heads, c.nkv, c.hd);
+    return hy::paged_batch_ws(batch, n_heads, c);
 }
 
 int hy_paged_attention(const float* q, uint32_t n_heads, const hy_paged_cache* cache, const hy_paged_batch* batch,

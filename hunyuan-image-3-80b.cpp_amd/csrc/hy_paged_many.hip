@@ -514,7 +514,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 dst = a.out + ((int64_t)row * a.nh + head) * HD;
                 f = l_run == 0.0f ? 0.0f : down / l_run;
             } else {
-                float* const slot = a.ws + (size_t)slot_id * part_slot_floats(PM_M, HD);
+                float* const slot = a.ws + ps.ws + (size_t)slot_id * part_slot_floats(PM_M, HD);
                 dst = slot + my * HD;
                 if (h == 0) {
                     slot[PM_M * HD + my] = m_run;

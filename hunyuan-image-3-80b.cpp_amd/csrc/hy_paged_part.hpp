@@ -2,7 +2,7 @@
 //
 // A request's rows (token x query head of one kv head, token-major) fall into tiles of M; an
 // item is a (request, kv head, tile) and its nominal length the keys that its last token sees
-// if causal.  All items of a batch in a row (requests, then kv heads, then tiles) are cut into
+// if causal, plus what starting an item costs.  All items of a batch in a row (requests, then kv heads, then tiles) are cut into
 // equal stretches, one per worker: however ragged the lengths, every worker has the same share.
 // Lengths are in device memory, so every work group sums them itself (part_sums).  An item
 // inside one worker's stretch is written by it; one that is cut leaves a partial result per
@@ -19,11 +19,14 @@ struct PartShape {
     int G, tau;                // query heads of a kv head; nominal tokens per tile, max(M / G, 1)
     int64_t rows_lo, rows_hi;  // requests with rows_lo < rows <= rows_hi belong to this launch
     int workers;
-    int min_keys;              // of a stretch
+    int extra;                 // keys that starting an item is worth
+    int unit;                  // nominal length of the shortest stretch, a power of two
+    size_t ws;                 // floats of the workspace before this launch's slots
 };
-inline PartShape part_shape(int m_shift, int G, int64_t rows_lo, int64_t rows_hi, int workers, int min_keys) {
+inline PartShape part_shape(int m_shift, int G, int64_t rows_lo, int64_t rows_hi, int workers, int extra, int unit,
+                            size_t ws) {
     const int M = 1 << m_shift;
-    return {M, m_shift, G, M / G > 1 ? M / G : 1, rows_lo, rows_hi, workers, min_keys};
+    return {M, m_shift, G, M / G > 1 ? M / G : 1, rows_lo, rows_hi, workers, extra, unit, ws};
 }
 
 // a value that all lanes share, in scalar registers
@@ -35,7 +38,7 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 struct PartReq {
     int start, n, kv;   // first row, rows (tokens), keys
     int tiles, full;    // tiles of its rows; those whose nominal tokens do not reach past the last
-    int64_t base, head; // keys before its first token; nominal length of a head's tiles
+    int64_t base, head; // keys before its first token, and extra; nominal length of a head's tiles
     // nominal length of tiles 0 .. k - 1
     __device__ __forceinline__ int64_t upto(int tau, int64_t k) const {
         const int64_t f = min(k, (int64_t)full);
@@ -44,10 +47,11 @@ struct PartReq {
 };
 
 __device__ __forceinline__ PartReq part_req(const PartShape& p, int start, int n, int kv) {
-    PartReq q{start, n, kv, 0, n / p.tau, max(kv - n, 0), 0};
+    PartReq q{start, n, kv, 0, n / p.tau, max(kv - n, 0) + p.extra, 0};
     const int64_t rows = (int64_t)n * p.G;
     if (rows > p.rows_lo && rows <= p.rows_hi) q.tiles = (int)((rows + p.M - 1) >> p.m_shift);
-    q.head = q.upto(p.tau, q.tiles);
+    // whole units: where stretches are one unit, short requests share no worker
+    q.head = (q.upto(p.tau, q.tiles) + p.unit - 1) & ~(int64_t)(p.unit - 1);
     return q;
 }
 
@@ -105,7 +109,7 @@ __device__ __forceinline__ int64_t part_sums(const PagedAttnArgs& a, const PartS
 
 __device__ __forceinline__ int64_t part_stretch(const PartShape& p, int64_t total) {
     // workers is a power of two
-    return max((total + p.workers - 1) >> (31 - __builtin_clz(p.workers)), (int64_t)p.min_keys);
+    return max((total + p.workers - 1) >> (31 - __builtin_clz(p.workers)), (int64_t)p.unit);
 }
 
 struct PartItem {
@@ -154,12 +158,12 @@ __device__ __forceinline__ PartItem part_find(const PagedAttnArgs& a, const Part
         t = min(uniform((int)(2.0f * yf * __builtin_amdgcn_rcpf(b + __builtin_amdgcn_sqrtf(b * b + 2.0f * p.tau * yf)))),
                 it.q.tiles - 1);
         while (t > 0 && it.q.upto(p.tau, t) > y) t--;
-        while (t + 1 < it.q.tiles && it.q.upto(p.tau, t + 1) <= y) t++;
+        while (t + 1 < it.q.tiles && it.q.upto(p.tau, t + 1) <= y) t++;  // the last one ends with its head
     }
     it.tile = t;
     const int64_t t0 = it.q.upto(p.tau, t);
     it.at += t0;
-    it.len = it.q.upto(p.tau, t + 1) - t0;
+    it.len = (t + 1 < it.q.tiles ? it.q.upto(p.tau, t + 1) : it.q.head) - t0;
     return it;
 }
 
