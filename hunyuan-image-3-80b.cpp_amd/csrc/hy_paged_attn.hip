@@ -100,6 +100,7 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && NT == 2 
     const int G = ps.G, pmask = (1 << a.c.shift) - 1;
     const float qscale = a.scale * 1.4426950408889634f;
 
+    PartJob job{};
     while (x < x_end) {
         const PartItem it = part_find(a, ps, sums, x);
         const int64_t p0 = x - it.at, p1 = min(x_end - it.at, it.len);  // this piece
@@ -138,6 +139,7 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && NT == 2 
         const int blocks = (last + 31) / 32;
         const int t0 = part_block(p0, it.len, blocks) * (32 / KB), t1 = part_block(p1, it.len, blocks) * (32 / KB);
 
+        job = part_job(ps, it, p0, p1, stretch, worker, n_live);
         const int slot_id = p0 == 0 && p1 == it.len ? -1 : 2 * worker + (p0 == 0 ? 1 : 0);  // -1: all of it is here
 
         // q: scaled by scale * log2(e) (scores in the base-2 domain); f16: by a power of two that
@@ -427,42 +429,44 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && NT == 2 
                     }
         }
     }
+    if (lane == 0) part_jobs(a, ps, HD)[worker] = job;
 }
 
-// Joins the pieces of every cut item: a team of THREADS / JOBS threads per worker w takes the
-// item that w begins and another ends, HD / 4 threads a row, 4 dims each.  The pieces' statistics
-// and sums are fetched PJ at a time, which is what a join of few rows waits for.
-template <int HD, int JOBS>
-__device__ __forceinline__ void join(const PagedAttnArgs& a, const PartShape& ps, PartSums<256>& sums, int group,
-                                     int split, int splits) {
-    const int64_t total = part_sums(a, ps, sums);
-    const int64_t stretch = part_stretch(ps, total);
-    constexpr int TEAM = 256 / JOBS;  // a wave at least
-    constexpr int PJ = JOBS > 1 ? 8 : 2;  // items of many rows rarely have more than 2 pieces
-    const int w0 = uniform(group * JOBS + (int)threadIdx.x / TEAM), tt = threadIdx.x % TEAM;
-    const int64_t cut = ((int64_t)w0 + 1) * stretch;  // the end of worker w0's stretch
-    if (cut >= total) return;
-    const PartItem it = part_find(a, ps, sums, cut);
-    if (it.at >= cut || it.at < cut - stretch) return;  // begins here, or was begun by another
-    const int64_t past = it.at + it.len - cut;           // beyond w0's stretch
-    int n_piece = 1 + uniform((int)((float)past * __builtin_amdgcn_rcpf((float)stretch)));
-    while ((int64_t)(n_piece - 1) * stretch >= past) n_piece--;
-    while ((int64_t)(n_piece - 1) * stretch < past) n_piece++;
-    const int n_live = min(it.q.n * ps.G - it.tile * ps.M, ps.M);
+// Joins the pieces of the items that are cut, from the jobs the workers left: work group (w, split)
+// takes every splits-th set of rows of worker w's; in it, HD / 4 threads take 4 dims each of
+// a row and every PL-th piece of it, PJ pieces at a time, and the PL groups of a row meet in LDS.
+// Bound by what a work group gets from memory at once, hence rows and pieces spread as far as
+// they go.
+constexpr int PJ = 4;
+
+template <int HD>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartShape few, PartShape many, int few_splits,
+                                                        int many_splits) {
+    __shared__ float meet[6][256];
+    const int b = (int)blockIdx.x - few.workers * few_splits;
+    const PartShape& ps = b < 0 ? few : many;
+    const int splits = b < 0 ? few_splits : many_splits, at = b < 0 ? (int)blockIdx.x : b;
+    const int w0 = at / splits, split = at - w0 * splits;
+    const PartJob job = part_jobs(a, ps, HD)[w0];
+    const int n_piece = uniform(job.n_piece), n_live = uniform(job.n_live);
+    if (n_piece == 0) return;
     const size_t sf = part_slot_floats(ps.M, HD);
     const float* const first = a.ws + ps.ws + (size_t)(2 * w0 + 1) * sf;
     const float* const rest = a.ws + ps.ws + (size_t)(2 * w0) * sf;  // piece k > 0: + 2 k slots
-    constexpr int TR = HD / 4, RPB = TEAM / TR;  // threads per row, rows at a time
-    const int d = tt % TR * 4;
-    for (int i = split * RPB + tt / TR; i < n_live; i += RPB * splits) {
+    constexpr int TR = HD / 4, GROUPS = 256 / TR;
+    int pl_n = 1;
+    while (pl_n < 8 && pl_n * PJ < n_piece) pl_n *= 2;
+    const int tid = threadIdx.x, d = tid % TR * 4, pl = tid / TR % pl_n, rs = tid / TR / pl_n, rs_n = GROUPS / pl_n;
+    for (int i0 = split * rs_n; i0 < n_live; i0 += rs_n * splits) {  // the same for the work group
+        const int i = min(i0 + rs, n_live - 1);
         float m = -INFINITY, l = 0.0f;
         v4f_t o = v4f_t{};
-        for (int k0 = 0; k0 < n_piece; k0 += PJ) {
+        for (int k0 = pl; k0 < n_piece; k0 += pl_n * PJ) {
             float mk[PJ], lk[PJ];
             v4f_t ok[PJ];
 #pragma unroll
             for (int j = 0; j < PJ; j++) {
-                const int k = min(k0 + j, n_piece - 1);
+                const int k = min(k0 + j * pl_n, n_piece - 1);
                 const float* const s = k == 0 ? first : rest + (size_t)(2 * k) * sf;
                 mk[j] = s[ps.M * HD + i];
                 lk[j] = s[ps.M * (HD + 1) + i];
@@ -479,16 +483,40 @@ __device__ __forceinline__ void join(const PagedAttnArgs& a, const PartShape& ps
 #pragma unroll
             for (int j = 0; j < PJ; j++) {
                 const float f = __builtin_amdgcn_exp2f(mk[j] - ref);
-                if (k0 + j < n_piece) {
+                if (k0 + j * pl_n < n_piece) {
                     l += f * lk[j];
                     o += f * ok[j];
                 }
             }
         }
-        const int rho = it.tile * ps.M + i, tok = rho / ps.G;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        *reinterpret_cast<v4f_t*>(a.out + ((int64_t)(it.q.start + tok) * a.nh + it.g * ps.G + rho - tok * ps.G) * HD +
-                                  d) = o * inv;
+        if (pl_n > 1) {
+            __syncthreads();  // the last rows' are read
+            meet[4][tid] = m;
+            meet[5][tid] = l;
+#pragma unroll
+            for (int j = 0; j < 4; j++) meet[j][tid] = o[j];
+            __syncthreads();
+            if (pl == 0) {
+                float mn = m;
+                for (int k = 1; k < pl_n; k++) mn = fmaxf(mn, meet[4][tid + k * TR]);
+                const float ref = mn == -INFINITY ? 0.0f : mn, alpha = __builtin_amdgcn_exp2f(m - ref);
+                l *= alpha;
+                o *= alpha;
+                for (int k = 1; k < pl_n; k++) {
+                    const int from = tid + k * TR;
+                    const float f = __builtin_amdgcn_exp2f(meet[4][from] - ref);
+                    l += f * meet[5][from];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[j] += f * meet[j][from];
+                }
+            }
+        }
+        if (pl == 0 && i0 + rs < n_live) {
+            const int rho = job.rho0 + i, tok = rho / ps.G;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            *reinterpret_cast<v4f_t*>(a.out + ((int64_t)(job.start + tok) * a.nh + job.g * ps.G + rho - tok * ps.G) * HD +
+                                      d) = o * inv;
+        }
     }
 }
 
@@ -496,21 +524,7 @@ constexpr int PF_GROUPS = 512;  // two per CU
 constexpr int PF_WORKERS = PF_GROUPS * PF_WAVES;
 constexpr int PF_MAX_M = 32;
 constexpr int PF_MAX_ROWS = PF_MAX_M;  // rows of a request up to which the stream takes it
-// Rows over work groups until a round or two are left, as each round is a trip to memory (24 rows
-// of 8 pieces: 24 us in one work group, 15 in four).
-constexpr int PJ_FEW_ROWS = 8, PJ_MANY_SPLITS = 4;
-
-// first few.workers / 4 x few.M / 8 work groups for the stream's items, then many.workers x
-// PJ_MANY_SPLITS for the others'
-template <int HD>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartShape few, PartShape many) {
-    __shared__ PartSums<256> sums;
-    const int splits = few.M / PJ_FEW_ROWS, few_groups = few.workers / 4 * splits, b = (int)blockIdx.x - few_groups;
-    if (b < 0)
-        join<HD, 4>(a, few, sums, (int)blockIdx.x / splits, (int)blockIdx.x % splits, splits);
-    else
-        join<HD, 1>(a, many, sums, b / PJ_MANY_SPLITS, b % PJ_MANY_SPLITS, PJ_MANY_SPLITS);
-}
+constexpr int PJ_ROWS = 8, PJ_MANY_SPLITS = 32;  // rows of a stream's item per work group; a tile's work groups
 
 // which launches a batch takes: workers 0: not that one
 struct PaPlan {
@@ -524,14 +538,14 @@ static PaPlan pa_plan(int n_req, int max_new, int G, int hd) {
     // Starting an item is worth 16 keys of a full stream, 256 of a many-row tile (20 000 of its 3500
     // to 6500 cycles per 32 keys); a stretch is 64 keys at least, 128.
     p.few = part_shape(rows > 16 ? 5 : 4, G, 0, many ? PF_MAX_ROWS : ALL, few ? PF_WORKERS : 0, 16, 64, 0);
-    const size_t few_ws = few ? 2 * (size_t)PF_WORKERS * part_slot_floats(p.few.M, hd) : 0;
+    const size_t few_ws = part_ws_floats(p.few.workers, p.few.M, hd);
     p.many = part_shape(PM_TILE_SHIFT, G, few ? PF_MAX_ROWS : 0, ALL, many ? PM_WORKERS : 0, 256, 128, few_ws);
     return p;
 }
 
 size_t paged_attn_ws_bytes(int n_req, int max_new, int G, int hd) {
     const PaPlan p = pa_plan(n_req, max_new, G, hd);
-    return 4 * (p.many.ws + 2 * (size_t)p.many.workers * part_slot_floats(PM_TILE, hd));
+    return 4 * (p.many.ws + part_ws_floats(p.many.workers, PM_TILE, hd));
 }
 
 template <class E, int HD>
@@ -554,11 +568,12 @@ hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s)
             big ? launch_few<__bf16, 128>(a, p.few, s) : launch_few<__bf16, 64>(a, p.few, s);
     }
     if (p.many.workers) (void)launch_paged_many(a, p.many, s);
-    const dim3 grid(p.few.workers / 4 * (p.few.M / PJ_FEW_ROWS) + p.many.workers * PJ_MANY_SPLITS);
+    const int splits = p.few.M / PJ_ROWS;
+    const dim3 grid(p.few.workers * splits + p.many.workers * PJ_MANY_SPLITS);
     if (big)
-        hipLaunchKernelGGL(paged_join_kernel<128>, grid, dim3(256), 0, s, a, p.few, p.many);
+        hipLaunchKernelGGL(paged_join_kernel<128>, grid, dim3(256), 0, s, a, p.few, p.many, splits, PJ_MANY_SPLITS);
     else
-        hipLaunchKernelGGL(paged_join_kernel<64>, grid, dim3(256), 0, s, a, p.few, p.many);
+        hipLaunchKernelGGL(paged_join_kernel<64>, grid, dim3(256), 0, s, a, p.few, p.many, splits, PJ_MANY_SPLITS);
     return hipGetLastError();
 }
 

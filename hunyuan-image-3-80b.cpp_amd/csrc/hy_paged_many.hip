@@ -93,6 +93,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
     const int64_t x_end = min(x + stretch, total);
     const int G = ps.G, pmask = (1 << a.c.shift) - 1;
 
+    PartJob job{};
     while (x < x_end) {
         const PartItem it = part_find(a, ps, sums, x);
         const int64_t p0 = x - it.at, p1 = min(x_end - it.at, it.len);
@@ -125,6 +126,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         const int blocks = (tile_last + 31) / 32;
         const int kb0 = part_block(p0, it.len, blocks), kb1 = part_block(p1, it.len, blocks);
         const int my_kb1 = min((last + 31) / 32, kb1);
+        job = part_job(ps, it, p0, p1, stretch, worker, n_live);
         const int slot_id = p0 == 0 && p1 == it.len ? -1 : 2 * worker + (p0 == 0 ? 1 : 0);  // -1: all of it is here
 
         // ---- loads and stores of blocks
@@ -536,6 +538,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         }
         __syncthreads();  // last_s and the buffers are free
     }
+    if (tid == 0) part_jobs(a, ps, HD)[worker] = job;
 }
 
 template <class E>

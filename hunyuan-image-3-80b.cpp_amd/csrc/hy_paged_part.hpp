@@ -167,6 +167,14 @@ __device__ __forceinline__ PartItem part_find(const PagedAttnArgs& a, const Part
     return it;
 }
 
+// floor(x / n) for 0 <= x, 0 < n
+__device__ __forceinline__ int part_quotient(int64_t x, int64_t n) {
+    int k = uniform((int)((float)x * __builtin_amdgcn_rcpf((float)n)));
+    while ((int64_t)k * n > x) k--;
+    while ((int64_t)(k + 1) * n <= x) k++;
+    return k;
+}
+
 // the block where a piece ending at place y of an item of nominal length len ends: rounded, but
 // growing with y and the same for both who share the cut
 __device__ __forceinline__ int part_block(int64_t y, int64_t len, int blocks) {
@@ -216,6 +224,29 @@ __device__ __forceinline__ void slow_rows(const PagedAttnArgs& a, const int* tro
 // of an item it begins and another ends, in 2 w + 1.  A slot: [M][hd] unnormalised output,
 // [M] running maximum, [M] sum.
 __host__ __device__ __forceinline__ size_t part_slot_floats(int M, int hd) { return (size_t)M * (hd + 2); }
+
+// What worker w leaves for the join: the item that it begins and others end.
+struct PartJob {
+    int n_piece;    // w's own and those of the workers after it; 0: no such item
+    int n_live;     // rows
+    int start;      // the request's first row
+    int rho0;       // the tile's first row (token x head) of the request
+    int g, pad[3];  // kv head
+};
+// floats of a launch's workspace: slots, then jobs
+__host__ __device__ __forceinline__ size_t part_ws_floats(int workers, int M, int hd) {
+    return workers * (2 * part_slot_floats(M, hd) + sizeof(PartJob) / 4);
+}
+__device__ __forceinline__ PartJob* part_jobs(const PagedAttnArgs& a, const PartShape& p, int hd) {
+    return reinterpret_cast<PartJob*>(a.ws + p.ws + 2 * (size_t)p.workers * part_slot_floats(p.M, hd));
+}
+// the job that a piece [p0, p1) of an item makes of worker w
+__device__ __forceinline__ PartJob part_job(const PartShape& p, const PartItem& it, int64_t p0, int64_t p1, int64_t stretch,
+                                            int w, int n_live) {
+    PartJob j{0, n_live, it.q.start, it.tile * p.M, it.g, {}};
+    if (p0 == 0 && p1 < it.len) j.n_piece = part_quotient(it.at + it.len - 1, stretch) - w + 1;
+    return j;
+}
 
 // requests of many rows: tiles of PM_TILE rows, PM_WORKERS work groups (hy_paged_many.hip)
 constexpr int PM_TILE_SHIFT = 8, PM_TILE = 1 << PM_TILE_SHIFT, PM_WORKERS = 256;
