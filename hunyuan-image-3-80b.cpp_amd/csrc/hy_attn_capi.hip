@@ -20,6 +20,7 @@
 
 namespace hy {
 int set_last_error(int code, const std::string& msg);  // hy_capi.hip
+int moe_layer_check(const hy_moe_ctx* c, uint32_t layer, uint32_t T);  // hy_capi.hip
 int moe_hidden(const hy_moe_ctx* c);                   // hy_capi.hip
 int moe_device(const hy_moe_ctx* c);
 const GgufFile& gguf_file(const hy_gguf* g);           // host/hy_gguf.cpp
@@ -240,10 +241,8 @@ int check_paged(const hy_attn_ctx* c, uint32_t layer, const hy_paged_cache* cach
     st->cache.k = static_cast<uint8_t*>(st->cache.k) + layer * cache->layer_stride * el;
     st->cache.v = static_cast<uint8_t*>(st->cache.v) + layer * cache->layer_stride * el;
     st->batch = b;
-    const size_t need = hy::paged_batch_ws(b, (uint32_t)c->nh, st->cache);
-    if (!st->ws || st->ws_bytes < need)
-        return fail(HY_ERR_INVALID, "workspace of %zu bytes at %p: %zu bytes needed", st->ws_bytes, st->ws, need);
-    return HY_OK;
+    HY_TRY(hy::paged_rotary_check(c->cfg.rope_theta, st->cos_t, st->sin_t, st->n_pos, c->cfg.rms_norm_eps));
+    return hy::paged_ws_check(b, (uint32_t)c->nh, st->cache, st->ws, st->ws_bytes);
 }
 
 // run() over a paged cache
@@ -769,6 +768,7 @@ int hy_model_forward_paged(hy_model_ctx* m, const int32_t* ids, const hy_paged_c
     for (uint32_t l = 0; l < (uint32_t)m->L; l++) {  // every layer, before anything is launched
         PagedStep st{{}, nullptr, nullptr, nullptr, 0, ws, ws_bytes};
         HY_TRY(check_paged(c, l, cache, batch, &st));
+        HY_TRY(hy::moe_layer_check(m->moe, l, batch->n_rows));
     }
     const int T = (int)batch->n_rows;
     const float eps = m->cfg.attn.rms_norm_eps;

@@ -17,6 +17,10 @@
 #include "hy_rules.hpp"
 #include "../host/hy_gguf.hpp"
 
+namespace hy {
+int moe_layer_check(const hy_moe_ctx* c, uint32_t layer, uint32_t T);
+}
+
 namespace {
 
 thread_local std::string g_last_error;
@@ -266,11 +270,8 @@ int alloc_layer(hy_moe_ctx* c, LayerW& L) {
 // Q8_0 form of x (the stack's fused RMSNorm + quantization wrote them).
 int forward_impl(hy_moe_ctx* c, uint32_t layer, const float* x, uint32_t T, float* out, const float* resid,
                  hipStream_t s, bool prequant = false) {
-    if (layer >= c->layers.size()) return fail(HY_ERR_INVALID, "layer %u out of range", layer);
+    HY_TRY(hy::moe_layer_check(c, layer, T));
     const LayerW& L = c->layers[layer];
-    if (!L.loaded) return fail(HY_ERR_STATE, "layer %u has no weights", layer);
-    if (T == 0 || T > c->cfg.max_tokens)
-        return fail(HY_ERR_INVALID, "T=%u must be in 1..max_tokens=%u", T, c->cfg.max_tokens);
     if (!x || !out) return fail(HY_ERR_INVALID, "null x/out");
     c->last_stream = s;
     const int H = c->H, I = c->I, E = c->E, K = c->K, wt = c->cfg.wtype;
@@ -471,6 +472,13 @@ namespace hy {
 int set_last_error(int code, const std::string& msg) {
     g_last_error = msg;
     return code;
+}
+int moe_layer_check(const hy_moe_ctx* c, uint32_t layer, uint32_t T) {
+    if (layer >= c->layers.size()) return fail(HY_ERR_INVALID, "layer %u out of range", layer);
+    if (!c->layers[layer].loaded) return fail(HY_ERR_STATE, "layer %u has no weights", layer);
+    if (T == 0 || T > c->cfg.max_tokens)
+        return fail(HY_ERR_INVALID, "T=%u must be in 1..max_tokens=%u", T, c->cfg.max_tokens);
+    return HY_OK;
 }
 int moe_hidden(const hy_moe_ctx* c) { return c ? c->H : 0; }
 int moe_device(const hy_moe_ctx* c) { return c ? c->cfg.device : -1; }

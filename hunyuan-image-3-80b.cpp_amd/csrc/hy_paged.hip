@@ -201,7 +201,7 @@ template <class E>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
     const int heads = a.nh + a.c.nkv, hd = a.c.hd;
     const int groups = (heads + PA_HEADS - 1) / PA_HEADS;
-    const int64_t wid = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
+    const int64_t wid = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + threadIdx.x / WAVE;
     if (wid >= (int64_t)a.n_rows * groups) return;
     const int t = (int)(wid / groups), h0 = (int)(wid % groups) * PA_HEADS, l = threadIdx.x % WAVE;
     const int slot = a.slots[t], pos = a.positions[t];
@@ -242,7 +242,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
 
 hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
     const int64_t waves = (int64_t)a.n_rows * ((a.nh + a.c.nkv + PA_HEADS - 1) / PA_HEADS);
-    const dim3 grid((unsigned)((waves + 3) / 4));
+    // a launch has fewer than 2^32 threads along x
+    const int64_t groups = (waves + 3) / 4, gx = groups < 1 << 22 ? groups : 1 << 22;
+    const dim3 grid((unsigned)gx, (unsigned)((groups + gx - 1) / gx));
     if (a.c.type == HY_TYPE_F32)
         hipLaunchKernelGGL(paged_append_kernel<float>, grid, dim3(256), 0, s, a);
     else if (a.c.type == HY_TYPE_F16)

@@ -14,9 +14,10 @@
 // matrix cores multiply exactly -- a f16 cache: two f16 pieces (22 bits, q scaled per row by a
 // power of two, p by 2^14); a bf16 cache: three bf16 pieces (24 bits) -- while K and V go in as
 // they are.  f32 caches use the fp32 MFMAs.
-// Keys that a row does not see get weight 0; 0 times an infinity or NaN in their V would
-// still be felt, so where some rows do not see a key, V is looked at, and if it is not
-// finite the piece is computed again key by key (slow_rows).
+// Keys that a row does not see get weight 0, but 0 times an infinity or NaN in their V would
+// still be felt.  Keys that no row sees (a page's unwritten end) have their V zeroed; where
+// some rows do not see a key, V is looked at, and if it is not finite the piece is computed again
+// key by key (slow_rows).
 #include "hy_device.hpp"
 #include "hy_lds.hpp"
 #include "hy_paged.hpp"
@@ -340,9 +341,14 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && NT == 2 
 #pragma unroll
                 for (int u = 0; u < KT; u++)
 #pragma unroll
-                    for (int v = 0; v < 4; v++)
+                    for (int v = 0; v < 4; v++) {
+                        const bool gone = t * KB + 16 * u + 4 * g4 + v >= last || vpage[u] < 0;
 #pragma unroll
-                        for (int w = 0; w < VL * VW; w++) odd |= P::odd((uint32_t)vx[u][v][w]);
+                        for (int w = 0; w < VL * VW; w++) {
+                            vx[u][v][w] = gone ? 0 : vx[u][v][w];
+                            odd |= P::odd((uint32_t)vx[u][v][w]);
+                        }
+                    }
             }
             if constexpr (F32T) {
 #pragma unroll
@@ -567,7 +573,7 @@ hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s)
         else
             big ? launch_few<__bf16, 128>(a, p.few, s) : launch_few<__bf16, 64>(a, p.few, s);
     }
-    if (p.many.workers) (void)launch_paged_many(a, p.many, s);
+    if (p.many.workers) launch_paged_many(a, p.many, s);
     const int splits = p.few.M / PJ_ROWS;
     const dim3 grid(p.few.workers * splits + p.many.workers * PJ_MANY_SPLITS);
     if (big)

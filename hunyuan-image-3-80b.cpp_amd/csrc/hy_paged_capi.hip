@@ -59,6 +59,15 @@ int sizes_check(uint32_t n_req, uint32_t n_rows, uint32_t page_size, uint32_t ma
     return HY_OK;
 }
 
+int verify_check(uint32_t n_req, uint32_t n_rows, uint32_t vocab) {
+    if (n_req == 0 || n_req > (uint32_t)hy::PG_MAX_REQ || n_rows == 0 || n_rows > 1u << 20 || vocab == 0 ||
+        vocab > 1u << 22)
+        return fail(HY_ERR_INVALID, "n_req=%u n_rows=%u vocab=%u out of range", n_req, n_rows, vocab);
+    if ((uint64_t)n_rows * vocab > 1ull << 36)  // 256 GiB of logits, the most that one launch covers
+        return fail(HY_ERR_UNSUPPORTED, "n_rows=%u of vocab=%u: 2^36 logits at most", n_rows, vocab);
+    return HY_OK;
+}
+
 }  // namespace
 
 namespace hy {
@@ -105,18 +114,24 @@ int paged_batch_check(const hy_paged_batch* b, const PagedView& c, bool writes) 
     return HY_OK;
 }
 
-int paged_append(const float* qkv, uint32_t n_rows, uint32_t n_heads, const PagedView& c, const int32_t* positions,
-                 const int32_t* slots, float theta, const float* cos_t, const float* sin_t, uint32_t n_pos,
-                 const float* q_norm, const float* k_norm, float eps, float* q, hipStream_t s) {
-    if (!qkv || !positions || !slots || !q) return fail(HY_ERR_INVALID, "null pointer");
-    if (n_rows == 0 || n_rows > 1u << 20) return fail(HY_ERR_INVALID, "n_rows=%u must be in 1..2^20", n_rows);
+int paged_rotary_check(float theta, const float* cos_t, const float* sin_t, uint32_t n_pos, float eps) {
     if ((cos_t == nullptr) != (sin_t == nullptr)) return fail(HY_ERR_INVALID, "give both rotary tables or neither");
     if (cos_t && (n_pos == 0 || n_pos > 1u << 30)) return fail(HY_ERR_INVALID, "n_pos=%u must be in 1..2^30", n_pos);
     if (!cos_t && !(theta == 0.0f || (theta > 0.0f && std::isfinite(theta))))
         return fail(HY_ERR_INVALID, "theta=%g must be positive, or 0 for no rotation", theta);
     if (!(eps >= 0.0f)) return fail(HY_ERR_INVALID, "eps=%g must not be negative", eps);
-    if (!aligned(qkv, 16) || !aligned(q, 16) || (q_norm && !aligned(q_norm, 16)) || (k_norm && !aligned(k_norm, 16)) ||
-        (cos_t && (!aligned(cos_t, 16) || !aligned(sin_t, 16))))
+    if (cos_t && (!aligned(cos_t, 16) || !aligned(sin_t, 16)))
+        return fail(HY_ERR_INVALID, "rotary tables must be aligned to 16 bytes");
+    return HY_OK;
+}
+
+int paged_append(const float* qkv, uint32_t n_rows, uint32_t n_heads, const PagedView& c, const int32_t* positions,
+                 const int32_t* slots, float theta, const float* cos_t, const float* sin_t, uint32_t n_pos,
+                 const float* q_norm, const float* k_norm, float eps, float* q, hipStream_t s) {
+    if (!qkv || !positions || !slots || !q) return fail(HY_ERR_INVALID, "null pointer");
+    if (n_rows == 0 || n_rows > 1u << 20) return fail(HY_ERR_INVALID, "n_rows=%u must be in 1..2^20", n_rows);
+    HY_TRY(paged_rotary_check(theta, cos_t, sin_t, n_pos, eps));
+    if (!aligned(qkv, 16) || !aligned(q, 16) || (q_norm && !aligned(q_norm, 16)) || (k_norm && !aligned(k_norm, 16)))
         return fail(HY_ERR_INVALID, "f32 arrays must be aligned to 16 bytes");
     PagedAppendArgs a{qkv,   (int)n_rows, (int)n_heads, c,      positions, slots, cos_t, sin_t,
                       (int)n_pos, cos_t ? 2 : theta > 0.0f ? 1 : 0, q_norm, k_norm, eps, q, {}};
@@ -131,14 +146,19 @@ size_t paged_batch_ws(const hy_paged_batch* b, uint32_t n_heads, const PagedView
                                (int)n_heads / c.nkv, c.hd);
 }
 
+int paged_ws_check(const hy_paged_batch* b, uint32_t n_heads, const PagedView& c, const void* ws, size_t ws_bytes) {
+    const size_t need = paged_batch_ws(b, n_heads, c);
+    if (!ws || ws_bytes < need || !aligned(ws, 16))
+        return fail(HY_ERR_INVALID, "workspace of %zu bytes at %p: %zu bytes aligned to 16 needed", ws_bytes, ws, need);
+    return HY_OK;
+}
+
 int paged_attention(const float* q, uint32_t n_heads, const PagedView& c, const hy_paged_batch* b, float scale,
                     float* out, void* ws, size_t ws_bytes, hipStream_t s) {
     if (!q || !out) return fail(HY_ERR_INVALID, "null q/out");
     if (!std::isfinite(scale)) return fail(HY_ERR_INVALID, "scale is not finite");
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(HY_ERR_INVALID, "q and out must be aligned to 16 bytes");
-    const size_t need = paged_batch_ws(b, n_heads, c);
-    if (!ws || ws_bytes < need || !aligned(ws, 16))
-        return fail(HY_ERR_INVALID, "workspace of %zu bytes at %p: %zu bytes aligned to 16 needed", ws_bytes, ws, need);
+    HY_TRY(paged_ws_check(b, n_heads, c, ws, ws_bytes));
     const PagedAttnArgs a{q, out, c, (int)n_heads, (int)b->n_req, (int)b->n_rows, (int)b->max_pages, b->q_start_dev,
                           b->kv_len_dev, b->table_dev, b->seen_dev, scale, static_cast<float*>(ws)};
     HIP_TRY(launch_paged_attn(a, (int)(b->max_new < b->n_rows ? b->max_new : b->n_rows), s));
@@ -190,11 +210,7 @@ int hy_paged_attention(const float* q, uint32_t n_heads, const hy_paged_cache* c
 }
 
 size_t hy_verify_drafts_ws(uint32_t n_req, uint32_t n_rows, uint32_t vocab) {
-    if (n_req == 0 || n_req > (uint32_t)hy::PG_MAX_REQ || n_rows == 0 || n_rows > 1u << 20 || vocab == 0 ||
-        vocab > 1u << 22) {
-        (void)fail(HY_ERR_INVALID, "n_req=%u n_rows=%u vocab=%u out of range", n_req, n_rows, vocab);
-        return 0;
-    }
+    if (verify_check(n_req, n_rows, vocab) != HY_OK) return 0;
     return hy::verify_ws_bytes((int)n_req, (int)n_rows, (int)vocab);
 }
 
@@ -205,8 +221,8 @@ int hy_verify_drafts(const float* logits, const float* draft_probs, const int32_
     if (!logits || !ids || !q_start || !u_accept || !u_sample || !accepted || !tokens)
         return fail(HY_ERR_INVALID, "null pointer");
     if (max_new == 0 || max_new > 1u << 20) return fail(HY_ERR_INVALID, "max_new=%u must be in 1..2^20", max_new);
-    const size_t need = hy_verify_drafts_ws(n_req, n_rows, vocab);
-    if (!need) return HY_ERR_INVALID;
+    HY_TRY(verify_check(n_req, n_rows, vocab));
+    const size_t need = hy::verify_ws_bytes((int)n_req, (int)n_rows, (int)vocab);
     if (!ws || ws_bytes < need || !aligned(ws, 16))
         return fail(HY_ERR_INVALID, "workspace of %zu bytes at %p: %zu bytes aligned to 16 needed", ws_bytes, ws, need);
     const hy::VerifyArgs a{logits, draft_probs, ids, q_start, (int)n_req, (int)n_rows, (int)max_new, (int)vocab,

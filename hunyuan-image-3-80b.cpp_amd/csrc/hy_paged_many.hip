@@ -549,14 +549,13 @@ static void launch(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
         hipLaunchKernelGGL((paged_many_kernel<E, 64>), dim3(ps.workers), dim3(PM_THREADS), 0, s, a, ps);
 }
 
-hipError_t launch_paged_many(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
+void launch_paged_many(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
     if (a.c.type == HY_TYPE_F32)
         launch<float>(a, ps, s);
     else if (a.c.type == HY_TYPE_F16)
         launch<_Float16>(a, ps, s);
     else
         launch<__bf16>(a, ps, s);
-    return hipGetLastError();
 }
 
 }  // namespace hy

@@ -250,6 +250,6 @@ __device__ __forceinline__ PartJob part_job(const PartShape& p, const PartItem& 
 
 // requests of many rows: tiles of PM_TILE rows, PM_WORKERS work groups (hy_paged_many.hip)
 constexpr int PM_TILE_SHIFT = 8, PM_TILE = 1 << PM_TILE_SHIFT, PM_WORKERS = 256;
-hipError_t launch_paged_many(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s);
+void launch_paged_many(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s);
 
 }  // namespace hy

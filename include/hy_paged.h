@@ -115,8 +115,10 @@ int hy_rope_qknorm_paged(const float* qkv_dev, uint32_t n_rows, uint32_t n_heads
 /* out[t][h] = sum_j p_j v_j, p = softmax_j(scale q[t][h] . k_j) over the keys row t sees
  * (hy_paged_batch); zero where it sees none.  q, out [n_rows][n_heads][head_dim] f32;
  * query head h reads kv head h / (n_heads / n_kv_heads).  Products and sums have f32
- * accuracy whatever the cache's type.  A key that a row does not see does not touch it,
- * whatever it holds.  ws_dev: hy_paged_attention_ws bytes (0 for bad arguments), aligned
+ * accuracy whatever the cache's type, relative to the largest elements of q, of a key and
+ * of a value row: one below 2^-16 of its vector's largest is taken to 2^-39 of that, values
+ * to 2^-98 at least.  A key that a row does not see does not touch it, whatever it holds; an
+ * infinity or NaN in q or in a key that a row sees makes the row NaN.  ws_dev: hy_paged_attention_ws bytes (0 for bad arguments), aligned
  * to 16 bytes, contents indifferent. */
 size_t hy_paged_attention_ws(uint32_t n_heads, const hy_paged_cache* cache, const hy_paged_batch* batch);
 int hy_paged_attention(const float* q_dev, uint32_t n_heads, const hy_paged_cache* cache, const hy_paged_batch* batch,
@@ -130,7 +132,7 @@ int hy_paged_attention(const float* q_dev, uint32_t n_heads, const hy_paged_cach
  * in order: x_{i+1} is accepted if u_accept[row i] * q(x_{i+1}) < p(x_{i+1}).  At the first
  * refusal the next token is drawn from max(p - q, 0) / sum (from p where that is 0
  * everywhere), after n accepted drafts from p of the last row; drawn by inversion: the
- * lowest index whose running sum exceeds u_sample[r] times the whole.  Temperature 0 or
+ * lowest index whose running sum exceeds u_sample[r] times the whole.  n_rows * vocab <= 2^36.  Temperature 0 or
  * less: x is accepted if it is the largest logit (equal ones: the lowest index), which is
  * also the next token.  Numbers are computed in 64 bits.  Outputs:
  *   accepted [n_req]           accepted drafts; -1 for a request without rows or with more

@@ -164,3 +164,12 @@ def test_context_calls_refuse_null(hy):
     L = hy.lib()
     assert L.hy_attn_forward_paged(None, 0, P, _cache(hy), _batch(hy), None, None, 0, P, P, 1 << 40, None) == INVALID
     assert L.hy_model_forward_paged(None, P, _cache(hy), _batch(hy), P, P, 1 << 40, None) == INVALID
+
+
+def test_verify_refuses_what_no_launch_covers(hy):
+    L = hy.lib()
+    n_rows, vocab = 1 << 20, (1 << 16) + 1     # past 2^36 logits
+    assert L.hy_verify_drafts_ws(4, n_rows, vocab) == 0
+    assert L.hy_verify_drafts(P, None, P, P, 4, n_rows, 5, vocab, None, P, P, P, P, P, 1 << 62, None) == UNSUPPORTED
+    assert L.hy_last_error().decode()
+    assert L.hy_verify_drafts_ws(4, n_rows, vocab - 1) > 0

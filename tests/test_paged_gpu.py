@@ -922,3 +922,136 @@ def test_speculative_decoding_equals_greedy_decoding(gpu):
     assert accepted_in_all > 10
     for d, w in zip(done, want):
         assert d[:steps] == w[:len(d)][:steps]
+
+
+# ------------------------------------------------------------------ the ends of the ranges
+
+def test_append_of_more_waves_than_one_grid_dimension_holds(gpu):
+    """2^20 rows of 253 heads: 2^32 threads.  Only a few rows have a slot, so little is touched."""
+    T, nh, nkv, hd, page = 1 << 20, 252, 1, 64, 16
+    row = (nh + 2 * nkv) * hd
+    qkv, qb = gpu.Buf(4 * T * row), gpu.Buf(4 * T * nh * hd)
+    rng = np.random.default_rng(60)
+    live = np.array([0, 1, 77777, T // 2, T - 2, T - 1])
+    x = rng.standard_normal((len(live), row)).astype(np.float32)
+    slots, pos = np.full(T, -1, np.int32), np.zeros(T, np.int32)
+    slots[live], pos[live] = np.arange(len(live)) + 3, live
+    put = lambda at, a: gpu.check(gpu.lib().hy_memcpy_h2d(at, a.ctypes.data, a.nbytes))  # noqa: E731
+    for i, t in enumerate(live):
+        put(qkv.ptr + 4 * int(t) * row, np.ascontiguousarray(x[i]))
+    pool = Pool(2, page, nkv, hd, F32, fill=7.0)
+    kb, vb = upload(gpu, pool)
+    gpu.rope_qknorm_paged(qkv, T, nh, cache_of(gpu, pool, kb, vb), dev(gpu, pos), dev(gpu, slots), 1e4, None, None, 0,
+                          None, None, 1e-5, qb)
+    gpu.sync()
+    q, k, v, qm, km = append_ref(x, nh, nkv, hd, pos[live], 1e4, None, None, None, None, 1e-5)
+    got, gk, gv = np.empty((nh, hd), np.float32), kb.numpy(), vb.numpy()
+    for i, t in enumerate(live):
+        gpu.check(gpu.lib().hy_memcpy_d2h(got.ctypes.data, qb.ptr + 4 * int(t) * nh * hd, got.nbytes))
+        assert (np.abs(got - q[i]) <= APPEND_TOL * qm[i]).all()
+        p, o = divmod(int(slots[t]), page)
+        assert (np.abs(pool.at(gk, p, o) - k[i]) <= APPEND_TOL * km[i] + EPS32 * np.abs(k[i])).all()
+        np.testing.assert_array_equal(pool.at(gv, p, o), v[i].astype(np.float32))
+    qkv.free()
+    qb.free()
+
+
+def test_model_of_a_padded_batch(gpu):
+    """Rows behind the last sequence and rows of a request that got no pages change nothing for
+    the others, whatever their ids."""
+    m, nh, nkv, hd, V, L = greedy_model(gpu)
+    rng = np.random.default_rng(61)
+    page, n_pages, max_pages = 8, 6, 8
+    news = [9, 23, 30, 1]                     # 2 + 3 + (4: refused) + 1 pages of 6
+
+    def run(news, pad):
+        pool = Pool(n_pages * L, page, nkv, hd, F32, fill=np.nan)
+        kb, vb = upload(gpu, pool)
+        cache = gpu.PagedCache(kb, vb, F32, n_pages, page, nkv, hd, layer_stride=n_pages * nkv * page * hd)
+        n = len(news)
+        p = PlanBufs(gpu, np.zeros(n), news, np.zeros(n), np.zeros((n, max_pages)), np.arange(n_pages), n_pages,
+                     sum(news) + pad, page, n_pages)
+        p.run()
+        batch = gpu.PagedBatch(n, p.n_rows, max_pages, max(news), p.q_start, p.kv_len, p.table, p.positions, p.slots)
+        ids = np.full(p.n_rows, -5, np.int32)
+        at = 0
+        for new, seq in zip(news, (seqs[0], seqs[1], seqs[2], seqs[3])):
+            ids[at:at + new] = seq[:new]
+            at += new
+        if pad:
+            ids[at:] = 2 ** 31 - 1
+        logits = gpu.Buf.empty((p.n_rows, V))
+        ws = Ws(gpu, nh, cache, batch)
+        m.forward_paged(dev(gpu, ids), cache, batch, logits, ws.b, ws.n)
+        return p.status.numpy().tolist(), logits.numpy(), p
+
+    seqs = [rng.integers(0, V, 40) for _ in range(4)]
+    st, got, p = run(news, 7)
+    # the request that lacks pages, and those that lack them behind it
+    assert st == [0, 0, 1, 1]
+    for r in range(2):
+        lb = gpu.Buf.empty((news[r], V))
+        m.forward(dev(gpu, seqs[r][:news[r]], np.int32), news[r], lb)
+        want = lb.numpy()
+        g = got[sum(news[:r]):sum(news[:r + 1])]
+        assert np.isfinite(g).all()
+        # two f32 evaluations of two layers, as far apart as the layer test's, and their
+        # experts' products
+        assert np.linalg.norm(g - want) <= 1e-4 * np.linalg.norm(want)
+    m.close()
+
+
+def test_model_refuses_before_it_writes(gpu):
+    """A layer without experts: refused with the cache as it was."""
+    H, I, E, K, nh, nkv, hd, V, L = 256, 128, 8, 2, 8, 2, 64, 500, 2
+    m = gpu.Model(H, I, E, K, gpu.F32, nh, nkv, hd, V, L, 64)
+    m.synth_globals(seed=3, std=0.5)
+    for l in range(L):
+        m.attn.synth(l, seed=7 + l, std=0.08)
+    m.moe.synth(0, seed=9, std=0.05)
+    pool = Pool(4 * L, 16, nkv, hd, F16, fill=3.0)
+    kb, vb = upload(gpu, pool)
+    cache = gpu.PagedCache(kb, vb, F16, 4, 16, nkv, hd, layer_stride=4 * nkv * 16 * hd)
+    i32 = lambda *a: dev(gpu, np.array(a, np.int32))  # noqa: E731
+    batch = gpu.PagedBatch(1, 2, 4, 2, i32(0, 2), i32(2), i32(0, 1, 2, 3), i32(0, 1), i32(0, 1))
+    ws = Ws(gpu, nh, cache, batch)
+    logits = dev(gpu, np.full((2, V), 8.0, np.float32))
+    call = lambda w, n: m.forward_paged(i32(4, 5), cache, batch, logits, w, n)  # noqa: E731
+    with pytest.raises(gpu.HyError):
+        call(ws.b, ws.n)
+    m.moe.synth(1, seed=10, std=0.05)
+    with pytest.raises(gpu.HyError):
+        call(ws.b, ws.n - 1)
+
+    class Odd:
+        ptr = ws.b.ptr + 4
+    with pytest.raises(gpu.HyError):
+        call(Odd, ws.n)
+    gpu.sync()
+    np.testing.assert_array_equal(kb.numpy(), pool.k)
+    np.testing.assert_array_equal(vb.numpy(), pool.v)
+    assert (logits.numpy() == 8.0).all()
+    call(ws.b, ws.n)
+    assert np.isfinite(logits.numpy()).all() and (kb.numpy() != pool.k).any()
+    m.close()
+
+
+def test_attention_unwritten_page_ends_take_no_longer_path(gpu):
+    """What lies behind a request's last key in its page may be anything, infinities and NaN among
+    it: the sums are the same bits as over zeros there."""
+    rng = np.random.default_rng(62)
+    for wtype in (F32, F16, BF16):
+        outs = []
+        pool, table, q_start, kv_len = make_batch(rng, [(700, 1), (37, 1), (90, 3), (200, 1)], 64, 2, 128, wtype)
+        q = rng.standard_normal((q_start[-1], 8, 128)).astype(np.float32)
+        used = np.zeros((pool.n_pages, 64), bool)
+        for r, kv in enumerate(kv_len):
+            for j in range(kv):
+                used[table[r, j // 64], j % 64] = True
+        for fill in (0.0, np.nan, np.inf):
+            for p, i in np.argwhere(~used):
+                for a in (pool.k, pool.v):
+                    pool.put(a, p, i, R.encode(np.full((2, 128), fill, np.float32), wtype))
+            outs.append(attend(gpu, q, pool, q_start, kv_len, table, 0.1))
+        np.testing.assert_array_equal(outs[0], outs[1])
+        np.testing.assert_array_equal(outs[0], outs[2])
