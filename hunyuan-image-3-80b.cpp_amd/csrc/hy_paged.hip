@@ -5,6 +5,7 @@
 //    [rows][nh][hd], keys and values to their slots in the cache's type.
 #include "hy_device.hpp"
 #include "hy_paged.hpp"
+#include "hy_paged_split.hpp"
 
 namespace hy {
 
@@ -184,73 +185,105 @@ hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------- rotary + QK-norm + write
-// One wave per (row, group of PA_HEADS heads), lane l the pair (2l, 2l + 1) of every head:
-// the angle is formed once per wave.  An angle is kept as a fraction of a turn in 64 bits,
-// position times turns per position minus its whole part, so a far position costs no
-// accuracy; sine and cosine of the remaining |x| <= pi are f32.
-constexpr int PA_HEADS = 4;
+// The units of a row are its heads in memory order: nh query heads, nkv key heads, nkv value
+// heads.  A work group takes a group of PA_STEPS * 64 / (HD / 4) units of four consecutive rows, a
+// row per wave (neighbouring rows are neighbours in a page); HD / 4 lanes share a unit, 4 dims
+// (16 bytes) each, and all loads of a wave go out before anything else.  An angle is kept as a
+// fraction of a turn in 64 bits, position times turns per position minus its whole part, so a
+// far position costs no accuracy; sine and cosine of the rest are f32.
+// Bound by memory: 4096 rows of 48 heads of 128 (205 MB) 33 us in caches, 50 from memory (PENDING);
+// 5 rows 4.4 us, all of it latency.
+constexpr int PA_STEPS = 4;
 
-template <class E>
-__device__ __forceinline__ void store_pair(E* p, float a, float b) {
-    typedef E v2 __attribute__((ext_vector_type(2)));
-    const v2 r = {(E)a, (E)b};  // to nearest, ties to even
-    *reinterpret_cast<v2*>(p) = r;
+template <int CTRL>
+__device__ __forceinline__ float dpp_f(float v) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, false));
 }
 
-template <class E>
+template <class E, int HD>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
-    const int heads = a.nh + a.c.nkv, hd = a.c.hd;
-    const int groups = (heads + PA_HEADS - 1) / PA_HEADS;
-    const int64_t wid = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + threadIdx.x / WAVE;
-    if (wid >= (int64_t)a.n_rows * groups) return;
-    const int t = (int)(wid / groups), h0 = (int)(wid % groups) * PA_HEADS, l = threadIdx.x % WAVE;
+    constexpr int LPU = HD / 4, UNITS = PA_STEPS * WAVE / LPU;
+    const int units = a.nh + 2 * a.c.nkv, groups = (units + UNITS - 1) / UNITS;
+    const int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    const int t = (int)(b / groups) * 4 + (int)threadIdx.x / WAVE, u0 = (int)(b % groups) * UNITS;
+    if (t >= a.n_rows) return;
+    const int l = threadIdx.x % WAVE, d = 4 * (l % LPU);
+    const float* const row = a.qkv + (int64_t)t * units * HD + d;
+    v4f_t x[PA_STEPS];
+#pragma unroll
+    for (int s = 0; s < PA_STEPS; s++)
+        x[s] = *reinterpret_cast<const v4f_t*>(row + (int64_t)min(u0 + (s * WAVE + l) / LPU, units - 1) * HD);
     const int slot = a.slots[t], pos = a.positions[t];
     if (slot < 0 || (slot >> a.c.shift) >= a.c.n_pages) return;
     if (a.rotate == 2 && (pos < 0 || pos >= a.n_pos)) return;
-    if (2 * l >= hd) return;  // head_dim 64: half a wave (the sums below stay inside it)
-    float cs = 1.0f, sn = 0.0f;
-    if (a.rotate == 1) {
-        double turn = (double)pos * a.freq[l];
-        turn -= rint(turn);
-        sincosf((float)(turn * 6.283185307179586), &sn, &cs);
-    } else if (a.rotate == 2) {
-        cs = a.cos_t[(int64_t)pos * hd + 2 * l];
-        sn = a.sin_t[(int64_t)pos * hd + 2 * l];
+    float cs[2] = {1.0f, 1.0f}, sn[2] = {0.0f, 0.0f};
+    if (u0 < a.nh + a.c.nkv) {  // not values alone
+        if (a.rotate == 1) {
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                double turn = (double)pos * a.freq[d / 2 + p];
+                turn -= rint(turn);
+                sincospif((float)(2.0 * turn), &sn[p], &cs[p]);
+            }
+        } else if (a.rotate == 2) {
+            const v4f_t c = *reinterpret_cast<const v4f_t*>(a.cos_t + (int64_t)pos * HD + d);
+            const v4f_t s = *reinterpret_cast<const v4f_t*>(a.sin_t + (int64_t)pos * HD + d);
+            cs[0] = c[0], cs[1] = c[2], sn[0] = s[0], sn[1] = s[2];
+        }
     }
-    const float* const row = a.qkv + (int64_t)t * (a.nh + 2 * a.c.nkv) * hd + 2 * l;
+    const v4f_t one = {1.0f, 1.0f, 1.0f, 1.0f};
+    const v4f_t wq = a.q_norm ? *reinterpret_cast<const v4f_t*>(a.q_norm + d) : one;
+    const v4f_t wk = a.k_norm ? *reinterpret_cast<const v4f_t*>(a.k_norm + d) : one;
     const int64_t cell = (int64_t)(slot >> a.c.shift) * a.c.page_stride +
-                         (int64_t)(slot & ((1 << a.c.shift) - 1)) * a.c.token_stride + 2 * l;
-    for (int hh = h0; hh < min(h0 + PA_HEADS, heads); hh++) {
-        const float2 x = *reinterpret_cast<const float2*>(row + (int64_t)hh * hd);
-        const float y0 = x.x * cs - x.y * sn, y1 = x.x * sn + x.y * cs;
-        float ss = y0 * y0 + y1 * y1;
-        for (int d = hd / 4; d >= 1; d >>= 1) ss += shfl_xor(ss, d);
-        const float rms = 1.0f / sqrtf(ss / (float)hd + a.eps);
-        const float* const w = hh < a.nh ? a.q_norm : a.k_norm;
-        const float w0 = w ? w[2 * l] : 1.0f, w1 = w ? w[2 * l + 1] : 1.0f;
-        if (hh < a.nh) {
-            *reinterpret_cast<float2*>(a.q + ((int64_t)t * a.nh + hh) * hd + 2 * l) =
-                make_float2(y0 * rms * w0, y1 * rms * w1);
-        } else {
-            const int g = hh - a.nh;
-            const float2 v = *reinterpret_cast<const float2*>(row + (int64_t)(hh + a.c.nkv) * hd);
-            store_pair(static_cast<E*>(a.c.k) + cell + g * a.c.head_stride, y0 * rms * w0, y1 * rms * w1);
-            store_pair(static_cast<E*>(a.c.v) + cell + g * a.c.head_stride, v.x, v.y);
+                         (int64_t)(slot & ((1 << a.c.shift) - 1)) * a.c.token_stride + d;
+#pragma unroll
+    for (int s = 0; s < PA_STEPS; s++) {
+        const int u = u0 + (s * WAVE + l) / LPU;
+        v4f_t y;
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            y[2 * p] = x[s][2 * p] * cs[p] - x[s][2 * p + 1] * sn[p];
+            y[2 * p + 1] = x[s][2 * p] * sn[p] + x[s][2 * p + 1] * cs[p];
+        }
+        float ss = (y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]);
+        ss += dpp_f<0x128>(ss);  // rotations by 8 .. 1 in 16 lanes
+        ss += dpp_f<0x124>(ss);
+        ss += dpp_f<0x122>(ss);
+        ss += dpp_f<0x121>(ss);
+        if constexpr (LPU == 32) ss = fadd_row(ss);
+        const float rms = 1.0f / sqrtf(ss / (float)HD + a.eps);
+        if (u < a.nh) {
+            *reinterpret_cast<v4f_t*>(a.q + ((int64_t)t * a.nh + u) * HD + d) = y * rms * wq;
+        } else if (u < units) {
+            const bool key = u < a.nh + a.c.nkv;
+            const v4f_t z = key ? y * rms * wk : x[s];
+            E* const pool = static_cast<E*>(key ? a.c.k : a.c.v);
+            typedef E v4 __attribute__((ext_vector_type(4)));  // to nearest, ties to even
+            *reinterpret_cast<v4*>(pool + cell + (u - a.nh - (key ? 0 : a.c.nkv)) * a.c.head_stride) =
+                __builtin_convertvector(z, v4);
         }
     }
 }
 
-hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
-    const int64_t waves = (int64_t)a.n_rows * ((a.nh + a.c.nkv + PA_HEADS - 1) / PA_HEADS);
+template <class E>
+static void append(const PagedAppendArgs& a, hipStream_t s) {
+    const int units = a.nh + 2 * a.c.nkv, per = PA_STEPS * WAVE * 4 / a.c.hd;
     // a launch has fewer than 2^32 threads along x
-    const int64_t groups = (waves + 3) / 4, gx = groups < 1 << 22 ? groups : 1 << 22;
-    const dim3 grid((unsigned)gx, (unsigned)((groups + gx - 1) / gx));
-    if (a.c.type == HY_TYPE_F32)
-        hipLaunchKernelGGL(paged_append_kernel<float>, grid, dim3(256), 0, s, a);
-    else if (a.c.type == HY_TYPE_F16)
-        hipLaunchKernelGGL(paged_append_kernel<_Float16>, grid, dim3(256), 0, s, a);
+    const int64_t n = (int64_t)((a.n_rows + 3) / 4) * ((units + per - 1) / per), gx = n < 1 << 22 ? n : 1 << 22;
+    const dim3 grid((unsigned)gx, (unsigned)((n + gx - 1) / gx));
+    if (a.c.hd == 128)
+        hipLaunchKernelGGL((paged_append_kernel<E, 128>), grid, dim3(256), 0, s, a);
     else
-        hipLaunchKernelGGL(paged_append_kernel<__bf16>, grid, dim3(256), 0, s, a);
+        hipLaunchKernelGGL((paged_append_kernel<E, 64>), grid, dim3(256), 0, s, a);
+}
+
+hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
+    if (a.c.type == HY_TYPE_F32)
+        append<float>(a, s);
+    else if (a.c.type == HY_TYPE_F16)
+        append<_Float16>(a, s);
+    else
+        append<__bf16>(a, s);
     return hipGetLastError();
 }
 
