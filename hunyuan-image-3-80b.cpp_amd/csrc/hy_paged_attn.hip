@@ -440,12 +440,10 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && NT == 2 
 
 // Joins the pieces of the items that are cut, from the jobs the workers left: work group (w, split)
 // takes every splits-th set of rows of worker w's; in it, HD / 4 threads take 4 dims each of
-// a row and every PL-th piece of it, PJ pieces at a time, and the PL groups of a row meet in LDS.
-// Bound by what a work group gets from memory at once, hence rows and pieces spread as far as
-// they go.
-constexpr int PJ = 4;
-
-template <int HD>
+// a row and every pl_n-th piece of it, PJ pieces at a time, and the pl_n groups of a row meet in
+// LDS.  Bound by the partial results' bytes (4 TB/s of them for tiles of 256 rows), for short ones
+// by the latency of job, pieces and result: hence rows and pieces spread as far as they go.
+template <int HD, int PJ>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartShape few, PartShape many, int few_splits,
                                                         int many_splits) {
     __shared__ float meet[6][256];
@@ -530,7 +528,7 @@ constexpr int PF_GROUPS = 512;  // two per CU
 constexpr int PF_WORKERS = PF_GROUPS * PF_WAVES;
 constexpr int PF_MAX_M = 32;
 constexpr int PF_MAX_ROWS = PF_MAX_M;  // rows of a request up to which the stream takes it
-constexpr int PJ_ROWS = 8, PJ_MANY_SPLITS = 32;  // rows of a stream's item per work group; a tile's work groups
+constexpr int PJ_ROWS = 8;  // rows of a stream's item per work group of the join
 
 // which launches a batch takes: workers 0: not that one
 struct PaPlan {
@@ -542,8 +540,9 @@ static PaPlan pa_plan(int n_req, int max_new, int G, int hd) {
     const bool many = rows > PF_MAX_ROWS, few = !many || n_req > 1;
     PaPlan p;
     // Starting an item is worth 16 keys of a full stream, 256 of a many-row tile (20 000 of its 3500
-    // to 6500 cycles per 32 keys); a stretch is 64 keys at least, 128.
-    p.few = part_shape(rows > 16 ? 5 : 4, G, 0, many ? PF_MAX_ROWS : ALL, few ? PF_WORKERS : 0, 16, 64, 0);
+    // to 6500 cycles per 32 keys); a stretch is 32 keys at least (64: one request of
+    // 1000 keys 12.6 us, 32: 10.2), 128.
+    p.few = part_shape(rows > 16 ? 5 : 4, G, 0, many ? PF_MAX_ROWS : ALL, few ? PF_WORKERS : 0, 16, 32, 0);
     const size_t few_ws = part_ws_floats(p.few.workers, p.few.M, hd);
     p.many = part_shape(PM_TILE_SHIFT, G, few ? PF_MAX_ROWS : 0, ALL, many ? PM_WORKERS : 0, 256, 128, few_ws);
     return p;
@@ -575,11 +574,18 @@ hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s)
     }
     if (p.many.workers) launch_paged_many(a, p.many, s);
     const int splits = p.few.M / PJ_ROWS;
-    const dim3 grid(p.few.workers * splits + p.many.workers * PJ_MANY_SPLITS);
-    if (big)
-        hipLaunchKernelGGL(paged_join_kernel<128>, grid, dim3(256), 0, s, a, p.few, p.many, splits, PJ_MANY_SPLITS);
+    const int many_splits = a.c.hd / 4;  // a tile of few pieces: one set of rows per work group
+    const dim3 grid(p.few.workers * splits + p.many.workers * many_splits);
+    // Items of 32 pieces and more: eight pieces at a time (1000 keys, one request: 4.0 us, by fours
+    // 5.6), elsewhere four, of half the registers (32 requests of 24 rows: 11.4, by eights 12.8).
+    const bool long_ = !p.many.workers && a.n_req * a.c.nkv * 32 <= p.few.workers;
+    const auto join = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, p.few, p.many, splits, many_splits);
+    };
+    if (long_)
+        big ? join(paged_join_kernel<128, 8>) : join(paged_join_kernel<64, 8>);
     else
-        hipLaunchKernelGGL(paged_join_kernel<64>, grid, dim3(256), 0, s, a, p.few, p.many, splits, PJ_MANY_SPLITS);
+        big ? join(paged_join_kernel<128, 4>) : join(paged_join_kernel<64, 4>);
     return hipGetLastError();
 }
 

@@ -9,6 +9,8 @@
 // piece, joined afterwards.  A piece [x0, x1) of an item of nominal length W takes the
 // key blocks from x0 B / W to x1 B / W (part_block) of the item's real B.
 #pragma once
+#include <type_traits>
+
 #include "hy_device.hpp"
 #include "hy_paged.hpp"
 
@@ -72,6 +74,27 @@ __device__ __forceinline__ void part_load(const PagedAttnArgs& a, int r, int& st
     kv = min(max(k, 0), a.max_pages << a.c.shift);
 }
 
+// inclusive sum over the lanes: shifts inside 16 lanes, then the rows' last lanes to those behind
+// (vector operations: six steps of shuffles take 1 us)
+__device__ __forceinline__ int64_t part_scan(int64_t v) {
+    const auto step = [&](auto shr) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(shr)::value, 0xF, 0xF, false);
+        const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), decltype(shr)::value, 0xF, 0xF, false);
+        v += (int64_t)((uint64_t)(uint32_t)hi << 32 | lo);
+    };
+    step(std::integral_constant<int, 0x111>{});
+    step(std::integral_constant<int, 0x112>{});
+    step(std::integral_constant<int, 0x114>{});
+    step(std::integral_constant<int, 0x118>{});
+    const auto row_sum = [&](int l) {
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)v, l));
+    };
+    const int64_t r0 = row_sum(15), r1 = r0 + row_sum(31), r2 = r1 + row_sum(47);
+    const int lane = threadIdx.x % WAVE;
+    return v + (lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r1 : r2);
+}
+
 // fills s; returns the sum of all nominal lengths
 template <int THREADS>
 __device__ __forceinline__ int64_t part_sums(const PagedAttnArgs& a, const PartShape& p, PartSums<THREADS>& s) {
@@ -87,12 +110,7 @@ __device__ __forceinline__ int64_t part_sums(const PagedAttnArgs& a, const PartS
             s.kv[r] = kv;
         }
     }
-    int64_t v = mine;
-#pragma unroll
-    for (int d = 1; d < WAVE; d <<= 1) {
-        const int64_t o = __shfl_up(v, d, WAVE);
-        if (tid % WAVE >= d) v += o;
-    }
+    const int64_t v = part_scan(mine);
     if (tid % WAVE == WAVE - 1) s.wave[tid / WAVE] = v;
     __syncthreads();
     int64_t before = 0, total = 0;
