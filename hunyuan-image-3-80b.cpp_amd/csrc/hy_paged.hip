@@ -242,8 +242,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
         v4f_t y;
 #pragma unroll
         for (int p = 0; p < 2; p++) {
-            y[2 * p] = x[s][2 * p] * cs[p] - x[s][2 * p + 1] * sn[p];
-            y[2 * p + 1] = x[s][2 * p] * sn[p] + x[s][2 * p + 1] * cs[p];
+            y[2 * p] = fmaf(x[s][2 * p], cs[p], -(x[s][2 * p + 1] * sn[p]));
+            y[2 * p + 1] = fmaf(x[s][2 * p], sn[p], x[s][2 * p + 1] * cs[p]);
         }
         float ss = (y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]);
         ss += dpp_f<0x128>(ss);  // rotations by 8 .. 1 in 16 lanes

@@ -279,20 +279,30 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && NT == 2 
             for (int c = 0; c < NT; c++)
 #pragma unroll
                 for (int u = 0; u < KT; u++) {
-                    v4f_t acc = v4f_t{};
+                    if constexpr (F32T) {
+                        // four sums (two, where registers are short) of their part of the dims: an f32
+                        // score of one chain of 128 terms is off by twice as much, and each product
+                        // would wait for the last
+                        constexpr int CH = NT == 2 && HD == 128 ? 2 : 4;
+                        v4f_t acc[CH] = {};
 #pragma unroll
-                    for (int n = 0; n < NQ; n++) {
-                        if constexpr (F32T) {
+                        for (int n = 0; n < NQ; n++) {
                             const v4f_t k = __builtin_bit_cast(v4f_t, kx[u][n]);
 #pragma unroll
                             for (int j = 0; j < 4; j++)
-                                acc = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j], qx[c][4 * n + j], acc, 0, 0, 0);
-                        } else {
+                                acc[j % CH] =
+                                    __builtin_amdgcn_mfma_f32_16x16x4f32(k[j], qx[c][4 * n + j], acc[j % CH], 0, 0, 0);
+                        }
+                        s[c][u] = acc[0] + acc[1];
+                        if constexpr (CH == 4) s[c][u] += acc[2] + acc[3];
+                    } else {
+                        v4f_t acc = v4f_t{};
+#pragma unroll
+                        for (int n = 0; n < NQ; n++)
 #pragma unroll
                             for (int q = PC - 1; q >= 0; q--) acc = P::mfma(kx[u][n], qf[c][n][q], acc);
-                        }
+                        s[c][u] = acc;
                     }
-                    s[c][u] = acc;
                 }
             __builtin_amdgcn_sched_barrier(0);
             if (t + 1 < t1) load_k(t + 1);
