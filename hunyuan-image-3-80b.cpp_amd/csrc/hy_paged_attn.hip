@@ -104,17 +104,18 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && NT == 2 
     PartJob job{};
     while (x < x_end) {
         const PartItem it = part_find(a, ps, sums, x);
-        const int64_t p0 = x - it.at, p1 = min(x_end - it.at, it.len);  // this piece
+        const int p0 = (int)(x - it.at), p1 = (int)min(x_end - it.at, (int64_t)it.len);  // this piece
         x = it.at + p1;
 
         // rows of this lane's columns; rows past the last repeat it and are not stored
         const int n_live = min(it.q.n * G - it.tile * ps.M, ps.M);
+        const int rho0 = it.tile * ps.M, tok0 = part_quotient(rho0, G);
         int row[NT], head[NT], end[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            const int rho = it.tile * ps.M + min(16 * t + i, n_live - 1), tok = rho / G;
+            const int rho = rho0 + min(16 * t + i, n_live - 1) - tok0 * G, tok1 = part_div(rho, G), tok = tok0 + tok1;
             row[t] = it.q.start + tok;
-            head[t] = it.g * G + rho - tok * G;
+            head[t] = it.g * G + rho - tok1 * G;
             end[t] = a.seen ? min(a.seen[row[t]], it.q.kv) : it.q.kv - it.q.n + tok + 1;
         }
         int last, first;  // the most and the fewest keys that a row sees
@@ -131,16 +132,15 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && NT == 2 
                 first = min(first, shfl_xor(first, d));
             }
         } else {
-            const int rho = it.tile * ps.M;
-            first = it.q.kv - it.q.n + rho / G + 1;
-            last = max(it.q.kv - it.q.n + (rho + n_live - 1) / G + 1, 0);
+            first = it.q.kv - it.q.n + tok0 + 1;
+            last = max(it.q.kv - it.q.n + tok0 + part_div(rho0 - tok0 * G + n_live - 1, G) + 1, 0);
         }
         last = uniform(last);
         first = uniform(first);
         const int blocks = (last + 31) / 32;
         const int t0 = part_block(p0, it.len, blocks) * (32 / KB), t1 = part_block(p1, it.len, blocks) * (32 / KB);
 
-        job = part_job(ps, it, p0, p1, stretch, worker, n_live);
+        job = part_job(ps, it, p0, p1, stretch, n_live);
         const int slot_id = p0 == 0 && p1 == it.len ? -1 : 2 * worker + (p0 == 0 ? 1 : 0);  // -1: all of it is here
 
         // q: scaled by scale * log2(e) (scores in the base-2 domain); f16: by a power of two that

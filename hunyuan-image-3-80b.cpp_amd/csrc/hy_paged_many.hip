@@ -96,13 +96,14 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
     PartJob job{};
     while (x < x_end) {
         const PartItem it = part_find(a, ps, sums, x);
-        const int64_t p0 = x - it.at, p1 = min(x_end - it.at, it.len);
+        const int p0 = (int)(x - it.at), p1 = (int)min(x_end - it.at, (int64_t)it.len);
         x = it.at + p1;
         const int kv = it.q.kv;
         const int n_live = min(it.q.n * G - it.tile * PM_M, PM_M);
         // this lane's row (the last one again past the end) and the keys it sees
-        const int my = 32 * wv + lr, rho = it.tile * PM_M + min(my, n_live - 1), tok = rho / G;
-        const int row = it.q.start + tok, head = it.g * G + rho - tok * G;
+        const int tok0 = part_quotient(it.tile * PM_M, G);
+        const int my = 32 * wv + lr, rho = it.tile * PM_M + min(my, n_live - 1) - tok0 * G, tok1 = part_div(rho, G);
+        const int tok = tok0 + tok1, row = it.q.start + tok, head = it.g * G + rho - tok1 * G;
         const int end = a.seen ? min(a.seen[row], kv) : kv - it.q.n + tok + 1;
         int last = end, first = end;  // the most and the fewest keys that a row of the wave sees
         if (a.seen) {
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         const int blocks = (tile_last + 31) / 32;
         const int kb0 = part_block(p0, it.len, blocks), kb1 = part_block(p1, it.len, blocks);
         const int my_kb1 = min((last + 31) / 32, kb1);
-        job = part_job(ps, it, p0, p1, stretch, worker, n_live);
+        job = part_job(ps, it, p0, p1, stretch, n_live);
         const int slot_id = p0 == 0 && p1 == it.len ? -1 : 2 * worker + (p0 == 0 ? 1 : 0);  // -1: all of it is here
 
         // ---- loads and stores of blocks

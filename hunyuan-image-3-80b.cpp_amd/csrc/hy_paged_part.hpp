@@ -9,6 +9,8 @@
 // piece, joined afterwards.  A piece [x0, x1) of an item of nominal length W takes the
 // key blocks from x0 B / W to x1 B / W (part_block) of the item's real B.
 #pragma once
+#include <limits.h>
+
 #include <type_traits>
 
 #include "hy_device.hpp"
@@ -41,19 +43,32 @@ struct PartReq {
     int start, n, kv;   // first row, rows (tokens), keys
     int tiles, full;    // tiles of its rows; those whose nominal tokens do not reach past the last
     int64_t base, head; // keys before its first token, and extra; nominal length of a head's tiles
-    // nominal length of tiles 0 .. k - 1
-    __device__ __forceinline__ int64_t upto(int tau, int64_t k) const {
-        const int64_t f = min(k, (int64_t)full);
-        return k * base + (int64_t)tau * (f * (f + 1) / 2) + (k - f) * n;
+    // nominal length of tiles 0 .. k - 1; I: what holds the request's
+    template <class I>
+    __device__ __forceinline__ I upto(int tau, I k) const {
+        const I f = min(k, (I)full);
+        return k * (I)base + (I)tau * (f * (f + 1) / 2) + (k - f) * (I)n;
     }
 };
 
+// n / d for 0 <= n <= 2^20, 0 < d: n + 1/2 keeps 1 / (2 d) from the next whole number, the
+// reciprocal is off by 2^-22 of the quotient
+__device__ __forceinline__ int part_div(int n, int d) { return (int)(((float)n + 0.5f) * __builtin_amdgcn_rcpf((float)d)); }
+// floor(x / n) for 0 <= x, 0 < n, the same for the wave: an estimate in f32, then a step either way
+template <class I>
+__device__ __forceinline__ int part_quotient(I x, I n) {
+    int k = uniform((int)((float)x * __builtin_amdgcn_rcpf((float)n)));
+    while ((I)k * n > x) k--;
+    while (x - (I)k * n >= n) k++;
+    return k;
+}
+
 __device__ __forceinline__ PartReq part_req(const PartShape& p, int start, int n, int kv) {
-    PartReq q{start, n, kv, 0, n / p.tau, max(kv - n, 0) + p.extra, 0};
+    PartReq q{start, n, kv, 0, part_div(n, p.tau), max(kv - n, 0) + p.extra, 0};
     const int64_t rows = (int64_t)n * p.G;
     if (rows > p.rows_lo && rows <= p.rows_hi) q.tiles = (int)((rows + p.M - 1) >> p.m_shift);
     // whole units: where stretches are one unit, short requests share no worker
-    q.head = (q.upto(p.tau, q.tiles) + p.unit - 1) & ~(int64_t)(p.unit - 1);
+    q.head = (q.upto<int64_t>(p.tau, q.tiles) + p.unit - 1) & ~(int64_t)(p.unit - 1);
     return q;
 }
 
@@ -133,9 +148,29 @@ __device__ __forceinline__ int64_t part_stretch(const PartShape& p, int64_t tota
 struct PartItem {
     PartReq q;
     int r, g, tile;
-    int64_t at;   // where the item starts in the row of all items
-    int64_t len;  // its nominal length
+    int64_t at;  // where the item starts in the row of all items
+    int len;     // its nominal length: the keys, at most 2^30, and the tokens
 };
+
+// kv head and tile of place y of a request
+template <class I>
+__device__ __forceinline__ void part_place(const PartShape& p, PartItem& it, I y) {
+    it.g = part_quotient(y, (I)it.q.head);
+    y -= (I)it.q.head * it.g;
+    I t = 0;  // upto(t) <= y < upto(t + 1)
+    if (it.q.tiles > 1) {
+        // tiles of full size: t base + tau t (t + 1) / 2 = y
+        const float b = (float)(I)it.q.base + 0.5f * p.tau, yf = (float)y;
+        t = min(uniform((int)(2.0f * yf * __builtin_amdgcn_rcpf(b + __builtin_amdgcn_sqrtf(b * b + 2.0f * p.tau * yf)))),
+                it.q.tiles - 1);
+        while (t > 0 && it.q.upto(p.tau, t) > y) t--;
+        while (t + 1 < it.q.tiles && it.q.upto<I>(p.tau, t + 1) <= y) t++;  // the last one ends with its head
+    }
+    it.tile = (int)t;
+    const I t0 = it.q.upto(p.tau, t);
+    it.at += it.q.head * it.g + t0;
+    it.len = (int)((t + 1 < it.q.tiles ? it.q.upto<I>(p.tau, t + 1) : (I)it.q.head) - t0);
+}
 
 // the item at place x (0 <= x < total), the same for the whole wave
 template <int THREADS>
@@ -163,39 +198,17 @@ __device__ __forceinline__ PartItem part_find(const PagedAttnArgs& a, const Part
         if (x - it.at < it.q.head * a.c.nkv) break;
         it.at += it.q.head * a.c.nkv;
     }
-    // estimates in f32, then a step either way
-    it.g = uniform((int)((float)(x - it.at) * __builtin_amdgcn_rcpf((float)it.q.head)));
-    while (it.q.head * it.g > x - it.at) it.g--;
-    while (it.q.head * (it.g + 1) <= x - it.at) it.g++;
-    it.at += it.q.head * it.g;
-    const int64_t y = x - it.at;  // upto(tile) <= y < upto(tile + 1)
-    int t = 0;
-    if (it.q.tiles > 1) {
-        // tiles of full size: t base + tau t (t + 1) / 2 = y
-        const float b = (float)it.q.base + 0.5f * p.tau, yf = (float)y;
-        t = min(uniform((int)(2.0f * yf * __builtin_amdgcn_rcpf(b + __builtin_amdgcn_sqrtf(b * b + 2.0f * p.tau * yf)))),
-                it.q.tiles - 1);
-        while (t > 0 && it.q.upto(p.tau, t) > y) t--;
-        while (t + 1 < it.q.tiles && it.q.upto(p.tau, t + 1) <= y) t++;  // the last one ends with its head
-    }
-    it.tile = t;
-    const int64_t t0 = it.q.upto(p.tau, t);
-    it.at += t0;
-    it.len = (t + 1 < it.q.tiles ? it.q.upto(p.tau, t + 1) : it.q.head) - t0;
+    const int64_t y = x - it.at;
+    if (it.q.head * a.c.nkv < 1ll << 31)  // 32 bits: a third of the instructions
+        part_place<int>(p, it, (int)y);
+    else
+        part_place<int64_t>(p, it, y);
     return it;
-}
-
-// floor(x / n) for 0 <= x, 0 < n
-__device__ __forceinline__ int part_quotient(int64_t x, int64_t n) {
-    int k = uniform((int)((float)x * __builtin_amdgcn_rcpf((float)n)));
-    while ((int64_t)k * n > x) k--;
-    while ((int64_t)(k + 1) * n <= x) k++;
-    return k;
 }
 
 // the block where a piece ending at place y of an item of nominal length len ends: rounded, but
 // growing with y and the same for both who share the cut
-__device__ __forceinline__ int part_block(int64_t y, int64_t len, int blocks) {
+__device__ __forceinline__ int part_block(int y, int len, int blocks) {
     return y >= len ? blocks : min(uniform((int)((float)y * ((float)blocks / (float)len))), blocks);
 }
 
@@ -258,11 +271,12 @@ __host__ __device__ __forceinline__ size_t part_ws_floats(int workers, int M, in
 __device__ __forceinline__ PartJob* part_jobs(const PagedAttnArgs& a, const PartShape& p, int hd) {
     return reinterpret_cast<PartJob*>(a.ws + p.ws + 2 * (size_t)p.workers * part_slot_floats(p.M, hd));
 }
-// the job that a piece [p0, p1) of an item makes of worker w
-__device__ __forceinline__ PartJob part_job(const PartShape& p, const PartItem& it, int64_t p0, int64_t p1, int64_t stretch,
-                                            int w, int n_live) {
+// the job that a piece [p0, p1) of an item makes of its worker
+__device__ __forceinline__ PartJob part_job(const PartShape& p, const PartItem& it, int p0, int p1, int64_t stretch,
+                                            int n_live) {
     PartJob j{0, n_live, it.q.start, it.tile * p.M, it.g, {}};
-    if (p0 == 0 && p1 < it.len) j.n_piece = part_quotient(it.at + it.len - 1, stretch) - w + 1;
+    if (p0 == 0 && p1 < it.len)  // the other pieces are a stretch each, the last one's rest aside
+        j.n_piece = 2 + part_quotient(it.len - 1 - p1, (int)min(stretch, (int64_t)INT_MAX));
     return j;
 }
 
