@@ -12,8 +12,8 @@ namespace hy {
 // ---------------------------------------------------------------- tables and slots
 // One work group, a request (or PER consecutive ones) per thread: sums over requests (rows, pages
 // given back, pages taken) by scans, then the pages and the rows one per thread, whose request a
-// search in LDS finds.  All of it is latency: 8 requests 6 us, 1024 requests 11.  Rows beyond
-// PL_ROWS go to a second launch over the whole chip (16 000 rows in one work group: 40 us).
+// search in LDS finds.  All of it is latency: 8 requests 3.7 us, 1024 requests 7.8.  Rows beyond
+// PL_ROWS go to a second launch over the whole chip (4.1 us; 16 000 rows in one work group: 40).
 // Sums saturate at PL_CAP, which is past every bound that they are compared with.
 constexpr int PL_CAP = (1 << 30) - 1, PL_ROWS = 4096;
 
@@ -191,7 +191,7 @@ hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t s) {
 // (16 bytes) each, and all loads of a wave go out before anything else.  An angle is kept as a
 // fraction of a turn in 64 bits, position times turns per position minus its whole part, so a
 // far position costs no accuracy; sine and cosine of the rest are f32.
-// Bound by memory: 4096 rows of 48 heads of 128 (205 MB) 33 us in caches, 50 from memory (PENDING);
+// Bound by memory: 4096 rows of 48 heads of 128 (205 MB) 33 us in caches, 40 from memory (5.2 TB/s);
 // 5 rows 4.4 us, all of it latency.
 constexpr int PA_STEPS = 4;
 

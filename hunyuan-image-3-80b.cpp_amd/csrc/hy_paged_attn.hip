@@ -12,12 +12,16 @@
 //  * softmax statistics: one query row per lane, joined over the four g.
 // f32 accuracy from 16-bit operands: q and the probabilities are split into pieces that the
 // matrix cores multiply exactly -- a f16 cache: two f16 pieces (22 bits, q scaled per row by a
-// power of two, p by 2^14); a bf16 cache: three bf16 pieces (24 bits) -- while K and V go in as
-// they are.  f32 caches use the fp32 MFMAs.
+// power of two, weights by 2^6); a bf16 cache: three bf16 pieces (24 bits) -- while K and V go in
+// as they are.  f32 caches use the fp32 MFMAs.
 // Keys that a row does not see get weight 0, but 0 times an infinity or NaN in their V would
 // still be felt.  Keys that no row sees (a page's unwritten end) have their V zeroed; where
 // some rows do not see a key, V is looked at, and if it is not finite the piece is computed again
 // key by key (slow_rows).
+// Bound by the bytes of K and V: 64 single tokens over bf16 caches of up to 8000 keys (1.24 GB)
+// 225 us, 5.5 TB/s; 32 requests of 6 tokens over f16 caches of up to 2900 keys (255 MB) 60 us, of
+// which some 10 are the start (7000 cycles from launch to the first loads) and the end; one token
+// over 1000 f32 keys 10 us, all of it that latency.
 #include "hy_device.hpp"
 #include "hy_lds.hpp"
 #include "hy_paged.hpp"

@@ -16,9 +16,15 @@
 // Blocks of 32 keys: every thread loads its share of a block of K and V one block ahead,
 // splits it and stores the pieces to LDS, K as it is and V transposed, both in MFMA operand
 // order.  Scores are computed transposed, S^T = K Q^T, so a query's statistics stay in its
-// lane pair and its weights are the operand of O^T += V^T W^T as they lie.  The two waves of
-// a SIMD run half a block apart: one multiplies the last block's weights with V while the other
-// is at this block's scores, so one's softmax runs under the other's products.
+// lane pair and its weights are the operand of O^T += V^T W^T as they lie.
+//
+// Bound by instruction issue and the power it draws: a SIMD's two waves take, per block and head_dim
+// 128 of a bf16 cache, 2100 cycles for the 64 products and 2700 for the vector operations (half
+// of them the softmax), of 4700 measured; matrix and vector work of different waves do not overlap
+// here (running the waves half a block apart changed nothing), and the clock falls to 1.6 GHz under
+// it.  2048 rows of 32 heads behind 8192 keys, f32: 1.09 ms, 283 TFLOP/s of attention and three times
+// that of f16 products (a large f16 matrix product reaches 1110); head_dim 64, five prompts of up
+// to 1500 tokens, f16: 67 us, of which 20 000 cycles (10 us) per piece go to its first loads.
 //
 // Keys that no row sees are stored as zeros and masked; where V holds an infinity or NaN, which 0
 // times a weight would not keep out, the piece is computed again key by key (slow_rows).
@@ -67,7 +73,7 @@ struct PmLds {
     // V: per piece 4 chunks (2 c + h: keys 16 c + 4 h .. + 3 and 16 c + 8 + 4 h .. + 3) of HD dims
     // x 16 bytes, even dims before odd ones
     static constexpr int CHUNK_V = HD * 16, PIECE_V = 4 * CHUNK_V, BUF_V = KP * PIECE_V;
-    static constexpr int OFF_V = 2 * BUF_K, BYTES = OFF_V + 3 * BUF_V;
+    static constexpr int OFF_V = 2 * BUF_K, BYTES = OFF_V + 2 * BUF_V;
 };
 
 template <class E, int HD>
@@ -79,12 +85,12 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
     constexpr int KL = HD / 8;  // threads per key of K
     constexpr int RING = KP == 2 ? 2 : 3;  // operands read ahead of the products (registers allowing)
     __shared__ __attribute__((aligned(1024))) uint8_t lds[L::BYTES];
-    __shared__ __attribute__((aligned(16))) float k_fac[3][32], v_exp[3][32], v_inv[3][32];
+    __shared__ __attribute__((aligned(16))) float k_fac[2][32], v_exp[2][32], v_inv[2][32];
     __shared__ int odd_s;  // an infinity or NaN in this piece's V
     __shared__ int last_s[PM_WAVES];
     __shared__ PartSums<PM_THREADS> sums;
     const int tid = threadIdx.x, lane = tid % WAVE, lr = lane % 32, h = lane / 32;
-    const int wv = __builtin_amdgcn_readfirstlane(tid / WAVE), lag = wv / 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const int64_t total = part_sums(a, ps, sums);
     const int64_t stretch = part_stretch(ps, total);
     // neighbouring stretches, which share kv heads, on one XCD (work groups go round the XCDs)
@@ -193,9 +199,9 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 tab2 = entries(seg + 1);
             }
         };
-        // block kb, r = kb % 3
-        auto put_k = [&](int kb, int r) {
-            uint8_t* const d = k_dst + (kb & 1) * L::BUF_K;
+        // block kb, r = kb % 2
+        auto put_k = [&](int r) {
+            uint8_t* const d = k_dst + r * L::BUF_K;
             if constexpr (!SCALED) {
                 if (k_mine) *reinterpret_cast<v4i_t*>(d) = kx[0];
             } else {
@@ -369,7 +375,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         v4i_t pf[2][2];  // the weights' pieces, keys 16 c .. in step c
         // scores of block kb and its weights' pieces
         auto scores = [&](int kb, int r) {
-            const uint8_t* const kb_ = lds + (kb & 1) * L::BUF_K + h * L::CHUNK_K + lr * 16;
+            const uint8_t* const kb_ = lds + r * L::BUF_K + h * L::CHUNK_K + lr * 16;
             v4i_t kf[RING][KP];
             auto read = [&](int c) {
 #pragma unroll
@@ -473,25 +479,20 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             }
         };
 
-        int r = kb0 % 3, before = 0;  // kb % 3, (kb - 1) % 3
         if (kb0 < kb1) {
-            put_k(kb0, r);
+            put_k(kb0 & 1);
             load_k(kb0 + 1);
         }
         for (int kb = kb0; kb < kb1; kb++) {
-            const int next = r == 2 ? 0 : r + 1;
+            const int r = kb & 1;
             put_v(kb, r);
             load_v(kb + 1);
-            __syncthreads();  // block kb is in LDS; K of block kb - 1 and V of kb - 2 are read out
-            if (lag == 1 && kb > kb0 && kb - 1 < my_kb1) values(before);
+            __syncthreads();  // block kb is in LDS, block kb - 1 read out
             if (kb < my_kb1) scores(kb, r);
-            if (kb + 1 < kb1) put_k(kb + 1, next);
+            if (kb + 1 < kb1) put_k(r ^ 1);
             load_k(kb + 2);
-            if (lag == 0 && kb < my_kb1) values(r);
-            before = r;
-            r = next;
+            if (kb < my_kb1) values(r);
         }
-        if (lag == 1 && my_kb1 == kb1 && kb0 < kb1) values(before);
         l_run = fadd_half(l_run);
 
         // l carries the weights' factor too, scaled values have one of their own
