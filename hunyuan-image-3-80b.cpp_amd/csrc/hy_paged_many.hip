@@ -149,15 +149,24 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             const int e = trow[p];
             return e >= 0 && e < a.c.n_pages;
         };
-        auto entries = [&](int seg) {
-            const int p = seg * 64 + lane;
-            const int e = p < n_tab ? trow[p] : 0;
-            const bool ok = e >= 0 && e < a.c.n_pages;
-            bad |= (bool)__any(!ok);
-            return ok ? e * a.c.page_stride : 0;
+        auto entry = [&](int seg) { return trow[min(seg * 64 + lane, max(n_tab - 1, 0))]; };
+        auto page_at = [&](int seg, int e) {
+            const bool there = seg * 64 + lane < n_tab, ok = e >= 0 && e < a.c.n_pages;
+            bad |= (bool)__any(there && !ok);
+            return there && ok ? e * a.c.page_stride : 0;
         };
         int seg = (kb0 * 32) >> (a.c.shift + 6);
-        int64_t tab = entries(seg), tab2 = entries(seg + 1);
+        const int e1 = entry(seg), e2 = entry(seg + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        // q's dims 16 c + 8 h .. + 7: on their way before the pages are known
+        const float* const qp = a.q + ((int64_t)row * a.nh + head) * HD + 8 * h;
+        v4f_t q[NC][2];
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) q[c][u] = *reinterpret_cast<const v4f_t*>(qp + 16 * c + 4 * u);
+        __builtin_amdgcn_sched_barrier(0);
+        int64_t tab = page_at(seg, e1), tab2 = page_at(seg + 1, e2);
         auto lane64 = [](int64_t v, int l) {
             return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) |
                              (uint32_t)__builtin_amdgcn_readlane((int)v, l));
@@ -196,7 +205,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             if (s != seg) {
                 seg = s;
                 tab = tab2;
-                tab2 = entries(seg + 1);
+                tab2 = page_at(seg + 1, entry(seg + 1));
             }
         };
         // block kb, r = kb % 2
@@ -333,22 +342,13 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             load_v(kb0);
         }
 
-        // ---- q: pieces of dims 16 c + 8 h .. + 7, times scale * log2(e) (scores in the base-2
-        // domain) and the row's power of two
+        // ---- q: its pieces, times scale * log2(e) (scores in the base-2 domain) and the row's power
+        // of two
         v4i_t qf[NC][2];
         float unscale;
         {
             const float qscale = a.scale * 1.4426950408889634f;
-            const float* const qp = a.q + ((int64_t)row * a.nh + head) * HD + 8 * h;
-            v4f_t q[NC][2];
             uint32_t big = 0;
-#pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    q[c][u] = *reinterpret_cast<const v4f_t*>(qp + 16 * c + 4 * u);
-                }
-            __builtin_amdgcn_sched_barrier(0);  // all of them in flight
 #pragma unroll
             for (int c = 0; c < NC; c++)
 #pragma unroll
