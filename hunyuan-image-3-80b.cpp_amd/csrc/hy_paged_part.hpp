@@ -2,11 +2,12 @@
 //
 // A request's rows (token x query head of one kv head, token-major) fall into tiles of M; an
 // item is a (request, kv head, tile) and its nominal length the keys that its last token sees
-// if causal, plus what starting an item costs.  All items of a batch in a row (requests, then kv heads, then tiles) are cut into
-// equal stretches, one per worker: however ragged the lengths, every worker has the same share.
-// Lengths are in device memory, so every work group sums them itself (part_sums).  An item
-// inside one worker's stretch is written by it; one that is cut leaves a partial result per
-// piece, joined afterwards.  A piece [x0, x1) of an item of nominal length W takes the
+// if causal, plus what starting an item costs.  All items of a batch in a row (requests, then kv
+// heads, then tiles) are cut into equal stretches, one per worker: however ragged the lengths,
+// every worker has the same share.  Lengths are in device memory, so every work group sums them
+// itself (part_sums).  An item inside one worker's stretch is written by it; one that is cut leaves
+// a partial result per piece, joined afterwards (joining the pieces of a work group's waves in LDS
+// first was tried: 32 requests of 24 rows 72.5 -> 70.4 us, one of 4 rows 14.1 -> 14.9).  A piece [x0, x1) of an item of nominal length W takes the
 // key blocks from x0 B / W to x1 B / W (part_block) of the item's real B.
 #pragma once
 #include <limits.h>
