@@ -2,7 +2,8 @@
 // (hy_paged_attention): out = sum_j softmax_j(scale q . k_j) v_j over the keys a row sees.
 //
 // paged_few_kernel: requests of few rows (single tokens, drafts).  A stream over K and V: one
-// wave works for itself on 16 NT rows (token x query head of a kv head) and goes over its keys
+// wave works for itself on 16 NT rows (token x query head of a kv head; 32 over 16-bit caches:
+// hy_paged_wide.hip) and goes over its keys
 // 32 (f32: 16) at a time, straight from memory into the operands of 16 x 16 MFMAs, without LDS
 // and barriers:
 //  * S^T = K Q^T: lane l = 16 g + i holds key i's dims, 16 bytes at a time;
@@ -19,9 +20,8 @@
 // some rows do not see a key, V is looked at, and if it is not finite the piece is computed again
 // key by key (slow_rows).
 // Bound by the bytes of K and V: 64 single tokens over bf16 caches of up to 8000 keys (1.24 GB)
-// 225 us, 5.5 TB/s; 32 requests of 6 tokens over f16 caches of up to 2900 keys (255 MB) 60 us, of
-// which some 10 are the start (7000 cycles from launch to the first loads) and the end; one token
-// over 1000 f32 keys 10 us, all of it that latency.
+// 225 us, 5.5 TB/s; one token over 1000 f32 keys 10 us, all of it latency (7000 cycles from launch
+// to the first loads).
 #include "hy_device.hpp"
 #include "hy_lds.hpp"
 #include "hy_paged.hpp"
@@ -30,60 +30,12 @@
 
 namespace hy {
 
-// the operand kinds of a cache type
-template <class E>
-struct PaType;
-template <>
-struct PaType<_Float16> {
-    static constexpr int PIECES = 2;
-    static __device__ __forceinline__ v4f_t mfma(v4i_t a, v4i_t b, v4f_t c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h16_t, a), __builtin_bit_cast(v8h16_t, b), c,
-                                                      0, 0, 0);
-    }
-    // two floats -> their pieces, packed
-    static __device__ __forceinline__ void split(float a, float b, uint32_t (&p)[2]) {
-        split_f16(a, b, p[0], p[1]);
-    }
-    static __device__ __forceinline__ bool odd(uint32_t w) {  // an infinity or NaN among the two
-        return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
-    }
-};
-template <>
-struct PaType<__bf16> {
-    static constexpr int PIECES = 3;
-    static __device__ __forceinline__ v4f_t mfma(v4i_t a, v4i_t b, v4f_t c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf_t, a), __builtin_bit_cast(v8bf_t, b), c,
-                                                       0, 0, 0);
-    }
-    static __device__ __forceinline__ void split(float a, float b, uint32_t (&p)[3]) {
-        uint32_t lost = 0;
-        const Split2 s = split2(a, b, lost);
-#pragma unroll
-        for (int i = 0; i < 3; i++) p[i] = s.p[i];
-    }
-    static __device__ __forceinline__ bool odd(uint32_t w) {
-        return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
-    }
-};
-template <>
-struct PaType<float> {
-    static constexpr int PIECES = 1;
-    static __device__ __forceinline__ bool odd(uint32_t w) { return (w & 0x7F800000u) == 0x7F800000u; }
-};
-
 // over lanes i, 16 + i, 32 + i, 48 + i
 __device__ __forceinline__ float group_max(float v) { return fmax_half(fmax_row(v)); }
 __device__ __forceinline__ float group_sum(float v) { return fadd_half(fadd_row(v)); }
 
-constexpr int PF_WAVES = 4;
-// The running maximum that weights are relative to is left behind while a block's scores do not
-// pass it by more than PA_LAG (base 2): weights are up to 2^PA_LAG, and the sums are rescaled
-// once or twice per row instead of at every new maximum.
-constexpr float PA_LAG = 8.0f;
-constexpr float PF_PSCALE = 64.0f;  // of the weights' f16 pieces: below 2^14 with PA_LAG
-
 template <class E, int HD, int NT>
-__global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && NT == 2 && HD == 128 ? 1 : 2) void paged_few_kernel(PagedAttnArgs a, PartShape ps) {
+__global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttnArgs a, PartShape ps) {
     using P = PaType<E>;
     constexpr bool F32T = sizeof(E) == 4, F16T = std::is_same<E, _Float16>::value;
     constexpr int KB = F32T ? 16 : 32;       // keys per turn
@@ -538,8 +490,6 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartSh
     }
 }
 
-constexpr int PF_GROUPS = 512;  // two per CU
-constexpr int PF_WORKERS = PF_GROUPS * PF_WAVES;
 constexpr int PF_MAX_M = 32;
 constexpr int PF_MAX_ROWS = PF_MAX_M;  // rows of a request up to which the stream takes it
 constexpr int PJ_ROWS = 8;  // rows of a stream's item per work group of the join
@@ -569,17 +519,22 @@ size_t paged_attn_ws_bytes(int n_req, int max_new, int G, int hd) {
 
 template <class E, int HD>
 static void launch_few(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s) {
-    if (ps.M == 32)
-        hipLaunchKernelGGL((paged_few_kernel<E, HD, 2>), dim3(PF_GROUPS), dim3(WAVE * PF_WAVES), 0, s, a, ps);
-    else
-        hipLaunchKernelGGL((paged_few_kernel<E, HD, 1>), dim3(PF_GROUPS), dim3(WAVE * PF_WAVES), 0, s, a, ps);
+    if constexpr (sizeof(E) == 4) {
+        if (ps.M == 32) {
+            hipLaunchKernelGGL((paged_few_kernel<E, HD, 2>), dim3(PF_GROUPS), dim3(WAVE * PF_WAVES), 0, s, a, ps);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((paged_few_kernel<E, HD, 1>), dim3(PF_GROUPS), dim3(WAVE * PF_WAVES), 0, s, a, ps);
 }
 
 hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s) {
     const PaPlan p = pa_plan(a.n_req, max_new, a.nh / a.c.nkv, a.c.hd);
     const bool big = a.c.hd == 128;
     if (p.few.workers) {
-        if (a.c.type == HY_TYPE_F32)
+        if (a.c.type != HY_TYPE_F32 && p.few.M == 32)
+            launch_paged_wide(a, p.few, s);
+        else if (a.c.type == HY_TYPE_F32)
             big ? launch_few<float, 128>(a, p.few, s) : launch_few<float, 64>(a, p.few, s);
         else if (a.c.type == HY_TYPE_F16)
             big ? launch_few<_Float16, 128>(a, p.few, s) : launch_few<_Float16, 64>(a, p.few, s);

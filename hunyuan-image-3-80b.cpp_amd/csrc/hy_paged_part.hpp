@@ -281,6 +281,15 @@ __device__ __forceinline__ PartJob part_job(const PartShape& p, const PartItem& 
     return j;
 }
 
+// requests of few rows: PF_WORKERS waves, each for itself (hy_paged_attn.hip, hy_paged_wide.hip)
+constexpr int PF_WAVES = 4, PF_GROUPS = 512, PF_WORKERS = PF_GROUPS * PF_WAVES;  // two work groups per CU
+// The running maximum that weights are relative to is left behind while a block's scores do not
+// pass it by more than PA_LAG (base 2): weights are up to 2^PA_LAG, and the sums are rescaled
+// once or twice per row instead of at every new maximum.
+constexpr float PA_LAG = 8.0f;
+constexpr float PF_PSCALE = 64.0f;  // of the weights' f16 pieces: below 2^14 with PA_LAG
+void launch_paged_wide(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s);
+
 // requests of many rows: tiles of PM_TILE rows, PM_WORKERS work groups (hy_paged_many.hip)
 constexpr int PM_TILE_SHIFT = 8, PM_TILE = 1 << PM_TILE_SHIFT, PM_WORKERS = 256;
 void launch_paged_many(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s);

@@ -2,6 +2,7 @@
 // attention's kernels: x = hi + lo, each rounded to nearest, 2^-24 of x left out as long as the
 // pieces are normal numbers (which the callers' powers of two see to).
 #pragma once
+#include "hy_lds.hpp"
 #include "hy_split.hpp"
 
 namespace hy {
@@ -53,5 +54,51 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32
     asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(lo) : "v"(hi), "v"(a));
     asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(lo) : "v"(hi), "v"(b));
 }
+
+// the operand kinds of a cache type
+template <class E>
+struct PaType;
+template <>
+struct PaType<_Float16> {
+    static constexpr int PIECES = 2;
+    static __device__ __forceinline__ v4f_t mfma(v4i_t a, v4i_t b, v4f_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h16_t, a), __builtin_bit_cast(v8h16_t, b), c,
+                                                      0, 0, 0);
+    }
+    static __device__ __forceinline__ v16f_t mfma(v4i_t a, v4i_t b, v16f_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h16_t, a), __builtin_bit_cast(v8h16_t, b), c,
+                                                      0, 0, 0);
+    }
+    // two floats -> their pieces, packed
+    static __device__ __forceinline__ void split(float a, float b, uint32_t (&p)[2]) {
+        split_f16(a, b, p[0], p[1]);
+    }
+    static __device__ __forceinline__ bool odd(uint32_t w) {  // an infinity or NaN among the two
+        return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
+    }
+};
+template <>
+struct PaType<__bf16> {
+    static constexpr int PIECES = 3;
+    static __device__ __forceinline__ v4f_t mfma(v4i_t a, v4i_t b, v4f_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf_t, a), __builtin_bit_cast(v8bf_t, b), c,
+                                                       0, 0, 0);
+    }
+    static __device__ __forceinline__ v16f_t mfma(v4i_t a, v4i_t b, v16f_t c) { return mfma_bf16(a, b, c); }
+    static __device__ __forceinline__ void split(float a, float b, uint32_t (&p)[3]) {
+        uint32_t lost = 0;
+        const Split2 s = split2(a, b, lost);
+#pragma unroll
+        for (int i = 0; i < 3; i++) p[i] = s.p[i];
+    }
+    static __device__ __forceinline__ bool odd(uint32_t w) {
+        return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+    }
+};
+template <>
+struct PaType<float> {
+    static constexpr int PIECES = 1;
+    static __device__ __forceinline__ bool odd(uint32_t w) { return (w & 0x7F800000u) == 0x7F800000u; }
+};
 
 }  // namespace hy
