@@ -69,7 +69,7 @@ struct PagedAttnArgs {
     float* ws;
 };
 hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s);
-size_t paged_attn_ws_bytes(int n_req, int max_new, int G, int hd);
+size_t paged_attn_ws_bytes(int type, int n_req, int max_new, int G, int hd);
 
 struct VerifyArgs {
     const float* logits;

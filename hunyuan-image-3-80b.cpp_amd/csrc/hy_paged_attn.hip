@@ -490,30 +490,47 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartSh
     }
 }
 
-constexpr int PF_MAX_M = 32;
-constexpr int PF_MAX_ROWS = PF_MAX_M;  // rows of a request up to which the stream takes it
 constexpr int PJ_ROWS = 8;  // rows of a stream's item per work group of the join
 
 // which launches a batch takes: workers 0: not that one
 struct PaPlan {
     PartShape few, many;
 };
-static PaPlan pa_plan(int n_req, int max_new, int G, int hd) {
+constexpr int PF_ROWS = 32;
+// Rows of the largest request up to which the streams take a whole batch; past it they take the
+// requests of PF_ROWS rows at most (f16, 14 requests of up to 744 rows: 50, all up to 128 rows 62).
+// They read K and V once per 32 rows (from caches, past the first), but start quickly and need no
+// second launch; the tiles of 256 rows do more per key where there are rows enough.  Measured with
+// both, us:
+//  * head_dim 64, 16 bits: 4 requests of 1024 rows 31 by tiles, 25 by the stream; 6 requests of 2048
+//    behind 1000 keys 54, 48, of 4096 78, 85.  f32: 6 of 512 53, 42, 2 of 1024 behind 6000 keys 77, 119;
+//  * head_dim 128, more than two requests: f16, 16 of 128 behind 8000 keys 139, 138, of 256 203, 290;
+//    bf16, of 256 227, 214, 6 of 384 behind 1000 58, 59; f32, 8 of 64 behind 1000 60, 47, 16 of 96
+//    behind 8000 237, 319;
+//  * one or two requests of head_dim 128 are few items, which the stream cuts into more pieces than
+//    pay: 2 of 64 behind 6000, f16 42, 62.
+static int pf_max_rows(int type, int n_req, int hd) {
+    if (hd == 64) return type == HY_TYPE_F32 ? 512 : 2048;
+    if (n_req <= 2) return PF_ROWS;
+    return type == HY_TYPE_F32 ? 64 : type == HY_TYPE_F16 ? 128 : 256;
+}
+
+static PaPlan pa_plan(int type, int n_req, int max_new, int G, int hd) {
     const int64_t rows = (int64_t)max_new * G;  // of one request, at most
     constexpr int64_t ALL = (int64_t)1 << 62;
-    const bool many = rows > PF_MAX_ROWS, few = !many || n_req > 1;
+    const bool many = rows > pf_max_rows(type, n_req, hd), few = !many || n_req > 1;
     PaPlan p;
     // Starting an item is worth 16 keys of a full stream, 256 of a many-row tile (20 000 of its 3500
     // to 6500 cycles per 32 keys); a stretch is 32 keys at least (64: one request of
     // 1000 keys 12.6 us, 32: 10.2), 128.
-    p.few = part_shape(rows > 16 ? 5 : 4, G, 0, many ? PF_MAX_ROWS : ALL, few ? PF_WORKERS : 0, 16, 32, 0);
+    p.few = part_shape(rows > 16 ? 5 : 4, G, 0, many ? PF_ROWS : ALL, few ? PF_WORKERS : 0, 16, 32, 0);
     const size_t few_ws = part_ws_floats(p.few.workers, p.few.M, hd);
-    p.many = part_shape(PM_TILE_SHIFT, G, few ? PF_MAX_ROWS : 0, ALL, many ? PM_WORKERS : 0, 256, 128, few_ws);
+    p.many = part_shape(PM_TILE_SHIFT, G, few ? PF_ROWS : 0, ALL, many ? PM_WORKERS : 0, 256, 128, few_ws);
     return p;
 }
 
-size_t paged_attn_ws_bytes(int n_req, int max_new, int G, int hd) {
-    const PaPlan p = pa_plan(n_req, max_new, G, hd);
+size_t paged_attn_ws_bytes(int type, int n_req, int max_new, int G, int hd) {
+    const PaPlan p = pa_plan(type, n_req, max_new, G, hd);
     return 4 * (p.many.ws + part_ws_floats(p.many.workers, PM_TILE, hd));
 }
 
@@ -529,7 +546,7 @@ static void launch_few(const PagedAttnArgs& a, const PartShape& ps, hipStream_t 
 }
 
 hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s) {
-    const PaPlan p = pa_plan(a.n_req, max_new, a.nh / a.c.nkv, a.c.hd);
+    const PaPlan p = pa_plan(a.c.type, a.n_req, max_new, a.nh / a.c.nkv, a.c.hd);
     const bool big = a.c.hd == 128;
     if (p.few.workers) {
         if (a.c.type != HY_TYPE_F32 && p.few.M == 32)

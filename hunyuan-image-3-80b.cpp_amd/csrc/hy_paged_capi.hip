@@ -142,7 +142,7 @@ int paged_append(const float* qkv, uint32_t n_rows, uint32_t n_heads, const Page
 }
 
 size_t paged_batch_ws(const hy_paged_batch* b, uint32_t n_heads, const PagedView& c) {
-    return paged_attn_ws_bytes((int)b->n_req, (int)(b->max_new < b->n_rows ? b->max_new : b->n_rows),
+    return paged_attn_ws_bytes(c.type, (int)b->n_req, (int)(b->max_new < b->n_rows ? b->max_new : b->n_rows),
                                (int)n_heads / c.nkv, c.hd);
 }
 

@@ -1055,3 +1055,36 @@ def test_attention_unwritten_page_ends_take_no_longer_path(gpu):
             outs.append(attend(gpu, q, pool, q_start, kv_len, table, 0.1))
         np.testing.assert_array_equal(outs[0], outs[1])
         np.testing.assert_array_equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("wtype", [F32, F16, BF16])
+@pytest.mark.parametrize("nh,nkv,page,order,trash", [(8, 2, 8, "head", 0.0), (10, 2, 64, "token", np.nan),
+                                                     (16, 1, 32, "head", np.inf)])
+def test_attention_long_chunks_of_small_heads(gpu, wtype, nh, nkv, page, order, trash):
+    """More rows than the streams take for head_dim 64, beside requests of few rows."""
+    rng = np.random.default_rng(63 + nh)
+    n = 2100 // (nh // nkv) + 5
+    lens = [(n + 61, n), (40, 1), (90, 3), (0, 0), (200, 33)]
+    pool, table, q_start, kv_len = make_batch(rng, lens, page, nkv, 64, wtype, order, fill=trash)
+    q = rng.standard_normal((q_start[-1] + 2, nh, 64)).astype(np.float32)
+    args = (q, pool, q_start, kv_len, table, 0.125)
+    check_attention(attend(gpu, *args), *args)
+    seen = np.minimum(rng.integers(0, n + 90, q_start[-1] + 2), np.repeat(kv_len, np.diff(q_start)).max()).astype(np.int32)
+    seen[5:40] = 0
+    check_attention(attend(gpu, *args, seen=seen), *args, seen)
+
+
+@pytest.mark.parametrize("wtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_rows_around_the_streams_limits(gpu, wtype, hd):
+    """Row counts on both sides of every choice of kernel and tile: the same sums within rounding."""
+    rng = np.random.default_rng(64)
+    nh, nkv = 8, 2
+    for news in ((4, 4, 4), (5, 1, 3), (8, 8, 2), (9, 8, 2), (16, 2, 2), (17, 16, 1), (32, 31, 2), (33, 9, 8), (64, 20, 1),
+                 (65, 64, 3), (128, 7, 1), (129, 8, 9)):
+        lens = [(n + int(rng.integers(0, 80)), n) for n in news]
+        for part in (lens, lens[:2], lens[:1]):
+            pool, table, q_start, kv_len = make_batch(rng, part, 16, nkv, hd, wtype)
+            q = rng.standard_normal((q_start[-1], nh, hd)).astype(np.float32)
+            args = (q, pool, q_start, kv_len, table, hd ** -0.5)
+            check_attention(attend(gpu, *args), *args)
