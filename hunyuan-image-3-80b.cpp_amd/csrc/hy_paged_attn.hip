@@ -193,7 +193,8 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
             for (int u = 0; u < KT; u++) {
                 const int key = t * KB + 16 * u + 4 * g4;
                 vpage[u] = page_of(key);
-                const E* const vp = vbase + max(vpage[u], 0) * a.c.page_stride + (key & pmask) * a.c.token_stride + VD * i;
+                const E* const vp =
+                    vbase + max(vpage[u], 0) * a.c.page_stride + (key & pmask) * a.c.token_stride + VD * i;
 #pragma unroll
                 for (int v = 0; v < 4; v++)
 #pragma unroll
@@ -367,8 +368,11 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
 #pragma unroll
             for (int c = 0; c < NT; c++)
                 slow_rows<E, HD, 4>(
-                    a, trow, it.q.kv, t0 * KB, t1 * KB, end[c], a.q + ((int64_t)row[c] * a.nh + head[c]) * HD, kbase, vbase,
-                    [&](int n) { return F32T ? 64 * (n / 16) + 4 * (4 * g4 + n % 4) + n / 4 % 4 : VD * (4 * g4 + n % 4) + n / 4; },
+                    a, trow, it.q.kv, t0 * KB, t1 * KB, end[c], a.q + ((int64_t)row[c] * a.nh + head[c]) * HD, kbase,
+                    vbase,
+                    [&](int n) {
+                        return F32T ? 64 * (n / 16) + 4 * (4 * g4 + n % 4) + n / 4 % 4 : VD * (4 * g4 + n % 4) + n / 4;
+                    },
                     [&](int n, float v) { o[c][n / 4][n % 4] = v; }, [&](int n) { return o[c][n / 4][n % 4]; }, m_run[c],
                     l_run[c]);
         }
@@ -484,8 +488,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartSh
         if (pl == 0 && i0 + rs < n_live) {
             const int rho = job.rho0 + i, tok = rho / ps.G;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            *reinterpret_cast<v4f_t*>(a.out + ((int64_t)(job.start + tok) * a.nh + job.g * ps.G + rho - tok * ps.G) * HD +
-                                      d) = o * inv;
+            const int64_t head = (int64_t)(job.start + tok) * a.nh + job.g * ps.G + rho - tok * ps.G;
+            *reinterpret_cast<v4f_t*>(a.out + head * HD + d) = o * inv;
         }
     }
 }

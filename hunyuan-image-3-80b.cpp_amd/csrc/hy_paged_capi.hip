@@ -100,7 +100,8 @@ int paged_cache_check(const hy_paged_cache* c, uint32_t n_heads, PagedView* out)
     if (ps % unit || hs % unit || ts % unit || !aligned(c->k_dev, 16) || !aligned(c->v_dev, 16))
         return fail(HY_ERR_INVALID, "cache pointers and strides must be multiples of 16 bytes");
     if (ps >> 40 || hs >> 40) return fail(HY_ERR_INVALID, "cache stride of 2^40 or more elements");
-    if (ts > 1u << 24) return fail(HY_ERR_UNSUPPORTED, "token_stride=%llu: 2^24 elements at most", (unsigned long long)ts);
+    if (ts > 1u << 24)
+        return fail(HY_ERR_UNSUPPORTED, "token_stride=%llu: 2^24 elements at most", (unsigned long long)ts);
     *out = {c->k_dev, c->v_dev, (int64_t)ps, (int64_t)hs, (int64_t)ts, c->type, (int)c->n_pages, shift,
             (int)c->n_kv_heads, (int)c->head_dim};
     return HY_OK;

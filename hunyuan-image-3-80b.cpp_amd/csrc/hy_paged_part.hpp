@@ -7,8 +7,9 @@
 // every worker has the same share.  Lengths are in device memory, so every work group sums them
 // itself (part_sums).  An item inside one worker's stretch is written by it; one that is cut leaves
 // a partial result per piece, joined afterwards (joining the pieces of a work group's waves in LDS
-// first was tried: 32 requests of 24 rows 72.5 -> 70.4 us, one of 4 rows 14.1 -> 14.9).  A piece [x0, x1) of an item of nominal length W takes the
-// key blocks from x0 B / W to x1 B / W (part_block) of the item's real B.
+// first was tried: 32 requests of 24 rows 72.5 -> 70.4 us, one of 4 rows 14.1 -> 14.9).  A piece
+// [x0, x1) of an item of nominal length W takes the key blocks from x0 B / W to x1 B / W
+// (part_block) of the item's real B.
 #pragma once
 #include <limits.h>
 
@@ -54,7 +55,9 @@ struct PartReq {
 
 // n / d for 0 <= n <= 2^20, 0 < d: n + 1/2 keeps 1 / (2 d) from the next whole number, the
 // reciprocal is off by 2^-22 of the quotient
-__device__ __forceinline__ int part_div(int n, int d) { return (int)(((float)n + 0.5f) * __builtin_amdgcn_rcpf((float)d)); }
+__device__ __forceinline__ int part_div(int n, int d) {
+    return (int)(((float)n + 0.5f) * __builtin_amdgcn_rcpf((float)d));
+}
 // floor(x / n) for 0 <= x, 0 < n, the same for the wave: an estimate in f32, then a step either way
 template <class I>
 __device__ __forceinline__ int part_quotient(I x, I n) {
@@ -162,8 +165,8 @@ __device__ __forceinline__ void part_place(const PartShape& p, PartItem& it, I y
     if (it.q.tiles > 1) {
         // tiles of full size: t base + tau t (t + 1) / 2 = y
         const float b = (float)(I)it.q.base + 0.5f * p.tau, yf = (float)y;
-        t = min(uniform((int)(2.0f * yf * __builtin_amdgcn_rcpf(b + __builtin_amdgcn_sqrtf(b * b + 2.0f * p.tau * yf)))),
-                it.q.tiles - 1);
+        const float root = __builtin_amdgcn_sqrtf(b * b + 2.0f * p.tau * yf);
+        t = min(uniform((int)(2.0f * yf * __builtin_amdgcn_rcpf(b + root))), it.q.tiles - 1);
         while (t > 0 && it.q.upto(p.tau, t) > y) t--;
         while (t + 1 < it.q.tiles && it.q.upto<I>(p.tau, t + 1) <= y) t++;  // the last one ends with its head
     }

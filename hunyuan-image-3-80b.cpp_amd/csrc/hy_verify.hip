@@ -236,8 +236,8 @@ __global__ __launch_bounds__(VF_THREADS) void verify_rows_kernel(VerifyArgs a, V
 // Where request r, of rows lo .. hi - 1, ends: a row per wave, the last row always ends it.
 // found, ends: one per wave.
 template <int WAVES>
-__device__ __forceinline__ VfPick vf_decide(const VerifyArgs& a, const VfSlice* part, int r, int lo, int hi, VfPick* found,
-                                            int* ends) {
+__device__ __forceinline__ VfPick vf_decide(const VerifyArgs& a, const VfSlice* part, int r, int lo, int hi,
+                                            VfPick* found, int* ends) {
     const int V = a.vocab, S = vf_slices(V), lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, n = hi - lo;
     const float temp = a.temp ? a.temp[r] : 1.0f;
     const bool greedy = !(temp > 0.0f);
@@ -413,7 +413,8 @@ __global__ __launch_bounds__(VP_THREADS) void verify_pick_kernel(VerifyArgs a, c
         __syncthreads();
         const double mine_run = lane < VP_VEC * WAVES ? runs[lane] : 0.0;  // a run per lane
         const double run = wave_scan(mine_run);
-        const unsigned long long over = __ballot(mine_run > 0.0 && s_before + run > thr), some = __ballot(mine_run > 0.0);
+        const unsigned long long some = __ballot(mine_run > 0.0);
+        const unsigned long long over = __ballot(mine_run > 0.0 && s_before + run > thr);
         // no run: the sums of the slice and of its runs may round apart
         const int at = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
         const double at_before = s_before + read_lane(run - mine_run, max(at, 0));
@@ -448,7 +449,8 @@ __global__ __launch_bounds__(VP_THREADS) void verify_pick_kernel(VerifyArgs a, c
         tok = block_fold<VP_THREADS>(tok, pi, [](int u, int v) { return max(u, v); });
     }
     int* const out = a.tokens + (int64_t)r * a.max_new;
-    for (int i = tid; i < a.max_new; i += VP_THREADS) out[i] = i < p.accepted ? a.ids[lo + i + 1] : i == p.accepted ? tok : -1;
+    for (int i = tid; i < a.max_new; i += VP_THREADS)
+        out[i] = i < p.accepted ? a.ids[lo + i + 1] : i == p.accepted ? tok : -1;
     if (tid == 0) a.accepted[r] = p.accepted;
 }
 
@@ -469,7 +471,8 @@ hipError_t launch_verify_drafts(const VerifyArgs& a, hipStream_t s) {
     if (a.draft) {
         rest = reinterpret_cast<double*>(ws + al16(a.n_rows * S * sizeof(VfSlice)));
         pick = reinterpret_cast<VfPick*>(reinterpret_cast<uint8_t*>(rest) + al16(a.n_req * S * sizeof(double)));
-        hipLaunchKernelGGL(verify_rest_kernel, dim3((unsigned)(a.n_req * S)), dim3(VF_THREADS), 0, s, a, part, rest, pick);
+        hipLaunchKernelGGL(verify_rest_kernel, dim3((unsigned)(a.n_req * S)), dim3(VF_THREADS), 0, s, a, part, rest,
+                           pick);
     }
     hipLaunchKernelGGL(verify_pick_kernel, dim3((unsigned)a.n_req), dim3(VP_THREADS), 0, s, a, part, rest, pick);
     return hipGetLastError();
