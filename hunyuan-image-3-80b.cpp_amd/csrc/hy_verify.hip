@@ -281,7 +281,7 @@ __device__ __forceinline__ VfPick vf_decide(const VerifyArgs& a, const VfSlice* 
             e.row = row;
             e.x = word ? x : -1;
         }
-        __syncthreads();  // the last round's are read
+        __syncthreads();  // the last rows' are read
         if (lane == 0) {
             found[wave] = e;
             ends[wave] = end && i < n;
