@@ -60,8 +60,8 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
     PartJob job{};
     while (x < x_end) {
         const PartItem it = part_find(a, ps, sums, x);
-        const int p0 = (int)(x - it.at), p1 = (int)min(x_end - it.at, (int64_t)it.len);  // this piece
-        x = it.at + p1;
+        int p0, p1;
+        if (!part_piece(ps, it, x, x_end, p0, p1)) continue;
 
         // rows of this lane's columns; rows past the last repeat it and are not stored
         const int n_live = min(it.q.n * G - it.tile * ps.M, ps.M);
@@ -526,10 +526,12 @@ static PaPlan pa_plan(int type, int n_req, int max_new, int G, int hd) {
     PaPlan p;
     // Starting an item is worth 16 keys of a full stream, 256 of a many-row tile (20 000 of its 3500
     // to 6500 cycles per 32 keys); a stretch is 32 keys at least (64: one request of
-    // 1000 keys 12.6 us, 32: 10.2), 128.
-    p.few = part_shape(rows > 16 ? 5 : 4, G, 0, many ? PF_ROWS : ALL, few ? PF_WORKERS : 0, 16, 32, 0);
+    // 1000 keys 12.6 us, 32: 10.2), 128.  Cuts within 32, 128 of an item's end move there: a small
+    // piece costs its start and a partial result (2 requests of up to 172 tokens, f16, 53 -> 45 us,
+    // 88 drafts of up to 15 behind 5 keys 18 -> 15; 64 for the streams: a token over 1000 keys 12 -> 14).
+    p.few = part_shape(rows > 16 ? 5 : 4, G, 0, many ? PF_ROWS : ALL, few ? PF_WORKERS : 0, 16, 32, 32, 0);
     const size_t few_ws = part_ws_floats(p.few.workers, p.few.M, hd);
-    p.many = part_shape(PM_TILE_SHIFT, G, few ? PF_ROWS : 0, ALL, many ? PM_WORKERS : 0, 256, 128, few_ws);
+    p.many = part_shape(PM_TILE_SHIFT, G, few ? PF_ROWS : 0, ALL, many ? PM_WORKERS : 0, 256, 128, 128, few_ws);
     return p;
 }
 

@@ -102,8 +102,8 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
     PartJob job{};
     while (x < x_end) {
         const PartItem it = part_find(a, ps, sums, x);
-        const int p0 = (int)(x - it.at), p1 = (int)min(x_end - it.at, (int64_t)it.len);
-        x = it.at + p1;
+        int p0, p1;
+        if (!part_piece(ps, it, x, x_end, p0, p1)) continue;
         const int kv = it.q.kv;
         const int n_live = min(it.q.n * G - it.tile * PM_M, PM_M);
         // this lane's row (the last one again past the end) and the keys it sees

@@ -27,12 +27,13 @@ struct PartShape {
     int workers;
     int extra;                 // keys that starting an item is worth
     int unit;                  // nominal length of the shortest stretch, a power of two
+    int snap;                  // a cut nearer than this to an item's end moves there
     size_t ws;                 // floats of the workspace before this launch's slots
 };
 inline PartShape part_shape(int m_shift, int G, int64_t rows_lo, int64_t rows_hi, int workers, int extra, int unit,
-                            size_t ws) {
+                            int snap, size_t ws) {
     const int M = 1 << m_shift;
-    return {M, m_shift, G, M / G > 1 ? M / G : 1, rows_lo, rows_hi, workers, extra, unit, ws};
+    return {M, m_shift, G, M / G > 1 ? M / G : 1, rows_lo, rows_hi, workers, extra, unit, snap, ws};
 }
 
 // a value that all lanes share, in scalar registers
@@ -216,6 +217,22 @@ __device__ __forceinline__ int part_block(int y, int len, int blocks) {
     return y >= len ? blocks : min(uniform((int)((float)y * ((float)blocks / (float)len))), blocks);
 }
 
+// A worker's piece of the item at place x, [p0, p1) of it: where its stretch begins and ends, each
+// moved to the item's end that is nearer than p.snap (the neighbour moves it too).  x goes on to the
+// next item, or to x_end.  False: nothing of the item is the worker's.
+__device__ __forceinline__ bool part_piece(const PartShape& p, const PartItem& it, int64_t& x, int64_t x_end, int& p0,
+                                           int& p1) {
+    const auto cut = [&](int64_t at) {
+        if (at - it.at >= it.len) return it.len;
+        const int y = (int)(at - it.at);
+        return y < p.snap ? 0 : it.len - y < p.snap ? it.len : y;
+    };
+    p0 = x == it.at ? 0 : cut(x);
+    p1 = cut(x_end);
+    x = p1 == it.len ? it.at + it.len : x_end;
+    return p0 < p1;
+}
+
 // Attention of this lane's row over keys k0 .. k1 - 1, key by key in f32: what the kernels do
 // again where their V holds infinities or NaNs.  A key of weight 0 does not touch the row.
 // LPR lanes (l, l + 64 / LPR, ...) share a row, the i-th of a lane's HD / LPR dims is dim(i);
@@ -280,7 +297,7 @@ __device__ __forceinline__ PartJob part_job(const PartShape& p, const PartItem& 
                                             int n_live) {
     PartJob j{0, n_live, it.q.start, it.tile * p.M, it.g, {}};
     if (p0 == 0 && p1 < it.len)  // the other pieces are a stretch each, the last one's rest aside
-        j.n_piece = 2 + part_quotient(it.len - 1 - p1, (int)min(stretch, (int64_t)INT_MAX));
+        j.n_piece = 2 + part_quotient(max(it.len - max(p.snap, 1) - p1, 0), (int)min(stretch, (int64_t)INT_MAX));
     return j;
 }
 

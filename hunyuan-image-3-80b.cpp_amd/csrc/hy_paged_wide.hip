@@ -44,8 +44,8 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && HD == 12
     PartJob job{};
     while (x < x_end) {
         const PartItem it = part_find(a, ps, sums, x);
-        const int p0 = (int)(x - it.at), p1 = (int)min(x_end - it.at, (int64_t)it.len);  // this piece
-        x = it.at + p1;
+        int p0, p1;
+        if (!part_piece(ps, it, x, x_end, p0, p1)) continue;
 
         // this lane's row; rows past the last repeat it and are not stored
         const int n_live = min(it.q.n * G - it.tile * M, M);
