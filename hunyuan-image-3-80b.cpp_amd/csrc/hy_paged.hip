@@ -190,7 +190,7 @@ hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t s) {
 // row per wave (neighbouring rows are neighbours in a page); HD / 4 lanes share a unit, 4 dims
 // (16 bytes) each, and all loads of a wave go out before anything else.  An angle is kept as a
 // fraction of a turn in 64 bits, position times turns per position minus its whole part, so a
-// far position costs no accuracy; sine and cosine of the rest are f32.
+// far position costs no accuracy; sine and cosine are f32, of its f32 part, and turned by the rest.
 // Bound by memory: 4096 rows of 48 heads of 128 (205 MB) 33 us in caches, 40 from memory (5.2 TB/s);
 // 5 rows 4.4 us, all of it latency.
 constexpr int PA_STEPS = 4;
@@ -222,8 +222,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
 #pragma unroll
             for (int p = 0; p < 2; p++) {
                 double turn = (double)pos * a.freq[d / 2 + p];
-                turn -= rint(turn);
-                sincospif((float)(2.0 * turn), &sn[p], &cs[p]);
+                turn = 2.0 * (turn - rint(turn));  // in half turns
+                const float half = (float)turn, rest = (float)(turn - (double)half) * 3.14159265f;
+                float s0, c0;
+                sincospif(half, &s0, &c0);
+                sn[p] = fmaf(rest, c0, s0);
+                cs[p] = fmaf(-rest, s0, c0);
             }
         } else if (a.rotate == 2) {
             const v4f_t c = *reinterpret_cast<const v4f_t*>(a.cos_t + (int64_t)pos * HD + d);
@@ -251,7 +255,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
         ss += dpp_f<0x122>(ss);
         ss += dpp_f<0x121>(ss);
         if constexpr (LPU == 32) ss = fadd_row(ss);
-        const float rms = 1.0f / sqrtf(ss / (float)HD + a.eps);
+        // 1 / sqrt rounded once: the 64-bit estimate (2^-24) and a step of Newton's, fewer operations than
+        // an f32 root and quotient
+        const double ms = fma((double)ss, 1.0 / HD, (double)a.eps), e = __builtin_amdgcn_rsq(ms);
+        const float rms = ms > 0.0 && ms < (double)INFINITY ? (float)fma(0.5 * e, fma(-ms * e, e, 1.0), e) : (float)e;
         if (u < a.nh) {
             *reinterpret_cast<v4f_t*>(a.q + ((int64_t)t * a.nh + u) * HD + d) = y * rms * wq;
         } else if (u < units) {
