@@ -524,12 +524,14 @@ static PaPlan pa_plan(int type, int n_req, int max_new, int G, int hd) {
     constexpr int64_t ALL = (int64_t)1 << 62;
     const bool many = rows > pf_max_rows(type, n_req, hd), few = !many || n_req > 1;
     PaPlan p;
+    // Beside chunks the stream's requests are mostly single tokens: 16 rows (12 requests of chunks and
+    // tokens, bf16, 414 -> 406 us; 32 rows would spare drafts a second reading of K and V).
     // Starting an item is worth 16 keys of a full stream, 256 of a many-row tile (20 000 of its 3500
     // to 6500 cycles per 32 keys); a stretch is 32 keys at least (64: one request of
     // 1000 keys 12.6 us, 32: 10.2), 128.  Cuts within 32, 128 of an item's end move there: a small
     // piece costs its start and a partial result (2 requests of up to 172 tokens, f16, 53 -> 45 us,
     // 88 drafts of up to 15 behind 5 keys 18 -> 15; 64 for the streams: a token over 1000 keys 12 -> 14).
-    p.few = part_shape(rows > 16 ? 5 : 4, G, 0, many ? PF_ROWS : ALL, few ? PF_WORKERS : 0, 16, 32, 32, 0);
+    p.few = part_shape(rows > 16 && !many ? 5 : 4, G, 0, many ? PF_ROWS : ALL, few ? PF_WORKERS : 0, 16, 32, 32, 0);
     const size_t few_ws = part_ws_floats(p.few.workers, p.few.M, hd);
     p.many = part_shape(PM_TILE_SHIFT, G, few ? PF_ROWS : 0, ALL, many ? PM_WORKERS : 0, 256, 128, 128, few_ws);
     return p;

@@ -18,9 +18,9 @@
 // order.  Scores are computed transposed, S^T = K Q^T, so a query's statistics stay in its
 // lane pair and its weights are the operand of O^T += V^T W^T as they lie.
 //
-// Bound by instruction issue and the power it draws: a SIMD's two waves take, per block and head_dim
-// 128 of a bf16 cache, 2100 cycles for the 64 products and 2700 for the vector operations (half
-// of them the softmax), of 4700 measured; matrix and vector work of different waves do not overlap
+// Bound by instruction issue and the power it draws: a SIMD's two waves have, per block and head_dim
+// 128 of a bf16 cache, 64 products (20 cycles each back to back, 33 from one wave) and 2700 cycles
+// of vector operations (half of them the softmax), and take 4700; matrix and vector work of different waves do not overlap
 // here (running the waves half a block apart changed nothing), and the clock falls to 1.6 GHz under
 // it.  2048 rows of 32 heads behind 8192 keys, f32: 1.09 ms, 283 TFLOP/s of attention and three times
 // that of f16 products (a large f16 matrix product reaches 1110); head_dim 64, five prompts of up
