@@ -136,8 +136,14 @@ int paged_append(const float* qkv, uint32_t n_rows, uint32_t n_heads, const Page
         return fail(HY_ERR_INVALID, "f32 arrays must be aligned to 16 bytes");
     PagedAppendArgs a{qkv,   (int)n_rows, (int)n_heads, c,      positions, slots, cos_t, sin_t,
                       (int)n_pos, cos_t ? 2 : theta > 0.0f ? 1 : 0, q_norm, k_norm, eps, q, {}};
-    for (int i = 0; i < c.hd / 2; i++)
-        a.freq[i] = theta > 0.0f ? std::pow((double)theta, -2.0 * i / c.hd) / 6.283185307179586476925 : 0.0;
+    if (a.rotate == 1) {  // theta^(-2 (8 p + r) / hd) as a product: 16 powers, not 64 (0.6 us of the call)
+        double low[8];
+        for (int r = 0; r < 8; r++) low[r] = std::pow((double)theta, -2.0 * r / c.hd) / 6.283185307179586476925;
+        for (int p = 0; p < c.hd / 16; p++) {
+            const double high = std::pow((double)theta, -16.0 * p / c.hd);
+            for (int r = 0; r < 8; r++) a.freq[8 * p + r] = high * low[r];
+        }
+    }
     HIP_TRY(launch_paged_append(a, s));
     return HY_OK;
 }
