@@ -120,7 +120,7 @@ int hy_rope_qknorm_paged(const float* qkv_dev, uint32_t n_rows, uint32_t n_heads
  * to 2^-98 at least.  A key that a row does not see does not touch it, whatever it holds; an
  * infinity or NaN in q or in a key that a row sees makes the row NaN.  ws_dev:
  * hy_paged_attention_ws bytes (0 for bad arguments; by the cache's and the batch's sizes,
- * 137 MB at most), aligned to 16 bytes, contents indifferent. */
+ * 103 MB at most), aligned to 16 bytes, contents indifferent. */
 size_t hy_paged_attention_ws(uint32_t n_heads, const hy_paged_cache* cache, const hy_paged_batch* batch);
 int hy_paged_attention(const float* q_dev, uint32_t n_heads, const hy_paged_cache* cache, const hy_paged_batch* batch,
                        float scale, float* out_dev, void* ws_dev, size_t ws_bytes, void* stream);

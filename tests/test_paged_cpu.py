@@ -173,3 +173,16 @@ def test_verify_refuses_what_no_launch_covers(hy):
     assert L.hy_verify_drafts(P, None, P, P, 4, n_rows, 5, vocab, None, P, P, P, P, P, 1 << 62, None) == UNSUPPORTED
     assert L.hy_last_error().decode()
     assert L.hy_verify_drafts_ws(4, n_rows, vocab - 1) > 0
+
+
+def test_workspace_is_bounded(hy):
+    """What the header promises, over every choice of kernels."""
+    L = hy.lib()
+    for t in (0, 1, 30):
+        for hd in (64, 128):
+            for nkv, nh in ((1, 1), (1, 64), (8, 32), (8, 1024)):
+                for n_req in (1, 2, 3, 4096):
+                    for max_new in (0, 1, 4, 8, 16, 33, 700, 1 << 20):
+                        n = L.hy_paged_attention_ws(nh, _cache(hy, type=t, head_dim=hd, n_kv_heads=nkv),
+                                                    _batch(hy, n_req=n_req, n_rows=1 << 20, max_new=max_new))
+                        assert 0 < n <= 103_000_000
