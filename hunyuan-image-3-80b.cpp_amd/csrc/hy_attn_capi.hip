@@ -765,6 +765,8 @@ int hy_model_forward_paged(hy_model_ctx* m, const int32_t* ids, const hy_paged_c
     if (!m) return fail(HY_ERR_INVALID, "null ctx");
     if (!ids || !logits) return fail(HY_ERR_INVALID, "null ids/logits");
     hy_attn_ctx* c = m->attn;
+    if (cache && m->L > 1 && cache->layer_stride == 0)
+        return fail(HY_ERR_INVALID, "layer_stride=0: the %d layers would share one pool", (int)m->L);
     for (uint32_t l = 0; l < (uint32_t)m->L; l++) {  // every layer, before anything is launched
         PagedStep st{{}, nullptr, nullptr, nullptr, 0, ws, ws_bytes};
         HY_TRY(check_paged(c, l, cache, batch, &st));

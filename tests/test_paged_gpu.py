@@ -1088,3 +1088,18 @@ def test_attention_rows_around_the_streams_limits(gpu, wtype, hd):
             q = rng.standard_normal((q_start[-1], nh, hd)).astype(np.float32)
             args = (q, pool, q_start, kv_len, table, hd ** -0.5)
             check_attention(attend(gpu, *args), *args)
+
+
+def test_model_refuses_layers_that_share_a_pool(gpu):
+    m, nh, nkv, hd, V, L = greedy_model(gpu)
+    pool = Pool(4, 16, nkv, hd, F32, fill=3.0)
+    kb, vb = upload(gpu, pool)
+    i32 = lambda *a: dev(gpu, np.array(a, np.int32))  # noqa: E731
+    cache = cache_of(gpu, pool, kb, vb)
+    batch = gpu.PagedBatch(1, 2, 4, 2, i32(0, 2), i32(2), i32(0, 1, 2, 3), i32(0, 1), i32(0, 1))
+    ws, logits = Ws(gpu, nh, cache, batch), gpu.Buf.empty((2, V))
+    with pytest.raises(gpu.HyError):
+        m.forward_paged(i32(4, 5), cache, batch, logits, ws.b, ws.n)
+    gpu.sync()
+    np.testing.assert_array_equal(kb.numpy(), pool.k)
+    m.close()
