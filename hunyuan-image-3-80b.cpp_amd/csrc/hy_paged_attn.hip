@@ -411,16 +411,13 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
 // Joins the pieces of the items that are cut, from the jobs the workers left: work group (w, split)
 // takes every splits-th set of rows of worker w's; in it, HD / 4 threads take 4 dims each of
 // a row and every pl_n-th piece of it, PJ pieces at a time, and the pl_n groups of a row meet in
-// LDS.  Bound by the partial results' bytes (4 TB/s of them for tiles of 256 rows), for short ones
+// LDS.  In slots by lanes neighbouring threads are neighbouring rows, eight of them (128 bytes), and
+// eight threads of a row 128 bytes of the output; in slots by rows they are a row's.  Bound by the partial results' bytes (4 TB/s of them for tiles of 256 rows), for short ones
 // by the latency of job, pieces and result: hence rows and pieces spread as far as they go.
-template <int HD, int PJ>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartShape few, PartShape many, int few_splits,
-                                                        int many_splits) {
-    __shared__ float meet[6][256];
-    const int b = (int)blockIdx.x - few.workers * few_splits;
-    const PartShape& ps = b < 0 ? few : many;
-    const int splits = b < 0 ? few_splits : many_splits, at = b < 0 ? (int)blockIdx.x : b;
-    const int w0 = at / splits, split = at - w0 * splits;
+// one of splits work groups for worker w0's item; LANES: of part_at's slots
+template <int HD, int PJ, bool LANES>
+__device__ __forceinline__ void join_item(const PagedAttnArgs& a, const PartShape& ps, int w0, int split, int splits,
+                                          float (&meet)[6][256]) {
     const PartJob job = part_jobs(a, ps, HD)[w0];
     const int n_piece = uniform(job.n_piece), n_live = uniform(job.n_live);
     if (n_piece == 0) return;
@@ -430,9 +427,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartSh
     constexpr int TR = HD / 4, GROUPS = 256 / TR;
     int pl_n = 1;
     while (pl_n < 8 && pl_n * PJ < n_piece) pl_n *= 2;
-    const int tid = threadIdx.x, d = tid % TR * 4, pl = tid / TR % pl_n, rs = tid / TR / pl_n, rs_n = GROUPS / pl_n;
+    const int tid = threadIdx.x, rs_n = GROUPS / pl_n;
+    const int d = (LANES ? tid / 8 : tid) % TR * 4, group = LANES ? tid % 8 + tid / (8 * TR) * 8 : tid / TR;
+    const int pl = LANES ? group / rs_n : group % pl_n, rs = LANES ? group % rs_n : group / pl_n;
     for (int i0 = split * rs_n; i0 < n_live; i0 += rs_n * splits) {  // the same for the work group
-        const int i = min(i0 + rs, n_live - 1);
+        const int i = min(i0 + rs, n_live - 1), at = LANES ? part_at(HD, i, d) : i * HD + d;
         float m = -INFINITY, l = 0.0f;
         v4f_t o = v4f_t{};
         for (int k0 = pl; k0 < n_piece; k0 += pl_n * PJ) {
@@ -444,7 +443,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartSh
                 const float* const s = k == 0 ? first : rest + (size_t)(2 * k) * sf;
                 mk[j] = s[ps.M * HD + i];
                 lk[j] = s[ps.M * (HD + 1) + i];
-                ok[j] = *reinterpret_cast<const v4f_t*>(s + i * HD + d);
+                ok[j] = *reinterpret_cast<const v4f_t*>(s + at);
             }
             __builtin_amdgcn_sched_barrier(0);
             float mn = m;
@@ -464,6 +463,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartSh
             }
         }
         if (pl_n > 1) {
+            // the thread of the row's next group: group + 1 by rows, group + rs_n by lanes, whose low
+            // three bits are in tid's
+            const auto other = [&](int k) {
+                if (!LANES) return tid + k * TR;
+                const int g = group + k * rs_n;
+                return tid / 8 % TR * 8 + g % 8 + g / 8 * (8 * TR);
+            };
             __syncthreads();  // the last rows' are read
             meet[4][tid] = m;
             meet[5][tid] = l;
@@ -472,12 +478,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartSh
             __syncthreads();
             if (pl == 0) {
                 float mn = m;
-                for (int k = 1; k < pl_n; k++) mn = fmaxf(mn, meet[4][tid + k * TR]);
+                for (int k = 1; k < pl_n; k++) mn = fmaxf(mn, meet[4][other(k)]);
                 const float ref = mn == -INFINITY ? 0.0f : mn, alpha = __builtin_amdgcn_exp2f(m - ref);
                 l *= alpha;
                 o *= alpha;
                 for (int k = 1; k < pl_n; k++) {
-                    const int from = tid + k * TR;
+                    const int from = other(k);
                     const float f = __builtin_amdgcn_exp2f(meet[4][from] - ref);
                     l += f * meet[5][from];
 #pragma unroll
@@ -492,6 +498,18 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartSh
             *reinterpret_cast<v4f_t*>(a.out + head * HD + d) = o * inv;
         }
     }
+}
+
+// MANY: with both in it the kernel has 78 registers, for streams alone 56
+template <int HD, int PJ, bool MANY>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartShape few, PartShape many, int few_splits,
+                                                        int many_splits) {
+    __shared__ float meet[6][256];
+    const int b = (int)blockIdx.x - few.workers * few_splits;
+    if (!MANY || b < 0)
+        join_item<HD, PJ, false>(a, few, blockIdx.x / few_splits, blockIdx.x % few_splits, few_splits, meet);
+    else
+        join_item<HD, PJ, true>(a, many, b / many_splits, b % many_splits, many_splits, meet);
 }
 
 constexpr int PJ_ROWS = 8;  // rows of a stream's item per work group of the join
@@ -572,14 +590,16 @@ hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s)
     const dim3 grid(p.few.workers * splits + p.many.workers * many_splits);
     // Items of 32 pieces and more: eight pieces at a time (1000 keys, one request: 4.0 us, by fours
     // 5.6), elsewhere four, of half the registers (32 requests of 24 rows: 11.4, by eights 12.8).
-    const bool long_ = !p.many.workers && a.n_req * a.c.nkv * 32 <= p.few.workers;
+    const bool long_ = a.n_req * a.c.nkv * 32 <= p.few.workers;
     const auto join = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, p.few, p.many, splits, many_splits);
     };
-    if (long_)
-        big ? join(paged_join_kernel<128, 8>) : join(paged_join_kernel<64, 8>);
+    if (p.many.workers)
+        big ? join(paged_join_kernel<128, 4, true>) : join(paged_join_kernel<64, 4, true>);
+    else if (long_)
+        big ? join(paged_join_kernel<128, 8, false>) : join(paged_join_kernel<64, 8, false>);
     else
-        big ? join(paged_join_kernel<128, 4>) : join(paged_join_kernel<64, 4>);
+        big ? join(paged_join_kernel<128, 4, false>) : join(paged_join_kernel<64, 4, false>);
     return hipGetLastError();
 }
 

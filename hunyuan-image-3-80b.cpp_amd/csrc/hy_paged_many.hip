@@ -519,7 +519,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 f = l_run == 0.0f ? 0.0f : down / l_run;
             } else {
                 float* const slot = a.ws + ps.ws + (size_t)slot_id * part_slot_floats(PM_M, HD);
-                dst = slot + my * HD;
+                dst = slot + 32 * wv * HD + 4 * lane;  // part_at
                 if (h == 0) {
                     slot[PM_M * HD + my] = m_run;
                     slot[PM_M * (HD + 1) + my] = l_run;
@@ -529,10 +529,11 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             for (int d = 0; d < ND / 2; d++)
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
-                    float* const p = dst + 2 * (32 * d + 8 * u + 4 * h);
+                    float* const p = dst + (slot_id < 0 ? 2 * (32 * d + 8 * u + 4 * h) : 512 * (4 * d + u));
+                    const int next = slot_id < 0 ? 4 : 256;
 #pragma unroll
                     for (int v = 0; v < 2; v++)
-                        *reinterpret_cast<v4f_t*>(p + 4 * v) =
+                        *reinterpret_cast<v4f_t*>(p + v * next) =
                             (v4f_t){o[d][4 * u + 2 * v], o[d + ND / 2][4 * u + 2 * v], o[d][4 * u + 2 * v + 1],
                                     o[d + ND / 2][4 * u + 2 * v + 1]} *
                             f;
