@@ -373,8 +373,8 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
                     [&](int n) {
                         return F32T ? 64 * (n / 16) + 4 * (4 * g4 + n % 4) + n / 4 % 4 : VD * (4 * g4 + n % 4) + n / 4;
                     },
-                    [&](int n, float v) { o[c][n / 4][n % 4] = v; }, [&](int n) { return o[c][n / 4][n % 4]; }, m_run[c],
-                    l_run[c]);
+                    [&](int n, float v) { o[c][n / 4][n % 4] = v; },
+                    [&](int n) { return o[c][n / 4][n % 4]; }, m_run[c], l_run[c]);
         }
         float* const slot = a.ws + ps.ws + (size_t)max(slot_id, 0) * part_slot_floats(ps.M, HD);
 #pragma unroll
@@ -412,8 +412,9 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
 // takes every splits-th set of rows of worker w's; in it, HD / 4 threads take 4 dims each of
 // a row and every pl_n-th piece of it, PJ pieces at a time, and the pl_n groups of a row meet in
 // LDS.  In slots by lanes neighbouring threads are neighbouring rows, eight of them (128 bytes), and
-// eight threads of a row 128 bytes of the output; in slots by rows they are a row's.  Bound by the partial results' bytes (4 TB/s of them for tiles of 256 rows), for short ones
-// by the latency of job, pieces and result: hence rows and pieces spread as far as they go.
+// eight threads of a row 128 bytes of the output; in slots by rows they are a row's.  Bound by the
+// partial results' bytes (4 TB/s of them for tiles of 256 rows), for short ones by the latency of
+// job, pieces and result: hence rows and pieces spread as far as they go.
 // one of splits work groups for worker w0's item; LANES: of part_at's slots
 template <int HD, int PJ, bool LANES>
 __device__ __forceinline__ void join_item(const PagedAttnArgs& a, const PartShape& ps, int w0, int split, int splits,
