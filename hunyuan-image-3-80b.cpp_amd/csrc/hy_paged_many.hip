@@ -22,9 +22,10 @@
 // 128 of a bf16 cache, 64 products (20 cycles each back to back, 33 from one wave) and 2700 cycles
 // of vector operations (half of them the softmax), and take 4700; matrix and vector work of
 // different waves do not overlap here (running the waves half a block apart changed nothing), and
-// the clock falls to 1.6 GHz under it.  2048 rows of 32 heads behind 8192 keys, f32: 1.09 ms, 283 TFLOP/s of attention and three times
-// that of f16 products (a large f16 matrix product reaches 1110); head_dim 64, five prompts of up
-// to 1500 tokens, f16: 61 us, of which 20 000 cycles (10 us) per piece go to its start and end.
+// the clock falls to 1.6 GHz under it.  2048 rows of 32 heads behind 8192 keys, f32: 1.08 ms back to
+// back, 286 TFLOP/s of attention and three times that of f16 products (a large f16 matrix product
+// reaches 1110); head_dim 64, five prompts of up to 1500 tokens, f16: 61 us, of which 20 000 cycles
+// (10 us) per piece go to its start and end.
 //
 // Keys that no row sees are stored as zeros and masked; where V holds an infinity or NaN, which 0
 // times a weight would not keep out, the piece is computed again key by key (slow_rows).
