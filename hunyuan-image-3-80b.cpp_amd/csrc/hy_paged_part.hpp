@@ -46,11 +46,13 @@ struct PartReq {
     int start, n, kv;   // first row, rows (tokens), keys
     int tiles, full;    // tiles of its rows; those whose nominal tokens do not reach past the last
     int64_t base, head; // keys before its first token, and extra; nominal length of a head's tiles
-    // nominal length of tiles 0 .. k - 1; I: what holds the request's
+    // nominal length of tiles 0 .. k - 1; I: what holds the request's.  f (f + 1) is formed without a
+    // sign: tiles of one token reach 2^32 with it where half of it still fits I
     template <class I>
-    __device__ __forceinline__ I upto(int tau, I k) const {
-        const I f = min(k, (I)full);
-        return k * (I)base + (I)tau * (f * (f + 1) / 2) + (k - f) * (I)n;
+    __host__ __device__ __forceinline__ I upto(int tau, I k) const {
+        const I f = k < (I)full ? k : (I)full;
+        typedef typename std::make_unsigned<I>::type U;
+        return k * (I)base + (I)tau * (I)((U)f * (U)(f + 1) / 2) + (k - f) * (I)n;
     }
 };
 
