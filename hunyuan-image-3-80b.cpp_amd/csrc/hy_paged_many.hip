@@ -11,7 +11,11 @@
 // 2^-27 of their vector's largest keep all bits of a piece, none is off by more than 2^-38 of it).  K's
 // factor is undone on the scores.  V's, 2^e_j, joins the weights: with R the running
 // maximum of s_j + e_j the accumulators sum w_j v_j 2^-e_j, w_j = 2^(s_j + e_j - R),
-// and w_j 2^-e_j = 2^(s_j - R), which leaves out = O / l in any reference R.
+// and w_j 2^-e_j = 2^(s_j - R), which leaves out = O / l in any reference R.  e_j lies in
+// PM_ELO .. PM_EHI: then a w_j that l is formed from stays above 2^-126 wherever 2^(s_j - R) counts
+// in l (2^-30 of its largest term: -30 + PM_ELO - PM_EHI + PM_WUP > -126), within a piece
+// and where pieces meet.  A row of zeros takes PM_ELO, which raises no R above the others'; smaller
+// values share it; a piece with larger ones is computed again key by key.
 //
 // Blocks of 32 keys: every thread loads its share of a block of K and V one block ahead,
 // splits it and stores the pieces to LDS, K as it is and V transposed, both in MFMA operand
@@ -28,7 +32,8 @@
 // (10 us) per piece go to its start and end.
 //
 // Keys that no row sees are stored as zeros and masked; where V holds an infinity or NaN, which 0
-// times a weight would not keep out, the piece is computed again key by key (slow_rows).
+// times a weight would not keep out, or 2^35 and more under scaling, the piece is computed again
+// key by key (slow_rows).
 #include "hy_device.hpp"
 #include "hy_lds.hpp"
 #include "hy_paged.hpp"
@@ -40,7 +45,8 @@ namespace hy {
 constexpr int PM_WAVES = 8, PM_THREADS = WAVE * PM_WAVES, PM_M = PM_TILE;
 static_assert(PM_M == 32 * PM_WAVES && PM_WORKERS % 8 == 0, "32 rows per wave, whole XCDs");
 constexpr int PM_UP = 14;   // q's and K's largest elements go to [2^14, 2^15)
-constexpr int PM_VUP = 13;  // V's to [2^13, 2^14): 2^-e of an e up to 126 is a normal number
+constexpr int PM_VUP = 13;  // V's to [2^13, 2^14)
+constexpr int PM_ELO = -60, PM_EHI = 34;  // exponents that V's rows are scaled by
 // The running maximum R that weights are relative to is left behind while a block does not pass
 // it by more than PM_LAG: weights are up to 2^PM_LAG, and the sums are rescaled once or twice
 // per row instead of at every new maximum.  Weights carry a factor 2^PM_WUP.
@@ -87,7 +93,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
     constexpr int RING = KP == 2 ? 2 : 3;  // operands read ahead of the products (registers allowing)
     __shared__ __attribute__((aligned(1024))) uint8_t lds[L::BYTES];
     __shared__ __attribute__((aligned(16))) float k_fac[2][32], v_exp[2][32], v_inv[2][32];
-    __shared__ int odd_s;  // an infinity or NaN in this piece's V
+    __shared__ int odd_s;  // V of this piece that the scaled products do not take
     __shared__ int last_s[PM_WAVES];
     __shared__ PartSums<PM_THREADS> sums;
     const int tid = threadIdx.x, lane = tid % WAVE, lr = lane % 32, h = lane / 32;
@@ -192,7 +198,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         v4i_t kx[KP];
         typedef typename std::conditional<KP == 2, uint2, uint32_t>::type vrow_t;
         vrow_t vx[4];
-        uint32_t v_big = 0;  // the largest magnitude of V's: whether one was infinite or no number
+        uint32_t v_big = 0;  // the largest magnitude of V's: whether one was infinite, no number, or past PM_EHI
         auto load_k = [&](int kb) {
             const char* const p = reinterpret_cast<const char*>(kg + cell_of(kb * 32 + (wv * KPW) % 32));
 #pragma unroll
@@ -293,8 +299,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 const auto umax = [](uint32_t p, uint32_t q) { return max(p, q); };
                 b = with_half(with_row(b, umax), umax);
                 v_big = max(v_big, b);
-                // (no exponent of its own for a row of zeros: it has to share the sum's range)
-                const int e = b >= 0x7f800000u || b == 0 ? 0 : min(exponent(b, -60), 126);
+                const int e = min(exponent(b, PM_ELO), PM_EHI);
                 if (lane < 4) {
                     v_exp[r][4 * wv + lane] = (float)e;
                     v_inv[r][4 * wv + lane] = pow2(-e);
@@ -499,7 +504,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         // l carries the weights' factor too, scaled values have one of their own
         float down = SCALED ? pow2(-PM_VUP) : 1.0f;
         if constexpr (SCALED)
-            v_big = v_big >= 0x7f800000u;
+            v_big = v_big >= (uint32_t)(127 + PM_EHI + 1) << 23;
         else
             v_big = (v_big & 0xffffu) >= 0x7c00u || v_big >= 0x7c000000u;
         if (__any(v_big != 0)) odd_s = 1;
@@ -509,8 +514,9 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 a, trow, kv, kb0 * 32, my_kb1 * 32, end, a.q + ((int64_t)row * a.nh + head) * HD, kg, vg,
                 [&](int i) { return 2 * (32 * (i / 16 % (ND / 2)) + 8 * (i % 16 / 4) + 4 * h + i % 4) + i / (8 * ND); },
                 [&](int i, float v) { o[i / 16][i % 16] = v; }, [&](int i) { return o[i / 16][i % 16]; }, m_run, l_run);
-            down = pow2(PM_WUP);  // as the other pieces of its item
-            l_run *= down;
+            // as the other pieces of its item; in the reference, the sums of large values have no room for it
+            down = 1.0f;
+            m_run += (float)PM_WUP;
         }
         if (my < n_live) {
             float* dst;

@@ -3,8 +3,8 @@ import numpy as np
 import pytest
 
 import paged_ref as R
-from paged_ref import F16
-from test_paged_gpu import attend, make_batch
+from paged_ref import BF16, F16, F32
+from test_paged_gpu import attend, check_attention, make_batch
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +28,57 @@ def test_attention_long_request_in_tiles_of_one_token(gpu):
         w /= np.maximum(w.sum(-1, keepdims=True), 1e-300)
         bound = R.attention_bound((np.abs(x) @ np.abs(k).T).max(-1) * hd ** -0.5, w @ np.abs(v), hd, 40)
         assert (np.abs(got[t0:t0 + 5000] - w @ v) <= bound).all()
+
+
+# max_new that sends a request of 40 rows and 4 query heads per kv head to the streams' tiles of 16
+# rows, of 32, and to the tiles of 256
+KERNELS = {"stream16": 1, "stream32": 8, "tiles": 1 << 20}
+
+
+def at(pool, a, table, r, j):
+    """Storage [nkv][hd] of a's (pool.k or pool.v) key j of request r."""
+    return pool.at(a, table[r, j // pool.page], j % pool.page)
+
+
+def scale_values(pool, f):
+    """Values of a pool by a factor per [page][position]."""
+    pool.v = R.encode(R.decode(pool.v, pool.wtype).astype(np.float32) * f[:, None, :, None].astype(np.float32), pool.wtype)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("wtype,scale", [(F32, 1.0), (F32, 1e-6), (F32, 1e-10), (F16, 1.0), (F16, 1e-3), (BF16, 1.0),
+                                         (BF16, 1e-6), (BF16, 1e-10)])
+def test_attention_zero_value_rows(gpu, wtype, scale, kernel):
+    """Keys whose value is zero take their weight and leave the others' accuracy alone, whatever size
+    the others' values have."""
+    rng = np.random.default_rng(71)
+    for zeros in ((150,), range(0, 300, 3), range(300)):
+        pool, table, q_start, kv_len = make_batch(rng, [(300, 40)], 16, 2, 128, wtype)
+        scale_values(pool, np.full((pool.n_pages, 16), scale))
+        for j in zeros:
+            at(pool, pool.v, table, 0, j)[:] = 0
+        q = (rng.standard_normal((40, 8, 128)) * 0.5).astype(np.float32)
+        args = (q, pool, q_start, kv_len, table, 128 ** -0.5)
+        check_attention(attend(gpu, *args, max_new=KERNELS[kernel]), *args)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("small,big,kv", [(0.01, 1e28, 300), (0.01, 1e28, 3000), (1e-15, 1e10, 300), (1e-17, 3e10, 3000),
+                                          (0.01, 1e38, 300), (1e-6, 1e12, 3000)])
+@pytest.mark.parametrize("wtype", [F32, BF16])
+def test_attention_values_of_very_different_size(gpu, wtype, small, big, kv, kernel):
+    """Equal scores: the weight of a small value counts in full beside a large one, in one piece and
+    over many, and rows that do not see the large one keep the small ones' accuracy."""
+    rng = np.random.default_rng(72)
+    pool, table, q_start, kv_len = make_batch(rng, [(kv, 40)], 16, 2, 128, wtype)
+    pool.k[:] = 0
+    f = np.full((pool.n_pages, 16), small)
+    for j in [kv - 30] if big > 1e30 else [kv - 30, 40, kv // 2]:
+        f[table[0, j // 16], j % 16] = big
+    scale_values(pool, f)
+    q = rng.standard_normal((40, 8, 128)).astype(np.float32)
+    args = (q, pool, q_start, kv_len, table, 128 ** -0.5)
+    check_attention(attend(gpu, *args, max_new=KERNELS[kernel]), *args)
+    seen = rng.integers(0, kv + 1, 40).astype(np.int32)
+    seen[:9] = (40, 41, 39, 7, kv // 2, kv // 2 + 1, kv - 30, kv - 29, kv)
+    check_attention(attend(gpu, *args, seen=seen, max_new=KERNELS[kernel]), *args, seen)
