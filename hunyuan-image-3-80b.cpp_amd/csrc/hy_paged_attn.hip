@@ -268,6 +268,17 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
 #pragma unroll
             for (int u = 0; u < KT; u++) none |= vpage[u] < 0;
             const bool edge = (t + 1) * KB > first || __any(none);
+            uint32_t top = 0;
+#pragma unroll
+            for (int c = 0; c < NT; c++)
+#pragma unroll
+                for (int u = 0; u < KT; u++) top = top_bits<4>(s[c][u], top);
+            if (__any(top >= PA_MINUS_INF)) {
+#pragma unroll
+                for (int c = 0; c < NT; c++)
+#pragma unroll
+                    for (int u = 0; u < KT; u++) minus_inf_to_nan<4>(s[c][u]);
+            }
 #pragma unroll
             for (int c = 0; c < NT; c++) {
                 if (edge) {  // wave-uniform

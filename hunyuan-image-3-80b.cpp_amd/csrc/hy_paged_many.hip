@@ -218,8 +218,12 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         // block kb, r = kb % 2
         auto put_k = [&](int r) {
             uint8_t* const d = k_dst + r * L::BUF_K;
+            // a key with an infinity makes NaN of every score (a row's q with one does by its pieces):
+            // through its factor, or its element x becomes 0 x + x
             if constexpr (!SCALED) {
-                if (k_mine) *reinterpret_cast<v4i_t*>(d) = kx[0];
+                const v8h16_t x = __builtin_bit_cast(v8h16_t, kx[0]);
+                const v8h16_t y = __builtin_elementwise_fma(x, (v8h16_t)((_Float16)0), x);
+                if (k_mine) *reinterpret_cast<v8h16_t*>(d) = y;
             } else {
                 float f[8];
                 uint32_t big = 0;
@@ -254,7 +258,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 if (k_mine) {
                     *reinterpret_cast<v4i_t*>(d) = hi;
                     if constexpr (KP == 2) *reinterpret_cast<v4i_t*>(d + L::PIECE_K) = lo;
-                    if (k_ch == 0) k_fac[r][k_key] = pow2(e - PM_UP);
+                    if (k_ch == 0) k_fac[r][k_key] = big < 0x7f800000u ? pow2(e - PM_UP) : __builtin_nanf("");
                 }
             }
         };

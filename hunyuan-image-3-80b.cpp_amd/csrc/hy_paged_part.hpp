@@ -235,6 +235,25 @@ __device__ __forceinline__ bool part_piece(const PartShape& p, const PartItem& i
     return p0 < p1;
 }
 
+// A score of -inf comes from an infinity in q or in the key (or, over f32 and bf16 caches, from
+// products past f32's range): it becomes NaN, as one of +inf does in its weight, or the row would
+// go on as if the key were masked, and one with no other score as if it saw nothing.  -inf has the
+// largest bits but for NaNs', so the streams look for it by a maximum of whole numbers (0 to 2 %
+// of their time; 1 to 3 % of the tiles', which mark such keys as they store them instead, 0 to 1 %).
+constexpr uint32_t PA_MINUS_INF = 0xff800000u;
+template <int N, class V>
+__device__ __forceinline__ uint32_t top_bits(const V& s, uint32_t top = 0) {
+#pragma unroll
+    for (int v = 0; v < N; v++) top = max(top, __float_as_uint(s[v]));
+    return top;
+}
+template <int N, class V>
+__device__ __forceinline__ void minus_inf_to_nan(V& s) {
+    asm volatile("");  // behind a branch, not done without one
+#pragma unroll
+    for (int v = 0; v < N; v++) s[v] = s[v] == -INFINITY ? __builtin_nanf("") : s[v];
+}
+
 // Attention of this lane's row over keys k0 .. k1 - 1, key by key in f32: what the kernels do
 // again where their V holds infinities or NaNs.  A key of weight 0 does not touch the row.
 // LPR lanes (l, l + 64 / LPR, ...) share a row, the i-th of a lane's HD / LPR dims is dim(i);
@@ -261,6 +280,7 @@ __device__ __forceinline__ void slow_rows(const PagedAttnArgs& a, const int* tro
         for (int i = 0; i < N; i++) s = fmaf(qk[dim(i)] * qscale, (float)kg[at + dim(i)], s);
 #pragma unroll
         for (int d = 32; d >= 64 / LPR; d >>= 1) s += shfl_xor(s, d);
+        if (s == -INFINITY) s = __builtin_nanf("");
         if (key >= end) s = -INFINITY;
         const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
         const float alpha = __builtin_amdgcn_exp2f(m - ref), p = __builtin_amdgcn_exp2f(s - ref);

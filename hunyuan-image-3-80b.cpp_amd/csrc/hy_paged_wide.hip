@@ -171,6 +171,7 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && HD == 12
             __builtin_amdgcn_sched_barrier(0);
             if (t + 1 < t1) load_k(t + 1);
             __builtin_amdgcn_sched_barrier(0);
+            if (__any(top_bits<16>(s) >= PA_MINUS_INF)) minus_inf_to_nan<16>(s);
             const bool edge = (t + 1) * KB > first || (vpage[0] | vpage[1] | vpage[2] | vpage[3]) < 0;
             if (edge) {  // wave-uniform
                 asm volatile("");

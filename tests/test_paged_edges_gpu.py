@@ -82,3 +82,47 @@ def test_attention_values_of_very_different_size(gpu, wtype, small, big, kv, ker
     seen = rng.integers(0, kv + 1, 40).astype(np.int32)
     seen[:9] = (40, 41, 39, 7, kv // 2, kv // 2 + 1, kv - 30, kv - 29, kv)
     check_attention(attend(gpu, *args, seen=seen, max_new=KERNELS[kernel]), *args, seen)
+
+
+def check_rows(got, want, bound, rows):
+    """Rows x heads of a mask: finite, and within bound of want."""
+    assert np.isfinite(got[rows]).all() and (np.abs(got - want)[rows] <= bound[rows]).all()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("wtype", [F32, F16, BF16])
+def test_attention_infinities_make_rows_nan(gpu, wtype, sign, kernel):
+    """One infinite element of a key or of q: NaN wherever a row sees it, whatever its product's sign,
+    whichever kernel, on the key-by-key path too; other rows and heads notice nothing."""
+    rng = np.random.default_rng(73)
+    kv, n, j = 300, 40, 275              # row i sees keys 0 .. 260 + i
+    for odd_value in (False, True):
+        pool, table, q_start, kv_len = make_batch(rng, [(kv, n)], 16, 2, 128, wtype)
+        q = rng.standard_normal((n, 8, 128)).astype(np.float32)
+        q[:, :, 17] = np.where(rng.random((n, 8)) < 0.5, 1.0, -1.0)
+        args = (q, pool, q_start, kv_len, table, 128 ** -0.5)
+        want, dot, pv = R.attention(*args)
+        bound = R.attention_bound(dot, pv, 128, kv)
+        hit = np.zeros((n, 8), bool)
+        hit[j - 260:, :4] = True
+        key, value = at(pool, pool.k, table, 0, j), at(pool, pool.v, table, 0, kv - 1)
+        key[0, 17] = R.encode(np.float32([sign * np.inf]), wtype)[0]
+        if odd_value:                    # of the last row's own key: the pieces with it go key by key
+            value[0, :] = R.encode(np.float32([np.nan]), wtype)[0]
+        got = attend(gpu, *args, max_new=KERNELS[kernel])
+        assert np.isnan(got[hit]).all()
+        check_rows(got, want, bound, ~hit)
+        # q: every key has the other sign there, so that every score is -inf
+        pool.k[..., 17] = R.encode(np.float32([-sign]), wtype)[0]
+        q[:, :, 17] = 1.0
+        want, dot, pv = R.attention(*args)
+        bound = R.attention_bound(dot, pv, 128, kv)
+        hit[:] = False
+        q[7, 2, 17] = q[39, 5, 17] = sign * np.inf
+        hit[7, 2] = hit[39, 5] = True
+        got = attend(gpu, *args, max_new=KERNELS[kernel])
+        assert np.isnan(got[hit]).all()
+        if odd_value:
+            hit[39, :4] = True           # they see the value that is NaN
+        check_rows(got, want, bound, ~hit)
