@@ -138,7 +138,7 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
                 float up = 1.0f;
                 if constexpr (F16T) {
                     big = group_max(big);
-                    const int e = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -100), 100);
+                    const int e = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -100), 127);
                     up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
                     unscale[t] = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
                 }

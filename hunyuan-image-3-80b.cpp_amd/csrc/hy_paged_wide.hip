@@ -94,7 +94,7 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && HD == 12
             float up = 1.0f;
             if constexpr (F16T) {
                 big = fmax_half(big);
-                const int e = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -100), 100);
+                const int e = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -100), 127);
                 up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
                 unscale = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
             }

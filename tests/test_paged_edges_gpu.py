@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import paged_ref as R
-from paged_ref import BF16, F16, F32
+from paged_ref import BF16, EPS32, F16, F32
 from test_paged_gpu import attend, check_attention, make_batch
 
 pytestmark = pytest.mark.gpu
@@ -126,3 +126,29 @@ def test_attention_infinities_make_rows_nan(gpu, wtype, sign, kernel):
         if odd_value:
             hit[39, :4] = True           # they see the value that is NaN
         check_rows(got, want, bound, ~hit)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("wtype", [F32, F16, BF16])
+def test_attention_large_queries(gpu, wtype, kernel):
+    """Scores of 1e35: the best key takes all, where it leads by more than an f32 product's error."""
+    rng = np.random.default_rng(74)
+    pool, table, q_start, kv_len = make_batch(rng, [(300, 40)], 16, 2, 128, wtype)
+    q = (rng.standard_normal((40, 8, 128)) * 1e35).astype(np.float32)
+    args = (q, pool, q_start, kv_len, table, 128 ** -0.5)
+    got = attend(gpu, *args, max_new=KERNELS[kernel])
+    assert np.isfinite(got).all()
+    k = np.stack([R.decode(at(pool, pool.k, table, 0, j), wtype) for j in range(300)])
+    v = np.stack([R.decode(at(pool, pool.v, table, 0, j), wtype) for j in range(300)])
+    clear = 0
+    for t in range(40):
+        for h in range(8):
+            s = k[:261 + t, h // 4] @ q[t, h].astype(np.float64)
+            best = np.argsort(s)[-2:]
+            if s[best[1]] - s[best[0]] > (128 + 8) * 2 * EPS32 * (np.abs(k[:, h // 4]) @ np.abs(q[t, h])).max() * 2:
+                clear += 1
+                # a weight of one, in pieces of 22 bits, and the division; small elements to 2^-38 of
+                # their row's largest
+                x = v[best[1], h // 4]
+                assert (np.abs(got[t, h] - x) <= 8 * EPS32 * np.abs(x) + 2.0 ** -38 * np.abs(x).max()).all()
+    assert clear > 250
