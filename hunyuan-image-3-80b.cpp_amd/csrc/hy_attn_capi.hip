@@ -259,7 +259,8 @@ int run_paged(hy_attn_ctx* c, const AttnLayer& W, const float* x, const PagedSte
     HY_TRY(timed(c, AK_ROPE, s, [&] {
         return call(hy::paged_append(c->qkv, st.batch->n_rows, (uint32_t)c->nh, st.cache, st.batch->positions_dev,
                                      st.batch->slots_dev, c->cfg.rope_theta, st.cos_t, st.sin_t, st.n_pos, W.q_norm,
-                                     W.k_norm, c->cfg.rms_norm_eps, c->q, s));
+                                     W.k_norm, c->cfg.rms_norm_eps, c->q, s, c->merged,
+                                     st.batch->q_start_dev + st.batch->n_req));
     }));
     HY_TRY(rc);
     HY_TRY(timed(c, AK_ATTN, s, [&] {

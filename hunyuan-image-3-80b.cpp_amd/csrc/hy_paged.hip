@@ -214,8 +214,20 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
     for (int s = 0; s < PA_STEPS; s++)
         x[s] = *reinterpret_cast<const v4f_t*>(row + (int64_t)min(u0 + (s * WAVE + l) / LPU, units - 1) * HD);
     const int slot = a.slots[t], pos = a.positions[t];
-    if (slot < 0 || (slot >> a.c.shift) >= a.c.n_pages) return;
-    if (a.rotate == 2 && (pos < 0 || pos >= a.n_pos)) return;
+    // What a layer goes on with comes from this call alone: a row of nobody has an attention of zeros,
+    // a skipped one a query of zeros.
+    const auto clear = [&](float* to) {
+#pragma unroll
+        for (int s = 0; s < PA_STEPS; s++) {
+            const int u = u0 + (s * WAVE + l) / LPU;
+            if (u < a.nh) *reinterpret_cast<v4f_t*>(to + ((int64_t)t * a.nh + u) * HD + d) = v4f_t{};
+        }
+    };
+    if (a.merged && t >= a.row_end[0]) clear(a.merged);
+    if (slot < 0 || (slot >> a.c.shift) >= a.c.n_pages || (a.rotate == 2 && (pos < 0 || pos >= a.n_pos))) {
+        if (a.merged) clear(a.q);
+        return;
+    }
     float cs[2] = {1.0f, 1.0f}, sn[2] = {0.0f, 0.0f};
     if (u0 < a.nh + a.c.nkv) {  // not values alone
         if (a.rotate == 1) {

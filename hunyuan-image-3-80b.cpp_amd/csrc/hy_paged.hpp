@@ -51,6 +51,8 @@ struct PagedAppendArgs {
     const float* k_norm;
     float eps;
     float* q;
+    float* merged;       // of a layer: the attention's output [rows][nh][hd]; null: rows without a slot are
+    const int* row_end;  // left alone; and the first row that belongs to nobody
     double freq[PG_MAX_HD / 2];  // turns per position of pair i: theta^(-2i / hd) / (2 pi)
 };
 hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s);
@@ -93,7 +95,8 @@ int paged_batch_check(const hy_paged_batch* b, const PagedView& c, bool writes);
 int paged_rotary_check(float theta, const float* cos_t, const float* sin_t, uint32_t n_pos, float eps);
 int paged_append(const float* qkv, uint32_t n_rows, uint32_t n_heads, const PagedView& c, const int32_t* positions,
                  const int32_t* slots, float theta, const float* cos_t, const float* sin_t, uint32_t n_pos,
-                 const float* q_norm, const float* k_norm, float eps, float* q, hipStream_t s);
+                 const float* q_norm, const float* k_norm, float eps, float* q, hipStream_t s,
+                 float* merged = nullptr, const int32_t* row_end = nullptr);
 size_t paged_batch_ws(const hy_paged_batch* b, uint32_t n_heads, const PagedView& c);
 int paged_ws_check(const hy_paged_batch* b, uint32_t n_heads, const PagedView& c, const void* ws, size_t ws_bytes);
 int paged_attention(const float* q, uint32_t n_heads, const PagedView& c, const hy_paged_batch* b, float scale,

@@ -128,14 +128,15 @@ int paged_rotary_check(float theta, const float* cos_t, const float* sin_t, uint
 
 int paged_append(const float* qkv, uint32_t n_rows, uint32_t n_heads, const PagedView& c, const int32_t* positions,
                  const int32_t* slots, float theta, const float* cos_t, const float* sin_t, uint32_t n_pos,
-                 const float* q_norm, const float* k_norm, float eps, float* q, hipStream_t s) {
+                 const float* q_norm, const float* k_norm, float eps, float* q, hipStream_t s,
+                 float* merged, const int32_t* row_end) {
     if (!qkv || !positions || !slots || !q) return fail(HY_ERR_INVALID, "null pointer");
     if (n_rows == 0 || n_rows > 1u << 20) return fail(HY_ERR_INVALID, "n_rows=%u must be in 1..2^20", n_rows);
     HY_TRY(paged_rotary_check(theta, cos_t, sin_t, n_pos, eps));
     if (!aligned(qkv, 16) || !aligned(q, 16) || (q_norm && !aligned(q_norm, 16)) || (k_norm && !aligned(k_norm, 16)))
         return fail(HY_ERR_INVALID, "f32 arrays must be aligned to 16 bytes");
     PagedAppendArgs a{qkv,   (int)n_rows, (int)n_heads, c,      positions, slots, cos_t, sin_t,
-                      (int)n_pos, cos_t ? 2 : theta > 0.0f ? 1 : 0, q_norm, k_norm, eps, q, {}};
+                      (int)n_pos, cos_t ? 2 : theta > 0.0f ? 1 : 0, q_norm, k_norm, eps, q, merged, row_end, {}};
     if (a.rotate == 1) {  // theta^(-2 (8 p + r) / hd) as a product: 16 powers, not 64 (0.6 us of the call)
         double low[8];
         for (int r = 0; r < 8; r++) low[r] = std::pow((double)theta, -2.0 * r / c.hd) / 6.283185307179586476925;

@@ -151,10 +151,10 @@ int hy_verify_drafts(const float* logits_dev, const float* draft_probs_dev, cons
                      int32_t* accepted_dev, int32_t* tokens_dev, void* ws_dev, size_t ws_bytes, void* stream);
 
 /* hy_attn_forward over a paged cache: out = o_proj(attention of the batch's rows), the
- * rows' keys and values written to `layer`'s pool first.  x, out [n_rows][hidden]; rows
- * that belong to nobody read x and leave out undefined.  1D rotary positions
- * (rope_theta), or the tables of hy_rope_qknorm_paged.  The cache's heads are the
- * context's; n_rows <= max_tokens. */
+ * rows' keys and values written to `layer`'s pool first.  x, out [n_rows][hidden].  Rows
+ * that belong to nobody get zeros; a row without a slot, or with a position outside the
+ * tables, has a query of zeros.  1D rotary positions (rope_theta), or the tables of
+ * hy_rope_qknorm_paged.  The cache's heads are the context's; n_rows <= max_tokens. */
 int hy_attn_forward_paged(hy_attn_ctx* ctx, uint32_t layer, const float* x_dev, const hy_paged_cache* cache,
                           const hy_paged_batch* batch, const float* cos_dev, const float* sin_dev, uint32_t n_pos,
                           float* out_dev, void* ws_dev, size_t ws_bytes, void* stream);

@@ -3,8 +3,8 @@ import numpy as np
 import pytest
 
 import paged_ref as R
-from paged_ref import BF16, EPS32, F16, F32
-from test_paged_gpu import attend, check_attention, make_batch
+from paged_ref import BF16, EPS32, F16, F32, Pool
+from test_paged_gpu import Ws, attend, cache_of, check_attention, dev, make_batch, upload
 
 pytestmark = pytest.mark.gpu
 
@@ -152,3 +152,39 @@ def test_attention_large_queries(gpu, wtype, kernel):
                 x = v[best[1], h // 4]
                 assert (np.abs(got[t, h] - x) <= 8 * EPS32 * np.abs(x) + 2.0 ** -38 * np.abs(x).max()).all()
     assert clear > 250
+
+
+def layer(gpu):
+    att = gpu.Attn(512, 8, 2, 128, 32)
+    att.synth(0, seed=5, std=0.05)
+    return att
+
+
+def test_layer_rows_of_nobody_keep_nothing_of_earlier_calls(gpu):
+    """Rows behind the last sequence give zeros, and a row without a slot the same as in a new context;
+    the other rows' bits do not depend on what ran before either."""
+    rng = np.random.default_rng(75)
+    nh, nkv, hd, page = 8, 2, 128, 16
+    i32 = lambda a: dev(gpu, a, np.int32)  # noqa: E731
+    x = rng.standard_normal((12, 512)).astype(np.float32)
+    pool = Pool(4, page, nkv, hd, F16)
+
+    def step(att, x, n, slots):
+        kb, vb = upload(gpu, pool)
+        cache = cache_of(gpu, pool, kb, vb)
+        batch = gpu.PagedBatch(1, len(x), 2, n, i32([0, n]), i32([n]), i32([1, 3]), i32(range(len(x))), i32(slots))
+        ws, out = Ws(gpu, nh, cache, batch), dev(gpu, np.full(x.shape, 7.0, np.float32))
+        att.forward_paged(dev(gpu, x), cache, batch, out, ws.b, ws.n)
+        return out.numpy()
+
+    slots = page + np.arange(12)
+    few = np.where(np.arange(12) < 8, slots, -1)
+    few[5] = 4 * page + 1                                # outside the pool: no key, and no query
+    for padding in (few, np.where(np.arange(12) == 5, -1, slots)):  # rows of nobody with slots too
+        used, new = layer(gpu), layer(gpu)
+        step(used, np.full((12, 512), np.nan, np.float32), 12, slots)
+        got, want = step(used, x, 8, padding), step(new, x, 8, padding)
+        assert np.isfinite(got).all() and (got[8:] == 0).all()
+        np.testing.assert_array_equal(got, want)
+        used.close()
+        new.close()
