@@ -23,6 +23,7 @@ int set_last_error(int code, const std::string& msg);  // hy_capi.hip
 int moe_layer_check(const hy_moe_ctx* c, uint32_t layer, uint32_t T);  // hy_capi.hip
 int moe_hidden(const hy_moe_ctx* c);                   // hy_capi.hip
 int moe_device(const hy_moe_ctx* c);
+bool moe_drops_tokens(const hy_moe_ctx* c);
 const GgufFile& gguf_file(const hy_gguf* g);           // host/hy_gguf.cpp
 }
 
@@ -766,6 +767,9 @@ int hy_model_forward_paged(hy_model_ctx* m, const int32_t* ids, const hy_paged_c
     if (!m) return fail(HY_ERR_INVALID, "null ctx");
     if (!ids || !logits) return fail(HY_ERR_INVALID, "null ids/logits");
     hy_attn_ctx* c = m->attn;
+    if (hy::moe_drops_tokens(m->moe))
+        return fail(HY_ERR_UNSUPPORTED,
+                    "drop_tokens: a request's experts would depend on the other requests' rows and on rows of nobody");
     if (cache && m->L > 1 && cache->layer_stride == 0)
         return fail(HY_ERR_INVALID, "layer_stride=0: the %d layers would share one pool", (int)m->L);
     for (uint32_t l = 0; l < (uint32_t)m->L; l++) {  // every layer, before anything is launched

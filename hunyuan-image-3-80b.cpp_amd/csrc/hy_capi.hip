@@ -482,6 +482,7 @@ int moe_layer_check(const hy_moe_ctx* c, uint32_t layer, uint32_t T) {
 }
 int moe_hidden(const hy_moe_ctx* c) { return c ? c->H : 0; }
 int moe_device(const hy_moe_ctx* c) { return c ? c->cfg.device : -1; }
+bool moe_drops_tokens(const hy_moe_ctx* c) { return c->cfg.drop_tokens != 0; }
 const GgufFile& gguf_file(const hy_gguf* g);  // host/hy_gguf.cpp
 }  // namespace hy
 

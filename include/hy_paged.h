@@ -160,7 +160,8 @@ int hy_attn_forward_paged(hy_attn_ctx* ctx, uint32_t layer, const float* x_dev, 
                           float* out_dev, void* ws_dev, size_t ws_bytes, void* stream);
 
 /* hy_model_forward over a paged cache of num_layers pools: ids int32 [n_rows], logits
- * [n_rows][vocab]; 1D rotary positions. */
+ * [n_rows][vocab]; 1D rotary positions.  HY_ERR_UNSUPPORTED for a model with drop_tokens:
+ * an expert's capacity would be shared with the other requests and with rows of nobody. */
 int hy_model_forward_paged(hy_model_ctx* ctx, const int32_t* ids_dev, const hy_paged_cache* cache,
                            const hy_paged_batch* batch, float* logits_dev, void* ws_dev, size_t ws_bytes,
                            void* stream);

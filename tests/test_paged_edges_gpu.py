@@ -1,4 +1,6 @@
 """Paged serving on the GPU at the ends of its ranges, against plain numpy in 64 bits."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -188,3 +190,36 @@ def test_layer_rows_of_nobody_keep_nothing_of_earlier_calls(gpu):
         np.testing.assert_array_equal(got, want)
         used.close()
         new.close()
+
+
+def test_model_that_drops_tokens_is_refused(gpu):
+    """Under token dropping a request's experts depend on the rows beside it, those of nobody among
+    them: refused, with nothing written."""
+    H, nh, nkv, hd, V, L, T = 256, 8, 2, 64, 500, 2, 32
+    mc = gpu.Config(H, 128, 8, 2, L, T, gpu.F32, 1, 1, 1.0, 0, 0, 0, 0)
+    mc.drop_tokens, mc.capacity_factor, mc.min_capacity = 1, 1.0, 1
+    ac = gpu.AttnConfig(H, nh, nkv, hd, L, T, 0, 1e-5, 10000.0, 0)
+    h = C.c_void_p()
+    gpu.check(gpu.lib().hy_model_create(C.byref(gpu.ModelConfig(mc, ac, V)), C.byref(h)))
+    m = gpu.Model.__new__(gpu.Model)
+    m.h, m.H, m.V, m.L = h, H, V, L
+    m.attn = gpu.Attn(H, nh, nkv, hd, T, handle=C.c_void_p(gpu.lib().hy_model_attn(h)))
+    m.moe = gpu.Moe.__new__(gpu.Moe)
+    m.moe.h, m.moe.owned = gpu.lib().hy_model_moe(h), False
+    m.moe.H, m.moe.I, m.moe.E, m.moe.K, m.moe.wtype = H, 128, 8, 2, gpu.F32
+    m.synth_globals(seed=3, std=0.5)
+    for l in range(L):
+        m.attn.synth(l, seed=7 + l, std=0.08)
+        m.moe.synth(l, seed=9 + l, std=0.05)
+    pool = Pool(4 * L, 16, nkv, hd, F32, fill=3.0)
+    kb, vb = upload(gpu, pool)
+    i32 = lambda *a: dev(gpu, np.array(a, np.int32))  # noqa: E731
+    cache = gpu.PagedCache(kb, vb, F32, 4, 16, nkv, hd, layer_stride=4 * nkv * 16 * hd)
+    batch = gpu.PagedBatch(1, 2, 4, 2, i32(0, 2), i32(2), i32(0, 1, 2, 3), i32(0, 1), i32(0, 1))
+    ws, logits = Ws(gpu, nh, cache, batch), dev(gpu, np.full((2, V), 8.0, np.float32))
+    with pytest.raises(gpu.HyError, match="drop"):
+        m.forward_paged(i32(4, 5), cache, batch, logits, ws.b, ws.n)
+    gpu.sync()
+    np.testing.assert_array_equal(kb.numpy(), pool.k)
+    assert (logits.numpy() == 8.0).all()
+    m.close()
