@@ -225,6 +225,23 @@ struct PagedStep {
     size_t ws_bytes;
 };
 
+// Do `layers` pools, `stride` elements apart, share no element?  Side by side, or each inside the gaps
+// of the last one's smallest stride above `stride`.
+bool pools_apart(const hy::PagedView& v, uint64_t stride, size_t layers) {
+    typedef unsigned __int128 wide;  // 2^28 pages of 2^40 elements
+    const wide n[] = {(wide)v.n_pages, (wide)v.nkv, (wide)1 << v.shift};
+    const wide st[] = {(wide)v.page_stride, (wide)v.head_stride, (wide)v.token_stride};
+    wide inside = v.hd, above = 0;  // what a pool spans without its strides from `stride` on; the least of those
+    for (int i = 0; i < 3; i++) {
+        if (n[i] == 1) continue;
+        if (st[i] < stride)
+            inside += (n[i] - 1) * st[i];
+        else if (!above || st[i] < above)
+            above = st[i];
+    }
+    return inside <= stride && (!above || (layers - 1) * (wide)stride + inside <= above);
+}
+
 int check_paged(const hy_attn_ctx* c, uint32_t layer, const hy_paged_cache* cache, const hy_paged_batch* b,
                 PagedStep* st) {
     HY_TRY(check_layer(c, layer, true));
@@ -239,6 +256,9 @@ int check_paged(const hy_attn_ctx* c, uint32_t layer, const hy_paged_cache* cach
     if (cache->layer_stride * el % 16 || cache->layer_stride >> 44)
         return fail(HY_ERR_INVALID, "layer_stride=%llu must be a multiple of 16 bytes below 2^44 elements",
                     (unsigned long long)cache->layer_stride);
+    if (c->layers.size() > 1 && !pools_apart(st->cache, cache->layer_stride, c->layers.size()))
+        return fail(HY_ERR_INVALID, "layer_stride=%llu: pools of the %zu layers would overlap",
+                    (unsigned long long)cache->layer_stride, c->layers.size());
     st->cache.k = static_cast<uint8_t*>(st->cache.k) + layer * cache->layer_stride * el;
     st->cache.v = static_cast<uint8_t*>(st->cache.v) + layer * cache->layer_stride * el;
     st->batch = b;
@@ -770,8 +790,6 @@ int hy_model_forward_paged(hy_model_ctx* m, const int32_t* ids, const hy_paged_c
     if (hy::moe_drops_tokens(m->moe))
         return fail(HY_ERR_UNSUPPORTED,
                     "drop_tokens: a request's experts would depend on the other requests' rows and on rows of nobody");
-    if (cache && m->L > 1 && cache->layer_stride == 0)
-        return fail(HY_ERR_INVALID, "layer_stride=0: the %d layers would share one pool", (int)m->L);
     for (uint32_t l = 0; l < (uint32_t)m->L; l++) {  // every layer, before anything is launched
         PagedStep st{{}, nullptr, nullptr, nullptr, 0, ws, ws_bytes};
         HY_TRY(check_paged(c, l, cache, batch, &st));

@@ -48,8 +48,9 @@ typedef struct {
     uint64_t page_stride;  /* elements */
     uint64_t head_stride;
     uint64_t token_stride; /* 2^24 at most */
-    uint64_t layer_stride; /* elements from one layer's pool to the next (calls with a layer); 0 only
-                            * where there is one */
+    uint64_t layer_stride; /* elements from one layer's pool to the next (calls with a context); pools of
+                            * several layers lie side by side, or interleaved by page, head or
+                            * position; looked at only where there are several */
 } hy_paged_cache;
 
 /* The requests of one step.  Request r has the token rows q_start[r] .. q_start[r + 1] - 1

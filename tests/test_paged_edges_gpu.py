@@ -223,3 +223,43 @@ def test_model_that_drops_tokens_is_refused(gpu):
     np.testing.assert_array_equal(kb.numpy(), pool.k)
     assert (logits.numpy() == 8.0).all()
     m.close()
+
+
+def test_layers_that_would_overlap_are_refused(gpu):
+    """A context of several layers: pools that share elements are refused for every layer, pools side by
+    side, interleaved by page, by position and by head are taken."""
+    H, nh, nkv, hd, page, n_pages, L = 256, 8, 2, 64, 16, 4, 3
+    att = gpu.Attn(H, nh, nkv, hd, 16, num_layers=L)
+    for l in range(L):
+        att.synth(l, seed=5 + l, std=0.05)
+    one = n_pages * nkv * page * hd
+    kb, vb = gpu.Buf(2 * L * (one + 64)), gpu.Buf(2 * L * (one + 64))
+    i32 = lambda n: dev(gpu, np.zeros(n, np.int32))  # noqa: E731
+    x, out = dev(gpu, np.zeros((8, H), np.float32)), gpu.Buf.empty((8, H))
+
+    def call(layer, layer_stride, strides=(0, 0, 0)):
+        c = gpu.PagedCache(kb, vb, F16, n_pages, page, nkv, hd, strides, layer_stride)
+        b = gpu.PagedBatch(1, 8, 4, 8, i32(2), i32(1), i32(4), i32(8), i32(8))
+        ws = Ws(gpu, nh, c, b)
+        att.forward_paged(x, c, b, out, ws.b, ws.n, layer=layer)
+
+    per = nkv * page * hd                                   # of a page
+    good = [(one, (0, 0, 0)), (one + 64, (0, 0, 0)),        # one behind the other
+            (per, (L * per, page * hd, hd)),                # a page's layers together
+            (hd, (L * per, L * page * hd, L * hd)),         # a position's
+            (page * hd, (L * per, L * page * hd, hd)),      # a head's
+            (per, (L * per, hd, nkv * hd))]                 # pages of [position][head], their layers together
+    for stride, strides in good:
+        for layer in range(L):
+            call(layer, stride, strides)
+    bad = [(0, (0, 0, 0)), (8, (0, 0, 0)), (hd, (0, 0, 0)), (per, (0, 0, 0)), (one - 8, (0, 0, 0)),
+           (per, ((L - 1) * per, page * hd, hd)),           # too few elements between pages
+           (per - 8, (L * per, page * hd, hd)),
+           (hd - 8, (L * per, L * page * hd, L * hd)),
+           (hd, (L * per, L * page * hd, (L - 1) * hd))]
+    for stride, strides in bad:
+        for layer in range(L):
+            with pytest.raises(gpu.HyError, match="layer_stride"):
+                call(layer, stride, strides)
+    gpu.sync()
+    att.close()
