@@ -385,6 +385,9 @@ __global__ __launch_bounds__(VP_THREADS) void verify_pick_kernel(VerifyArgs a, c
             s = s_any;
             s_before = any_before;
         }
+        // no weight anywhere: rows of no request, whose slices nobody wrote (row starts out of order)
+        const bool none = s < 0;
+        s = max(s, 0);
         // in the slice: VP_VEC x WAVES runs of 4 x 64 tokens (load_slice's order), their sums, then
         // the lanes of the run that u falls into
         const float* const dr = minus && !whole ? a.draft + (int64_t)p.row * V : nullptr;
@@ -416,7 +419,7 @@ __global__ __launch_bounds__(VP_THREADS) void verify_pick_kernel(VerifyArgs a, c
         const unsigned long long some = __ballot(mine_run > 0.0);
         const unsigned long long over = __ballot(mine_run > 0.0 && s_before + run > thr);
         // no run: the sums of the slice and of its runs may round apart
-        const int at = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
+        const int at = none ? -1 : over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
         const double at_before = s_before + read_lane(run - mine_run, max(at, 0));
         tok = -1;
         if (at >= 0 && at % WAVES == wave) {

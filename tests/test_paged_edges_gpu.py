@@ -6,7 +6,7 @@ import pytest
 
 import paged_ref as R
 from paged_ref import BF16, EPS32, F16, F32, Pool
-from test_paged_gpu import Ws, attend, cache_of, check_attention, dev, make_batch, upload
+from test_paged_gpu import VerifyBufs, Ws, attend, cache_of, check_attention, dev, make_batch, upload
 
 pytestmark = pytest.mark.gpu
 
@@ -263,3 +263,19 @@ def test_layers_that_would_overlap_are_refused(gpu):
                 call(layer, stride, strides)
     gpu.sync()
     att.close()
+
+
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_row_starts_out_of_order(gpu, probs):
+    """Starts that go back leave rows that no request's slices were written for: over a workspace of
+    zeros their tokens are -1 or of the vocabulary, and nothing outside the logits is read."""
+    rng = np.random.default_rng(76)
+    V, n = 20000, 9
+    logits = rng.standard_normal((n, V)).astype(np.float32)
+    draft = np.full((n, V), 1 / V, np.float32) if probs else None
+    for starts in ([0, 3, 1, 4], [5, 2, 9, 0], [0, 9, 9, 3], [7, 9, 0, 5]):
+        b = VerifyBufs(gpu, logits, draft, np.arange(n), starts, None, np.full(n, 0.9), np.full(3, 0.5), n)
+        b.ws = dev(gpu, np.zeros(b.n // 4 + 1, np.float32))
+        b.run()
+        accepted, tokens = b.result()
+        assert ((accepted >= -1) & (accepted < n)).all() and ((tokens >= -1) & (tokens < V)).all()
