@@ -9,11 +9,15 @@
  * without a context run on the calling thread's current device (hy_set_device), which the
  * stream and all pointers belong to.  Every call only launches kernels on its stream: it
  * returns without waiting, allocates nothing, and can be captured into a graph.  Calls
- * that overlap in time need workspaces of their own, captured graphs among them.
+ * that overlap in time, captured graphs among them, need workspaces of their own, and
+ * contexts of their own where they take one.
  *
  * One step of a server: hy_paged_plan (tables, slots), hy_model_forward_paged (every
- * layer: hy_rope_qknorm_paged, hy_paged_attention), hy_verify_drafts (accepted tokens,
- * which give the next step's lengths).  No counterpart in the reference, whose KVCache
+ * layer: hy_rope_qknorm_paged, hy_paged_attention), hy_verify_drafts (accepted tokens).
+ * Request r brought new[r] rows, of a prompt or its last token and drafts.  With
+ * status[r] = 0, cached[r] grows by the rows whose tokens were given (a prompt's), and by
+ * 1 + accepted for those that were verified; with any other status its rows computed
+ * nothing, cached[r] stays, and they come again.  No counterpart in the reference, whose KVCache
  * (src/hunyuan_image_gen.h:179-193) holds one sequence in one piece.
  */
 #ifndef HY_PAGED_H
@@ -128,7 +132,12 @@ int hy_paged_attention(const float* q_dev, uint32_t n_heads, const hy_paged_cach
                        float scale, float* out_dev, void* ws_dev, size_t ws_bytes, void* stream);
 
 /* The verification of drafted tokens by speculative sampling.  Request r's rows
- * q_start[r] .. q_start[r + 1] - 1 of ids are its last token and its drafts x_1 .. x_n;
+ * q_start[r] .. q_start[r + 1] - 1 of ids are its last token and its drafts x_1 .. x_n: every
+ * row after the first is taken for a draft.  Rows that are none (a prompt's but the last, those of a
+ * request that was not served) are kept apart by a q_start of its own with two entries per
+ * request, [start, start + context rows]: the even results, of context rows, mean nothing (with
+ * more than max_new rows they are -1), the odd ones are of the rows behind, -1 where there are
+ * none.  So a prompt's last piece has one verified row, its last token, and gets its first new token.
  * row i of logits is the target's prediction of what follows row i, and row i of
  * draft_probs [n_rows][vocab] the distribution that x_{i+1} was drawn from (NULL: drafts
  * without probabilities, as certain).  With p = softmax(logits / temperature[r]) (NULL: 1),

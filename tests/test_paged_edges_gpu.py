@@ -6,7 +6,8 @@ import pytest
 
 import paged_ref as R
 from paged_ref import BF16, EPS32, F16, F32, Pool
-from test_paged_gpu import VerifyBufs, Ws, attend, cache_of, check_attention, dev, make_batch, upload
+from test_paged_gpu import (PlanBufs, VerifyBufs, Ws, attend, cache_of, check_attention, dev, greedy_model, make_batch,
+                            upload)
 
 pytestmark = pytest.mark.gpu
 
@@ -279,3 +280,86 @@ def test_verify_row_starts_out_of_order(gpu, probs):
         b.run()
         accepted, tokens = b.result()
         assert ((accepted >= -1) & (accepted < n)).all() and ((tokens >= -1) & (tokens < V)).all()
+
+
+def test_server_step_with_prompts_drafts_and_waiting_requests(gpu):
+    """The loop that include/hy_paged.h describes, with everything in one step: prompts in pieces,
+    last tokens with drafts, requests that find no pages and come again (where nobody finds any, the last
+    one gives up its pages and starts again with what it has), rows of nobody.
+    Verification takes all rows' logits as they are, two row starts per request.  The text equals
+    greedy decoding by hy_model_forward."""
+    m, nh, nkv, hd, V, L = greedy_model(gpu)
+    rng = np.random.default_rng(77)
+    prompts = [rng.integers(0, V, n).tolist() for n in (9, 23, 1, 14)]
+    n, steps, piece, max_drafts = len(prompts), 12, 8, 4
+    asked, want = [len(p) for p in prompts], []
+    for p in prompts:
+        seq = list(p)
+        for _ in range(steps):
+            lb = gpu.Buf.empty((len(seq), V))
+            m.forward(dev(gpu, seq, np.int32), len(seq), lb)
+            last = np.sort(lb.numpy()[-1])
+            assert last[-1] - last[-2] > 1e-4 * abs(last[-1])  # no near tie decides
+            seq.append(int(np.argmax(lb.numpy()[-1])))
+        want.append(seq[len(p):])
+    page, n_pages, max_pages = 8, 8, 8
+    pool = Pool(n_pages * L, page, nkv, hd, F32, fill=np.nan)
+    kb, vb = upload(gpu, pool)
+    cache = gpu.PagedCache(kb, vb, F32, n_pages, page, nkv, hd, layer_stride=n_pages * nkv * page * hd)
+    held, table = np.zeros(n, np.int32), np.zeros((n, max_pages), np.int32)
+    free, n_free, cached = rng.permutation(n_pages).astype(np.int32), n_pages, np.zeros(n, np.int64)
+    done, kinds, accepted_drafts = [[] for _ in prompts], set(), 0
+    drafts = [[] for _ in prompts]
+    for _ in range(80):
+        if min(len(d) for d in done) >= steps:
+            break
+        rows, context = [], []
+        for r, p in enumerate(prompts):                      # p: what runs without drafts
+            if len(done[r]) >= steps:                        # ended: its pages go back
+                rows.append([])
+                context.append(0)
+                cached[r] = 0
+            elif cached[r] < len(p):                         # a piece of the prompt
+                rows.append(p[cached[r]:cached[r] + piece])
+                context.append(len(rows[-1]) - (cached[r] + len(rows[-1]) == len(p)))
+            else:
+                rows.append([done[r][-1]] + drafts[r])
+                context.append(0)
+        new = np.array([len(x) for x in rows])
+        n_rows = int(new.sum()) + 2
+        plan = PlanBufs(gpu, cached, new, held, table, free, n_free, n_rows, page, n_pages)
+        plan.run(in_place=True)
+        batch = gpu.PagedBatch(n, n_rows, max_pages, int(new.max()), plan.q_start, plan.kv_len, plan.table,
+                               plan.positions, plan.slots)
+        ids = np.array(sum(rows, []) + [V + 3, -1], np.int32)
+        logits, ws = gpu.Buf.empty((n_rows, V)), Ws(gpu, nh, cache, batch)
+        m.forward_paged(dev(gpu, ids), cache, batch, logits, ws.b, ws.n)
+        start = np.concatenate([[0], np.cumsum(new)])
+        starts = np.append(np.stack([start[:-1], start[:-1] + context], 1).ravel(), start[-1])
+        ver = VerifyBufs(gpu, np.zeros((n_rows, V), np.float32), None, ids, starts, np.zeros(2 * n), np.zeros(n_rows),
+                         np.zeros(2 * n), 1 + max_drafts)
+        ver.logits = logits
+        ver.run()
+        accepted, tokens = (x[1::2] for x in ver.result())
+        held, table, free, n_free = plan.held.numpy(), plan.table.numpy(), plan.free.numpy(), int(plan.n_free.numpy()[0])
+        status = plan.status.numpy()
+        kinds.add(tuple(sorted({"waits" if s else "prompt" if c else "drafts" if len(x) > 1 else "token"
+                                for s, c, x in zip(status, context, rows) if len(x)})))
+        if not any(len(x) and not s for s, x in zip(status, rows)):
+            r = max(r for r in range(n) if rows[r] and held[r])
+            prompts[r], cached[r], drafts[r] = prompts[r] + done[r][len(prompts[r]) - asked[r]:], 0, []
+        for r in range(n):
+            if status[r] or not rows[r]:
+                continue
+            cached[r] += context[r]
+            if context[r] < len(rows[r]):
+                cached[r] += 1 + accepted[r]
+                done[r] += tokens[r, :accepted[r] + 1].tolist()
+                accepted_drafts += int(accepted[r])
+            else:
+                assert accepted[r] == -1
+            known = want[r][len(done[r]):len(done[r]) + int(rng.integers(0, max_drafts + 1))]
+            drafts[r] = [t if rng.random() < 0.8 else (t + 1) % V for t in known]
+    m.close()
+    assert [d[:steps] for d in done] == want
+    assert accepted_drafts > 8 and any({"waits", "drafts", "prompt"} <= set(k) for k in kinds), kinds
