@@ -123,8 +123,12 @@ int hy_rope_qknorm_paged(const float* qkv_dev, uint32_t n_rows, uint32_t n_heads
  * query head h reads kv head h / (n_heads / n_kv_heads).  Products and sums have f32
  * accuracy whatever the cache's type, relative to the largest elements of q, of a key and
  * of a value row: one below 2^-16 of its vector's largest is taken to 2^-39 of that, values
- * to 2^-98 at least.  A key that a row does not see does not touch it, whatever it holds; an
- * infinity or NaN in q or in a key that a row sees makes the row NaN.  ws_dev:
+ * to 2^-98 at least.  Small weights over f16 caches, and over the others in long chunks small
+ * products of a weight and its value row, are taken to 2^-31 of the row's largest.  Values
+ * up to 2^96 sum without overflow; scores past f32's range are not defined.
+ * A key that a row does not see does not touch it, whatever it holds; an infinity or NaN in q
+ * or in a key that a row sees makes the row NaN, one in a value makes that element infinite
+ * or NaN (with a weight of 0 it may be left out).  ws_dev:
  * hy_paged_attention_ws bytes (0 for bad arguments; by the cache's and the batch's sizes,
  * 103 MB at most), aligned to 16 bytes, contents indifferent. */
 size_t hy_paged_attention_ws(uint32_t n_heads, const hy_paged_cache* cache, const hy_paged_batch* batch);
@@ -132,12 +136,7 @@ int hy_paged_attention(const float* q_dev, uint32_t n_heads, const hy_paged_cach
                        float scale, float* out_dev, void* ws_dev, size_t ws_bytes, void* stream);
 
 /* The verification of drafted tokens by speculative sampling.  Request r's rows
- * q_start[r] .. q_start[r + 1] - 1 of ids are its last token and its drafts x_1 .. x_n: every
- * row after the first is taken for a draft.  Rows that are none (a prompt's but the last, those of a
- * request that was not served) are kept apart by a q_start of its own with two entries per
- * request, [start, start + context rows]: the even results, of context rows, mean nothing (with
- * more than max_new rows they are -1), the odd ones are of the rows behind, -1 where there are
- * none.  So a prompt's last piece has one verified row, its last token, and gets its first new token.
+ * q_start[r] .. q_start[r + 1] - 1 of ids are its last token and its drafts x_1 .. x_n;
  * row i of logits is the target's prediction of what follows row i, and row i of
  * draft_probs [n_rows][vocab] the distribution that x_{i+1} was drawn from (NULL: drafts
  * without probabilities, as certain).  With p = softmax(logits / temperature[r]) (NULL: 1),
@@ -153,7 +152,13 @@ int hy_paged_attention(const float* q_dev, uint32_t n_heads, const hy_paged_cach
  *                              that gives no distribution (a logit that is NaN or +inf, all
  *                              -inf) ends its request with next token -1.
  * Drafts outside 0..vocab-1 are refused.  u in [0, 1).  ws_dev: hy_verify_drafts_ws bytes
- * (0 for bad arguments), aligned to 16 bytes, contents indifferent. */
+ * (0 for bad arguments), aligned to 16 bytes, contents indifferent.
+ *
+ * Every row after a request's first is taken for a draft.  Rows that are none (a prompt's but
+ * its last) are kept apart by a q_start of this call's own, with two entries per request:
+ * its start, and its start + such rows.  Results 2 r are theirs and mean nothing (-1 for more
+ * than max_new rows); results 2 r + 1 are of the rows behind, -1 where there are none.  So
+ * the last piece of a prompt has one row here, its last token, and gets the first new token. */
 size_t hy_verify_drafts_ws(uint32_t n_req, uint32_t n_rows, uint32_t vocab);
 int hy_verify_drafts(const float* logits_dev, const float* draft_probs_dev, const int32_t* ids_dev,
                      const int32_t* q_start_dev, uint32_t n_req, uint32_t n_rows, uint32_t max_new, uint32_t vocab,

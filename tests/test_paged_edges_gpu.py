@@ -363,3 +363,37 @@ def test_server_step_with_prompts_drafts_and_waiting_requests(gpu):
     m.close()
     assert [d[:steps] for d in done] == want
     assert accepted_drafts > 8 and any({"waits", "drafts", "prompt"} <= set(k) for k in kinds), kinds
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("wtype", [F32, F16, BF16])
+def test_attention_small_weights_of_large_values(gpu, wtype, kernel):
+    """Weights down to 2^-40 of the largest, of values up to 2^25 times the others'.  Beside an f32
+    evaluation's error: over f16 a weight is off by up to 2^-31 of the largest one (f16 pieces of
+    2^6 times it end at 2^-24, half a step 2^-25), in the tiles of the others a weight times 2^e,
+    e the exponent of its value row's largest, by as much of the largest such product."""
+    rng = np.random.default_rng(79)
+    kv, n, hd = 300, 40, 128
+    pool, table, q_start, kv_len = make_batch(rng, [(kv, n)], 16, 2, hd, wtype, k_std=0.01)
+    q = (rng.standard_normal((n, 8, hd)) * 0.01).astype(np.float32)
+    q[:, :, 0] = 8.0
+    depth = rng.integers(0, 41, kv)
+    depth[0] = 0
+    for j in range(kv):
+        at(pool, pool.k, table, 0, j)[:, 0] = R.encode(np.full(2, -depth[j] * np.log(2) * hd ** 0.5 / 8, np.float32), wtype)
+        x = rng.standard_normal((2, hd)).astype(np.float32) * np.float32(2.0 ** -10 if depth[j] < 20 else 2.0 ** 13)
+        at(pool, pool.v, table, 0, j)[:] = R.encode(x, wtype)
+    args = (q, pool, q_start, kv_len, table, hd ** -0.5)
+    want, dot, pv = R.attention(*args)
+    bound = R.attention_bound(dot, pv, hd, kv)
+    k = np.stack([R.decode(at(pool, pool.k, table, 0, j), wtype) for j in range(kv)])
+    v = np.abs(np.stack([R.decode(at(pool, pool.v, table, 0, j), wtype) for j in range(kv)]))
+    for t in range(n):
+        for h in range(8):
+            p = R.softmax64(k[:kv - n + t + 1, h // 4] @ q[t, h].astype(np.float64) * hd ** -0.5)
+            seen = v[:len(p), h // 4]
+            size = 2.0 ** np.floor(np.log2(seen.max(1)))
+            bound[t, h] += 2.0 ** -31 * (p.max() * seen.sum(0) if wtype == F16
+                                         else (p * size).max() * (seen / size[:, None]).sum(0))
+    got = attend(gpu, *args, max_new=KERNELS[kernel])
+    assert (np.abs(got - want) <= bound).all()
