@@ -397,3 +397,57 @@ def test_attention_small_weights_of_large_values(gpu, wtype, kernel):
                                          else (p * size).max() * (seen / size[:, None]).sum(0))
     got = attend(gpu, *args, max_new=KERNELS[kernel])
     assert (np.abs(got - want) <= bound).all()
+
+
+def test_captured_model_step(gpu):
+    """hy_model_forward_paged of a padded batch in one graph, replayed with other contents, with eager
+    calls of another context and synchronizations between: every replay equals the eager call."""
+    rng = np.random.default_rng(78)
+    nh, nkv, hd, page, V, L = 8, 2, 64, 8, 500, 2
+    n_pages, max_pages, lens = 20, 5, [(17, 9), (30, 1), (6, 6)]
+
+    class Step:
+        def __init__(self):
+            self.m = greedy_model(gpu)[0]
+            self.pool = Pool(n_pages * L, page, nkv, hd, BF16)
+            self.kb, self.vb = upload(gpu, self.pool)
+            self.cache = gpu.PagedCache(self.kb, self.vb, BF16, n_pages, page, nkv, hd,
+                                        layer_stride=n_pages * nkv * page * hd)
+            self.n_rows = 18
+            i32 = lambda a: dev(gpu, a, np.int32)  # noqa: E731
+            table = np.arange(15).reshape(3, 5)
+            pos = [kv - n + i for kv, n in lens for i in range(n)]
+            req = [r for r, (_, n) in enumerate(lens) for _ in range(n)]
+            slots = [table[r, p // page] * page + p % page for r, p in zip(req, pos)] + [-1, -1]
+            self.batch = gpu.PagedBatch(3, self.n_rows, max_pages, 9, i32([0, 9, 10, 16]), i32([kv for kv, _ in lens]),
+                                        i32(table), i32(pos + [0, 0]), i32(slots))
+            self.ids, self.logits = i32(np.zeros(18)), dev(gpu, np.zeros((18, V), np.float32))
+            self.ws = Ws(gpu, nh, self.cache, self.batch)
+
+        def fill(self, ids):
+            gpu.check(gpu.lib().hy_memcpy_h2d(self.ids.ptr, ids.ctypes.data, ids.nbytes))
+
+        def run(self, st):
+            self.m.forward_paged(self.ids, self.cache, self.batch, self.logits, self.ws.b, self.ws.n, st)
+
+    st, a, b = gpu.Stream(), Step(), Step()
+    a.run(st.h)                      # what a first call sets up is set up
+    st.synchronize()
+    g = gpu.Graph(st, lambda: a.run(st.h))
+    try:
+        for rep in range(4):
+            ids = rng.integers(0, V, 18).astype(np.int32)
+            a.fill(ids)
+            b.fill(ids)
+            b.run(st.h)
+            st.synchronize()
+            g.launch()
+            st.synchronize()
+            for p, q in ((a.kb, b.kb), (a.vb, b.vb), (a.logits, b.logits)):
+                np.testing.assert_array_equal(p.numpy(), q.numpy())
+            assert np.isfinite(a.logits.numpy()).all()
+    finally:
+        g.close()
+        st.close()
+        a.m.close()
+        b.m.close()
