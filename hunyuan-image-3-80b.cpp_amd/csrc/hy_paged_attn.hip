@@ -555,7 +555,8 @@ static PaPlan pa_plan(int type, int n_req, int max_new, int G, int hd) {
     const bool many = rows > pf_max_rows(type, n_req, hd), few = !many || n_req > 1;
     PaPlan p;
     // Beside chunks the stream's requests are mostly single tokens: 16 rows (12 requests of chunks and
-    // tokens, bf16, 414 -> 406 us; 32 rows would spare drafts a second reading of K and V).
+    // tokens, bf16, 414 -> 406 us; 32 rows would spare drafts beside chunks a second reading of K and V,
+    // which was not timed).
     // Starting an item is worth 16 keys of a full stream, 256 of a many-row tile (20 000 of its 3500
     // to 6500 cycles per 32 keys); a stretch is 32 keys at least (64: one request of
     // 1000 keys 12.6 us, 32: 10.2), 128.  Cuts within 32, 128 of an item's end move there: a small

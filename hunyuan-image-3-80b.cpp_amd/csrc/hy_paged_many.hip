@@ -23,13 +23,14 @@
 // lane pair and its weights are the operand of O^T += V^T W^T as they lie.
 //
 // Bound by instruction issue and the power it draws: a SIMD's two waves have, per block and head_dim
-// 128 of a bf16 cache, 64 products (20 cycles each back to back, 33 from one wave) and 2700 cycles
-// of vector operations (half of them the softmax), and take 4700; matrix and vector work of
-// different waves do not overlap here (running the waves half a block apart changed nothing), and
-// the clock falls to 1.6 GHz under it.  2048 rows of 32 heads behind 8192 keys, f32: 1.08 ms back to
-// back, 286 TFLOP/s of attention and three times that of f16 products (a large f16 matrix product
-// reaches 1110); head_dim 64, five prompts of up to 1500 tokens, f16: 61 us, of which 20 000 cycles
-// (10 us) per piece go to its start and end.
+// 128 of a bf16 cache, 64 products (32 cycles each, 2050) and 2700 cycles of vector operations
+// (half of them the softmax), and take 4700, about their sum (running the waves half a block apart
+// changed nothing; what keeps the two kinds of work apart is not known), and the clock falls to
+// 1.6 GHz under it.  2048 rows of 32 heads behind 8192 keys, f32: 0.93 ms (the first passes of
+// a run 1.07), 330 TFLOP/s of attention and three times that of f16 products (a large f16 matrix
+// product reaches 1110, the instruction alone 2090); head_dim 64, five prompts of up to 1500 tokens,
+// f16: 61 us, of which 20 000 cycles (10 us) per piece go to its start and end.  The f32 kernel
+// of head_dim 128 spills 36 vector registers, the others none.
 //
 // Keys that no row sees are stored as zeros and masked; where V holds an infinity or NaN, which 0
 // times a weight would not keep out, or 2^35 and more under scaling, the piece is computed again

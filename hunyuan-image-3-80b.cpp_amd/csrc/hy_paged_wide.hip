@@ -10,7 +10,9 @@
 // the exponent, so a row's sum carries it too.
 // Bound by the bytes of K and V and by what a wave does between its loads: 32 requests of 6 tokens
 // over f16 caches of up to 2900 keys (255 MB) 67 us (on 16 x 16 tiles 74), 3.8 TB/s, of which
-// some 10 us are the start and the end of a launch.
+// some 10 us are the start and the end of a launch.  At head_dim 128 the f16 kernel spills 35
+// registers, and the bf16 one, of three pieces, has one wave per SIMD (365 registers; not
+// timed by itself).
 #include "hy_device.hpp"
 #include "hy_paged.hpp"
 #include "hy_paged_part.hpp"
