@@ -125,7 +125,7 @@ int hy_rope_qknorm_paged(const float* qkv_dev, uint32_t n_rows, uint32_t n_heads
  * of a value row: one below 2^-16 of its vector's largest is taken to 2^-39 of that, values
  * to 2^-98 at least.  Small weights over f16 caches, and over the others in long chunks small
  * products of a weight and its value row, are taken to 2^-31 of the row's largest.  Values
- * up to 2^96 sum without overflow; scores past f32's range are not defined.
+ * up to 2^88 sum without overflow; scores past f32's range are not defined.
  * A key that a row does not see does not touch it, whatever it holds; an infinity or NaN in q
  * or in a key that a row sees makes the row NaN, one in a value makes that element infinite
  * or NaN (with a weight of 0 it may be left out).  ws_dev:
