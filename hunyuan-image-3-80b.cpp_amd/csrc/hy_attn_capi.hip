@@ -225,8 +225,8 @@ struct PagedStep {
     size_t ws_bytes;
 };
 
-// Do `layers` pools, `stride` elements apart, share no element?  Side by side, or each inside the gaps
-// of the last one's smallest stride above `stride`.
+// Do `layers` pools, `stride` elements apart, share no element?  Side by side, or all of them within one
+// step of the pool's smallest stride from `stride` on.
 bool pools_apart(const hy::PagedView& v, uint64_t stride, size_t layers) {
     typedef unsigned __int128 wide;  // 2^28 pages of 2^40 elements
     const wide n[] = {(wide)v.n_pages, (wide)v.nkv, (wide)1 << v.shift};
