@@ -7,7 +7,7 @@
  * `stream` = hipStream_t as void* (NULL: default stream), HY_OK or a negative hy_status
  * with hy_last_error() set; arguments are checked before anything is launched.  Calls
  * without a context run on the calling thread's current device (hy_set_device), which the
- * stream and all pointers belong to.  Every call only launches kernels on its stream: it
+ * stream and all pointers belong to.  Every call only queues work on its stream: it
  * returns without waiting, allocates nothing, and can be captured into a graph.  Calls
  * that overlap in time, captured graphs among them, need workspaces of their own, and
  * contexts of their own where they take one.
