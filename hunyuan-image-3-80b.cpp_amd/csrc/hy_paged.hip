@@ -5,6 +5,7 @@
 //    [rows][nh][hd], keys and values to their slots in the cache's type.
 #include "hy_device.hpp"
 #include "hy_paged.hpp"
+#include "hy_paged_rotary.hpp"
 #include "hy_paged_split.hpp"
 
 namespace hy {
@@ -188,17 +189,11 @@ hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t s) {
 // The units of a row are its heads in memory order: nh query heads, nkv key heads, nkv value
 // heads.  A work group takes a group of PA_STEPS * 64 / (HD / 4) units of four consecutive rows, a
 // row per wave (neighbouring rows are neighbours in a page); HD / 4 lanes share a unit, 4 dims
-// (16 bytes) each, and all loads of a wave go out before anything else.  An angle is kept as a
-// fraction of a turn in 64 bits, position times turns per position minus its whole part, so a
-// far position costs no accuracy; sine and cosine are f32, of its f32 part, and turned by the rest.
+// (16 bytes) each, and all loads of a wave go out before anything else.  Angles and norm:
+// hy_paged_rotary.hpp.
 // Bound by memory: 4096 rows of 48 heads of 128 (205 MB) 33 us in caches, 40 from memory (5.2 TB/s);
 // 5 rows 4.4 us, all of it latency.
 constexpr int PA_STEPS = 4;
-
-template <int CTRL>
-__device__ __forceinline__ float dpp_f(float v) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, false));
-}
 
 template <class E, int HD>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
@@ -232,15 +227,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
     if (u0 < a.nh + a.c.nkv) {  // not values alone
         if (a.rotate == 1) {
 #pragma unroll
-            for (int p = 0; p < 2; p++) {
-                double turn = (double)pos * a.freq[d / 2 + p];
-                turn = 2.0 * (turn - rint(turn));  // in half turns
-                const float half = (float)turn, rest = (float)(turn - (double)half) * 3.14159265f;
-                float s0, c0;
-                sincospif(half, &s0, &c0);
-                sn[p] = fmaf(rest, c0, s0);
-                cs[p] = fmaf(-rest, s0, c0);
-            }
+            for (int p = 0; p < 2; p++) rope_angle(pos, a.freq[d / 2 + p], sn[p], cs[p]);
         } else if (a.rotate == 2) {
             const v4f_t c = *reinterpret_cast<const v4f_t*>(a.cos_t + (int64_t)pos * HD + d);
             const v4f_t s = *reinterpret_cast<const v4f_t*>(a.sin_t + (int64_t)pos * HD + d);
@@ -261,16 +248,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
             y[2 * p] = fmaf(x[s][2 * p], cs[p], -(x[s][2 * p + 1] * sn[p]));
             y[2 * p + 1] = fmaf(x[s][2 * p], sn[p], x[s][2 * p + 1] * cs[p]);
         }
-        float ss = (y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]);
-        ss += dpp_f<0x128>(ss);  // rotations by 8 .. 1 in 16 lanes
-        ss += dpp_f<0x124>(ss);
-        ss += dpp_f<0x122>(ss);
-        ss += dpp_f<0x121>(ss);
-        if constexpr (LPU == 32) ss = fadd_row(ss);
-        // 1 / sqrt rounded once: the 64-bit estimate (2^-24) and a step of Newton's, fewer operations than
-        // an f32 root and quotient
-        const double ms = fma((double)ss, 1.0 / HD, (double)a.eps), e = __builtin_amdgcn_rsq(ms);
-        const float rms = ms > 0.0 && ms < (double)INFINITY ? (float)fma(0.5 * e, fma(-ms * e, e, 1.0), e) : (float)e;
+        const float rms = head_rms<HD>(y, a.eps);
         if (u < a.nh) {
             *reinterpret_cast<v4f_t*>(a.q + ((int64_t)t * a.nh + u) * HD + d) = y * rms * wq;
         } else if (u < units) {

@@ -18,6 +18,8 @@ struct PagedView {
     int type, n_pages, shift, nkv, hd;               // page_size = 1 << shift
 };
 
+struct PagedViewI8;  // hy_int8.hpp
+
 struct PagedPlanArgs {
     const int* cached;
     const int* add;
@@ -90,13 +92,14 @@ hipError_t launch_verify_drafts(const VerifyArgs& a, hipStream_t s);
 size_t verify_ws_bytes(int n_req, int n_rows, int vocab);
 
 // host checks shared by the calls (hy_paged_capi.hip): HY_OK, or a status with the last error set
-int paged_cache_check(const hy_paged_cache* cache, uint32_t n_heads, PagedView* out);
+// only: the one type that is taken; 0: those of hy_paged.h
+int paged_cache_check(const hy_paged_cache* cache, uint32_t n_heads, PagedView* out, int only = 0);
 int paged_batch_check(const hy_paged_batch* b, const PagedView& c, bool writes);
 int paged_rotary_check(float theta, const float* cos_t, const float* sin_t, uint32_t n_pos, float eps);
 int paged_append(const float* qkv, uint32_t n_rows, uint32_t n_heads, const PagedView& c, const int32_t* positions,
                  const int32_t* slots, float theta, const float* cos_t, const float* sin_t, uint32_t n_pos,
                  const float* q_norm, const float* k_norm, float eps, float* q, hipStream_t s,
-                 float* merged = nullptr, const int32_t* row_end = nullptr);
+                 float* merged = nullptr, const int32_t* row_end = nullptr, const PagedViewI8* i8 = nullptr);
 size_t paged_batch_ws(const hy_paged_batch* b, uint32_t n_heads, const PagedView& c);
 int paged_ws_check(const hy_paged_batch* b, uint32_t n_heads, const PagedView& c, const void* ws, size_t ws_bytes);
 int paged_attention(const float* q, uint32_t n_heads, const PagedView& c, const hy_paged_batch* b, float scale,

@@ -6,7 +6,7 @@
 #include <cstdio>
 #include <string>
 
-#include "hy_paged.hpp"
+#include "hy_int8.hpp"
 
 namespace hy {
 int set_last_error(int code, const std::string& msg);  // hy_capi.hip
@@ -72,10 +72,11 @@ int verify_check(uint32_t n_req, uint32_t n_rows, uint32_t vocab) {
 
 namespace hy {
 
-int paged_cache_check(const hy_paged_cache* c, uint32_t n_heads, PagedView* out) {
+int paged_cache_check(const hy_paged_cache* c, uint32_t n_heads, PagedView* out, int only) {
     if (!c) return fail(HY_ERR_INVALID, "null cache");
     if (!c->k_dev || !c->v_dev) return fail(HY_ERR_INVALID, "null cache pointer");
-    if (c->type != HY_TYPE_F32 && c->type != HY_TYPE_F16 && c->type != HY_TYPE_BF16)
+    if (only && c->type != only) return fail(HY_ERR_UNSUPPORTED, "cache type %d: %d expected", c->type, only);
+    if (!only && c->type != HY_TYPE_F32 && c->type != HY_TYPE_F16 && c->type != HY_TYPE_BF16)
         return fail(HY_ERR_UNSUPPORTED, "cache type %d: F32, F16 or BF16 expected", c->type);
     const int shift = page_shift(c->page_size);
     if (shift < 0)
@@ -93,7 +94,7 @@ int paged_cache_check(const hy_paged_cache* c, uint32_t n_heads, PagedView* out)
         hs = ts * c->page_size;
         ps = hs * c->n_kv_heads;
     }
-    const uint64_t unit = c->type == HY_TYPE_F32 ? 4 : 8;  // 16 bytes
+    const uint64_t unit = c->type == HY_TYPE_F32 ? 4 : c->type == HY_TYPE_I8 ? 16 : 8;  // 16 bytes
     if (ts < c->head_dim || hs < c->head_dim || ps < c->head_dim)
         return fail(HY_ERR_INVALID, "cache strides %llu / %llu / %llu below head_dim", (unsigned long long)ps,
                     (unsigned long long)hs, (unsigned long long)ts);
@@ -129,7 +130,7 @@ int paged_rotary_check(float theta, const float* cos_t, const float* sin_t, uint
 int paged_append(const float* qkv, uint32_t n_rows, uint32_t n_heads, const PagedView& c, const int32_t* positions,
                  const int32_t* slots, float theta, const float* cos_t, const float* sin_t, uint32_t n_pos,
                  const float* q_norm, const float* k_norm, float eps, float* q, hipStream_t s,
-                 float* merged, const int32_t* row_end) {
+                 float* merged, const int32_t* row_end, const PagedViewI8* i8) {
     if (!qkv || !positions || !slots || !q) return fail(HY_ERR_INVALID, "null pointer");
     if (n_rows == 0 || n_rows > 1u << 20) return fail(HY_ERR_INVALID, "n_rows=%u must be in 1..2^20", n_rows);
     HY_TRY(paged_rotary_check(theta, cos_t, sin_t, n_pos, eps));
@@ -145,7 +146,7 @@ int paged_append(const float* qkv, uint32_t n_rows, uint32_t n_heads, const Page
             for (int r = 0; r < 8; r++) a.freq[8 * p + r] = high * low[r];
         }
     }
-    HIP_TRY(launch_paged_append(a, s));
+    HIP_TRY(i8 ? launch_paged_append_i8(a, *i8, s) : launch_paged_append(a, s));
     return HY_OK;
 }
 

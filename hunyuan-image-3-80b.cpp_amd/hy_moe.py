@@ -18,9 +18,11 @@ ROOT = os.path.dirname(HERE)
 HEADER = os.path.join(ROOT, "include", "hy_moe.h")
 ATTN_HEADER = os.path.join(ROOT, "include", "hy_attn.h")
 PAGED_HEADER = os.path.join(ROOT, "include", "hy_paged.h")
+INT8_HEADER = os.path.join(ROOT, "include", "hy_int8.h")
 
 F32, Q4_0, Q8_0 = 0, 2, 8
 F16, BF16 = 1, 30  # cache types besides F32
+I8 = 24            # of PagedCacheI8's pool
 PATH_AUTO, PATH_VALU, PATH_MFMA = 0, 1, 2
 TENSOR_X, TENSOR_ROUTER, TENSOR_GU, TENSOR_DN = 0, 1, 2, 3
 
@@ -66,6 +68,18 @@ class PagedCache(C.Structure):
     def __init__(self, k, v, wtype, n_pages, page_size, nkv, hd, strides=(0, 0, 0), layer_stride=0):
         super().__init__(k.ptr, v.ptr, wtype, n_pages, page_size, nkv, hd, *strides, layer_stride)
         self.keep = (k, v)
+
+
+class PagedCacheI8(C.Structure):
+    """hy_paged_cache_i8: a pool (PagedCache of type I8) with scales (objects with .ptr) per block of positions."""
+    _fields_ = [
+        ("pool", PagedCache), ("k_scale_dev", C.c_void_p), ("v_scale_dev", C.c_void_p), ("block", C.c_uint32),
+        ("layer_scale_stride", C.c_uint64),
+    ]
+
+    def __init__(self, pool, k_scale, v_scale, block, layer_scale_stride=0):
+        super().__init__(pool, k_scale.ptr, v_scale.ptr, block, layer_scale_stride)
+        self.keep = (pool, k_scale, v_scale)
 
 
 class PagedBatch(C.Structure):
@@ -183,6 +197,16 @@ _SIGS = {
                                         _vp, _vp, C.c_size_t, _vp]),
     "hy_model_forward_paged": (C.c_int, [_vp, _vp, C.POINTER(PagedCache), C.POINTER(PagedBatch), _vp, _vp,
                                          C.c_size_t, _vp]),
+    "hy_quantize_rows_i8": (C.c_int, [_vp, _u32, _u32, _vp, _vp, _vp]),
+    "hy_gemm_i8_ws": (C.c_size_t, [_u32, _u32, _u32]),
+    "hy_gemm_i8": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, C.c_size_t, _vp]),
+    "hy_linear_i8_ws": (C.c_size_t, [_u32, _u32, _u32]),
+    "hy_linear_i8": (C.c_int, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, C.c_size_t, _vp]),
+    "hy_rope_qknorm_paged_i8": (C.c_int, [_vp, _u32, _u32, C.POINTER(PagedCacheI8), _vp, _vp, _f, _vp, _vp, _u32, _vp,
+                                          _vp, _f, _vp, _vp]),
+    "hy_paged_attention_i8_ws": (C.c_size_t, [_u32, C.POINTER(PagedCacheI8), C.POINTER(PagedBatch)]),
+    "hy_paged_attention_i8": (C.c_int, [_vp, _u32, C.POINTER(PagedCacheI8), C.POINTER(PagedBatch), _f, _vp, _vp,
+                                        C.c_size_t, _vp]),
 }
 
 _lib = None
@@ -809,3 +833,59 @@ def verify_drafts(logits, draft_probs, ids, q_start, n_req, n_rows, max_new, voc
                                  q_start.ptr, n_req, n_rows, max_new, vocab,
                                  temperature.ptr if temperature is not None else None, u_accept.ptr, u_sample.ptr,
                                  accepted.ptr, tokens.ptr, ws.ptr, ws_bytes, stream))
+
+
+# ------------------------------------------------------------------ serving in 8 bits
+
+def _ptr(b):
+    return b.ptr if b is not None else None
+
+
+def quantize_rows_i8(x, rows, cols, codes, scales, stream=None):
+    """8-bit codes and scales of the rows of x (hy_quantize_rows_i8)."""
+    check(lib().hy_quantize_rows_i8(x.ptr, rows, cols, codes.ptr, scales.ptr, stream))
+
+
+def _ws(n):
+    if n == 0:
+        check(-1)
+    return n
+
+
+def gemm_i8_ws(T, hidden, n_out):
+    """Workspace bytes of gemm_i8."""
+    return _ws(lib().hy_gemm_i8_ws(T, hidden, n_out))
+
+
+def gemm_i8(x, x_scale, w, w_scale, resid, T, hidden, n_out, out, ws, ws_bytes, stream=None):
+    """The product of codes with their scales, resid (or None) added (hy_gemm_i8)."""
+    check(lib().hy_gemm_i8(x.ptr, x_scale.ptr, w.ptr, w_scale.ptr, _ptr(resid), T, hidden, n_out, out.ptr, ws.ptr,
+                           ws_bytes, stream))
+
+
+def linear_i8_ws(T, hidden, n_out):
+    """Workspace bytes of linear_i8."""
+    return _ws(lib().hy_linear_i8_ws(T, hidden, n_out))
+
+
+def linear_i8(x, w, w_scale, resid, T, hidden, n_out, out, ws, ws_bytes, stream=None):
+    """f32 tokens, quantized, times 8-bit weights (hy_linear_i8)."""
+    check(lib().hy_linear_i8(x.ptr, w.ptr, w_scale.ptr, _ptr(resid), T, hidden, n_out, out.ptr, ws.ptr, ws_bytes,
+                             stream))
+
+
+def rope_qknorm_paged_i8(qkv, n_rows, nh, cache, positions, slots, theta, cos, sin, n_pos, q_norm, k_norm, eps, q,
+                         stream=None):
+    """Rotary embedding, QK-norm and the write of an 8-bit cache (hy_rope_qknorm_paged_i8)."""
+    check(lib().hy_rope_qknorm_paged_i8(qkv.ptr, n_rows, nh, cache, positions.ptr, slots.ptr, theta, _ptr(cos),
+                                        _ptr(sin), n_pos, _ptr(q_norm), _ptr(k_norm), eps, q.ptr, stream))
+
+
+def paged_attention_i8_ws(nh, cache, batch):
+    """Workspace bytes of paged_attention_i8."""
+    return _ws(lib().hy_paged_attention_i8_ws(nh, cache, batch))
+
+
+def paged_attention_i8(q, nh, cache, batch, scale, out, ws, ws_bytes, stream=None):
+    """Attention of the batch's rows over an 8-bit cache (hy_paged_attention_i8)."""
+    check(lib().hy_paged_attention_i8(q.ptr, nh, cache, batch, scale, out.ptr, ws.ptr, ws_bytes, stream))
