@@ -57,13 +57,7 @@ hipError_t launch_paged_append_i8(const PagedAppendArgs& a, const PagedViewI8& v
 // host checks and calls that the C entries share (hy_int8_capi.hip)
 int paged_cache_i8_check(const hy_paged_cache_i8* cache, uint32_t n_heads, PagedViewI8* out);
 
-struct PagedAttnI8Args {
-    PagedAttnArgs a;
-    const float* ks;
-    const float* vs;
-    int bshift;
-};
-hipError_t launch_paged_attn_i8(const PagedAttnI8Args& a, int max_new, hipStream_t s);
+hipError_t launch_paged_attn_i8(const PagedAttnArgs& a, int max_new, hipStream_t s);
 size_t paged_attn_i8_ws_bytes(int n_req, int max_new, int G, int hd);
 
 }  // namespace hy

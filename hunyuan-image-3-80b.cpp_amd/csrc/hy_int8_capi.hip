@@ -88,9 +88,9 @@ int paged_attention_i8(const float* q, uint32_t n_heads, const PagedViewI8& v, c
     if (!std::isfinite(scale)) return fail(HY_ERR_INVALID, "scale is not finite");
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(HY_ERR_INVALID, "q and out must be aligned to 16 bytes");
     HY_TRY(ws_check(ws, ws_bytes, paged_batch_i8_ws(b, n_heads, v)));
-    const PagedAttnI8Args a{{q, out, v.c, (int)n_heads, (int)b->n_req, (int)b->n_rows, (int)b->max_pages,
-                             b->q_start_dev, b->kv_len_dev, b->table_dev, b->seen_dev, scale, static_cast<float*>(ws)},
-                            v.ks, v.vs, v.bshift};
+    const PagedAttnArgs a{q, out, v.c, (int)n_heads, (int)b->n_req, (int)b->n_rows, (int)b->max_pages, b->q_start_dev,
+                          b->kv_len_dev, b->table_dev, b->seen_dev, scale, static_cast<float*>(ws), v.ks, v.vs,
+                          v.bshift};
     HIP_TRY(launch_paged_attn_i8(a, (int)(b->max_new < b->n_rows ? b->max_new : b->n_rows), s));
     return HY_OK;
 }

@@ -71,6 +71,9 @@ struct PagedAttnArgs {
     const int* seen;  // or null: causal
     float scale;
     float* ws;
+    const float* ks;  // of an 8-bit cache: the scales, of blocks of 1 << bshift positions
+    const float* vs;
+    int bshift;
 };
 hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s);
 size_t paged_attn_ws_bytes(int type, int n_req, int max_new, int G, int hd);

@@ -151,6 +151,10 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
 #pragma unroll
                         for (int c = 0; c < PC; c++) qf[t][s][c][j] = (int)w[c];
                     }
+                if constexpr (F16T) {
+#pragma unroll
+                    for (int s = 0; s < NQ; s++) settle(qf[t][s][1]);
+                }
             }
         }
 
@@ -351,6 +355,10 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
 #pragma unroll
                             for (int q = 0; q < PC; q++) pf[c][q][2 * u + v] = (int)w[q];
                         }
+                if constexpr (F16T) {
+#pragma unroll
+                    for (int c = 0; c < NT; c++) settle(pf[c][1]);
+                }
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
                     v4i_t vf;  // dims VD i + d of keys 4 g4 .. + 3 of both tiles
@@ -526,10 +534,6 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartSh
 
 constexpr int PJ_ROWS = 8;  // rows of a stream's item per work group of the join
 
-// which launches a batch takes: workers 0: not that one
-struct PaPlan {
-    PartShape few, many;
-};
 constexpr int PF_ROWS = 32;
 // Rows of the largest request up to which the streams take a whole batch; past it they take the
 // requests of PF_ROWS rows at most (f16, 14 requests of up to 744 rows: 50, all up to 128 rows 62).
@@ -598,6 +602,11 @@ hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s)
             big ? launch_few<__bf16, 128>(a, p.few, s) : launch_few<__bf16, 64>(a, p.few, s);
     }
     if (p.many.workers) launch_paged_many(a, p.many, s);
+    return launch_paged_join(a, p, s);
+}
+
+hipError_t launch_paged_join(const PagedAttnArgs& a, const PaPlan& p, hipStream_t s) {
+    const bool big = a.c.hd == 128;
     const int splits = p.few.M / PJ_ROWS;
     const int many_splits = a.c.hd / 4;  // a tile of few pieces: one set of rows per work group
     const dim3 grid(p.few.workers * splits + p.many.workers * many_splits);

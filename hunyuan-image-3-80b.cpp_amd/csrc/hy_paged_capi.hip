@@ -169,7 +169,7 @@ int paged_attention(const float* q, uint32_t n_heads, const PagedView& c, const 
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(HY_ERR_INVALID, "q and out must be aligned to 16 bytes");
     HY_TRY(paged_ws_check(b, n_heads, c, ws, ws_bytes));
     const PagedAttnArgs a{q, out, c, (int)n_heads, (int)b->n_req, (int)b->n_rows, (int)b->max_pages, b->q_start_dev,
-                          b->kv_len_dev, b->table_dev, b->seen_dev, scale, static_cast<float*>(ws)};
+                          b->kv_len_dev, b->table_dev, b->seen_dev, scale, static_cast<float*>(ws), nullptr, nullptr, 0};
     HIP_TRY(launch_paged_attn(a, (int)(b->max_new < b->n_rows ? b->max_new : b->n_rows), s));
     return HY_OK;
 }

@@ -344,4 +344,11 @@ void launch_paged_wide(const PagedAttnArgs& a, const PartShape& ps, hipStream_t 
 constexpr int PM_TILE_SHIFT = 8, PM_TILE = 1 << PM_TILE_SHIFT, PM_WORKERS = 256;
 void launch_paged_many(const PagedAttnArgs& a, const PartShape& ps, hipStream_t s);
 
+// which launches a batch takes: workers 0: not that one
+struct PaPlan {
+    PartShape few, many;
+};
+// joins what both left in pieces (hy_paged_attn.hip)
+hipError_t launch_paged_join(const PagedAttnArgs& a, const PaPlan& p, hipStream_t s);
+
 }  // namespace hy

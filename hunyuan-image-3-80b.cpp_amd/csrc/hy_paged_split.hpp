@@ -54,6 +54,35 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32
     asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(lo) : "v"(hi), "v"(a));
     asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(lo) : "v"(hi), "v"(b));
 }
+// Two wait states have to pass before a matrix instruction reads what a vector instruction wrote.  The
+// compiler sees to that for its own instructions, not for those of inline asm: an operand of split_f16's
+// remainders goes through here first (without it an operand's last half was read before it was written).
+__device__ __forceinline__ void settle(v4i_t& x) { asm("s_nop 1" : "+v"(x)); }
+
+// 8-bit codes as f16, exactly: with its sign flipped and 0x64 above it a byte is 1024 + 128 + code.
+// four codes of a dword, in their order
+__device__ __forceinline__ uint32_t f16_less_1152(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h16_t, w) + (v2h16_t){(_Float16)-1152, (_Float16)-1152});
+}
+__device__ __forceinline__ void i8_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    w ^= 0x80808080u;
+    lo = f16_less_1152(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u));
+    hi = f16_less_1152(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u));
+}
+// byte d of a and of b
+__device__ __forceinline__ uint32_t i8_pair(uint32_t a, uint32_t b, int d) {
+    return f16_less_1152(__builtin_amdgcn_perm(b, a, 0x0c040c00u + 0x00010001u * d) ^ 0x64806480u);
+}
+// A scale of V: 2^ex mant, ex in -60 .. 34, and 2^-ex; mant in [1, 2) inside that range, NaN for an
+// infinity or NaN.
+struct I8Scale {
+    float ex, inv, mant;
+};
+__device__ __forceinline__ I8Scale i8_scale(float d) {
+    const int e = min(max((int)((__float_as_uint(d) >> 23) & 255) - 127, -60), 34);
+    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    return {(float)e, inv, fmaf(d, 0.0f, d) * inv};
+}
 
 // the operand kinds of a cache type
 template <class E>
