@@ -344,12 +344,20 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedA
     if (lane == 0) part_jobs(a, ps, HD)[worker] = job;
 }
 
+constexpr int PF_ROWS = 32;
+static int i8_max_rows(int n_req, int hd) {
+    if (hd == 64) return 2048;
+    return n_req <= 2 ? PF_ROWS : 128;
+}
+
 static PaPlan i8_plan(int n_req, int max_new, int G, int hd) {
     const int64_t rows = (int64_t)max_new * G;  // of one request, at most
     constexpr int64_t ALL = (int64_t)1 << 62;
+    const bool many = rows > i8_max_rows(n_req, hd), few = !many || n_req > 1;
     PaPlan p;
-    p.few = part_shape(rows > 16 ? 5 : 4, G, 0, ALL, PF_WORKERS, 16, 32, 32, 0);
-    p.many = part_shape(PM_TILE_SHIFT, G, 0, ALL, 0, 256, 128, 128, part_ws_floats(p.few.workers, p.few.M, hd));
+    p.few = part_shape(rows > 16 && !many ? 5 : 4, G, 0, many ? PF_ROWS : ALL, few ? PF_WORKERS : 0, 16, 32, 32, 0);
+    const size_t few_ws = part_ws_floats(p.few.workers, p.few.M, hd);
+    p.many = part_shape(PM_TILE_SHIFT, G, few ? PF_ROWS : 0, ALL, many ? PM_WORKERS : 0, 256, 128, 128, few_ws);
     return p;
 }
 
@@ -368,7 +376,8 @@ static void launch(const PagedAttnArgs& a, const PaPlan& p, hipStream_t s) {
 
 hipError_t launch_paged_attn_i8(const PagedAttnArgs& a, int max_new, hipStream_t s) {
     const PaPlan p = i8_plan(a.n_req, max_new, a.nh / a.c.nkv, a.c.hd);
-    a.c.hd == 128 ? launch<128>(a, p, s) : launch<64>(a, p, s);
+    if (p.few.workers) a.c.hd == 128 ? launch<128>(a, p, s) : launch<64>(a, p, s);
+    if (p.many.workers) launch_paged_many(a, p.many, s);
     return launch_paged_join(a, p, s);
 }
 

@@ -37,6 +37,7 @@
 // times a weight would not keep out, or 2^35 and more under scaling, the piece is computed again
 // key by key (slow_rows).
 #include "hy_device.hpp"
+#include "hy_int8.hpp"
 #include "hy_lds.hpp"
 #include "hy_paged.hpp"
 #include "hy_paged_part.hpp"
@@ -88,13 +89,14 @@ struct PmLds {
 template <class E, int HD>
 __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs a, PartShape ps) {
     using L = PmLds<E, HD>;
-    constexpr bool SCALED = !std::is_same<E, _Float16>::value;
+    constexpr bool I8 = std::is_same<E, int8_t>::value, SCALED = !std::is_same<E, _Float16>::value;
     constexpr int KP = L::KP;
     constexpr int NC = HD / 16, ND = HD / 32;
     constexpr int KL = HD / 8;  // threads per key of K
     constexpr int RING = KP == 2 ? 2 : 3;  // operands read ahead of the products (registers allowing)
     __shared__ __attribute__((aligned(1024))) uint8_t lds[L::BYTES];
-    __shared__ __attribute__((aligned(16))) float k_fac[2][32], v_exp[2][32], v_inv[2][32];
+    __shared__ __attribute__((aligned(16))) float k_fac[2][I8 ? 1 : 32], v_exp[2][I8 ? 1 : 32], v_inv[2][I8 ? 1 : 32];
+    __shared__ v4f_t i8_fac[2][I8 ? 8 : 1];  // of four keys: K's scale, V's 2^e as e and 2^-e, and its rest
     __shared__ int odd_s;  // V of this piece that the scaled products do not take
     __shared__ int last_s[PM_WAVES];
     __shared__ PartSums<PM_THREADS> sums;
@@ -176,6 +178,14 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             for (int u = 0; u < 2; u++) q[c][u] = *reinterpret_cast<const v4f_t*>(qp + 16 * c + 4 * u);
         __builtin_amdgcn_sched_barrier(0);
         int64_t tab = page_at(seg, e1), tab2 = page_at(seg + 1, e2);
+        // scales of an 8-bit cache: the same for the neighbouring keys that a wave loads
+        int ptab = e1, ptab2 = e2;
+        auto scale_of = [&](const float* scales, int key) {
+            const int i = (key >> a.c.shift) - seg * 64;
+            const int e = __builtin_amdgcn_readlane(i < 64 ? ptab : ptab2, i & 63);
+            const int64_t p = e >= 0 && e < a.c.n_pages ? e : 0;
+            return scales[((p * a.c.nkv + it.g) << (a.c.shift - a.bshift)) + ((key & pmask) >> a.bshift)];
+        };
         auto lane64 = [](int64_t v, int l) {
             return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) |
                              (uint32_t)__builtin_amdgcn_readlane((int)v, l));
@@ -197,24 +207,30 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         const uint32_t v_off = (((4 * wv) & in_page) * ts + 2 * (lane % (HD / 2))) * sizeof(E);
         uint8_t* const k_dst = lds + k_ch * L::CHUNK_K + k_key * 16;
         uint8_t* const v_dst = lds + L::OFF_V + (2 * (wv / 4) + wv % 2) * L::CHUNK_V + lane * 16 + 8 * (wv / 2 % 2);
-        v4i_t kx[KP];
-        typedef typename std::conditional<KP == 2, uint2, uint32_t>::type vrow_t;
+        typedef typename std::conditional<I8, uint2, v4i_t>::type krow_t;
+        krow_t kx[KP];
+        float k_scale = 0.0f, v_scale = 0.0f;
+        typedef typename std::conditional<KP == 2, uint2, typename std::conditional<I8, uint16_t, uint32_t>::type>::type vrow_t;
         vrow_t vx[4];
         uint32_t v_big = 0;  // the largest magnitude of V's: whether one was infinite, no number, or past PM_EHI
         auto load_k = [&](int kb) {
             const char* const p = reinterpret_cast<const char*>(kg + cell_of(kb * 32 + (wv * KPW) % 32));
 #pragma unroll
-            for (int u = 0; u < KP; u++) kx[u] = *reinterpret_cast<const v4i_t*>(p + k_off + 16 * u);
+            for (int u = 0; u < KP; u++) kx[u] = *reinterpret_cast<const krow_t*>(p + k_off + 16 * u);
+            if constexpr (I8) k_scale = scale_of(a.ks, kb * 32 + (wv * KPW) % 32);
         };
         auto load_v = [&](int kb) {
             const char* const p = reinterpret_cast<const char*>(vg + cell_of(kb * 32 + 4 * wv));
 #pragma unroll
             for (int j = 0; j < 4; j++) vx[j] = *reinterpret_cast<const vrow_t*>(p + (v_off + j * ts * sizeof(E)));
+            if constexpr (I8) v_scale = scale_of(a.vs, kb * 32 + 4 * wv);
             const int s = ((kb + 1) * 32) >> (a.c.shift + 6);  // the next call's
             if (s != seg) {
                 seg = s;
                 tab = tab2;
-                tab2 = page_at(seg + 1, entry(seg + 1));
+                ptab = ptab2;
+                ptab2 = entry(seg + 1);
+                tab2 = page_at(seg + 1, ptab2);
             }
         };
         // block kb, r = kb % 2
@@ -222,7 +238,15 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             uint8_t* const d = k_dst + r * L::BUF_K;
             // a key with an infinity makes NaN of every score (a row's q with one does by its pieces):
             // through its factor, or its element x becomes 0 x + x
-            if constexpr (!SCALED) {
+            if constexpr (I8) {
+                uint32_t w0, w1, w2, w3;
+                i8_to_f16(kx[0].x, w0, w1);
+                i8_to_f16(kx[0].y, w2, w3);
+                if (k_mine) {
+                    *reinterpret_cast<v4i_t*>(d) = v4i_t{(int)w0, (int)w1, (int)w2, (int)w3};
+                    if (k_ch == 0 && k_key % 4 == 0) i8_fac[r][k_key / 4][0] = fmaf(k_scale, 0.0f, k_scale);
+                }
+            } else if constexpr (!SCALED) {
                 const v8h16_t x = __builtin_bit_cast(v8h16_t, kx[0]);
                 const v8h16_t y = __builtin_elementwise_fma(x, (v8h16_t)((_Float16)0), x);
                 if (k_mine) *reinterpret_cast<v8h16_t*>(d) = y;
@@ -267,6 +291,21 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         auto put_v = [&](int kb, int r) {
             uint8_t* const d = v_dst + r * L::BUF_V;
             const int key0 = kb * 32 + 4 * wv;
+            if constexpr (I8) {
+                const I8Scale v = i8_scale(v_scale);
+                if (v_mine) {
+#pragma unroll
+                    for (int n = 0; n < 2; n++)
+                        *reinterpret_cast<uint2*>(d + n * (HD / 2) * 16) =
+                            make_uint2(i8_pair(vx[0], vx[1], n), i8_pair(vx[2], vx[3], n));
+                }
+                if (lane == 0) {
+                    i8_fac[r][wv][1] = v.ex;
+                    i8_fac[r][wv][2] = v.inv;
+                    i8_fac[r][wv][3] = v.mant;
+                }
+                return;
+            }
             if (bad || key0 + 4 > kv) {  // wave-uniform: keys that are not there are zeros
                 const bool ok = page_ok(key0);
 #pragma unroll
@@ -275,7 +314,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             }
             float f[4][2];
             uint32_t big[4];
-            if constexpr (SCALED) {
+            if constexpr (SCALED && !I8) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     uint32_t w0, w1;
@@ -291,7 +330,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                     f[j][1] = __uint_as_float(w1);
                 }
             }
-            if constexpr (SCALED) {
+            if constexpr (SCALED && !I8) {
                 // row j's largest: lanes of equal l % 4 share one row from the second step on
                 uint32_t b0 = lane & 1 ? big[1] : big[0], g0 = lane & 1 ? big[0] : big[1];
                 uint32_t b1 = lane & 1 ? big[3] : big[2], g1 = lane & 1 ? big[2] : big[3];
@@ -328,7 +367,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                         if constexpr (KP == 2) *reinterpret_cast<uint2*>(d + n * (HD / 2) * 16 + L::PIECE_V) = lo;
                     }
                 }
-            } else {
+            } else if constexpr (!I8) {
                 typedef unsigned short v2u16_t __attribute__((ext_vector_type(2)));
 #pragma unroll
                 for (int j = 0; j < 4; j++)
@@ -408,11 +447,17 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 s = mfma_f16(kf[c % RING][0], qf[c][0], s);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            v4f_t inv[4];
+            v4f_t inv[4], mant;
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 v4f_t fac, ex;
-                if constexpr (SCALED) {
+                if constexpr (I8) {
+                    const v4f_t f = i8_fac[r][2 * u + h];
+                    fac = v4f_t{f[0], f[0], f[0], f[0]};
+                    ex = v4f_t{f[1], f[1], f[1], f[1]};
+                    inv[u][0] = f[2];
+                    mant[u] = f[3];
+                } else if constexpr (SCALED) {
                     fac = *reinterpret_cast<const v4f_t*>(&k_fac[r][8 * u + 4 * h]);
                     ex = *reinterpret_cast<const v4f_t*>(&v_exp[r][8 * u + 4 * h]);
                     inv[u] = *reinterpret_cast<const v4f_t*>(&v_inv[r][8 * u + 4 * h]);
@@ -424,8 +469,9 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                     s[4 * u + v] = t;
                 }
             }
-            if (bad || kb * 32 + 32 > first) {  // wave-uniform
-                asm volatile("");               // a branch, not 80 operations more in every block
+            const bool edge = bad || kb * 32 + 32 > first;
+            if (edge) {            // wave-uniform
+                asm volatile("");  // a branch, not 80 operations more in every block
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     const int key = kb * 32 + 8 * u + 4 * h;
@@ -452,12 +498,27 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             const float up = ref - (float)PM_WUP;
 #pragma unroll
             for (int v = 0; v < 16; v++) {  // l_run: of this lane's keys; joined behind the loop
-                if constexpr (SCALED) {
+                if constexpr (I8) {
+                    s[v] = __builtin_amdgcn_exp2f(s[v] - up);
+                    l_run = fmaf(s[v], inv[v / 4][0], l_run);
+                    s[v] *= mant[v / 4];
+                } else if constexpr (SCALED) {
                     s[v] = __builtin_amdgcn_exp2f(s[v] - up);
                     l_run = fmaf(s[v], inv[v / 4][v % 4], l_run);
                 } else {
                     s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], unscale, -up));
                     l_run += s[v];
+                }
+            }
+            if (I8 && edge) {  // a scale that the row does not see may be NaN
+                asm volatile("");
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int key = kb * 32 + 8 * u + 4 * h;
+                    const bool ok = !bad || page_ok(key);
+#pragma unroll
+                    for (int v = 0; v < 4; v++)
+                        if (!ok || key + v >= end) s[4 * u + v] = 0.0f;
                 }
             }
 #pragma unroll
@@ -512,21 +573,24 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         l_run = fadd_half(l_run);
 
         // l carries the weights' factor too, scaled values have one of their own
-        float down = SCALED ? pow2(-PM_VUP) : 1.0f;
-        if constexpr (SCALED)
+        float down = SCALED && !I8 ? pow2(-PM_VUP) : 1.0f;
+        if constexpr (I8) {  // codes are finite, whatever they are
+        } else if constexpr (SCALED)
             v_big = v_big >= (uint32_t)(127 + PM_EHI + 1) << 23;
         else
             v_big = (v_big & 0xffffu) >= 0x7c00u || v_big >= 0x7c000000u;
-        if (__any(v_big != 0)) odd_s = 1;
-        __syncthreads();
-        if (odd_s) {  // again, key by key
-            slow_rows<E, HD, 2>(
-                a, trow, kv, kb0 * 32, my_kb1 * 32, end, a.q + ((int64_t)row * a.nh + head) * HD, kg, vg,
-                [&](int i) { return 2 * (32 * (i / 16 % (ND / 2)) + 8 * (i % 16 / 4) + 4 * h + i % 4) + i / (8 * ND); },
-                [&](int i, float v) { o[i / 16][i % 16] = v; }, [&](int i) { return o[i / 16][i % 16]; }, m_run, l_run);
-            // as the other pieces of its item; in the reference, the sums of large values have no room for it
-            down = 1.0f;
-            m_run += (float)PM_WUP;
+        if constexpr (!I8) {
+            if (__any(v_big != 0)) odd_s = 1;
+            __syncthreads();
+            if (odd_s) {  // again, key by key
+                slow_rows<E, HD, 2>(
+                    a, trow, kv, kb0 * 32, my_kb1 * 32, end, a.q + ((int64_t)row * a.nh + head) * HD, kg, vg,
+                    [&](int i) { return 2 * (32 * (i / 16 % (ND / 2)) + 8 * (i % 16 / 4) + 4 * h + i % 4) + i / (8 * ND); },
+                    [&](int i, float v) { o[i / 16][i % 16] = v; }, [&](int i) { return o[i / 16][i % 16]; }, m_run, l_run);
+                // as the other pieces of its item; in the reference, the sums of large values have no room for it
+                down = 1.0f;
+                m_run += (float)PM_WUP;
+            }
         }
         if (my < n_live) {
             float* dst;
@@ -574,6 +638,8 @@ void launch_paged_many(const PagedAttnArgs& a, const PartShape& ps, hipStream_t 
         launch<float>(a, ps, s);
     else if (a.c.type == HY_TYPE_F16)
         launch<_Float16>(a, ps, s);
+    else if (a.c.type == HY_TYPE_I8)
+        launch<int8_t>(a, ps, s);
     else
         launch<__bf16>(a, ps, s);
 }
