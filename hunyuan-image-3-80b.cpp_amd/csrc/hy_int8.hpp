@@ -47,9 +47,9 @@ struct GemmI8Args {
     const float* resid;   // [T][N] or null
     float* out;           // [T][N]
     int T, K, N;
-    void* part;           // gemm_i8_ws_bytes
+    const float* xf;      // the tokens in f32, of calls that gemm_i8_takes_f32; x and xs are not read then
 };
-size_t gemm_i8_ws_bytes(int T, int K, int N);
+bool gemm_i8_takes_f32(const GemmI8Args& a);
 hipError_t launch_gemm_i8(const GemmI8Args& a, hipStream_t s);
 
 hipError_t launch_paged_append_i8(const PagedAppendArgs& a, const PagedViewI8& v, hipStream_t s);

@@ -111,7 +111,7 @@ int hy_quantize_rows_i8(const float* x, uint32_t rows, uint32_t cols, int8_t* co
 
 size_t hy_gemm_i8_ws(uint32_t T, uint32_t hidden, uint32_t n_out) {
     if (gemm_sizes_check(T, hidden, n_out) != HY_OK) return 0;
-    return hy::gemm_i8_ws_bytes((int)T, (int)hidden, (int)n_out);
+    return 16;  // the present kernels need none
 }
 
 int hy_gemm_i8(const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale, const float* resid,
@@ -122,7 +122,7 @@ int hy_gemm_i8(const int8_t* x, const float* x_scale, const int8_t* w, const flo
     if (!aligned(x_scale, 4) || !aligned(w_scale, 4) || !aligned(out, 4) || !aligned(resid, 4))
         return fail(HY_ERR_INVALID, "f32 arrays must be aligned to 4 bytes");
     HY_TRY(ws_check(ws, ws_bytes, hy_gemm_i8_ws(T, hidden, n_out)));
-    const hy::GemmI8Args a{x, x_scale, w, w_scale, resid, out, (int)T, (int)hidden, (int)n_out, ws};
+    const hy::GemmI8Args a{x, x_scale, w, w_scale, resid, out, (int)T, (int)hidden, (int)n_out, nullptr};
     HIP_TRY(hy::launch_gemm_i8(a, static_cast<hipStream_t>(stream)));
     return HY_OK;
 }
@@ -130,7 +130,7 @@ int hy_gemm_i8(const int8_t* x, const float* x_scale, const int8_t* w, const flo
 // codes, scales, and the product's own
 size_t hy_linear_i8_ws(uint32_t T, uint32_t hidden, uint32_t n_out) {
     if (gemm_sizes_check(T, hidden, n_out) != HY_OK) return 0;
-    return (size_t)T * hidden + al16((size_t)T * 4) + hy::gemm_i8_ws_bytes((int)T, (int)hidden, (int)n_out);
+    return (size_t)T * hidden + al16((size_t)T * 4) + hy_gemm_i8_ws(T, hidden, n_out);
 }
 
 int hy_linear_i8(const float* x, const int8_t* w, const float* w_scale, const float* resid, uint32_t T,
@@ -144,9 +144,11 @@ int hy_linear_i8(const float* x, const int8_t* w, const float* w_scale, const fl
     int8_t* const codes = static_cast<int8_t*>(ws);
     float* const scales = reinterpret_cast<float*>(codes + (size_t)T * hidden);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const hy::GemmI8Args a{codes, scales, w, w_scale, resid, out, (int)T, (int)hidden, (int)n_out,
-                           codes + (size_t)T * hidden + al16((size_t)T * 4)};
-    HIP_TRY(hy::launch_quantize_rows(x, (int)T, (int)hidden, codes, scales, s));
+    hy::GemmI8Args a{codes, scales, w, w_scale, resid, out, (int)T, (int)hidden, (int)n_out, nullptr};
+    if (hy::gemm_i8_takes_f32(a))
+        a.xf = x;
+    else
+        HIP_TRY(hy::launch_quantize_rows(x, (int)T, (int)hidden, codes, scales, s));
     HIP_TRY(hy::launch_gemm_i8(a, s));
     return HY_OK;
 }

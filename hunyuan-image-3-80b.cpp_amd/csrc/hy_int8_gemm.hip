@@ -1,9 +1,12 @@
 // hy_int8_gemm.hip -- products of tokens and weights in 8-bit integers (hy_gemm_i8, hy_linear_i8) and
 // the quantization of rows that they are fed by (hy_quantize_rows_i8).
+#include <cmath>
+
 #include "hy_device.hpp"
 #include "hy_int8.hpp"
 #include "hy_lds.hpp"
 #include "hy_mfma.hpp"
+#include "hy_split.hpp"
 
 namespace hy {
 
@@ -64,199 +67,237 @@ hipError_t launch_quantize_rows(const float* x, int rows, int cols, int8_t* code
 }
 
 // ---------------------------------------------------------------- products of few tokens
-// A stream over the weights: a work group of GS_WAVES waves takes 16 NT channels of 16 TT tokens, each
-// wave a part of the reduction, straight from memory into the operands of v_mfma_i32_16x16x64_i8 (lane l:
-// 16 bytes of row l % 16 at k offset 16 (l / 16), of A and of B alike; result v is A's row 4 (l / 16) + v, B's
-// row l % 16), GS_D steps of 64 ahead.  The waves' sums meet in LDS: whole numbers, so in any order.
-constexpr int GS_WAVES = 4;
+// A stream over the weights: a work group of GS_WAVES waves takes 16 channels of 16 tokens, each wave a part of
+// the reduction, straight from memory into the operands of v_mfma_i32_16x16x64_i8 (lane l: 16 bytes of row
+// l % 16 at k offset 16 (l / 16), of A and of B alike; result v is A's row 4 (l / 16) + v, B's row l % 16),
+// GS_DEPTH steps of 64 ahead.  The waves' sums meet in LDS: whole numbers, so in any order.
+// FUSED: the tokens are f32, up to GF_TOKENS of them, and every work group quantizes them for itself while its
+// first weights are on their way, which spares a launch (one token, 4096 x 6144: TODO us, in two launches TODO).
+// Bound by latency: 25 MB of weights would take 5 us at a copy's rate.
+constexpr int GS_WAVES = 4, GS_THREADS = WAVE * GS_WAVES, GS_DEPTH = 8;
+constexpr int GF_TOKENS = 4, GF_WIDTH = 8192;
 
-template <int NT, int TT, int D>
-__global__ __launch_bounds__(WAVE * GS_WAVES) void gemm_i8_stream_kernel(GemmI8Args a, int tiles_n) {
-    constexpr int BN = 16 * NT, BT = 16 * TT;
-    __shared__ int sum[BT * BN];
+template <bool FUSED>
+__global__ __launch_bounds__(GS_THREADS) void gemm_i8_stream_kernel(GemmI8Args a, int tiles_n) {
+    __shared__ int sum[256];
+    __shared__ __attribute__((aligned(16))) int8_t codes[FUSED ? GF_TOKENS : 1][FUSED ? GF_WIDTH : 16];
+    __shared__ uint32_t part[FUSED ? GF_TOKENS : 1][GS_WAVES];
     const int tid = threadIdx.x, lane = tid % WAVE, r = lane % 16, g = lane / 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-    const int n0 = (int)(b % tiles_n) * BN;
-    const int64_t t64 = b / tiles_n * BT;
+    const int n0 = (int)(b % tiles_n) * 16;
+    const int64_t t64 = b / tiles_n * 16;
     if (t64 >= a.T) return;
     const int t0 = (int)t64;
     const int steps = (a.K + 63) / 64, s0 = steps * wave / GS_WAVES, s1 = steps * (wave + 1) / GS_WAVES;
-    const int8_t* wp[NT];
-    const int8_t* xp[TT];
-#pragma unroll
-    for (int i = 0; i < NT; i++) wp[i] = a.w + (int64_t)min(n0 + 16 * i + r, a.N - 1) * a.K;
-#pragma unroll
-    for (int j = 0; j < TT; j++) xp[j] = a.x + (int64_t)min(t0 + 16 * j + r, a.T - 1) * a.K;
-    v4i_t wf[D][NT], xf[D][TT];
-    // steps past the last are read again and not used; behind the reduction's end the weights count as 0
+    const int8_t* const wp = a.w + (int64_t)min(n0 + r, a.N - 1) * a.K;
+    const int8_t* const xp = FUSED ? codes[min(r, a.T - 1)] : a.x + (int64_t)min(t0 + r, a.T - 1) * a.K;
+    v4i_t wf[GS_DEPTH], xf[GS_DEPTH];
+    // steps past the last are read again and not used
+    const auto at = [&](int s) { return min(64 * min(s, s1 - 1) + 16 * g, a.K - 16); };
     const auto load = [&](int s, int d) {
-        const int k = 64 * min(s, s1 - 1) + 16 * g, at = min(k, a.K - 16);
-#pragma unroll
-        for (int i = 0; i < NT; i++) wf[d][i] = *reinterpret_cast<const v4i_t*>(wp[i] + at);
-#pragma unroll
-        for (int j = 0; j < TT; j++) xf[d][j] = *reinterpret_cast<const v4i_t*>(xp[j] + at);
+        wf[d] = *reinterpret_cast<const v4i_t*>(wp + at(s));
+        if constexpr (!FUSED) xf[d] = *reinterpret_cast<const v4i_t*>(xp + at(s));
     };
-    v4i_t acc[TT][NT] = {};
     if (s0 < s1) {
 #pragma unroll
-        for (int d = 0; d < D; d++) load(s0 + d, d);
+        for (int d = 0; d < GS_DEPTH; d++) load(s0 + d, d);
     }
-    for (int i = tid; i < BT * BN; i += WAVE * GS_WAVES) sum[i] = 0;
-    __syncthreads();
-    for (int s = s0; s < s1; s += D) {
+    sum[tid] = 0;
+    float xs[GF_TOKENS];
+    if constexpr (FUSED) {
+        __builtin_amdgcn_sched_barrier(0);
+        uint32_t big[GF_TOKENS];
 #pragma unroll
-        for (int d = 0; d < D; d++) {
-            if (s + d < s1) {  // the same for the wave
-                if (64 * (s + d) + 64 > a.K) {
-                    const bool gone = 64 * (s + d) + 16 * g >= a.K;
+        for (int t = 0; t < GF_TOKENS; t++) {
+            big[t] = 0;
+            if (t >= a.T) continue;  // the same for the work group
+            for (int c = 4 * tid; c < a.K; c += 4 * GS_THREADS) {
+                const v4f_t v = *reinterpret_cast<const v4f_t*>(a.xf + (int64_t)t * a.K + c);
 #pragma unroll
-                    for (int i = 0; i < NT; i++) wf[d][i] = gone ? v4i_t{} : wf[d][i];
-                }
-#pragma unroll
-                for (int j = 0; j < TT; j++)
-#pragma unroll
-                    for (int i = 0; i < NT; i++)
-                        acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[d][j], wf[d][i], acc[j][i], 0, 0, 0);
+                for (int j = 0; j < 4; j++) big[t] = max(big[t], __float_as_uint(v[j]) & 0x7fffffffu);
             }
-            load(s + D + d, d);
+#pragma unroll
+            for (int m = 32; m; m >>= 1) big[t] = max(big[t], (uint32_t)shfl_xor((int)big[t], m));
+            if (lane == 0) part[t][wave] = big[t];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < GF_TOKENS; t++) {
+            if (t >= a.T) continue;
+#pragma unroll
+            for (int w = 0; w < GS_WAVES; w++) big[t] = max(big[t], part[t][w]);
+            const QuantScale q = quant_scale(big[t]);
+            xs[t] = q.d;
+            for (int c = 4 * tid; c < a.K; c += 4 * GS_THREADS) {
+                const v4f_t v = *reinterpret_cast<const v4f_t*>(a.xf + (int64_t)t * a.K + c);
+                *reinterpret_cast<uint32_t*>(&codes[t][c]) = quant4(v[0], v[1], v[2], v[3], q.inv);
+            }
+        }
+    }
+    __syncthreads();
+    v4i_t acc = {};
+    for (int s = s0; s < s1; s += GS_DEPTH) {
+#pragma unroll
+        for (int d = 0; d < GS_DEPTH; d++) {
+            if (s + d < s1) {  // the same for the wave
+                if constexpr (FUSED) xf[d] = *reinterpret_cast<const v4i_t*>(xp + at(s + d));
+                // behind the reduction's end the weights count as 0
+                if (64 * (s + d) + 64 > a.K) wf[d] = 64 * (s + d) + 16 * g >= a.K ? v4i_t{} : wf[d];
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[d], wf[d], acc, 0, 0, 0);
+            }
+            load(s + GS_DEPTH + d, d);
         }
     }
 #pragma unroll
-    for (int j = 0; j < TT; j++)
-#pragma unroll
-        for (int i = 0; i < NT; i++)
-#pragma unroll
-            for (int v = 0; v < 4; v++) atomicAdd(&sum[(16 * j + 4 * g + v) * BN + 16 * i + r], acc[j][i][v]);
+    for (int v = 0; v < 4; v++) atomicAdd(&sum[(4 * g + v) * 16 + r], acc[v]);
     __syncthreads();
-    for (int i = tid; i < BT * BN; i += WAVE * GS_WAVES) {
-        const int t = t0 + i / BN, n = n0 + i % BN;
-        if (t >= a.T || n >= a.N) continue;
-        const int64_t at = (int64_t)t * a.N + n;
-        float y = (float)sum[i] * a.xs[t] * a.ws[n];
-        if (a.resid) y += a.resid[at];
-        a.out[at] = y;
+    const int row = tid / 16, t = t0 + row, n = n0 + tid % 16;
+    if (t >= a.T || n >= a.N) return;
+    float scale;
+    if constexpr (FUSED) {
+        scale = xs[0];
+#pragma unroll
+        for (int i = 1; i < GF_TOKENS; i++) scale = row == i ? xs[i] : scale;
+    } else {
+        scale = a.xs[t];
     }
+    const int64_t o = (int64_t)t * a.N + n;
+    float y = (float)sum[tid] * scale * a.ws[n];
+    if (a.resid) y += a.resid[o];
+    a.out[o] = y;
 }
 
 // ---------------------------------------------------------------- products of many tokens
-// Tiles of 128 tokens x 256 channels: a work group of four waves, each 64 tokens x 128 channels (2 x 4
-// results of v_mfma_i32_32x32x32_i8: lane l holds 16 bytes of row l % 32 at k offset 16 (l / 32); result v
-// is A's row 8 (v / 4) + 4 (l / 32) + v % 4, B's row l % 32; A is the tokens, so that a store's lanes are
-// neighbouring channels).  Stages of 64 bytes of the reduction are copied from memory into a ring of three
-// in LDS, two of them on their way while one is multiplied; one barrier per stage.
-// A row of a stage is four pieces of 16 bytes; piece c lies in place c ^ (row / 4 % 4), so that
-// 16 rows' reads of one piece touch every bank once.  The copies' places are fixed, so they fetch
-// the pieces swapped.
-constexpr int GT_BT = 128, GT_BN = 256, GT_KB = 64, GT_RING = 3, GT_WAVES = 4;
-constexpr int GT_A = GT_BT * GT_KB, GT_STAGE = GT_A + GT_BN * GT_KB;
-constexpr int GT_COPIES = GT_STAGE / 1024 / GT_WAVES;  // of 1 KB per wave and stage
-static_assert(GT_BT == 128 && GT_BN == 256 && GT_COPIES == 6, "8 copies of tokens, 16 of weights");
+// Tiles of BT tokens x BN channels, WT x WN waves, results of v_mfma_i32_32x32x32_i8 (lane l holds 16 bytes of
+// row l % 32 at k offset 16 (l / 32); result v is A's row 8 (v / 4) + 4 (l / 32) + v % 4, B's row l % 32; A is
+// the tokens, so that a store's lanes are neighbouring channels).  Stages of KB bytes of the reduction are
+// copied from memory into a ring in LDS, all but the one that is multiplied on their way; one barrier
+// per stage; operands are read from LDS one step of 32 ahead of their products.
+// Piece c (16 bytes) of a stage's row lies in place c ^ swap(row), so that 16 rows' reads of one piece touch
+// every bank once.  The copies' places are fixed, so they fetch the pieces swapped.
+// Rows of 128 bytes: with 64 the copies are half as fast (a request of the L2 is 64 bytes of a line of
+// 128).  What bounds the tiles of 256 x 256: see launch_gemm_i8.
+template <int BT_, int BN_, int WT_, int WN_, int RING_, int KB_>
+struct GtShape {
+    static constexpr int BT = BT_, BN = BN_, WT = WT_, WN = WN_, RING = RING_, KB = KB_;
+    static constexpr int PIECES = KB / 16, ROWS = 64 / PIECES, Q = KB / 32;  // of a row, of a copy, products deep
+    static constexpr int WAVES = WT * WN, THREADS = WAVE * WAVES;
+    static constexpr int MT = BT / WT / 32, NT = BN / WN / 32;  // 32 x 32 results of a wave
+    static constexpr int A = BT * KB, STAGE = A + BN * KB, LDS = RING * STAGE;
+    // copies of 1 KB per wave and stage, of tokens and of both; copy i of wave w is the stage's KB i WAVES + w
+    static constexpr int COPIES_A = A / 1024 / WAVES, COPIES = STAGE / 1024 / WAVES;
+    static_assert(COPIES * WAVES * 1024 == STAGE && MT * 32 * WT == BT && NT * 32 * WN == BN, "whole copies and results");
+    static_assert(COPIES_A * WAVES * 1024 == A && ROWS * WAVES % (256 / KB * PIECES) == 0, "one swap per lane");
+    __device__ static __forceinline__ int swap(int row) { return row / (256 / KB) % PIECES; }
+};
 
 __device__ const int8_t i8_zeros[16] = {};
 
-__global__ __launch_bounds__(WAVE * GT_WAVES, 2) void gemm_i8_tile_kernel(GemmI8Args a, int tiles_n, int tiles) {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[GT_RING * GT_STAGE];
+template <class S>
+__device__ __forceinline__ void gemm_i8_tile(const GemmI8Args& a, int t0, int n0, uint8_t* lds) {
     const int tid = threadIdx.x, lane = tid % WAVE, lr = lane % 32, h = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-    // tiles in bands of 8 x 256 channels, tokens outer; neighbouring ones on one XCD (work groups go round
-    // the XCDs): 64 that run there at once share 8 x 8 rows and columns of tiles
-    const int per = (tiles + 7) / 8, o = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-    if ((int)(blockIdx.x / 8) >= per || o >= tiles) return;
-    const int tiles_t = tiles / tiles_n, band = o / (8 * tiles_t), width = min(8, tiles_n - 8 * band);
-    const int in_band = o - band * 8 * tiles_t;
-    const int n0 = (8 * band + in_band % width) * GT_BN, t0 = in_band / width * GT_BT;
-    const int K = a.K, stages = (K + GT_KB - 1) / GT_KB;
+    const int K = a.K, stages = (K + S::KB - 1) / S::KB;
 
-    // copy i of this wave: 16 rows x 64 bytes from row 16 (6 wave + i) of the stage on (tokens, then weights)
-    uint32_t off[GT_COPIES];
-    const int piece = (lane % 4) ^ (lane / 16);
+    uint32_t off[S::COPIES];
+    const int piece = (lane % S::PIECES) ^ S::swap(lane / S::PIECES + S::ROWS * wave);
     const __amdgpu_buffer_rsrc_t xr = buf_rsrc(a.x + (int64_t)t0 * K), wr = buf_rsrc(a.w + (int64_t)n0 * K);
 #pragma unroll
-    for (int i = 0; i < GT_COPIES; i++) {
-        const int row = 16 * (GT_COPIES * wave + i) + lane / 4;
-        const int clamped = row < GT_BT ? min(row, a.T - 1 - t0) : min(row - GT_BT, a.N - 1 - n0);
+    for (int i = 0; i < S::COPIES; i++) {
+        const int row = S::ROWS * (i * S::WAVES + wave) + lane / S::PIECES;
+        const int clamped = row < S::BT ? min(row, a.T - 1 - t0) : min(row - S::BT, a.N - 1 - n0);
         off[i] = (uint32_t)clamped * K + 16 * piece;
     }
     const auto copy = [&](int s) {
-        uint8_t* const dst = lds + (s % GT_RING) * GT_STAGE + GT_COPIES * 1024 * wave;
-        if (64 * s + 64 <= K) {
+        uint8_t* const dst = lds + (s % S::RING) * S::STAGE + 1024 * wave;
+        if (S::KB * s + S::KB <= K) {
 #pragma unroll
-            for (int i = 0; i < GT_COPIES; i++)
-                b2l(GT_COPIES * wave + i < GT_A / 1024 ? xr : wr, dst + 1024 * i, off[i], 64 * s);
+            for (int i = 0; i < S::COPIES; i++)
+                b2l(i < S::COPIES_A ? xr : wr, dst + 1024 * S::WAVES * i, off[i], S::KB * s);
         } else {  // the reduction ends inside the stage: zeros behind it
 #pragma unroll
-            for (int i = 0; i < GT_COPIES; i++) {
-                const int8_t* const base =
-                    GT_COPIES * wave + i < GT_A / 1024 ? a.x + (int64_t)t0 * K : a.w + (int64_t)n0 * K;
-                g2l16(64 * s + 16 * piece < K ? base + off[i] + 64 * s : i8_zeros, dst + 1024 * i);
+            for (int i = 0; i < S::COPIES; i++) {
+                const int8_t* const base = i < S::COPIES_A ? a.x + (int64_t)t0 * K : a.w + (int64_t)n0 * K;
+                g2l16(S::KB * s + 16 * piece < K ? base + off[i] + S::KB * s : i8_zeros, dst + 1024 * S::WAVES * i);
             }
         }
     };
-    v16i_t acc[2][4];
+    v16i_t acc[S::MT][S::NT];
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int i = 0; i < S::MT; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = v16i_t{};
-    // this lane's rows of the wave's tokens and channels; rows 32 apart are 2 KB apart
-    const int wt = wave % 2, wn = wave / 2;
-    const uint32_t a_row = lds_off(lds) + (uint32_t)(64 * wt + lr) * GT_KB;
-    const uint32_t b_row = lds_off(lds) + GT_A + (uint32_t)(128 * wn + lr) * GT_KB;
-    const uint32_t p0 = 16 * ((0 + h) ^ (lr / 4 % 4)), p1 = 16 * ((2 + h) ^ (lr / 4 % 4));
+        for (int j = 0; j < S::NT; j++) acc[i][j] = v16i_t{};
+    // this lane's rows of the wave's tokens and channels
+    const int wt = wave % S::WT, wn = wave / S::WT;
+    const uint32_t a_row = lds_off(lds) + (uint32_t)(32 * S::MT * wt + lr) * S::KB;
+    const uint32_t b_row = lds_off(lds) + S::A + (uint32_t)(32 * S::NT * wn + lr) * S::KB;
+    uint32_t place[S::Q];
+#pragma unroll
+    for (int q = 0; q < S::Q; q++) place[q] = 16 * ((2 * q + h) ^ S::swap(lr));
 
-    copy(0);
-    if (stages > 1) copy(1);
+    v4i_t af[2][S::MT], bf[2][S::NT];
+    const auto read = [&](int s, int q) {
+        const uint32_t at = (uint32_t)(s % S::RING) * S::STAGE + place[q];
+        static_for<S::MT>([&](auto i) { af[q % 2][i] = lds_b128_at<32 * S::KB * i>(a_row + at); });
+        static_for<S::NT>([&](auto j) { bf[q % 2][j] = lds_b128_at<32 * S::KB * j>(b_row + at); });
+    };
+    const auto multiply = [&](int q) {
+#pragma unroll
+        for (int i = 0; i < S::MT; i++) lds_pin(af[q][i]);
+#pragma unroll
+        for (int j = 0; j < S::NT; j++) lds_pin(bf[q][j]);
+        __builtin_amdgcn_s_setprio(1);  // a wave with its operands goes first: 8192 tokens 302 -> 290 us
+#pragma unroll
+        for (int j = 0; j < S::NT; j++)
+#pragma unroll
+            for (int i = 0; i < S::MT; i++)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(af[q][i], bf[q][j], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int s = 0; s < S::RING; s++)
+        if (s < stages) copy(s);
+    wait_copies<S::COPIES, S::RING - 1>(stages - 1);
+    __syncthreads();
+    read(0, 0);
     for (int s = 0; s < stages; s++) {
-        wait_copies<GT_COPIES, 1>(stages - 1 - s);  // this stage's are there, the next one's may be on their way
-        __syncthreads();                            // the others' too; all have read stage s - 1 out
-        if (s + 2 < stages) copy(s + 2);
-        const uint32_t slot = (uint32_t)(s % GT_RING) * GT_STAGE;
-        v4i_t af[2][2], bf[2][4];
-        const auto read = [&](int q, uint32_t p) {
-            const uint32_t ab = a_row + slot + p, bb = b_row + slot + p;
-            af[q][0] = lds_b128_at<0>(ab);
-            bf[q][0] = lds_b128_at<0>(bb);
-            bf[q][1] = lds_b128_at<2048>(bb);
-            af[q][1] = lds_b128_at<2048>(ab);
-            bf[q][2] = lds_b128_at<4096>(bb);
-            bf[q][3] = lds_b128_at<6144>(bb);
-        };
-        const auto pin = [&](int q) {
-            lds_pin(af[q][0]), lds_pin(af[q][1]);
-            lds_pin(bf[q][0]), lds_pin(bf[q][1]), lds_pin(bf[q][2]), lds_pin(bf[q][3]);
-        };
-        const auto multiply = [&](int q) {
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(af[q][i], bf[q][j], acc[i][j], 0, 0, 0);
-        };
-        read(0, p0);
-        read(1, p1);
-        lds_wait_upto<6>();
-        pin(0);
-        multiply(0);
-        lds_wait_upto<0>();
-        pin(1);
-        multiply(1);
+        for (int q = 0; q + 1 < S::Q; q++) {
+            read(s, q + 1);
+            lds_wait_upto<S::MT + S::NT>();
+            multiply(q % 2);
+        }
+        if (s + 1 < stages) {
+            // the next stage's copies have arrived, later ones' are on their way; this wave has read its part of
+            // the stage out (the wait is for LDS reads too)
+            wait_copies<S::COPIES, S::RING - 2>(stages - 2 - s);
+            __syncthreads();  // and so have the others
+            if (s + S::RING < stages) copy(s + S::RING);
+            read(s + 1, 0);
+            lds_wait_upto<S::MT + S::NT>();
+        } else {
+            lds_wait_upto<0>();
+        }
+        multiply((S::Q - 1) % 2);
     }
-    float wscale[4];
-    int n[4];
+    float wscale[S::NT];
+    int n[S::NT];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        n[j] = n0 + 128 * wn + 32 * j + lr;
+    for (int j = 0; j < S::NT; j++) {
+        n[j] = n0 + 32 * (S::NT * wn + j) + lr;
         wscale[j] = a.ws[min(n[j], a.N - 1)];
     }
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int i = 0; i < S::MT; i++)
 #pragma unroll
         for (int v = 0; v < 16; v++) {
-            const int t = t0 + 64 * wt + 32 * i + 8 * (v / 4) + 4 * h + v % 4;
+            const int t = t0 + 32 * (S::MT * wt + i) + 8 * (v / 4) + 4 * h + v % 4;
             if (t >= a.T) continue;
             const float xs = a.xs[t];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
+            for (int j = 0; j < S::NT; j++) {
                 if (n[j] >= a.N) continue;
                 const int64_t at = (int64_t)t * a.N + n[j];
                 float y = (float)acc[i][j][v] * xs * wscale[j];
@@ -266,29 +307,87 @@ __global__ __launch_bounds__(WAVE * GT_WAVES, 2) void gemm_i8_tile_kernel(GemmI8
         }
 }
 
-size_t gemm_i8_ws_bytes(int, int, int) { return 16; }
+constexpr int GT_XCDS = 8, GT_CUS = 32;  // of an XCD
 
-template <int NT, int TT, int D>
-static void stream(const GemmI8Args& a, hipStream_t s) {
-    const int tiles_n = (a.N + 16 * NT - 1) / (16 * NT);
-    const int64_t n = (int64_t)tiles_n * ((a.T + 16 * TT - 1) / (16 * TT)), gx = n < 1 << 22 ? n : 1 << 22;
-    const dim3 grid((unsigned)gx, (unsigned)((n + gx - 1) / gx));  // fewer than 2^32 threads along x
-    hipLaunchKernelGGL((gemm_i8_stream_kernel<NT, TT, D>), grid, dim3(WAVE * GS_WAVES), 0, s, a, tiles_n);
+// HALF: the shape of half a tile of channels, which what is left over of the last round falls into, or S itself
+template <class S, class HALF>
+__global__ __launch_bounds__(S::THREADS, S::WAVES / 4 * (S::LDS > 81920 ? 1 : 2)) void gemm_i8_tile_kernel(
+    GemmI8Args a, int tiles_n, int tiles) {
+    constexpr bool SPLIT = HALF::BN < S::BN;
+    static_assert(HALF::THREADS == S::THREADS && HALF::LDS <= S::LDS, "the same work group");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[S::LDS];
+    // tiles in bands of 8 of channels, tokens outer; neighbouring ones on one XCD (work groups go round the
+    // XCDs), where those that run at once share rows and columns of tiles
+    const int xcd = blockIdx.x % GT_XCDS, lo = (int)((int64_t)tiles * xcd / GT_XCDS);
+    const int mine = (int)((int64_t)tiles * (xcd + 1) / GT_XCDS) - lo, left = mine % GT_CUS;
+    const int whole = SPLIT && left <= GT_CUS / 2 ? mine - left : mine;
+    int i = blockIdx.x / GT_XCDS, half = -1;
+    if (i >= whole) {
+        half = (i - whole) % 2;
+        i = whole + (i - whole) / 2;
+    }
+    if (i >= mine) return;
+    const int o = lo + i, tiles_t = tiles / tiles_n, band = o / (8 * tiles_t), width = min(8, tiles_n - 8 * band);
+    const int in_band = o - band * 8 * tiles_t;
+    const int n0 = (8 * band + in_band % width) * S::BN, t0 = in_band / width * S::BT;
+    if (!SPLIT || half < 0) {
+        gemm_i8_tile<S>(a, t0, n0, lds);
+    } else if (n0 + half * HALF::BN < a.N) {
+        gemm_i8_tile<HALF>(a, t0, n0 + half * HALF::BN, lds);
+    }
 }
 
+template <bool FUSED>
+static void stream(const GemmI8Args& a, hipStream_t s) {
+    const int tiles_n = (a.N + 15) / 16;
+    const int64_t n = (int64_t)tiles_n * ((a.T + 15) / 16), gx = n < 1 << 22 ? n : 1 << 22;
+    const dim3 grid((unsigned)gx, (unsigned)((n + gx - 1) / gx));  // fewer than 2^32 threads along x
+    hipLaunchKernelGGL(gemm_i8_stream_kernel<FUSED>, grid, dim3(GS_THREADS), 0, s, a, tiles_n);
+}
+
+template <class S, class HALF = S>
+static void tiles(const GemmI8Args& a, hipStream_t s) {
+    const int tiles_n = (a.N + S::BN - 1) / S::BN, tiles = tiles_n * ((a.T + S::BT - 1) / S::BT);
+    const int per_xcd = (tiles + GT_XCDS - 1) / GT_XCDS + (HALF::BN < S::BN ? GT_CUS / 2 : 0);
+    hipLaunchKernelGGL((gemm_i8_tile_kernel<S, HALF>), dim3((unsigned)(GT_XCDS * per_xcd)), dim3(S::THREADS), 0, s, a,
+                       tiles_n, tiles);
+}
+typedef GtShape<256, 256, 4, 4, 2, 128> GtBig;
+typedef GtShape<256, 128, 4, 4, 2, 128> GtBigHalf;
+typedef GtShape<128, 128, 2, 4, 2, 128> GtMid;
+typedef GtShape<64, 64, 2, 2, 5, 128> GtSmall;
+
+// Which kernel, by what each takes at hidden 4096 (all in proportion to it), us:
+//  * the stream, for up to 4 tokens, or 16 of up to 2^14 channels.  4096 x 6144, 1 token 9.5, by small tiles
+//    13.5; 16 tokens 12.7, 13.5; x 133120, 1 token 117, 122; 16 tokens 191, 122;
+//  * tiles of 64 x 64: 14, or 6 and 36 ns per tile where that is more;
+//  * tiles of 128 x 128: 25, or 5 and 93 ns per tile;
+//  * tiles of 256 x 256: 70 per round of 256, 45 for a last round of up to 128, which takes half tiles.
+// 64, 128 and 256 wide tiles measured: 300 tokens x 4096 channels 18, 27, 33; 512 x 6144 34, 35, 44; 1024 x
+// 6144 60, 42, 49; 2048 x 6144 110, 75, 70; 4096 x 6144 226, 144, 127 (without half tiles 144); 64 x 133120 143,
+// 175, -; 256 x 133120 -, 243, 233.
+static double tiles_of(const GemmI8Args& a, int bt, int bn) {
+    return (double)((a.T + bt - 1) / bt) * ((a.N + bn - 1) / bn);
+}
+static bool by_stream(const GemmI8Args& a) { return a.T <= 4 || (a.T <= 16 && a.N <= 1 << 14); }
+
+bool gemm_i8_takes_f32(const GemmI8Args& a) { return a.T <= GF_TOKENS && a.K <= GF_WIDTH; }
+
 hipError_t launch_gemm_i8(const GemmI8Args& a, hipStream_t s) {
-    const int64_t tiles = (int64_t)((a.N + GT_BN - 1) / GT_BN) * ((a.T + GT_BT - 1) / GT_BT);
-    if (a.T > 64 && tiles >= 200) {
-        const int64_t per = (tiles + 7) / 8;
-        hipLaunchKernelGGL(gemm_i8_tile_kernel, dim3((unsigned)(8 * per)), dim3(WAVE * GT_WAVES), 0, s, a,
-                           (a.N + GT_BN - 1) / GT_BN, (int)tiles);
-    } else if (a.T > 32) {
-        stream<4, 4, 2>(a, s);
-    } else if (a.T > 16) {
-        a.N >= 32768 ? stream<4, 2, 4>(a, s) : stream<1, 2, 6>(a, s);
-    } else {
-        a.N >= 32768 ? stream<4, 1, 4>(a, s) : stream<1, 1, 8>(a, s);
+    if (by_stream(a)) {
+        a.xf ? stream<true>(a, s) : stream<false>(a, s);
+        return hipGetLastError();
     }
+    const double n64 = tiles_of(a, 64, 64), n128 = tiles_of(a, 128, 128), n256 = tiles_of(a, 256, 256);
+    const double small = fmax(14.0, 6.0 + 0.036 * n64), mid = fmax(25.0, 5.0 + 0.093 * n128);
+    const double rounds = floor(n256 / 256.0), left = n256 - 256.0 * rounds;
+    const double big = 70.0 * rounds + (left == 0.0 ? 0.0 : left <= 128.0 ? 45.0 : 70.0);
+    if (small <= mid && small <= big)
+        tiles<GtSmall>(a, s);
+    else if (mid <= big)
+        tiles<GtMid>(a, s);
+    else
+        tiles<GtBig, GtBigHalf>(a, s);
     return hipGetLastError();
 }
 

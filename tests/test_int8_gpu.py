@@ -46,7 +46,10 @@ def same_bits(a, b):
 SHAPES = [(1, 16, 1), (1, 4096, 6144), (2, 272, 33), (3, 48, 513), (5, 1040, 100), (16, 4096, 1000), (17, 144, 4096),
           (31, 2048, 65), (33, 4096, 257), (64, 1024, 512), (65, 2064, 130), (100, 32, 31), (128, 4096, 4096),
           (129, 528, 255), (200, 8192, 96), (256, 256, 256), (300, 4096, 1000), (511, 1008, 385), (700, 64, 2000),
-          (1025, 512, 300), (16, 16, 20000), (4096, 16, 5), (1, 131056, 40), (40, 131056, 9)]
+          (1025, 512, 300), (16, 16, 20000), (4096, 16, 5), (1, 131056, 40), (40, 131056, 9), (5, 272, 33000),
+          # tiles of 128 and of 256, with and without a last round of halves; reductions that end inside a stage
+          (1100, 400, 4200), (1000, 144, 6100), (2500, 272, 6144), (4100, 144, 4200), (4096, 80, 6145),
+          (3000, 2064, 11000)]
 
 
 @pytest.mark.parametrize("T,K,N", SHAPES)
