@@ -72,7 +72,7 @@ hipError_t launch_quantize_rows(const float* x, int rows, int cols, int8_t* code
 // l % 16 at k offset 16 (l / 16), of A and of B alike; result v is A's row 4 (l / 16) + v, B's row l % 16),
 // GS_DEPTH steps of 64 ahead.  The waves' sums meet in LDS: whole numbers, so in any order.
 // FUSED: the tokens are f32, up to GF_TOKENS of them, and every work group quantizes them for itself while its
-// first weights are on their way, which spares a launch (one token, 4096 x 6144: TODO us, in two launches TODO).
+// first weights are on their way, which spares a launch (one token, 4096 x 6144: 10.0 us, in two launches 9.9 + 2.6).
 // Bound by latency: 25 MB of weights would take 5 us at a copy's rate.
 constexpr int GS_WAVES = 4, GS_THREADS = WAVE * GS_WAVES, GS_DEPTH = 8;
 constexpr int GF_TOKENS = 4, GF_WIDTH = 8192;
@@ -194,7 +194,7 @@ struct GtShape {
 
 __device__ const int8_t i8_zeros[16] = {};
 
-template <class S>
+template <class S, bool ONCE>
 __device__ __forceinline__ void gemm_i8_tile(const GemmI8Args& a, int t0, int n0, uint8_t* lds) {
     const int tid = threadIdx.x, lane = tid % WAVE, lr = lane % 32, h = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
@@ -213,8 +213,12 @@ __device__ __forceinline__ void gemm_i8_tile(const GemmI8Args& a, int t0, int n0
         uint8_t* const dst = lds + (s % S::RING) * S::STAGE + 1024 * wave;
         if (S::KB * s + S::KB <= K) {
 #pragma unroll
-            for (int i = 0; i < S::COPIES; i++)
-                b2l(i < S::COPIES_A ? xr : wr, dst + 1024 * S::WAVES * i, off[i], S::KB * s);
+            for (int i = 0; i < S::COPIES; i++) {
+                if (i < S::COPIES_A)
+                    b2l(xr, dst + 1024 * S::WAVES * i, off[i], S::KB * s);
+                else
+                    b2l<16, ONCE ? HY_CPOL_NT : 0>(wr, dst + 1024 * S::WAVES * i, off[i], S::KB * s);
+            }
         } else {  // the reduction ends inside the stage: zeros behind it
 #pragma unroll
             for (int i = 0; i < S::COPIES; i++) {
@@ -309,8 +313,9 @@ __device__ __forceinline__ void gemm_i8_tile(const GemmI8Args& a, int t0, int n0
 
 constexpr int GT_XCDS = 8, GT_CUS = 32;  // of an XCD
 
-// HALF: the shape of half a tile of channels, which what is left over of the last round falls into, or S itself
-template <class S, class HALF>
+// HALF: the shape of half a tile of channels, which what is left over of the last round falls into, or S itself.
+// ONCE: the weights are read once and past the caches (tiles_once)
+template <class S, class HALF, bool ONCE>
 __global__ __launch_bounds__(S::THREADS, S::WAVES / 4 * (S::LDS > 81920 ? 1 : 2)) void gemm_i8_tile_kernel(
     GemmI8Args a, int tiles_n, int tiles) {
     constexpr bool SPLIT = HALF::BN < S::BN;
@@ -331,9 +336,9 @@ __global__ __launch_bounds__(S::THREADS, S::WAVES / 4 * (S::LDS > 81920 ? 1 : 2)
     const int in_band = o - band * 8 * tiles_t;
     const int n0 = (8 * band + in_band % width) * S::BN, t0 = in_band / width * S::BT;
     if (!SPLIT || half < 0) {
-        gemm_i8_tile<S>(a, t0, n0, lds);
+        gemm_i8_tile<S, ONCE>(a, t0, n0, lds);
     } else if (n0 + half * HALF::BN < a.N) {
-        gemm_i8_tile<HALF>(a, t0, n0 + half * HALF::BN, lds);
+        gemm_i8_tile<HALF, ONCE>(a, t0, n0 + half * HALF::BN, lds);
     }
 }
 
@@ -345,21 +350,33 @@ static void stream(const GemmI8Args& a, hipStream_t s) {
     hipLaunchKernelGGL(gemm_i8_stream_kernel<FUSED>, grid, dim3(GS_THREADS), 0, s, a, tiles_n);
 }
 
-template <class S, class HALF = S>
+template <class S, class HALF = S, bool ONCE = false>
 static void tiles(const GemmI8Args& a, hipStream_t s) {
     const int tiles_n = (a.N + S::BN - 1) / S::BN, tiles = tiles_n * ((a.T + S::BT - 1) / S::BT);
     const int per_xcd = (tiles + GT_XCDS - 1) / GT_XCDS + (HALF::BN < S::BN ? GT_CUS / 2 : 0);
-    hipLaunchKernelGGL((gemm_i8_tile_kernel<S, HALF>), dim3((unsigned)(GT_XCDS * per_xcd)), dim3(S::THREADS), 0, s, a,
+    hipLaunchKernelGGL((gemm_i8_tile_kernel<S, HALF, ONCE>), dim3((unsigned)(GT_XCDS * per_xcd)), dim3(S::THREADS), 0, s, a,
                        tiles_n, tiles);
+}
+// one row of tiles over weights that the Infinity Cache does not hold: past the caches (16 tokens x 133120 channels
+// 120 us, so 112; 20 x 6144, which it holds, 12.1 and 12.7)
+template <class S>
+static void tiles_once(const GemmI8Args& a, hipStream_t s) {
+    if (a.T <= S::BT && (size_t)a.N * a.K > INFINITY_CACHE)
+        tiles<S, S, true>(a, s);
+    else
+        tiles<S>(a, s);
 }
 typedef GtShape<256, 256, 4, 4, 2, 128> GtBig;
 typedef GtShape<256, 128, 4, 4, 2, 128> GtBigHalf;
 typedef GtShape<128, 128, 2, 4, 2, 128> GtMid;
 typedef GtShape<64, 64, 2, 2, 5, 128> GtSmall;
+typedef GtShape<32, 64, 1, 2, 4, 128> GtTiny;
 
 // Which kernel, by what each takes at hidden 4096 (all in proportion to it), us:
-//  * the stream, for up to 4 tokens, or 16 of up to 2^14 channels.  4096 x 6144, 1 token 9.5, by small tiles
-//    13.5; 16 tokens 12.7, 13.5; x 133120, 1 token 117, 122; 16 tokens 191, 122;
+//  * the stream, for up to 4 tokens and 128 MB of weights.  1 and 4 tokens x 6144 channels 9.3, 9.8, by tiles of
+//    32 x 64 10.9, 11.3; x 32000 30.5, 34.7 and 31.8, 32.4 (and a launch more where tokens are f32); x 133120
+//    117, 133 and 97, 102;
+//  * tiles of 32 x 64 for up to 32: 32 x 6144 12.6, by 64 x 64 14.5, 20 11.9 and 13.8, x 133120 128 and 129;
 //  * tiles of 64 x 64: 14, or 6 and 36 ns per tile where that is more;
 //  * tiles of 128 x 128: 25, or 5 and 93 ns per tile;
 //  * tiles of 256 x 256: 70 per round of 256, 45 for a last round of up to 128, which takes half tiles.
@@ -369,9 +386,11 @@ typedef GtShape<64, 64, 2, 2, 5, 128> GtSmall;
 static double tiles_of(const GemmI8Args& a, int bt, int bn) {
     return (double)((a.T + bt - 1) / bt) * ((a.N + bn - 1) / bn);
 }
-static bool by_stream(const GemmI8Args& a) { return a.T <= 4 || (a.T <= 16 && a.N <= 1 << 14); }
+static bool by_stream(const GemmI8Args& a) {
+    return a.T <= GF_TOKENS && a.K <= GF_WIDTH && (size_t)a.N * a.K <= (size_t)1 << 27;
+}
 
-bool gemm_i8_takes_f32(const GemmI8Args& a) { return a.T <= GF_TOKENS && a.K <= GF_WIDTH; }
+bool gemm_i8_takes_f32(const GemmI8Args& a) { return by_stream(a); }
 
 hipError_t launch_gemm_i8(const GemmI8Args& a, hipStream_t s) {
     if (by_stream(a)) {
@@ -382,8 +401,10 @@ hipError_t launch_gemm_i8(const GemmI8Args& a, hipStream_t s) {
     const double small = fmax(14.0, 6.0 + 0.036 * n64), mid = fmax(25.0, 5.0 + 0.093 * n128);
     const double rounds = floor(n256 / 256.0), left = n256 - 256.0 * rounds;
     const double big = 70.0 * rounds + (left == 0.0 ? 0.0 : left <= 128.0 ? 45.0 : 70.0);
-    if (small <= mid && small <= big)
-        tiles<GtSmall>(a, s);
+    if (a.T <= 32)
+        tiles_once<GtTiny>(a, s);
+    else if (small <= mid && small <= big)
+        tiles_once<GtSmall>(a, s);
     else if (mid <= big)
         tiles<GtMid>(a, s);
     else

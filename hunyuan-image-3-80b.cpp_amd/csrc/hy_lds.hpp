@@ -31,16 +31,16 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buf_rsrc(const void* uniform_b
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(uniform_base), (short)0, (int)0xffffffff, 0x00020000);
 }
 // global -> LDS copy of BYTES (4 or 16) per lane: lane l's bytes at base + lane_off +
-// s_off land at lds_wave_base + BYTES * l
-template <int BYTES = 16>
+// s_off land at lds_wave_base + BYTES * l.  CPOL: the cache policy
+template <int BYTES = 16, int CPOL = 0>
 __device__ __forceinline__ void b2l(__amdgpu_buffer_rsrc_t r, void* lds_wave_base, uint32_t lane_off,
                                     uint32_t s_off) {
     static_assert(BYTES == 4 || BYTES == 16, "4- or 16-byte copies");
     auto* l = (__attribute__((address_space(3))) void*)(lds_wave_base);
     if constexpr (BYTES == 4)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, l, 4, lane_off, s_off, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, l, 4, lane_off, s_off, 0, CPOL);
     else
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, l, 16, lane_off, s_off, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, l, 16, lane_off, s_off, 0, CPOL);
 }
 // s_waitcnt vmcnt(N) lgkmcnt(0) (gfx9 encoding: vmcnt[3:0] | expcnt[6:4] | lgkmcnt[11:8])
 #define MM_WAIT_VM_LGKM(N) __builtin_amdgcn_s_waitcnt(((N) & 0xF) | (0x7 << 4) | (((N) >> 4) << 14))
