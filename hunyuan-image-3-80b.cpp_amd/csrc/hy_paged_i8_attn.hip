@@ -253,17 +253,28 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedA
             __builtin_amdgcn_sched_barrier(0);
             const bool edge = (t + 1) * KB > first || __any((vpage[0] | vpage[1]) < 0);
             const int key0 = t * KB + 16 * g;
-#pragma unroll
-            for (int v = 0; v < 16; v++) s[v] = fmaf(s[v], fac[v / 8], ex[v / 8]);
             if (edge) {  // wave-uniform
                 asm volatile("");
 #pragma unroll
-                for (int v = 0; v < 16; v++)
+                for (int v = 0; v < 16; v++) {
+                    s[v] = fmaf(s[v], fac[v / 8], ex[v / 8]);  // before the mask: scales may be NaN
                     if (key0 + v >= end || vpage[v / 8] < 0) s[v] = -INFINITY;
-            }
-            float big = s[0];
+                }
 #pragma unroll
-            for (int v = 1; v < 16; v++) big = fmaxf(big, s[v]);
+                for (int h = 0; h < 2; h++) {
+                    fac[h] = 1.0f;
+                    ex[h] = 0.0f;
+                }
+            }
+            // scales are not negative: a half's largest score has its largest t
+            float big = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float m = s[8 * h];
+#pragma unroll
+                for (int v = 1; v < 8; v++) m = fmaxf(m, s[8 * h + v]);
+                big = fmaxf(big, fmaf(m, fac[h], ex[h]));
+            }
             if (__any(big > m_run + PA_LAG)) {
                 big = row_max<L>(big);
                 const float m = big > m_run + PA_LAG ? big : m_run;
@@ -275,8 +286,10 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedA
             }
             const float ref = (m_run == -INFINITY ? 0.0f : m_run) - 6.0f;  // weights are 2^6 times as large: PF_PSCALE
 #pragma unroll
+            for (int h = 0; h < 2; h++) ex[h] -= ref;
+#pragma unroll
             for (int v = 0; v < 16; v++) {
-                s[v] = __builtin_amdgcn_exp2f(s[v] - ref);
+                s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], fac[v / 8], ex[v / 8]));
                 l_run = fmaf(s[v], inv[v / 8], l_run);  // of this lane's keys; joined behind the loop
                 s[v] *= mant[v / 8];
             }

@@ -96,7 +96,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
     constexpr int RING = KP == 2 ? 2 : 3;  // operands read ahead of the products (registers allowing)
     __shared__ __attribute__((aligned(1024))) uint8_t lds[L::BYTES];
     __shared__ __attribute__((aligned(16))) float k_fac[2][I8 ? 1 : 32], v_exp[2][I8 ? 1 : 32], v_inv[2][I8 ? 1 : 32];
-    __shared__ v4f_t i8_fac[2][I8 ? 8 : 1];  // of four keys: K's scale, V's 2^e as e and 2^-e, and its rest
+    __shared__ v4f_t i8_fac[2][I8 ? 8 : 1];  // of four keys: K's scale, V's as its logarithm and its reciprocal
     __shared__ int odd_s;  // V of this piece that the scaled products do not take
     __shared__ int last_s[PM_WAVES];
     __shared__ PartSums<PM_THREADS> sums;
@@ -178,17 +178,24 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             for (int u = 0; u < 2; u++) q[c][u] = *reinterpret_cast<const v4f_t*>(qp + 16 * c + 4 * u);
         __builtin_amdgcn_sched_barrier(0);
         int64_t tab = page_at(seg, e1), tab2 = page_at(seg + 1, e2);
-        // scales of an 8-bit cache: the same for the neighbouring keys that a wave loads
-        int ptab = e1, ptab2 = e2;
-        auto scale_of = [&](const float* scales, int key) {
-            const int i = (key >> a.c.shift) - seg * 64;
-            const int e = __builtin_amdgcn_readlane(i < 64 ? ptab : ptab2, i & 63);
-            const int64_t p = e >= 0 && e < a.c.n_pages ? e : 0;
-            return scales[((p * a.c.nkv + it.g) << (a.c.shift - a.bshift)) + ((key & pmask) >> a.bshift)];
-        };
         auto lane64 = [](int64_t v, int l) {
             return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) |
                              (uint32_t)__builtin_amdgcn_readlane((int)v, l));
+        };
+        // scales of an 8-bit cache, where the pages' start as tab; one for the neighbouring keys that a wave loads
+        const int64_t page_scales = I8 ? (int64_t)a.c.nkv << (a.c.shift - a.bshift) : 0;
+        const int64_t head_scales = I8 ? (int64_t)it.g << (a.c.shift - a.bshift) : 0;
+        auto scales_at = [&](int seg, int e) {
+            return seg * 64 + lane < n_tab && e >= 0 && e < a.c.n_pages ? e * page_scales : 0;
+        };
+        int64_t stab = 0, stab2 = 0;
+        if constexpr (I8) {
+            stab = scales_at(seg, e1);
+            stab2 = scales_at(seg + 1, e2);
+        }
+        auto scale_of = [&](const float* scales, int key) {
+            const int p = (key >> a.c.shift) - seg * 64;
+            return scales[head_scales + (p < 64 ? lane64(stab, p) : lane64(stab2, p - 64)) + ((key & pmask) >> a.bshift)];
         };
         auto cell_of = [&](int key) {  // wave-uniform; keys up to 64 pages past those of load_v
             const int p = (key >> a.c.shift) - seg * 64;
@@ -228,9 +235,12 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             if (s != seg) {
                 seg = s;
                 tab = tab2;
-                ptab = ptab2;
-                ptab2 = entry(seg + 1);
-                tab2 = page_at(seg + 1, ptab2);
+                const int e = entry(seg + 1);
+                tab2 = page_at(seg + 1, e);
+                if constexpr (I8) {
+                    stab = stab2;
+                    stab2 = scales_at(seg + 1, e);
+                }
             }
         };
         // block kb, r = kb % 2
@@ -292,17 +302,18 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             uint8_t* const d = v_dst + r * L::BUF_V;
             const int key0 = kb * 32 + 4 * wv;
             if constexpr (I8) {
-                const I8Scale v = i8_scale(v_scale);
+                const bool tiny = v_scale < pow2(PM_ELO);  // the same for the wave: values of 0
                 if (v_mine) {
 #pragma unroll
-                    for (int n = 0; n < 2; n++)
-                        *reinterpret_cast<uint2*>(d + n * (HD / 2) * 16) =
-                            make_uint2(i8_pair(vx[0], vx[1], n), i8_pair(vx[2], vx[3], n));
+                    for (int n = 0; n < 2; n++) {
+                        const uint2 w = make_uint2(i8_pair(vx[0], vx[1], n), i8_pair(vx[2], vx[3], n));
+                        *reinterpret_cast<uint2*>(d + n * (HD / 2) * 16) = make_uint2(tiny ? 0 : w.x, tiny ? 0 : w.y);
+                    }
                 }
+                const float sv = tiny ? pow2(PM_ELO) : fmaf(v_scale, 0.0f, v_scale);  // an infinity becomes NaN
                 if (lane == 0) {
-                    i8_fac[r][wv][1] = v.ex;
-                    i8_fac[r][wv][2] = v.inv;
-                    i8_fac[r][wv][3] = v.mant;
+                    i8_fac[r][wv][1] = __builtin_amdgcn_logf(sv);
+                    i8_fac[r][wv][2] = __builtin_amdgcn_rcpf(sv);  // 2^-23 of the keys' weights in the sum
                 }
                 return;
             }
@@ -447,16 +458,17 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 s = mfma_f16(kf[c % RING][0], qf[c][0], s);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            v4f_t inv[4], mant;
+            v4f_t inv[4];
+            float i8_k[4], i8_v[4];  // of an 8-bit cache's scores: t = s i8_k + i8_v, formed in the exponential
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 v4f_t fac, ex;
                 if constexpr (I8) {
                     const v4f_t f = i8_fac[r][2 * u + h];
-                    fac = v4f_t{f[0], f[0], f[0], f[0]};
-                    ex = v4f_t{f[1], f[1], f[1], f[1]};
+                    i8_k[u] = f[0] * unscale;
+                    i8_v[u] = f[1];
                     inv[u][0] = f[2];
-                    mant[u] = f[3];
+                    continue;
                 } else if constexpr (SCALED) {
                     fac = *reinterpret_cast<const v4f_t*>(&k_fac[r][8 * u + 4 * h]);
                     ex = *reinterpret_cast<const v4f_t*>(&v_exp[r][8 * u + 4 * h]);
@@ -477,13 +489,30 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                     const int key = kb * 32 + 8 * u + 4 * h;
                     const bool ok = !bad || page_ok(key);
 #pragma unroll
-                    for (int v = 0; v < 4; v++)
+                    for (int v = 0; v < 4; v++) {
+                        if constexpr (I8) s[4 * u + v] = fmaf(s[4 * u + v], i8_k[u], i8_v[u]);  // before the mask: scales may be NaN
                         if (!ok || key + v >= end) s[4 * u + v] = -INFINITY;
+                    }
+                    if constexpr (I8) {
+                        i8_k[u] = 1.0f;
+                        i8_v[u] = 0.0f;
+                        inv[u][0] = inv[u][0] == inv[u][0] ? inv[u][0] : 0.0f;  // NaN: by the weights of rows that see it
+                    }
                 }
             }
-            float big = s[0];
+            float big;
+            if constexpr (I8) {  // scales are not negative: a group's largest score has its largest t
+                big = -INFINITY;
 #pragma unroll
-            for (int v = 1; v < 16; v++) big = fmaxf(big, s[v]);
+                for (int u = 0; u < 4; u++) {
+                    const float m = fmaxf(fmaxf(s[4 * u], s[4 * u + 1]), fmaxf(s[4 * u + 2], s[4 * u + 3]));
+                    big = fmaxf(big, fmaf(m, i8_k[u], i8_v[u]));
+                }
+            } else {
+                big = s[0];
+#pragma unroll
+                for (int v = 1; v < 16; v++) big = fmaxf(big, s[v]);
+            }
             if constexpr (!SCALED) big *= unscale;
             if (__any(big > m_run + PM_LAG)) {
                 big = fmax_half(big);
@@ -496,29 +525,21 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             }
             const float ref = m_run == -INFINITY ? 0.0f : m_run;
             const float up = ref - (float)PM_WUP;
+            if constexpr (I8) {
+#pragma unroll
+                for (int u = 0; u < 4; u++) i8_v[u] -= up;
+            }
 #pragma unroll
             for (int v = 0; v < 16; v++) {  // l_run: of this lane's keys; joined behind the loop
                 if constexpr (I8) {
-                    s[v] = __builtin_amdgcn_exp2f(s[v] - up);
+                    s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], i8_k[v / 4], i8_v[v / 4]));
                     l_run = fmaf(s[v], inv[v / 4][0], l_run);
-                    s[v] *= mant[v / 4];
                 } else if constexpr (SCALED) {
                     s[v] = __builtin_amdgcn_exp2f(s[v] - up);
                     l_run = fmaf(s[v], inv[v / 4][v % 4], l_run);
                 } else {
                     s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], unscale, -up));
                     l_run += s[v];
-                }
-            }
-            if (I8 && edge) {  // a scale that the row does not see may be NaN
-                asm volatile("");
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const int key = kb * 32 + 8 * u + 4 * h;
-                    const bool ok = !bad || page_ok(key);
-#pragma unroll
-                    for (int v = 0; v < 4; v++)
-                        if (!ok || key + v >= end) s[4 * u + v] = 0.0f;
                 }
             }
 #pragma unroll
