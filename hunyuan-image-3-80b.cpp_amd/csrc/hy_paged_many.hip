@@ -182,20 +182,36 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) |
                              (uint32_t)__builtin_amdgcn_readlane((int)v, l));
         };
-        // scales of an 8-bit cache, where the pages' start as tab; one for the neighbouring keys that a wave loads
-        const int64_t page_scales = I8 ? (int64_t)a.c.nkv << (a.c.shift - a.bshift) : 0;
-        const int64_t head_scales = I8 ? (int64_t)it.g << (a.c.shift - a.bshift) : 0;
-        auto scales_at = [&](int seg, int e) {
-            return seg * 64 + lane < n_tab && e >= 0 && e < a.c.n_pages ? e * page_scales : 0;
+        // scales of an 8-bit cache: those of 64 blocks of positions in the lanes, the next 64's, and the pages of
+        // the 64 behind them (a load per block of keys cost 10 % of a prompt)
+        auto scale_page = [&](int sseg) {
+            return trow[min((sseg * 64 + lane) >> (a.c.shift - a.bshift), max(n_tab - 1, 0))];
         };
-        int64_t stab = 0, stab2 = 0;
+        auto scale_from = [&](const float* scales, int sseg, int e) {
+            const int64_t p = e >= 0 && e < a.c.n_pages ? e : 0;
+            const int per_page = 1 << (a.c.shift - a.bshift);
+            return scales[(p * a.c.nkv + it.g) * per_page + ((sseg * 64 + lane) & (per_page - 1))];
+        };
+        int sseg = 0, sp = 0;
+        float ks = 0.0f, ks2 = 0.0f, vs2 = 0.0f;
+        // V's as their logarithms and reciprocals (to 2^-23 of the keys' weights in the sum); below the range the
+        // lowest logarithm and values of 0, an infinity as NaN
+        float v_log = 0.0f, v_rcp = 0.0f;
+        auto of_v = [&](float v) {
+            v = v < pow2(PM_ELO) ? pow2(PM_ELO) : fmaf(v, 0.0f, v);
+            v_log = __builtin_amdgcn_logf(v);
+            v_rcp = __builtin_amdgcn_rcpf(v);
+        };
         if constexpr (I8) {
-            stab = scales_at(seg, e1);
-            stab2 = scales_at(seg + 1, e2);
+            sseg = (kb0 * 32) >> (a.bshift + 6);
+            const int pg = scale_page(sseg), pg2 = scale_page(sseg + 1);
+            sp = scale_page(sseg + 2);
+            ks = scale_from(a.ks, sseg, pg);
+            of_v(scale_from(a.vs, sseg, pg));
+            ks2 = scale_from(a.ks, sseg + 1, pg2), vs2 = scale_from(a.vs, sseg + 1, pg2);
         }
-        auto scale_of = [&](const float* scales, int key) {
-            const int p = (key >> a.c.shift) - seg * 64;
-            return scales[head_scales + (p < 64 ? lane64(stab, p) : lane64(stab2, p - 64)) + ((key & pmask) >> a.bshift)];
+        auto lane_f = [](float v, int l) {
+            return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), l));
         };
         auto cell_of = [&](int key) {  // wave-uniform; keys up to 64 pages past those of load_v
             const int p = (key >> a.c.shift) - seg * 64;
@@ -216,7 +232,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         uint8_t* const v_dst = lds + L::OFF_V + (2 * (wv / 4) + wv % 2) * L::CHUNK_V + lane * 16 + 8 * (wv / 2 % 2);
         typedef typename std::conditional<I8, uint2, v4i_t>::type krow_t;
         krow_t kx[KP];
-        float k_scale = 0.0f, v_scale = 0.0f;
+        float k_scale = 0.0f, v_ex = 0.0f, v_in = 0.0f;
         typedef typename std::conditional<KP == 2, uint2, typename std::conditional<I8, uint16_t, uint32_t>::type>::type vrow_t;
         vrow_t vx[4];
         uint32_t v_big = 0;  // the largest magnitude of V's: whether one was infinite, no number, or past PM_EHI
@@ -224,22 +240,34 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             const char* const p = reinterpret_cast<const char*>(kg + cell_of(kb * 32 + (wv * KPW) % 32));
 #pragma unroll
             for (int u = 0; u < KP; u++) kx[u] = *reinterpret_cast<const krow_t*>(p + k_off + 16 * u);
-            if constexpr (I8) k_scale = scale_of(a.ks, kb * 32 + (wv * KPW) % 32);
+            if constexpr (I8) {  // up to 64 blocks of positions past those of load_v
+                const int b = ((kb * 32 + (wv * KPW) % 32) >> a.bshift) - sseg * 64;
+                k_scale = lane_f(b < 64 ? ks : ks2, b & 63);
+            }
         };
         auto load_v = [&](int kb) {
             const char* const p = reinterpret_cast<const char*>(vg + cell_of(kb * 32 + 4 * wv));
 #pragma unroll
             for (int j = 0; j < 4; j++) vx[j] = *reinterpret_cast<const vrow_t*>(p + (v_off + j * ts * sizeof(E)));
-            if constexpr (I8) v_scale = scale_of(a.vs, kb * 32 + 4 * wv);
+            if constexpr (I8) {
+                const int b = ((kb * 32 + 4 * wv) >> a.bshift) - sseg * 64;
+                v_ex = lane_f(v_log, b);
+                v_in = lane_f(v_rcp, b);
+            }
             const int s = ((kb + 1) * 32) >> (a.c.shift + 6);  // the next call's
             if (s != seg) {
                 seg = s;
                 tab = tab2;
-                const int e = entry(seg + 1);
-                tab2 = page_at(seg + 1, e);
-                if constexpr (I8) {
-                    stab = stab2;
-                    stab2 = scales_at(seg + 1, e);
+                tab2 = page_at(seg + 1, entry(seg + 1));
+            }
+            if constexpr (I8) {
+                const int t = ((kb + 1) * 32) >> (a.bshift + 6);
+                if (t != sseg) {
+                    sseg = t;
+                    ks = ks2;
+                    of_v(vs2);
+                    ks2 = scale_from(a.ks, sseg + 1, sp), vs2 = scale_from(a.vs, sseg + 1, sp);
+                    sp = scale_page(sseg + 2);
                 }
             }
         };
@@ -302,7 +330,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             uint8_t* const d = v_dst + r * L::BUF_V;
             const int key0 = kb * 32 + 4 * wv;
             if constexpr (I8) {
-                const bool tiny = v_scale < pow2(PM_ELO);  // the same for the wave: values of 0
+                const bool tiny = v_ex == (float)PM_ELO;  // the same for the wave: values of 0
                 if (v_mine) {
 #pragma unroll
                     for (int n = 0; n < 2; n++) {
@@ -310,10 +338,9 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                         *reinterpret_cast<uint2*>(d + n * (HD / 2) * 16) = make_uint2(tiny ? 0 : w.x, tiny ? 0 : w.y);
                     }
                 }
-                const float sv = tiny ? pow2(PM_ELO) : fmaf(v_scale, 0.0f, v_scale);  // an infinity becomes NaN
                 if (lane == 0) {
-                    i8_fac[r][wv][1] = __builtin_amdgcn_logf(sv);
-                    i8_fac[r][wv][2] = __builtin_amdgcn_rcpf(sv);  // 2^-23 of the keys' weights in the sum
+                    i8_fac[r][wv][1] = v_ex;
+                    i8_fac[r][wv][2] = v_in;
                 }
                 return;
             }
