@@ -14,6 +14,7 @@
 #include "../../include/hy_attn.h"
 #include "../host/hy_gguf.hpp"
 #include "hy_device.hpp"
+#include "hy_int8.hpp"
 #include "hy_launch.hpp"
 #include "hy_paged.hpp"
 #include "hy_rules.hpp"
@@ -76,6 +77,12 @@ struct AttnLayer {
     uint32_t cache_len = 0;
     bool loaded = false;
     bool has_in_norm = false;
+    void* i8 = nullptr;        // one allocation: the projections in 8 bits, of the weights that are loaded if has_i8
+    int8_t* qkv_q = nullptr;
+    float* qkv_s = nullptr;
+    int8_t* o_q = nullptr;
+    float* o_s = nullptr;
+    bool has_i8 = false;
 };
 
 size_t al256(size_t b) { return (b + 255) / 256 * 256; }
@@ -98,6 +105,8 @@ struct hy_attn_ctx {
     int decode_waves = 0;      // cap on the decode attention's waves (0: resident count)
     float* xn = nullptr;       // decoder layer: normed input [Tm][H]
     float* hres = nullptr;     // decoder layer: x + attention [Tm][H]
+    void* i8_ws = nullptr;     // of hy_linear_i8, once something is held in 8 bits
+    size_t i8_ws_bytes = 0;
     bool prof = false;
     std::vector<ProfRec> pending;
     std::vector<hipEvent_t> free_events;
@@ -117,6 +126,10 @@ struct hy_model_ctx {
     float* ha = nullptr;       // hidden ping-pong [Tm][H]
     float* hb = nullptr;
     float* normed = nullptr;   // [Tm][H]
+    void* i8 = nullptr;        // lm_head in 8 bits, of the one that is loaded if has_i8
+    int8_t* lm_q = nullptr;
+    float* lm_s = nullptr;
+    bool has_i8 = false;
 };
 
 namespace {
@@ -217,6 +230,8 @@ int run(hy_attn_ctx* c, const AttnLayer& W, const float* x, int T, int mode, con
 // what hy_attn_forward_paged and the paged decoder layer take besides x and out
 struct PagedStep {
     hy::PagedView cache;  // of the layer
+    hy::PagedViewI8 i8;   // and its scales, where the cache is one of 8 bits
+    bool is_i8;
     const hy_paged_batch* batch;
     const float* cos_t;
     const float* sin_t;
@@ -242,17 +257,24 @@ bool pools_apart(const hy::PagedView& v, uint64_t stride, size_t layers) {
     return inside <= stride && (!above || (layers - 1) * (wide)stride + inside <= above);
 }
 
-int check_paged(const hy_attn_ctx* c, uint32_t layer, const hy_paged_cache* cache, const hy_paged_batch* b,
-                PagedStep* st) {
+// cache8: its pool is `cache`, or null
+int check_paged(const hy_attn_ctx* c, uint32_t layer, const hy_paged_cache* cache, const hy_paged_cache_i8* cache8,
+                const hy_paged_batch* b, PagedStep* st) {
     HY_TRY(check_layer(c, layer, true));
-    HY_TRY(hy::paged_cache_check(cache, (uint32_t)c->nh, &st->cache));
+    st->is_i8 = cache8 != nullptr;
+    if (cache8) {
+        HY_TRY(hy::paged_cache_i8_check(cache8, (uint32_t)c->nh, &st->i8));
+        st->cache = st->i8.c;
+    } else {
+        HY_TRY(hy::paged_cache_check(cache, (uint32_t)c->nh, &st->cache));
+    }
     if (st->cache.nkv != c->nkv || st->cache.hd != c->hd)
         return fail(HY_ERR_INVALID, "the cache has %d heads of %d, the context %d of %d", st->cache.nkv, st->cache.hd,
                     c->nkv, c->hd);
     HY_TRY(hy::paged_batch_check(b, st->cache, true));
     if (b->n_rows > (uint32_t)c->Tm)
         return fail(HY_ERR_INVALID, "n_rows=%u exceeds max_tokens=%d", b->n_rows, c->Tm);
-    const uint64_t el = st->cache.type == HY_TYPE_F32 ? 4 : 2;
+    const uint64_t el = st->cache.type == HY_TYPE_F32 ? 4 : st->cache.type == HY_TYPE_I8 ? 1 : 2;
     if (cache->layer_stride * el % 16 || cache->layer_stride >> 44)
         return fail(HY_ERR_INVALID, "layer_stride=%llu must be a multiple of 16 bytes below 2^44 elements",
                     (unsigned long long)cache->layer_stride);
@@ -261,37 +283,90 @@ int check_paged(const hy_attn_ctx* c, uint32_t layer, const hy_paged_cache* cach
                     (unsigned long long)cache->layer_stride, c->layers.size());
     st->cache.k = static_cast<uint8_t*>(st->cache.k) + layer * cache->layer_stride * el;
     st->cache.v = static_cast<uint8_t*>(st->cache.v) + layer * cache->layer_stride * el;
+    if (cache8) {
+        const uint64_t scales = ((uint64_t)st->cache.n_pages * st->cache.nkv) << (st->cache.shift - st->i8.bshift);
+        if (c->layers.size() > 1 && (cache8->layer_scale_stride < scales || cache8->layer_scale_stride >> 44))
+            return fail(HY_ERR_INVALID, "layer_scale_stride=%llu: %llu scales per layer, below 2^44",
+                        (unsigned long long)cache8->layer_scale_stride, (unsigned long long)scales);
+        st->i8.c = st->cache;
+        st->i8.ks += layer * cache8->layer_scale_stride;
+        st->i8.vs += layer * cache8->layer_scale_stride;
+    }
     st->batch = b;
     HY_TRY(hy::paged_rotary_check(c->cfg.rope_theta, st->cos_t, st->sin_t, st->n_pos, c->cfg.rms_norm_eps));
-    return hy::paged_ws_check(b, (uint32_t)c->nh, st->cache, st->ws, st->ws_bytes);
+    return cache8 ? hy::paged_ws_i8_check(b, (uint32_t)c->nh, st->i8, st->ws, st->ws_bytes)
+                  : hy::paged_ws_check(b, (uint32_t)c->nh, st->cache, st->ws, st->ws_bytes);
 }
 
-// run() over a paged cache
+// run() over a paged cache; over one of 8 bits with the layer's projections in 8 bits where it has them
 int run_paged(hy_attn_ctx* c, const AttnLayer& W, const float* x, const PagedStep& st, float* out, hipStream_t s,
               const float* resid = nullptr) {
     const int T = (int)st.batch->n_rows;
-    HY_TRY(timed(c, AK_QKV, s,
-                 [&] { return hy::launch_gemm_nt_f32(x, W.qkv_w, nullptr, c->qkv, T, c->nqkv, c->H, s, c->gemm_ws); }));
-    int rc = HY_OK;  // the paged calls set their own errors
+    const bool q8 = st.is_i8 && W.has_i8;
+    int rc = HY_OK;  // the calls that set their own errors
     const auto call = [&](int r) {
         rc = r;
         return hipSuccess;
     };
+    HY_TRY(timed(c, AK_QKV, s, [&] {
+        return q8 ? call(hy_linear_i8(x, W.qkv_q, W.qkv_s, nullptr, (uint32_t)T, (uint32_t)c->H, (uint32_t)c->nqkv,
+                                      c->qkv, c->i8_ws, c->i8_ws_bytes, s))
+                  : hy::launch_gemm_nt_f32(x, W.qkv_w, nullptr, c->qkv, T, c->nqkv, c->H, s, c->gemm_ws);
+    }));
+    HY_TRY(rc);
     HY_TRY(timed(c, AK_ROPE, s, [&] {
         return call(hy::paged_append(c->qkv, st.batch->n_rows, (uint32_t)c->nh, st.cache, st.batch->positions_dev,
                                      st.batch->slots_dev, c->cfg.rope_theta, st.cos_t, st.sin_t, st.n_pos, W.q_norm,
                                      W.k_norm, c->cfg.rms_norm_eps, c->q, s, c->merged,
-                                     st.batch->q_start_dev + st.batch->n_req));
+                                     st.batch->q_start_dev + st.batch->n_req, st.is_i8 ? &st.i8 : nullptr));
     }));
     HY_TRY(rc);
     HY_TRY(timed(c, AK_ATTN, s, [&] {
-        return call(hy::paged_attention(c->q, (uint32_t)c->nh, st.cache, st.batch, 1.0f / sqrtf((float)c->hd),
-                                        c->merged, st.ws, st.ws_bytes, s));
+        const float scale = 1.0f / sqrtf((float)c->hd);
+        return call(st.is_i8 ? hy::paged_attention_i8(c->q, (uint32_t)c->nh, st.i8, st.batch, scale, c->merged, st.ws,
+                                                      st.ws_bytes, s)
+                             : hy::paged_attention(c->q, (uint32_t)c->nh, st.cache, st.batch, scale, c->merged, st.ws,
+                                                   st.ws_bytes, s));
     }));
     HY_TRY(rc);
-    return timed(c, AK_OPROJ, s, [&] {
-        return hy::launch_gemm_nt_f32(c->merged, W.o_w, resid, out, T, c->H, c->nh * c->hd, s, c->gemm_ws);
-    });
+    HY_TRY(timed(c, AK_OPROJ, s, [&] {
+        return q8 ? call(hy_linear_i8(c->merged, W.o_q, W.o_s, resid, (uint32_t)T, (uint32_t)(c->nh * c->hd),
+                                      (uint32_t)c->H, out, c->i8_ws, c->i8_ws_bytes, s))
+                  : hy::launch_gemm_nt_f32(c->merged, W.o_w, resid, out, T, c->H, c->nh * c->hd, s, c->gemm_ws);
+    }));
+    return rc;
+}
+
+// codes and scales of weights [rows][cols] each, in one allocation (kept where there is one already)
+int alloc_i8(void** base, const size_t (*shape)[2], int8_t** const* codes, float** const* scales, int n) {
+    size_t total = 0;
+    for (int i = 0; i < n; i++) total += al256(shape[i][0] * shape[i][1]) + al256(shape[i][0] * 4);
+    if (!*base && hipMalloc(base, total) != hipSuccess) {
+        *base = nullptr;
+        return fail(HY_ERR_NOMEM, "hipMalloc of %zu bytes for 8-bit weights failed", total);
+    }
+    uint8_t* p = static_cast<uint8_t*>(*base);
+    for (int i = 0; i < n; i++) {
+        *codes[i] = reinterpret_cast<int8_t*>(p);
+        p += al256(shape[i][0] * shape[i][1]);
+        *scales[i] = reinterpret_cast<float*>(p);
+        p += al256(shape[i][0] * 4);
+    }
+    return HY_OK;
+}
+
+// the workspace of the context's 8-bit products
+int alloc_i8_ws(hy_attn_ctx* c) {
+    if (c->i8_ws) return HY_OK;
+    const uint32_t nq = (uint32_t)(c->nh * c->hd), widest = (uint32_t)c->H > nq ? (uint32_t)c->H : nq;
+    const size_t bytes = hy_linear_i8_ws((uint32_t)c->Tm, widest, 1u << 22);
+    if (!bytes) return fail(HY_ERR_UNSUPPORTED, "hidden=%d, heads %u wide: the 8-bit products take less than 2^17", c->H, nq);
+    if (hipMalloc(&c->i8_ws, bytes) != hipSuccess) {
+        c->i8_ws = nullptr;
+        return fail(HY_ERR_NOMEM, "hipMalloc of %zu bytes for 8-bit tokens failed", bytes);
+    }
+    c->i8_ws_bytes = bytes;
+    return HY_OK;
 }
 
 // GGUF tensor -> f32 host copy (row-major as stored: ne0 innermost): F32, F16, BF16,
@@ -378,8 +453,11 @@ int hy_attn_destroy(hy_attn_ctx* c) {
         (void)hipEventDestroy(r.b);
     }
     for (auto e : c->free_events) (void)hipEventDestroy(e);
-    for (auto& L : c->layers)
+    for (auto& L : c->layers) {
         if (L.base) (void)hipFree(L.base);
+        if (L.i8) (void)hipFree(L.i8);
+    }
+    if (c->i8_ws) (void)hipFree(c->i8_ws);
     if (c->arena) (void)hipFree(c->arena);
     delete c;
     return HY_OK;
@@ -392,6 +470,7 @@ int hy_attn_upload(hy_attn_ctx* c, uint32_t layer, const float* qkv_w, const flo
     HIP_TRY(hipSetDevice(c->cfg.device));
     AttnLayer& L = c->layers[layer];
     HY_TRY(alloc_layer(c, L));
+    L.has_i8 = false;
     const size_t nq = (size_t)c->nh * c->hd;
     HIP_TRY(hipMemcpy(L.qkv_w, qkv_w, (size_t)c->nqkv * c->H * 4, hipMemcpyHostToDevice));
     HIP_TRY(hipMemcpy(L.o_w, o_w, (size_t)c->H * nq * 4, hipMemcpyHostToDevice));
@@ -424,6 +503,7 @@ int hy_attn_synth_layer(hy_attn_ctx* c, uint32_t layer, uint64_t seed, float std
     HIP_TRY(hipSetDevice(c->cfg.device));
     AttnLayer& L = c->layers[layer];
     HY_TRY(alloc_layer(c, L));
+    L.has_i8 = false;
     const float scale = std * hy::NORM_SCALE;
     const size_t nq = (size_t)c->nh * c->hd;
     HIP_TRY(hy::launch_synth_fill(L.qkv_w, (size_t)c->nqkv * c->H, hy::stream_key(seed, layer, hy::TENSOR_QKV, 0),
@@ -489,9 +569,37 @@ int hy_attn_forward_paged(hy_attn_ctx* c, uint32_t layer, const float* x, const 
                           const hy_paged_batch* batch, const float* cos_t, const float* sin_t, uint32_t n_pos,
                           float* out, void* ws, size_t ws_bytes, void* stream) {
     if (!x || !out) return fail(HY_ERR_INVALID, "null x/out");
-    PagedStep st{{}, nullptr, cos_t, sin_t, n_pos, ws, ws_bytes};
-    HY_TRY(check_paged(c, layer, cache, batch, &st));
+    PagedStep st{{}, {}, false, nullptr, cos_t, sin_t, n_pos, ws, ws_bytes};
+    HY_TRY(check_paged(c, layer, cache, nullptr, batch, &st));
     return run_paged(c, c->layers[layer], x, st, out, static_cast<hipStream_t>(stream));
+}
+
+int hy_attn_forward_paged_i8(hy_attn_ctx* c, uint32_t layer, const float* x, const hy_paged_cache_i8* cache,
+                             const hy_paged_batch* batch, const float* cos_t, const float* sin_t, uint32_t n_pos,
+                             float* out, void* ws, size_t ws_bytes, void* stream) {
+    if (!x || !out) return fail(HY_ERR_INVALID, "null x/out");
+    if (!cache) return fail(HY_ERR_INVALID, "null cache");
+    PagedStep st{{}, {}, false, nullptr, cos_t, sin_t, n_pos, ws, ws_bytes};
+    HY_TRY(check_paged(c, layer, &cache->pool, cache, batch, &st));
+    return run_paged(c, c->layers[layer], x, st, out, static_cast<hipStream_t>(stream));
+}
+
+int hy_attn_quantize_i8(hy_attn_ctx* c, uint32_t layer) {
+    HY_TRY(check_layer(c, layer, true));
+    HIP_TRY(hipSetDevice(c->cfg.device));
+    AttnLayer& L = c->layers[layer];
+    HY_TRY(alloc_i8_ws(c));
+    const size_t nq = (size_t)c->nh * c->hd, shape[2][2] = {{(size_t)c->nqkv, (size_t)c->H}, {(size_t)c->H, nq}};
+    int8_t** const codes[] = {&L.qkv_q, &L.o_q};
+    float** const scales[] = {&L.qkv_s, &L.o_s};
+    HIP_TRY(hipDeviceSynchronize());  // calls on the codes there were
+    L.has_i8 = false;
+    HY_TRY(alloc_i8(&L.i8, shape, codes, scales, 2));
+    HY_TRY(hy_quantize_rows_i8(L.qkv_w, (uint32_t)c->nqkv, (uint32_t)c->H, L.qkv_q, L.qkv_s, nullptr));
+    HY_TRY(hy_quantize_rows_i8(L.o_w, (uint32_t)c->H, (uint32_t)nq, L.o_q, L.o_s, nullptr));
+    HIP_TRY(hipDeviceSynchronize());
+    L.has_i8 = true;
+    return HY_OK;
 }
 
 int hy_attn_cache_reset(hy_attn_ctx* c) {
@@ -710,6 +818,7 @@ int hy_model_destroy(hy_model_ctx* m) {
     hy_attn_destroy(m->attn);
     hy_moe_destroy(m->moe);
     if (m->arena) (void)hipFree(m->arena);
+    if (m->i8) (void)hipFree(m->i8);
     delete m;
     return HY_OK;
 }
@@ -723,6 +832,7 @@ int hy_model_upload_globals(hy_model_ctx* m, const float* embedding, const float
     const size_t VH = (size_t)m->V * m->H;
     if (embedding) HIP_TRY(hipMemcpy(m->embed, embedding, VH * 4, hipMemcpyHostToDevice));
     if (final_norm) HIP_TRY(hipMemcpy(m->fnorm, final_norm, (size_t)m->H * 4, hipMemcpyHostToDevice));
+    if (lm_head) m->has_i8 = false;
     if (lm_head) HIP_TRY(hipMemcpy(m->lm_head, lm_head, VH * 4, hipMemcpyHostToDevice));
     return HY_OK;
 }
@@ -740,6 +850,7 @@ int hy_model_upload_globals_gguf(hy_model_ctx* m, const hy_gguf* g) {
 int hy_model_synth_globals(hy_model_ctx* m, uint64_t seed, float std) {
     if (!m) return fail(HY_ERR_INVALID, "null ctx");
     HIP_TRY(hipSetDevice(m->cfg.attn.device));
+    m->has_i8 = false;
     const size_t VH = (size_t)m->V * m->H;
     const float scale = std * hy::NORM_SCALE;
     HIP_TRY(hy::launch_synth_fill(m->embed, VH, hy::stream_key(seed, 0, hy::TENSOR_EMBED, 0), scale, nullptr));
@@ -782,17 +893,20 @@ int hy_model_forward(hy_model_ctx* m, const int32_t* ids, uint32_t T, const int3
     return HY_OK;
 }
 
-int hy_model_forward_paged(hy_model_ctx* m, const int32_t* ids, const hy_paged_cache* cache,
-                           const hy_paged_batch* batch, float* logits, void* ws, size_t ws_bytes, void* stream) {
-    if (!m) return fail(HY_ERR_INVALID, "null ctx");
+}  // extern "C"
+
+// over a paged cache; cache8: its pool is `cache`, or null
+static int forward_paged(hy_model_ctx* m, const int32_t* ids, const hy_paged_cache* cache,
+                         const hy_paged_cache_i8* cache8, const hy_paged_batch* batch, float* logits, void* ws,
+                         size_t ws_bytes, void* stream) {
     if (!ids || !logits) return fail(HY_ERR_INVALID, "null ids/logits");
     hy_attn_ctx* c = m->attn;
     if (hy::moe_drops_tokens(m->moe))
         return fail(HY_ERR_UNSUPPORTED,
                     "drop_tokens: a request's experts would depend on the other requests' rows and on rows of nobody");
     for (uint32_t l = 0; l < (uint32_t)m->L; l++) {  // every layer, before anything is launched
-        PagedStep st{{}, nullptr, nullptr, nullptr, 0, ws, ws_bytes};
-        HY_TRY(check_paged(c, l, cache, batch, &st));
+        PagedStep st{{}, {}, false, nullptr, nullptr, nullptr, 0, ws, ws_bytes};
+        HY_TRY(check_paged(c, l, cache, cache8, batch, &st));
         HY_TRY(hy::moe_layer_check(m->moe, l, batch->n_rows));
     }
     const int T = (int)batch->n_rows;
@@ -802,8 +916,8 @@ int hy_model_forward_paged(hy_model_ctx* m, const int32_t* ids, const hy_paged_c
     const float* cur = m->hb;
     for (uint32_t l = 0; l < (uint32_t)m->L; l++) {  // as hy_decoder_layer_forward
         const AttnLayer& W = c->layers[l];
-        PagedStep st{{}, nullptr, nullptr, nullptr, 0, ws, ws_bytes};
-        HY_TRY(check_paged(c, l, cache, batch, &st));
+        PagedStep st{{}, {}, false, nullptr, nullptr, nullptr, 0, ws, ws_bytes};
+        HY_TRY(check_paged(c, l, cache, cache8, batch, &st));
         float* dst = cur == m->ha ? m->hb : m->ha;
         HIP_TRY(W.has_in_norm ? hy::launch_rms_norm_w(cur, W.in_norm, T, m->H, eps, c->xn, s)
                               : hy::launch_rms_norm(cur, T, m->H, eps, c->xn, s));
@@ -812,7 +926,43 @@ int hy_model_forward_paged(hy_model_ctx* m, const int32_t* ids, const hy_paged_c
         cur = dst;
     }
     HIP_TRY(hy::launch_rms_norm_w(cur, m->fnorm, T, m->H, eps, m->normed, s));
+    if (cache8 && m->has_i8)
+        return hy_linear_i8(m->normed, m->lm_q, m->lm_s, nullptr, (uint32_t)T, (uint32_t)m->H, (uint32_t)m->V, logits,
+                            c->i8_ws, c->i8_ws_bytes, stream);
     HIP_TRY(hy::launch_gemm_nt_f32(m->normed, m->lm_head, nullptr, logits, T, m->V, m->H, s, c->gemm_ws));
+    return HY_OK;
+}
+
+extern "C" {
+
+int hy_model_forward_paged(hy_model_ctx* m, const int32_t* ids, const hy_paged_cache* cache,
+                           const hy_paged_batch* batch, float* logits, void* ws, size_t ws_bytes, void* stream) {
+    if (!m) return fail(HY_ERR_INVALID, "null ctx");
+    return forward_paged(m, ids, cache, nullptr, batch, logits, ws, ws_bytes, stream);
+}
+
+int hy_model_forward_paged_i8(hy_model_ctx* m, const int32_t* ids, const hy_paged_cache_i8* cache,
+                              const hy_paged_batch* batch, float* logits, void* ws, size_t ws_bytes, void* stream) {
+    if (!m) return fail(HY_ERR_INVALID, "null ctx");
+    if (!cache) return fail(HY_ERR_INVALID, "null cache");
+    return forward_paged(m, ids, &cache->pool, cache, batch, logits, ws, ws_bytes, stream);
+}
+
+int hy_model_quantize_i8(hy_model_ctx* m) {
+    if (!m) return fail(HY_ERR_INVALID, "null ctx");
+    for (uint32_t l = 0; l < (uint32_t)m->L; l++) HY_TRY(check_layer(m->attn, l, true));
+    HIP_TRY(hipSetDevice(m->cfg.attn.device));
+    HY_TRY(alloc_i8_ws(m->attn));
+    if ((uint32_t)m->V > 1u << 22) return fail(HY_ERR_UNSUPPORTED, "vocab=%d: the 8-bit products take 2^22 at most", m->V);
+    const size_t shape[1][2] = {{(size_t)m->V, (size_t)m->H}};
+    int8_t** const codes[] = {&m->lm_q};
+    float** const scales[] = {&m->lm_s};
+    HIP_TRY(hipDeviceSynchronize());  // calls on the codes there were
+    m->has_i8 = false;
+    HY_TRY(alloc_i8(&m->i8, shape, codes, scales, 1));
+    HY_TRY(hy_quantize_rows_i8(m->lm_head, (uint32_t)m->V, (uint32_t)m->H, m->lm_q, m->lm_s, nullptr));
+    for (uint32_t l = 0; l < (uint32_t)m->L; l++) HY_TRY(hy_attn_quantize_i8(m->attn, l));
+    m->has_i8 = true;
     return HY_OK;
 }
 

@@ -56,6 +56,9 @@ hipError_t launch_paged_append_i8(const PagedAppendArgs& a, const PagedViewI8& v
 
 // host checks and calls that the C entries share (hy_int8_capi.hip)
 int paged_cache_i8_check(const hy_paged_cache_i8* cache, uint32_t n_heads, PagedViewI8* out);
+int paged_ws_i8_check(const hy_paged_batch* b, uint32_t n_heads, const PagedViewI8& v, const void* ws, size_t ws_bytes);
+int paged_attention_i8(const float* q, uint32_t n_heads, const PagedViewI8& v, const hy_paged_batch* b, float scale,
+                       float* out, void* ws, size_t ws_bytes, hipStream_t s);
 
 hipError_t launch_paged_attn_i8(const PagedAttnArgs& a, int max_new, hipStream_t s);
 size_t paged_attn_i8_ws_bytes(int n_req, int max_new, int G, int hd);

@@ -77,9 +77,14 @@ int paged_cache_i8_check(const hy_paged_cache_i8* cache, uint32_t n_heads, Paged
     return HY_OK;
 }
 
-size_t paged_batch_i8_ws(const hy_paged_batch* b, uint32_t n_heads, const PagedViewI8& v) {
+static size_t paged_batch_i8_ws(const hy_paged_batch* b, uint32_t n_heads, const PagedViewI8& v) {
     return paged_attn_i8_ws_bytes((int)b->n_req, (int)(b->max_new < b->n_rows ? b->max_new : b->n_rows),
                                   (int)n_heads / v.c.nkv, v.c.hd);
+}
+
+int paged_ws_i8_check(const hy_paged_batch* b, uint32_t n_heads, const PagedViewI8& v, const void* ws,
+                      size_t ws_bytes) {
+    return ws_check(ws, ws_bytes, paged_batch_i8_ws(b, n_heads, v));
 }
 
 int paged_attention_i8(const float* q, uint32_t n_heads, const PagedViewI8& v, const hy_paged_batch* b, float scale,
@@ -87,7 +92,7 @@ int paged_attention_i8(const float* q, uint32_t n_heads, const PagedViewI8& v, c
     if (!q || !out) return fail(HY_ERR_INVALID, "null q/out");
     if (!std::isfinite(scale)) return fail(HY_ERR_INVALID, "scale is not finite");
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(HY_ERR_INVALID, "q and out must be aligned to 16 bytes");
-    HY_TRY(ws_check(ws, ws_bytes, paged_batch_i8_ws(b, n_heads, v)));
+    HY_TRY(paged_ws_i8_check(b, n_heads, v, ws, ws_bytes));
     const PagedAttnArgs a{q, out, v.c, (int)n_heads, (int)b->n_req, (int)b->n_rows, (int)b->max_pages, b->q_start_dev,
                           b->kv_len_dev, b->table_dev, b->seen_dev, scale, static_cast<float*>(ws), v.ks, v.vs,
                           v.bshift};

@@ -358,9 +358,16 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedA
 }
 
 constexpr int PF_ROWS = 32;
+// Rows of the largest request up to which the streams take a whole batch; past it they take the
+// requests of PF_ROWS rows at most, tiles of 256 rows the others.  Measured with both, us, stream and tiles:
+//  * head_dim 128, one or two requests are few items for the stream to cut: 2 of 64 rows behind 6000 keys 49,
+//    42, 1 of 64 52, 42.  More of them: 3 of 256 behind 6000 78, 91, 6 of 384 behind 1000 55, 59; 16 of 64
+//    behind 8000 133, 209, of 128 213, 219, of 256 371, 293, behind 1000 77, 64;
+//  * head_dim 64: 4 of 1024 25, 27, of 2048 39, 37; 6 of 1024 behind 1000 49, 53, of 2048 81, 78; 2 of 1024
+//    behind 6000 69, 72; 16 of 128 behind 8000 84, 96, of 256 140, 116.
 static int i8_max_rows(int n_req, int hd) {
-    if (hd == 64) return 2048;
-    return n_req <= 2 ? PF_ROWS : 128;
+    if (hd == 64) return n_req <= 8 ? 1536 : 128;
+    return n_req <= 2 ? PF_ROWS : n_req <= 8 ? 384 : 128;
 }
 
 static PaPlan i8_plan(int n_req, int max_new, int G, int hd) {

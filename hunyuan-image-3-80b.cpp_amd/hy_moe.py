@@ -207,6 +207,12 @@ _SIGS = {
     "hy_paged_attention_i8_ws": (C.c_size_t, [_u32, C.POINTER(PagedCacheI8), C.POINTER(PagedBatch)]),
     "hy_paged_attention_i8": (C.c_int, [_vp, _u32, C.POINTER(PagedCacheI8), C.POINTER(PagedBatch), _f, _vp, _vp,
                                         C.c_size_t, _vp]),
+    "hy_attn_quantize_i8": (C.c_int, [_vp, _u32]),
+    "hy_model_quantize_i8": (C.c_int, [_vp]),
+    "hy_attn_forward_paged_i8": (C.c_int, [_vp, _u32, _vp, C.POINTER(PagedCacheI8), C.POINTER(PagedBatch), _vp, _vp,
+                                           _u32, _vp, _vp, C.c_size_t, _vp]),
+    "hy_model_forward_paged_i8": (C.c_int, [_vp, _vp, C.POINTER(PagedCacheI8), C.POINTER(PagedBatch), _vp, _vp,
+                                            C.c_size_t, _vp]),
 }
 
 _lib = None
@@ -667,6 +673,16 @@ class Attn:
                                           sin.ptr if sin is not None else None, n_pos, out.ptr, ws.ptr, ws_bytes,
                                           stream))
 
+    def quantize_i8(self, layer=0):
+        """The layer's projections in 8 bits besides, for forward_paged_i8."""
+        check(lib().hy_attn_quantize_i8(self.h, layer))
+
+    def forward_paged_i8(self, x: Buf, cache, batch, out: Buf, ws: Buf, ws_bytes, cos=None, sin=None, n_pos=0,
+                         stream=None, layer=0):
+        """forward over a paged cache of 8 bits (PagedCacheI8, PagedBatch with positions and slots)."""
+        check(lib().hy_attn_forward_paged_i8(self.h, layer, x.ptr, cache, batch, _ptr(cos), _ptr(sin), n_pos, out.ptr,
+                                             ws.ptr, ws_bytes, stream))
+
     def set_input_norm(self, w=None, layer=0):
         """input_layernorm weight [H] (None: unit) for decoder_layer_forward."""
         if w is None:
@@ -762,6 +778,13 @@ class Model:
 
     def forward_paged(self, ids: Buf, cache, batch, logits: Buf, ws: Buf, ws_bytes, stream=None):
         check(lib().hy_model_forward_paged(self.h, ids.ptr, cache, batch, logits.ptr, ws.ptr, ws_bytes, stream))
+
+    def quantize_i8(self):
+        """Every layer's projections and the lm_head in 8 bits besides, for forward_paged_i8."""
+        check(lib().hy_model_quantize_i8(self.h))
+
+    def forward_paged_i8(self, ids: Buf, cache, batch, logits: Buf, ws: Buf, ws_bytes, stream=None):
+        check(lib().hy_model_forward_paged_i8(self.h, ids.ptr, cache, batch, logits.ptr, ws.ptr, ws_bytes, stream))
 
     def forward_hidden(self, embeds: Buf, T, hidden: Buf, n_layers=0, positions=None, stream=None):
         check(lib().hy_model_forward_hidden(self.h, embeds.ptr, T, positions.ptr if positions is not None else None,

@@ -76,8 +76,8 @@ typedef struct {
                                   * looked at only where there are several layers) */
 } hy_paged_cache_i8;
 
-/* hy_rope_qknorm_paged with the write of codes.  A key's norm(rotate(k)) is computed to 2^-45
- * and rounded to f32 once, so that its code does not depend on the order of a sum.  The rows of
+/* hy_rope_qknorm_paged with the write of codes.  A key's norm(rotate(k)) is computed in
+ * 64 bits and rounded to f32 once, so that its code does not depend on the order of a sum.  The rows of
  * a call that fall into one block of one page have to be neighbours among the rows, in the order
  * of their positions and without gaps, as hy_paged_plan gives them.  A block whose first position
  * is among them begins anew: its scale is theirs, its positions that are not written become
@@ -95,16 +95,36 @@ int hy_rope_qknorm_paged_i8(const float* qkv_dev, uint32_t n_rows, uint32_t n_he
                             const float* sin_dev, uint32_t n_pos, const float* q_norm_dev, const float* k_norm_dev,
                             float eps, float* q_dev, void* stream);
 
-/* hy_paged_attention over such a cache: k_j and v_j are code * scale.  The same accuracy; keys'
- * scales of any size as long as scores stay in f32's range, values' from 2^-60 to 2^34 (smaller ones
- * lose bits, to an absolute 2^-98; larger ones are not defined).  A row that sees a
- * key of a block whose key or value scale is infinite or NaN is NaN; a key that no row sees
- * touches none, whatever its block's scales.  ws_dev: hy_paged_attention_i8_ws bytes (0 for bad
+/* hy_paged_attention over such a cache: k_j and v_j are code * scale.  Products and sums have f32
+ * accuracy, relative to the largest elements of q, of a key and of a value row; products of a
+ * weight and its value's scale are taken to 2^-31 of the row's largest.  Scales are not negative;
+ * keys' are of any size as long as scores stay in f32's range, values' from 2^-59 to 2^34 (below that
+ * a value may count as 0, which is 2^-52 at most; larger ones are not defined).  A row that sees a
+ * key of a block whose key or value scale is infinite or NaN is NaN; a key that a row does not
+ * see does not touch it, whatever its block's scales.  ws_dev: hy_paged_attention_i8_ws bytes (0 for bad
  * arguments), aligned to 16 bytes, contents indifferent. */
 size_t hy_paged_attention_i8_ws(uint32_t n_heads, const hy_paged_cache_i8* cache, const hy_paged_batch* batch);
 int hy_paged_attention_i8(const float* q_dev, uint32_t n_heads, const hy_paged_cache_i8* cache,
                           const hy_paged_batch* batch, float scale, float* out_dev, void* ws_dev, size_t ws_bytes,
                           void* stream);
+
+/* ---- the layer and the backbone ------------------------------------------------ */
+
+/* Holds `layer`'s projections (hy_model_quantize_i8: every layer's, and the lm_head) in 8 bits
+ * besides f32: the two calls below take those from then on, until the weights are loaded anew.
+ * Allocates, and waits for the device; not while a stream is captured. */
+int hy_attn_quantize_i8(hy_attn_ctx* ctx, uint32_t layer);
+int hy_model_quantize_i8(hy_model_ctx* ctx);
+
+/* hy_attn_forward_paged and hy_model_forward_paged over a cache of 8 bits, with the products in
+ * f32, or in 8 bits of weights that are held so.  Of several layers the pools lie as there,
+ * the scales layer_scale_stride floats apart, at least as many as one layer has. */
+int hy_attn_forward_paged_i8(hy_attn_ctx* ctx, uint32_t layer, const float* x_dev, const hy_paged_cache_i8* cache,
+                             const hy_paged_batch* batch, const float* cos_dev, const float* sin_dev, uint32_t n_pos,
+                             float* out_dev, void* ws_dev, size_t ws_bytes, void* stream);
+int hy_model_forward_paged_i8(hy_model_ctx* ctx, const int32_t* ids_dev, const hy_paged_cache_i8* cache,
+                              const hy_paged_batch* batch, float* logits_dev, void* ws_dev, size_t ws_bytes,
+                              void* stream);
 
 #ifdef __cplusplus
 }

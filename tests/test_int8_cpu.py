@@ -158,6 +158,13 @@ def test_products_refused(hy):
         assert L.hy_quantize_rows_i8(*a.values(), None) == INVALID, kw
 
 
+def test_context_calls_refuse_null(hy):
+    L = hy.lib()
+    assert L.hy_attn_forward_paged_i8(None, 0, P, _cache(hy), _batch(hy), None, None, 0, P, P, 1 << 40, None) == INVALID
+    assert L.hy_model_forward_paged_i8(None, P, _cache(hy), _batch(hy), P, P, 1 << 40, None) == INVALID
+    assert L.hy_attn_quantize_i8(None, 0) == INVALID and L.hy_model_quantize_i8(None) == INVALID
+
+
 def test_workspace_is_bounded(hy):
     L = hy.lib()
     for hd in (64, 128):
