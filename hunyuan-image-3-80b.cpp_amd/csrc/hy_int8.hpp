@@ -61,6 +61,6 @@ int paged_attention_i8(const float* q, uint32_t n_heads, const PagedViewI8& v, c
                        float* out, void* ws, size_t ws_bytes, hipStream_t s);
 
 hipError_t launch_paged_attn_i8(const PagedAttnArgs& a, int max_new, hipStream_t s);
-size_t paged_attn_i8_ws_bytes(int n_req, int max_new, int G, int hd);
+size_t paged_attn_i8_ws_bytes(int n_req, int max_new, int G, int nkv, int hd);
 
 }  // namespace hy

@@ -79,7 +79,7 @@ int paged_cache_i8_check(const hy_paged_cache_i8* cache, uint32_t n_heads, Paged
 
 static size_t paged_batch_i8_ws(const hy_paged_batch* b, uint32_t n_heads, const PagedViewI8& v) {
     return paged_attn_i8_ws_bytes((int)b->n_req, (int)(b->max_new < b->n_rows ? b->max_new : b->n_rows),
-                                  (int)n_heads / v.c.nkv, v.c.hd);
+                                  (int)n_heads / v.c.nkv, v.c.nkv, v.c.hd);
 }
 
 int paged_ws_i8_check(const hy_paged_batch* b, uint32_t n_heads, const PagedViewI8& v, const void* ws,

@@ -370,32 +370,41 @@ static int i8_max_rows(int n_req, int hd) {
     return n_req <= 2 ? PF_ROWS : n_req <= 8 ? 384 : 128;
 }
 
-static PaPlan i8_plan(int n_req, int max_new, int G, int hd) {
+// Up to WIDE_ITEMS tiles of 32 rows half the workers, one wave per SIMD, take the stream: half the pieces to join.
+// head_dim 128, both numbers of workers, us: 32 requests of 6 tokens behind 2000 keys (256 tiles) 48, 63, behind
+// 6000 112, 117; 16 of 8 behind 8000 (128) 87, 90; 3 of 64 behind 6000 (192) 77, 82; 64 of 5 behind 3000 (512)
+// 111, 104; 16 of 32 behind 8000 (512) 220, 215.
+constexpr int WIDE_ITEMS = 256;
+
+static PaPlan i8_plan(int n_req, int max_new, int G, int nkv, int hd) {
     const int64_t rows = (int64_t)max_new * G;  // of one request, at most
     constexpr int64_t ALL = (int64_t)1 << 62;
     const bool many = rows > i8_max_rows(n_req, hd), few = !many || n_req > 1;
     PaPlan p;
-    p.few = part_shape(rows > 16 && !many ? 5 : 4, G, 0, many ? PF_ROWS : ALL, few ? PF_WORKERS : 0, 16, 32, 32, 0);
+    const bool wide = rows > 16 && !many, half = wide && (rows + 31) / 32 * n_req * nkv <= WIDE_ITEMS;
+    const int workers = !few ? 0 : half ? PF_WORKERS / 2 : PF_WORKERS;
+    p.few = part_shape(wide ? 5 : 4, G, 0, many ? PF_ROWS : ALL, workers, 16, 32, 32, 0);
     const size_t few_ws = part_ws_floats(p.few.workers, p.few.M, hd);
     p.many = part_shape(PM_TILE_SHIFT, G, few ? PF_ROWS : 0, ALL, many ? PM_WORKERS : 0, 256, 128, 128, few_ws);
     return p;
 }
 
-size_t paged_attn_i8_ws_bytes(int n_req, int max_new, int G, int hd) {
-    const PaPlan p = i8_plan(n_req, max_new, G, hd);
+size_t paged_attn_i8_ws_bytes(int n_req, int max_new, int G, int nkv, int hd) {
+    const PaPlan p = i8_plan(n_req, max_new, G, nkv, hd);
     return 4 * (p.many.ws + part_ws_floats(p.many.workers, PM_TILE, hd));
 }
 
 template <int HD>
 static void launch(const PagedAttnArgs& a, const PaPlan& p, hipStream_t s) {
+    const dim3 grid(p.few.workers / PF_WAVES), block(WAVE * PF_WAVES);
     if (p.few.M == 32)
-        hipLaunchKernelGGL((paged_i8_few_kernel<HD, 32>), dim3(PF_GROUPS), dim3(WAVE * PF_WAVES), 0, s, a, p.few);
+        hipLaunchKernelGGL((paged_i8_few_kernel<HD, 32>), grid, block, 0, s, a, p.few);
     else
-        hipLaunchKernelGGL((paged_i8_few_kernel<HD, 16>), dim3(PF_GROUPS), dim3(WAVE * PF_WAVES), 0, s, a, p.few);
+        hipLaunchKernelGGL((paged_i8_few_kernel<HD, 16>), grid, block, 0, s, a, p.few);
 }
 
 hipError_t launch_paged_attn_i8(const PagedAttnArgs& a, int max_new, hipStream_t s) {
-    const PaPlan p = i8_plan(a.n_req, max_new, a.nh / a.c.nkv, a.c.hd);
+    const PaPlan p = i8_plan(a.n_req, max_new, a.nh / a.c.nkv, a.c.nkv, a.c.hd);
     if (p.few.workers) a.c.hd == 128 ? launch<128>(a, p, s) : launch<64>(a, p, s);
     if (p.many.workers) launch_paged_many(a, p.many, s);
     return launch_paged_join(a, p, s);
