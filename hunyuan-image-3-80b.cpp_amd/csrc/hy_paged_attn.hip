@@ -151,10 +151,6 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
 #pragma unroll
                         for (int c = 0; c < PC; c++) qf[t][s][c][j] = (int)w[c];
                     }
-                if constexpr (F16T) {
-#pragma unroll
-                    for (int s = 0; s < NQ; s++) settle(qf[t][s][1]);
-                }
             }
         }
 
@@ -355,10 +351,6 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_few_kernel(PagedAttn
 #pragma unroll
                             for (int q = 0; q < PC; q++) pf[c][q][2 * u + v] = (int)w[q];
                         }
-                if constexpr (F16T) {
-#pragma unroll
-                    for (int c = 0; c < NT; c++) settle(pf[c][1]);
-                }
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
                     v4i_t vf;  // dims VD i + d of keys 4 g4 .. + 3 of both tiles

@@ -139,8 +139,6 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedA
                     qf[s][0][j] = (int)hi;
                     qf[s][1][j] = (int)lo;
                 }
-#pragma unroll
-            for (int s = 0; s < 2 * NL; s++) settle(qf[s][1]);
         }
 
         // block table: 64 entries in the lanes, the next 64 on their way
@@ -309,8 +307,6 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedA
                     pf[c][0][j] = (int)hi;
                     pf[c][1][j] = (int)lo;
                 }
-#pragma unroll
-            for (int c = 0; c < 2; c++) settle(pf[c][1]);
 #pragma unroll
             for (int c = 0; c < 2; c++)
 #pragma unroll

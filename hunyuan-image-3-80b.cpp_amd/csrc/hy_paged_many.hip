@@ -459,8 +459,6 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                     qf[c][0][j] = (int)w0;
                     qf[c][1][j] = (int)w1;
                 }
-#pragma unroll
-            for (int c = 0; c < NC; c++) settle(qf[c][1]);
         }
 
         v4i_t pf[2][2];  // the weights' pieces, keys 16 c .. in step c
@@ -578,8 +576,6 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                     pf[c][0][j] = (int)w0;
                     pf[c][1][j] = (int)w1;
                 }
-#pragma unroll
-            for (int c = 0; c < 2; c++) settle(pf[c][1]);
         };
         auto values = [&](int r) {
             const uint8_t* const vb = lds + L::OFF_V + r * L::BUF_V + h * L::CHUNK_V + lr * 16;

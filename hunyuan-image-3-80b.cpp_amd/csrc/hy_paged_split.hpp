@@ -47,17 +47,18 @@ __device__ __forceinline__ float fadd_row(float v) {
 __device__ __forceinline__ uint32_t pk_f16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f_t){a, b}, v2h16_t));
 }
-// pieces of two floats; the remainders x - hi are rounded as they are formed (v_fma_mixlo_f16 /
-// mixhi: hi's half times -1 plus x, one rounding)
+// Pieces of two floats; the remainders x - hi are rounded as they are formed (v_fma_mixlo_f16 / mixhi: hi's
+// half times -1 plus x, one rounding).  The compiler has to write those itself: a matrix instruction may read
+// a register two wait states after a vector instruction wrote it, and it sees to that for its own
+// instructions, not for those of inline asm (whose last half was read before it was written).
 __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
-    hi = pk_f16(a, b);
-    asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(lo) : "v"(hi), "v"(a));
-    asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(lo) : "v"(hi), "v"(b));
+    const v2h16_t h = __builtin_convertvector((v2f_t){a, b}, v2h16_t);
+    hi = __builtin_bit_cast(uint32_t, h);
+    float minus = -1.0f;
+    asm("" : "+s"(minus));  // or the product becomes a subtraction, which has no such form
+    lo = __builtin_bit_cast(uint32_t,
+                            (v2h16_t){(_Float16)fmaf((float)h[0], minus, a), (_Float16)fmaf((float)h[1], minus, b)});
 }
-// Two wait states have to pass before a matrix instruction reads what a vector instruction wrote.  The
-// compiler sees to that for its own instructions, not for those of inline asm: an operand of split_f16's
-// remainders goes through here first (without it an operand's last half was read before it was written).
-__device__ __forceinline__ void settle(v4i_t& x) { asm("s_nop 1" : "+v"(x)); }
 
 // 8-bit codes as f16, exactly: with its sign flipped and 0x64 above it a byte is 1024 + 128 + code.
 // four codes of a dword, in their order

@@ -109,10 +109,6 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && HD == 12
 #pragma unroll
                     for (int c = 0; c < PC; c++) qf[s][c][j] = (int)w[c];
                 }
-            if constexpr (F16T) {
-#pragma unroll
-                for (int s = 0; s < NQ; s++) settle(qf[s][1]);
-            }
         }
 
         // block table: 64 entries in the lanes, the next 64 on their way
@@ -227,10 +223,6 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, PaType<E>::PIECES == 3 && HD == 12
 #pragma unroll
                     for (int q = 0; q < PC; q++) pf[c][q][j] = (int)w[q];
                 }
-            if constexpr (F16T) {
-#pragma unroll
-                for (int c = 0; c < 2; c++) settle(pf[c][1]);
-            }
 #pragma unroll
             for (int c = 0; c < 2; c++)
 #pragma unroll
