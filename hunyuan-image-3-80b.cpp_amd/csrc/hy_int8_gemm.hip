@@ -177,7 +177,11 @@ __global__ __launch_bounds__(GS_THREADS) void gemm_i8_stream_kernel(GemmI8Args a
 // Piece c (16 bytes) of a stage's row lies in place c ^ swap(row), so that 16 rows' reads of one piece touch
 // every bank once.  The copies' places are fixed, so they fetch the pieces swapped.
 // Rows of 128 bytes: with 64 the copies are half as fast (a request of the L2 is 64 bytes of a line of
-// 128).  What bounds the tiles of 256 x 256: see launch_gemm_i8.
+// 128).
+// Bounds.  Tiles of 256 x 256 (4096 tokens x 4096 x 6144: 114 us, 1.8 PO/s; 8192^3 reaches 2.2, a library
+// product 2.09): the matrix pipe and the power it draws, the copies from the L2 and, at 6144 channels, one
+// and a half rounds of 256 work groups.  Small tiles (300 tokens x 4096 x 4096: 17 us, 0.6 PO/s): the copies, 168
+// MB from the L2 at 9 TB/s.  One row of tiles (16 tokens x 4096 x 133120: 111 us): the weights at 5.0 TB/s.
 template <int BT_, int BN_, int WT_, int WN_, int RING_, int KB_>
 struct GtShape {
     static constexpr int BT = BT_, BN = BN_, WT = WT_, WN = WN_, RING = RING_, KB = KB_;
@@ -369,7 +373,8 @@ static void tiles_once(const GemmI8Args& a, hipStream_t s) {
 typedef GtShape<256, 256, 4, 4, 2, 128> GtBig;
 typedef GtShape<256, 128, 4, 4, 2, 128> GtBigHalf;
 typedef GtShape<128, 128, 2, 4, 2, 128> GtMid;
-typedef GtShape<64, 64, 2, 2, 5, 128> GtSmall;
+typedef GtShape<64, 128, 2, 4, 3, 128> GtWide;
+typedef GtShape<64, 64, 2, 2, 4, 128> GtSmall;
 typedef GtShape<32, 64, 1, 2, 4, 128> GtTiny;
 
 // Which kernel, by what each takes at hidden 4096 (all in proportion to it), us:
@@ -377,12 +382,15 @@ typedef GtShape<32, 64, 1, 2, 4, 128> GtTiny;
 //    32 x 64 10.9, 11.3; x 32000 30.5, 34.7 and 31.8, 32.4 (and a launch more where tokens are f32); x 133120
 //    117, 133 and 97, 102;
 //  * tiles of 32 x 64 for up to 32: 32 x 6144 12.6, by 64 x 64 14.5, 20 11.9 and 13.8, x 133120 128 and 129;
-//  * tiles of 64 x 64: 14, or 6 and 36 ns per tile where that is more;
-//  * tiles of 128 x 128: 25, or 5 and 93 ns per tile;
+//  * tiles of 64 x 64: 17.5 for up to 512, which all run at once, then 6 and 38 ns per tile (rings of 5 stages, of
+//    which one work group fits a CU where there are more than 256: 18.9; of 64 x 32: 17.9);
+//  * tiles of 64 x 128, where all run at once: 18.5, or 12 and 38 ns per tile;
+//  * tiles of 128 x 128: 28, or 8 and 93 ns per tile;
 //  * tiles of 256 x 256: 70 per round of 256, 45 for a last round of up to 128, which takes half tiles.
-// 64, 128 and 256 wide tiles measured: 300 tokens x 4096 channels 18, 27, 33; 512 x 6144 34, 35, 44; 1024 x
-// 6144 60, 42, 49; 2048 x 6144 110, 75, 70; 4096 x 6144 226, 144, 127 (without half tiles 144); 64 x 133120 143,
-// 175, -; 256 x 133120 -, 243, 233.
+// 64 x 64, 64 x 128, 128 and 256 wide tiles measured: 300 tokens x 4096 channels 17.4, 18.8, 27, 33; 512 x 6144
+// 34, 27, 35, 44; 700 x 4096 31, 26, 29, -; 1024 x 4096 38, 31, 35, -; 1024 x 6144 58, 47, 42, 49; 2048 x 6144
+// 103, 84, 75, 70; 4096 x 6144 226, -, 144, 127 (without half tiles 144); 64 x 133120 140, 135, 175, -; 256 x
+// 133120 312, 266, 243, 233.
 static double tiles_of(const GemmI8Args& a, int bt, int bn) {
     return (double)((a.T + bt - 1) / bt) * ((a.N + bn - 1) / bn);
 }
@@ -397,14 +405,18 @@ hipError_t launch_gemm_i8(const GemmI8Args& a, hipStream_t s) {
         a.xf ? stream<true>(a, s) : stream<false>(a, s);
         return hipGetLastError();
     }
-    const double n64 = tiles_of(a, 64, 64), n128 = tiles_of(a, 128, 128), n256 = tiles_of(a, 256, 256);
-    const double small = fmax(14.0, 6.0 + 0.036 * n64), mid = fmax(25.0, 5.0 + 0.093 * n128);
+    const double n64 = tiles_of(a, 64, 64), nwide = tiles_of(a, 64, 128);
+    const double n128 = tiles_of(a, 128, 128), n256 = tiles_of(a, 256, 256);
+    const double small = n64 <= 512.0 ? 17.5 : 6.0 + 0.038 * n64, mid = fmax(28.0, 8.0 + 0.093 * n128);
+    const double wide = nwide <= 512.0 ? fmax(18.5, 12.0 + 0.038 * nwide) : HUGE_VAL;
     const double rounds = floor(n256 / 256.0), left = n256 - 256.0 * rounds;
     const double big = 70.0 * rounds + (left == 0.0 ? 0.0 : left <= 128.0 ? 45.0 : 70.0);
     if (a.T <= 32)
         tiles_once<GtTiny>(a, s);
-    else if (small <= mid && small <= big)
+    else if (small <= wide && small <= mid && small <= big)
         tiles_once<GtSmall>(a, s);
+    else if (wide <= mid && wide <= big)
+        tiles<GtWide>(a, s);
     else if (mid <= big)
         tiles<GtMid>(a, s);
     else

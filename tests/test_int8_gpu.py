@@ -63,6 +63,13 @@ def test_gemm(gpu, T, K, N):
         same_bits(b.result(), Q.gemm(x, xs, w, ws, resid))
 
 
+# tiles of 64 x 128; one row of tiles over weights of more than 256 MB, with a reduction that ends inside a stage
+@pytest.mark.parametrize("T,K,N", [(500, 272, 6100), (700, 2064, 4096), (20, 65520, 4200), (50, 65520, 4200),
+                                   (32, 65536, 4097), (64, 65536, 4097)])
+def test_gemm_wide_and_long(gpu, T, K, N):
+    test_gemm(gpu, T, K, N)
+
+
 @pytest.mark.parametrize("T,K,N", [(1, 4096, 300), (2, 64, 7), (3, 4112, 64), (8, 6160, 40), (17, 4096, 100),
                                    (70, 2048, 129), (300, 1024, 256), (600, 272, 70), (2, 131056, 8)])
 def test_linear(gpu, T, K, N):
