@@ -13,6 +13,7 @@ namespace hy {
 // ---------------------------------------------------------------- quantization of rows
 // A work group per row: largest magnitude (as bits, so that an infinity or NaN is among the largest),
 // then codes.  Rows up to QR_KEEP values stay in registers between the two, longer ones are read again.
+// Bound by memory: 4096 rows of 4096 20 us, 4.2 TB/s; few rows by latency, 4 us.
 constexpr int QR_THREADS = 256, QR_VEC = 4, QR_KEEP = QR_THREADS * QR_VEC * 4;
 
 __global__ __launch_bounds__(QR_THREADS) void quantize_rows_kernel(const float* __restrict__ x, int rows, int cols,
@@ -178,10 +179,10 @@ __global__ __launch_bounds__(GS_THREADS) void gemm_i8_stream_kernel(GemmI8Args a
 // every bank once.  The copies' places are fixed, so they fetch the pieces swapped.
 // Rows of 128 bytes: with 64 the copies are half as fast (a request of the L2 is 64 bytes of a line of
 // 128).
-// Bounds.  Tiles of 256 x 256 (4096 tokens x 4096 x 6144: 114 us, 1.8 PO/s; 8192^3 reaches 2.2, a library
+// Bounds.  Tiles of 256 x 256 (4096 tokens x 4096 x 6144: 112 us, 1.8 PO/s; 8192^3 reaches 2.17, a library
 // product 2.09): the matrix pipe and the power it draws, the copies from the L2 and, at 6144 channels, one
 // and a half rounds of 256 work groups.  Small tiles (300 tokens x 4096 x 4096: 17 us, 0.6 PO/s): the copies, 168
-// MB from the L2 at 9 TB/s.  One row of tiles (16 tokens x 4096 x 133120: 111 us): the weights at 5.0 TB/s.
+// MB from the L2 at 10 TB/s.  One row of tiles (16 tokens x 4096 x 133120: 111 us): the weights at 5.0 TB/s.
 template <int BT_, int BN_, int WT_, int WN_, int RING_, int KB_>
 struct GtShape {
     static constexpr int BT = BT_, BN = BN_, WT = WT_, WN = WN_, RING = RING_, KB = KB_;

