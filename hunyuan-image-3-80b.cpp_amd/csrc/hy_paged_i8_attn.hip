@@ -110,43 +110,6 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedA
         job = part_job(ps, it, p0, p1, stretch, n_live);
         const int slot_id = p0 == 0 && p1 == it.len ? -1 : 2 * worker + (p0 == 0 ? 1 : 0);  // -1: all of it is here
 
-        // q: scaled by scale * log2(e) and by a power of two that brings the row's largest to [2^13, 2^14)
-        const float* const qp = a.q + ((int64_t)row * a.nh + head) * HD;
-        v4i_t qf[2 * NL][2];
-        float unscale;
-        {
-            const float qscale = a.scale * 1.4426950408889634f;
-            v4f_t q[2 * NL][2];
-            float big = 0.0f;
-#pragma unroll
-            for (int s = 0; s < 2 * NL; s++)
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-                    q[s][u] = *reinterpret_cast<const v4f_t*>(qp + 16 * GQ * (s / 2) + 16 * g + 8 * (s % 2) + 4 * u);
-            __builtin_amdgcn_sched_barrier(0);  // all of them in flight
-#pragma unroll
-            for (int s = 0; s < 2 * NL; s++)
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    q[s][u] *= qscale;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) big = fmaxf(big, fabsf(q[s][u][j]));
-                }
-            big = row_max<L>(big);
-            const int e = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -100), 127);
-            const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
-            unscale = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
-#pragma unroll
-            for (int s = 0; s < 2 * NL; s++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    uint32_t hi, lo;
-                    split_f16(q[s][j / 2][2 * (j % 2)] * up, q[s][j / 2][2 * (j % 2) + 1] * up, hi, lo);
-                    qf[s][0][j] = (int)hi;
-                    qf[s][1][j] = (int)lo;
-                }
-        }
-
         // block table: 64 entries in the lanes, the next 64 on their way
         const int* const trow = a.table + (int64_t)it.r * a.max_pages;
         const int n_tab = (it.q.kv + pmask) >> a.c.shift;
@@ -157,6 +120,16 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedA
         };
         int seg = (t0 * KB) >> (a.c.shift + 6);
         int tab = entries(seg), tab2 = entries(seg + 1);
+        // q: scaled by scale * log2(e) and by a power of two that brings the row's largest to [2^13, 2^14)
+        const float* const qp = a.q + ((int64_t)row * a.nh + head) * HD;
+        v4i_t qf[2 * NL][2];
+        float unscale;
+        v4f_t q[2 * NL][2];
+#pragma unroll
+        for (int s = 0; s < 2 * NL; s++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                q[s][u] = *reinterpret_cast<const v4f_t*>(qp + 16 * GQ * (s / 2) + 16 * g + 8 * (s % 2) + 4 * u);
         const int8_t* const kbase = static_cast<const int8_t*>(a.c.k) + it.g * a.c.head_stride + 16 * g;
         const int8_t* const vbase = static_cast<const int8_t*>(a.c.v) + it.g * a.c.head_stride + VD * i;
 
@@ -211,6 +184,33 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedA
                 }
             }
         };
+
+        __builtin_amdgcn_sched_barrier(0);
+        {
+            const float qscale = a.scale * 1.4426950408889634f;
+            float big = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 2 * NL; s++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    q[s][u] *= qscale;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) big = fmaxf(big, fabsf(q[s][u][j]));
+                }
+            big = row_max<L>(big);
+            const int e = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -100), 127);
+            const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
+            unscale = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
+#pragma unroll
+            for (int s = 0; s < 2 * NL; s++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t hi, lo;
+                    split_f16(q[s][j / 2][2 * (j % 2)] * up, q[s][j / 2][2 * (j % 2) + 1] * up, hi, lo);
+                    qf[s][0][j] = (int)hi;
+                    qf[s][1][j] = (int)lo;
+                }
+        }
 
         acc_t o[VD];
 #pragma unroll
