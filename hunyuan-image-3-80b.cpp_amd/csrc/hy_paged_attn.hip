@@ -524,7 +524,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PartSh
         join_item<HD, PJ, true>(a, many, b / many_splits, b % many_splits, many_splits, meet);
 }
 
-constexpr int PJ_ROWS = 8;  // rows of a stream's item per work group of the join
+constexpr int PJ_ROWS = 8;  // rows of a stream's item per work group of the join, or with half the workers 4
 
 constexpr int PF_ROWS = 32;
 // Rows of the largest request up to which the streams take a whole batch; past it they take the
@@ -599,7 +599,7 @@ hipError_t launch_paged_attn(const PagedAttnArgs& a, int max_new, hipStream_t s)
 
 hipError_t launch_paged_join(const PagedAttnArgs& a, const PaPlan& p, hipStream_t s) {
     const bool big = a.c.hd == 128;
-    const int splits = p.few.M / PJ_ROWS;
+    const int splits = p.few.M / PJ_ROWS * (p.few.workers ? PF_WORKERS / p.few.workers : 1);
     const int many_splits = a.c.hd / 4;  // a tile of few pieces: one set of rows per work group
     const dim3 grid(p.few.workers * splits + p.many.workers * many_splits);
     // Items of 32 pieces and more: eight pieces at a time (1000 keys, one request: 4.0 us, by fours

@@ -57,7 +57,7 @@ __device__ __forceinline__ float row_sum(float v) {
 }
 
 template <int HD, int L>
-__global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedAttnArgs a, PartShape ps) {
+__global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedAttnArgs a, PartShape ps, float per_item) {
     using P = PaType<_Float16>;
     typedef typename I8Acc<L>::type acc_t;
     constexpr int GQ = WAVE / L;             // lanes of a row
@@ -72,7 +72,10 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedA
     const int lane = threadIdx.x % WAVE, i = lane % L, g = lane / L;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int64_t total = part_sums(a, ps, sums);
-    const int64_t stretch = part_stretch(ps, total);
+    // Pieces of few keys cost more in the join than they spare here: of an item of n keys sqrt(4 n) or more (one
+    // request of 4 tokens behind 4000 keys 21 us, so 19, behind 1000 15.4 and 13.6)
+    const int64_t least = uniform((int)__builtin_amdgcn_sqrtf((float)total * per_item));
+    const int64_t stretch = max(part_stretch(ps, total), least);
     const int worker = blockIdx.x * PF_WAVES + wave;
     int64_t x = worker * stretch;
     const int64_t x_end = min(x + stretch, total);
@@ -372,20 +375,27 @@ static int i8_max_rows(int n_req, int hd) {
     return n_req <= 2 ? PF_ROWS : n_req <= 8 ? 384 : 128;
 }
 
-// Up to WIDE_ITEMS tiles of 32 rows half the workers, one wave per SIMD, take the stream: half the pieces to join.
-// head_dim 128, both numbers of workers, us: 32 requests of 6 tokens behind 2000 keys (256 tiles) 48, 63, behind
-// 6000 112, 117; 16 of 8 behind 8000 (128) 87, 90; 3 of 64 behind 6000 (192) 77, 82; 64 of 5 behind 3000 (512)
-// 111, 104; 16 of 32 behind 8000 (512) 220, 215.
-constexpr int WIDE_ITEMS = 256;
+// Up to HALF_ITEMS items half the workers, one wave per SIMD, take the stream: half the pieces, and twice the work
+// groups for each item's join (launch_paged_join).  head_dim 128, all and half the workers, us:
+//  * 16 rows: one request of a token behind 1000 keys 14, 14, behind 120000 62, 52, of 4 behind 4000 37, 19; 8 of
+//    one behind 4000 25, 23, of 4 41, 27; 32 (256 items) of one behind 2000 35, 33, of 4 43, 35; 64 of one behind
+//    8000 (512) 134, not timed with half;
+//  * 32 rows: 32 of 6 behind 2000 (256) 48, 63, behind 6000 112, 117; 16 of 8 behind 8000 (128) 87, 90; 64 of 5
+//    behind 3000 (512) 104, 111; 16 of 32 behind 8000 (512) 215, 220.
+constexpr int HALF_ITEMS = 256;
+static int64_t i8_items(int64_t rows, int m_shift, int n_req, int nkv) {
+    return ((rows + (1 << m_shift) - 1) >> m_shift) * n_req * nkv;
+}
 
 static PaPlan i8_plan(int n_req, int max_new, int G, int nkv, int hd) {
     const int64_t rows = (int64_t)max_new * G;  // of one request, at most
     constexpr int64_t ALL = (int64_t)1 << 62;
     const bool many = rows > i8_max_rows(n_req, hd), few = !many || n_req > 1;
     PaPlan p;
-    const bool wide = rows > 16 && !many, half = wide && (rows + 31) / 32 * n_req * nkv <= WIDE_ITEMS;
+    const int shift = rows > 16 && !many ? 5 : 4;
+    const bool half = !many && i8_items(rows, shift, n_req, nkv) <= HALF_ITEMS;
     const int workers = !few ? 0 : half ? PF_WORKERS / 2 : PF_WORKERS;
-    p.few = part_shape(wide ? 5 : 4, G, 0, many ? PF_ROWS : ALL, workers, 16, 32, 32, 0);
+    p.few = part_shape(shift, G, 0, many ? PF_ROWS : ALL, workers, 16, 32, 32, 0);
     const size_t few_ws = part_ws_floats(p.few.workers, p.few.M, hd);
     p.many = part_shape(PM_TILE_SHIFT, G, few ? PF_ROWS : 0, ALL, many ? PM_WORKERS : 0, 256, 128, 128, few_ws);
     return p;
@@ -397,17 +407,20 @@ size_t paged_attn_i8_ws_bytes(int n_req, int max_new, int G, int nkv, int hd) {
 }
 
 template <int HD>
-static void launch(const PagedAttnArgs& a, const PaPlan& p, hipStream_t s) {
+static void launch(const PagedAttnArgs& a, const PaPlan& p, int max_new, hipStream_t s) {
+    // beside chunks there are fewer items than the batch could have: no least stretch
+    const int64_t items = i8_items((int64_t)max_new * p.few.G, p.few.m_shift, a.n_req, a.c.nkv);
+    const float per_item = p.many.workers ? 0.0f : 4.0f / (float)items;
     const dim3 grid(p.few.workers / PF_WAVES), block(WAVE * PF_WAVES);
     if (p.few.M == 32)
-        hipLaunchKernelGGL((paged_i8_few_kernel<HD, 32>), grid, block, 0, s, a, p.few);
+        hipLaunchKernelGGL((paged_i8_few_kernel<HD, 32>), grid, block, 0, s, a, p.few, per_item);
     else
-        hipLaunchKernelGGL((paged_i8_few_kernel<HD, 16>), grid, block, 0, s, a, p.few);
+        hipLaunchKernelGGL((paged_i8_few_kernel<HD, 16>), grid, block, 0, s, a, p.few, per_item);
 }
 
 hipError_t launch_paged_attn_i8(const PagedAttnArgs& a, int max_new, hipStream_t s) {
     const PaPlan p = i8_plan(a.n_req, max_new, a.nh / a.c.nkv, a.c.nkv, a.c.hd);
-    if (p.few.workers) a.c.hd == 128 ? launch<128>(a, p, s) : launch<64>(a, p, s);
+    if (p.few.workers) a.c.hd == 128 ? launch<128>(a, p, max_new, s) : launch<64>(a, p, max_new, s);
     if (p.many.workers) launch_paged_many(a, p.many, s);
     return launch_paged_join(a, p, s);
 }
