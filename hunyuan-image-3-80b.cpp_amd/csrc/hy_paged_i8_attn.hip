@@ -364,15 +364,15 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedA
 
 constexpr int PF_ROWS = 32;
 // Rows of the largest request up to which the streams take a whole batch; past it they take the
-// requests of PF_ROWS rows at most, tiles of 256 rows the others.  Measured with both, us, stream and tiles:
-//  * head_dim 128, one or two requests are few items for the stream to cut: 2 of 64 rows behind 6000 keys 49,
-//    42, 1 of 64 52, 42.  More of them: 3 of 256 behind 6000 78, 91, 6 of 384 behind 1000 55, 59; 16 of 64
-//    behind 8000 133, 209, of 128 213, 219, of 256 371, 293, behind 1000 77, 64;
-//  * head_dim 64: 4 of 1024 25, 27, of 2048 39, 37; 6 of 1024 behind 1000 49, 53, of 2048 81, 78; 2 of 1024
-//    behind 6000 69, 72; 16 of 128 behind 8000 84, 96, of 256 140, 116.
+// requests of PF_ROWS rows at most, tiles of 256 rows the others.  Requests x tokens (four rows each) behind keys,
+// streams and tiles, us:
+//  * head_dim 128: 1 x 16 behind 6000 33, 33, 4 x 16 41, 57, 8 x 16 59, 88, 16 x 16 110, 155; 1 x 32 43, 38, 4 x 32
+//    61, 61, 8 x 32 99, 93, behind 1000 38, 40, 16 x 32 behind 2000 78, 74; 8 x 64 behind 1000 58, 46, 16 x 64 81, 64;
+//  * head_dim 64: 16 x 16 behind 4000 38, 56, 8 x 32 39, 41, 16 x 32 60, 60; 2 x 64 29, 38, 4 x 64 42, 40, 8 x 64 63,
+//    50; 1 x 128 31, 37, 2 x 128 43, 42, 4 x 128 67, 52; 1 x 256 44, 40.
 static int i8_max_rows(int n_req, int hd) {
-    if (hd == 64) return n_req <= 8 ? 1536 : 128;
-    return n_req <= 2 ? PF_ROWS : n_req <= 8 ? 384 : 128;
+    if (hd == 64) return n_req > 6 ? 128 : 768 / n_req;
+    return 96;
 }
 
 // Up to HALF_ITEMS items half the workers, one wave per SIMD, take the stream: half the pieces, and twice the work
