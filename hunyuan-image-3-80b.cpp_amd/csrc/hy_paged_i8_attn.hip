@@ -410,7 +410,7 @@ template <int HD>
 static void launch(const PagedAttnArgs& a, const PaPlan& p, int max_new, hipStream_t s) {
     // beside chunks there are fewer items than the batch could have: no least stretch
     const int64_t items = i8_items((int64_t)max_new * p.few.G, p.few.m_shift, a.n_req, a.c.nkv);
-    const float per_item = p.many.workers ? 0.0f : 4.0f / (float)items;
+    const float per_item = p.many.workers || !items ? 0.0f : 4.0f / (float)items;
     const dim3 grid(p.few.workers / PF_WAVES), block(WAVE * PF_WAVES);
     if (p.few.M == 32)
         hipLaunchKernelGGL((paged_i8_few_kernel<HD, 32>), grid, block, 0, s, a, p.few, per_item);

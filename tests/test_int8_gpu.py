@@ -561,6 +561,20 @@ def test_attention_many_requests(gpu):
     check(attend(gpu, *args), *args)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n_req,new,kv", [(1, 1, 3000), (1, 4, 4000), (1, 6, 2500), (3, 4, 1500), (32, 1, 300), (33, 1, 300),
+                                          (32, 4, 200), (33, 4, 200), (32, 6, 150), (33, 6, 150), (1, 24, 900), (2, 32, 700),
+                                          (1, 64, 5000), (1, 130, 3000), (2, 96, 1200), (7, 33, 300)])
+def test_attention_pieces_and_workers(gpu, hd, n_req, new, kv):
+    """Few and many items (request x kv head x rows) for the streams' workers, and items in many pieces."""
+    rng = np.random.default_rng(n_req * 1000 + new)
+    lens = [(kv + int(rng.integers(0, 60)), new) for _ in range(n_req)]
+    p, table, q_start, kv_len = make_batch(rng, lens, 16, 8, hd, 16)
+    q = rng.standard_normal((q_start[-1], 32, hd)).astype(np.float32)
+    args = (q, p, q_start, kv_len, table, hd ** -0.5)
+    check(attend(gpu, *args), *args)
+
+
 @pytest.mark.parametrize("lens,block", [([(9000, 1), (20, 1)], 64), ([(20000, 3)], 16), ([(5000, 70)], 32)])
 def test_attention_long(gpu, lens, block):
     rng = np.random.default_rng(13)
