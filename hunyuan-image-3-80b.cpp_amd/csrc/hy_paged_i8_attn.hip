@@ -21,10 +21,10 @@
 // finite, whatever lies in memory.
 //
 // 32 heads over 8 kv heads of 128.  64 requests of one token behind 8000 keys: 125 us, 5.3 TB/s, the memory's
-// rate.  32 of six tokens behind 2900 keys (32 rows): 46 us, 2.9 TB/s; about 20 of them are a worker's start
+// rate.  32 of six tokens behind up to 2900 keys (32 rows): 45 us, 3.0 TB/s; about 20 of them are a worker's start
 // and end (finding its piece, q, the block table, the first keys; partial results), the rest is held up by what a
 // turn does in a row (turning codes into f16, products, maximum, exponentials, pieces): one wave per SIMD, or two
-// with twice the pieces, take the same.  One token behind 1000 keys: 8.4 us of latency, and 3.8 for the join.
+// with twice the pieces, take the same.  One token behind 1000 keys: 8.4 us of latency, and 3.5 for the join.
 #include "hy_device.hpp"
 #include "hy_int8.hpp"
 #include "hy_lds.hpp"
