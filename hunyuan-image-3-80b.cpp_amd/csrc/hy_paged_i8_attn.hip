@@ -20,7 +20,7 @@
 // Keys that a row does not see get weight 0, after the product with m, which may be NaN; codes are
 // finite, whatever lies in memory.
 //
-// 32 heads over 8 kv heads of 128.  64 requests of one token behind 8000 keys: 125 us, 5.3 TB/s, the memory's
+// 32 heads over 8 kv heads of 128.  64 requests of one token behind up to 8000 keys: 125 us, 5.3 TB/s, the memory's
 // rate.  32 of six tokens behind up to 2900 keys (32 rows): 45 us, 3.0 TB/s; about 20 of them are a worker's start
 // and end (finding its piece, q, the block table, the first keys; partial results), the rest is held up by what a
 // turn does in a row (turning codes into f16, products, maximum, exponentials, pieces): one wave per SIMD, or two
@@ -378,7 +378,7 @@ static int i8_max_rows(int n_req, int hd) {
 // Up to HALF_ITEMS items half the workers, one wave per SIMD, take the stream: half the pieces, and twice the work
 // groups for each item's join (launch_paged_join).  head_dim 128, all and half the workers, us:
 //  * 16 rows: one request of a token behind 1000 keys 14, 14, behind 120000 62, 52, of 4 behind 4000 37, 19; 8 of
-//    one behind 4000 25, 23, of 4 41, 27; 32 (256 items) of one behind 2000 35, 33, of 4 43, 35; 64 of one behind
+//    one behind 4000 25, 23, of 4 41, 27; 32 (256 items) of one behind 2000 35, 33, of 4 43, 35; 64 of one behind up to
 //    8000 (512) 134, not timed with half;
 //  * 32 rows: 32 of 6 behind 2000 (256) 48, 63, behind 6000 112, 117; 16 of 8 behind 8000 (128) 87, 90; 64 of 5
 //    behind 3000 (512) 104, 111; 16 of 32 behind 8000 (512) 215, 220.
