@@ -38,9 +38,9 @@
 // key by key (slow_rows).
 //
 // Caches of 8-bit integers (E = int8_t): codes are exact in f16 and take one piece; K's scale of a block joins the
-// scores, V's is split into a power of two, which joins the exponent as e_j does above, and 1 <= m < 2, which
-// multiplies the weight before its split.  Scales lie in the lanes of a wave, 64 blocks of the cache at a
-// time, and are read from there.  2048 rows of 32 heads behind 8192 keys: 637 us, 485 TFLOP/s of attention, 970
+// scores, V's, 2^(e + f) with e whole and 0 <= f < 1, the exponent: a weight is 2^(s + f + (e - R)), R a maximum of
+// s + e, and e - R comes first, so that nothing that counts is rounded at the size of e (2^-19 where that is 50).
+// Scales lie in the lanes of a wave, 64 blocks of the cache at a time, and are read from there.  2048 rows of 32 heads behind 8192 keys: 637 us, 485 TFLOP/s of attention, 970
 // of f16 products, matrix pipe 44 % and vector pipe 37 % of the cycles; five prompts of up to 1500 tokens,
 // head_dim 64: 75 us, a third of it waiting at barriers and for a piece's start.
 #include "hy_device.hpp"
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
     constexpr int RING = KP == 2 ? 2 : 3;  // operands read ahead of the products (registers allowing)
     __shared__ __attribute__((aligned(1024))) uint8_t lds[L::BYTES];
     __shared__ __attribute__((aligned(16))) float k_fac[2][I8 ? 1 : 32], v_exp[2][I8 ? 1 : 32], v_inv[2][I8 ? 1 : 32];
-    __shared__ v4f_t i8_fac[2][I8 ? 8 : 1];  // of four keys: K's scale, V's as its logarithm and its reciprocal
+    __shared__ v4f_t i8_fac[2][I8 ? 8 : 1];  // of four keys: K's scale, V's e, reciprocal and f
     __shared__ int odd_s;  // V of this piece that the scaled products do not take
     __shared__ int last_s[PM_WAVES];
     __shared__ PartSums<PM_THREADS> sums;
@@ -201,13 +201,16 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         };
         int sseg = 0, sp = 0;
         float ks = 0.0f, ks2 = 0.0f, vs2 = 0.0f;
-        // V's as their logarithms and reciprocals (to 2^-23 of the keys' weights in the sum); below the range the
-        // lowest logarithm and values of 0, an infinity as NaN
-        float v_log = 0.0f, v_rcp = 0.0f;
+        // V's as the two parts of their logarithms and their reciprocals (to 2^-23 of the keys' weights in the sum);
+        // below the range the lowest e and values of 0, an infinity as NaN
+        float v_e = 0.0f, v_f = 0.0f, v_rcp = 0.0f;
         auto of_v = [&](float v) {
             v = v < pow2(PM_ELO) ? pow2(PM_ELO) : fmaf(v, 0.0f, v);
-            v_log = __builtin_amdgcn_logf(v);
-            v_rcp = __builtin_amdgcn_rcpf(v);
+            const int e = min(exponent(__float_as_uint(v), PM_ELO), PM_EHI);
+            const float m = v * pow2(-e);
+            v_e = (float)e;
+            v_f = __builtin_amdgcn_logf(m);
+            v_rcp = __builtin_amdgcn_rcpf(m) * pow2(-e);
         };
         if constexpr (I8) {
             sseg = (kb0 * 32) >> (a.bshift + 6);
@@ -239,7 +242,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         uint8_t* const v_dst = lds + L::OFF_V + (2 * (wv / 4) + wv % 2) * L::CHUNK_V + lane * 16 + 8 * (wv / 2 % 2);
         typedef typename std::conditional<I8, uint2, v4i_t>::type krow_t;
         krow_t kx[KP];
-        float k_scale = 0.0f, v_ex = 0.0f, v_in = 0.0f;
+        float k_scale = 0.0f, v_ex = 0.0f, v_fr = 0.0f, v_in = 0.0f;
         typedef typename std::conditional<KP == 2, uint2, typename std::conditional<I8, uint16_t, uint32_t>::type>::type vrow_t;
         vrow_t vx[4];
         uint32_t v_big = 0;  // the largest magnitude of V's: whether one was infinite, no number, or past PM_EHI
@@ -258,7 +261,8 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             for (int j = 0; j < 4; j++) vx[j] = *reinterpret_cast<const vrow_t*>(p + (v_off + j * ts * sizeof(E)));
             if constexpr (I8) {
                 const int b = ((kb * 32 + 4 * wv) >> a.bshift) - sseg * 64;
-                v_ex = lane_f(v_log, b);
+                v_ex = lane_f(v_e, b);
+                v_fr = lane_f(v_f, b);
                 v_in = lane_f(v_rcp, b);
             }
             const int s = ((kb + 1) * 32) >> (a.c.shift + 6);  // the next call's
@@ -337,7 +341,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             uint8_t* const d = v_dst + r * L::BUF_V;
             const int key0 = kb * 32 + 4 * wv;
             if constexpr (I8) {
-                const bool tiny = v_ex == (float)PM_ELO;  // the same for the wave: values of 0
+                const bool tiny = v_ex + v_fr == (float)PM_ELO;  // the same for the wave: values of 0
                 if (v_mine) {
 #pragma unroll
                     for (int n = 0; n < 2; n++) {
@@ -348,6 +352,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 if (lane == 0) {
                     i8_fac[r][wv][1] = v_ex;
                     i8_fac[r][wv][2] = v_in;
+                    i8_fac[r][wv][3] = v_fr;
                 }
                 return;
             }
@@ -491,7 +496,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                 __builtin_amdgcn_sched_barrier(0);
             }
             v4f_t inv[4];
-            float i8_k[4], i8_v[4];  // of an 8-bit cache's scores: t = s i8_k + i8_v, formed in the exponential
+            float i8_k[4], i8_v[4], i8_f[4];  // of an 8-bit cache: K's factor, V's e and f
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 v4f_t fac, ex;
@@ -499,6 +504,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                     const v4f_t f = i8_fac[r][2 * u + h];
                     i8_k[u] = f[0] * unscale;
                     i8_v[u] = f[1];
+                    i8_f[u] = f[3];
                     inv[u][0] = f[2];
                     continue;
                 } else if constexpr (SCALED) {
@@ -513,27 +519,27 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
                     s[4 * u + v] = t;
                 }
             }
-            const bool edge = bad || kb * 32 + 32 > first;
-            if (edge) {            // wave-uniform
-                asm volatile("");  // a branch, not 80 operations more in every block
+            if (bad || kb * 32 + 32 > first) {  // wave-uniform
+                asm volatile("");               // a branch, not 80 operations more in every block
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     const int key = kb * 32 + 8 * u + 4 * h;
                     const bool ok = !bad || page_ok(key);
 #pragma unroll
-                    for (int v = 0; v < 4; v++) {
-                        if constexpr (I8) s[4 * u + v] = fmaf(s[4 * u + v], i8_k[u], i8_v[u]);  // before the mask: scales may be NaN
+                    for (int v = 0; v < 4; v++)
                         if (!ok || key + v >= end) s[4 * u + v] = -INFINITY;
-                    }
                     if constexpr (I8) {
-                        i8_k[u] = 1.0f;
-                        i8_v[u] = 0.0f;
-                        inv[u][0] = inv[u][0] == inv[u][0] ? inv[u][0] : 0.0f;  // NaN: by the weights of rows that see it
+                        // four keys of one block: what its scales are where this row sees none of them does not
+                        // matter, and a NaN is the row's where it sees one; -inf times a scale of 0 would be NaN
+                        const bool sees = ok && key < end;
+                        i8_k[u] = !sees || i8_k[u] < 0x1p-126f ? 0x1p-126f : i8_k[u];
+                        i8_f[u] = sees ? i8_f[u] : 0.0f;
+                        inv[u][0] = sees ? inv[u][0] : 0.0f;
                     }
                 }
             }
             float big;
-            if constexpr (I8) {  // scales are not negative: a group's largest score has its largest t
+            if constexpr (I8) {  // scales are not negative: a group's largest score has its largest s + e
                 big = -INFINITY;
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
@@ -559,7 +565,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
             const float up = ref - (float)PM_WUP;
             if constexpr (I8) {
 #pragma unroll
-                for (int u = 0; u < 4; u++) i8_v[u] -= up;
+                for (int u = 0; u < 4; u++) i8_v[u] = i8_f[u] + (i8_v[u] - up);
             }
 #pragma unroll
             for (int v = 0; v < 16; v++) {  // l_run: of this lane's keys; joined behind the loop
