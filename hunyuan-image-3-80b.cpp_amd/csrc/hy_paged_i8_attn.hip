@@ -16,8 +16,8 @@
 // K's scale joins the scores.  V's, 2^e m with 1 <= m < 2, joins the weights: with R the running maximum of
 // t_j = s_j + e_j (base 2), w_j = 2^(t_j - R) m_j goes into the products and l sums 2^(t_j - R) 2^-e_j, so
 // out = O / l whatever R; e is kept in -60 .. 34, so that no weight that counts in l underflows
-// (hy_paged_many.hip).
-// Keys that a row does not see get weight 0, after the product with m, which may be NaN; codes are
+// (hy_paged_many.hip).  e - R comes before s is added, so that nothing is rounded at the size of e.
+// Keys that a row does not see get a score of -inf, and factors that leave them a weight of 0; codes are
 // finite, whatever lies in memory.
 //
 // 32 heads over 8 kv heads of 128.  64 requests of one token behind up to 8000 keys: 125 us, 5.3 TB/s, the memory's
@@ -258,19 +258,19 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedA
             __builtin_amdgcn_sched_barrier(0);
             if (t + 1 < t1) load_k(t + 1);
             __builtin_amdgcn_sched_barrier(0);
-            const bool edge = (t + 1) * KB > first || __any((vpage[0] | vpage[1]) < 0);
             const int key0 = t * KB + 16 * g;
-            if (edge) {  // wave-uniform
+            if ((t + 1) * KB > first || __any((vpage[0] | vpage[1]) < 0)) {  // wave-uniform
                 asm volatile("");
 #pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    s[v] = fmaf(s[v], fac[v / 8], ex[v / 8]);  // before the mask: scales may be NaN
+                for (int v = 0; v < 16; v++)
                     if (key0 + v >= end || vpage[v / 8] < 0) s[v] = -INFINITY;
-                }
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    fac[h] = 1.0f;
-                    ex[h] = 0.0f;
+                    // eight keys of one block: what its scales are where this row sees none of them does not matter,
+                    // and a NaN is the row's where it sees one; -inf times a scale of 0 would be NaN
+                    const bool sees = key0 + 8 * h < end && vpage[h] >= 0;
+                    fac[h] = !sees || fac[h] < 0x1p-126f ? 0x1p-126f : fac[h];
+                    mant[h] = sees ? mant[h] : 0.0f;
                 }
             }
             // scales are not negative: a half's largest score has its largest t
@@ -299,12 +299,6 @@ __global__ __launch_bounds__(WAVE * PF_WAVES, 2) void paged_i8_few_kernel(PagedA
                 s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], fac[v / 8], ex[v / 8]));
                 l_run = fmaf(s[v], inv[v / 8], l_run);  // of this lane's keys; joined behind the loop
                 s[v] *= mant[v / 8];
-            }
-            if (edge) {
-                asm volatile("");
-#pragma unroll
-                for (int v = 0; v < 16; v++)
-                    if (key0 + v >= end || vpage[v / 8] < 0) s[v] = 0.0f;
             }
             v4i_t pf[2][2];
 #pragma unroll

@@ -48,3 +48,12 @@ def check_powers(gpu, lens, hd, bad_page=False):
                                      (64, [(200, 200)]), (64, [(2500, 250)])])
 def test_powers_of_two_tiles(gpu, hd, lens, bad_page):
     check_powers(gpu, lens, hd, bad_page)
+
+
+# streams of 16 and of 32 rows: turns that every row sees whole, and the last ones
+@pytest.mark.parametrize("bad_page", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lens", [[(50, 1)], [(700, 1), (20, 1), (130, 1)], [(300, 3), (17, 2)], [(6000, 4)], [(400, 7), (33, 5)],
+                                  [(2000, 8)]])
+def test_powers_of_two_streams(gpu, hd, lens, bad_page):
+    check_powers(gpu, lens, hd, bad_page)
