@@ -12,10 +12,6 @@ struct PagedViewI8 {
     float* vs;
     int bshift;  // block = 1 << bshift
 };
-// the scale of block b of head g of page p
-__host__ __device__ __forceinline__ int64_t scale_at(const PagedViewI8& v, int p, int g, int b) {
-    return (((int64_t)p * v.c.nkv + g) << (v.c.shift - v.bshift)) + b;
-}
 
 // codes of a group whose largest magnitude has the given bits: d, and 1 / d (0: all codes 0)
 struct QuantScale {
