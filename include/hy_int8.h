@@ -112,6 +112,8 @@ int hy_paged_attention_i8(const float* q_dev, uint32_t n_heads, const hy_paged_c
 
 /* Holds `layer`'s projections (hy_model_quantize_i8: every layer's, and the lm_head) in 8 bits
  * besides f32: the two calls below take those from then on, until the weights are loaded anew.
+ * A graph keeps the form it was captured with: over 8 bits it goes on with the codes there are, whatever is
+ * loaded behind it, until these calls are made again, which put the new ones in the same place.
  * Allocates, and waits for the device; not while a stream is captured. */
 int hy_attn_quantize_i8(hy_attn_ctx* ctx, uint32_t layer);
 int hy_model_quantize_i8(hy_model_ctx* ctx);

@@ -117,3 +117,47 @@ def test_model_over_steps(gpu, quantized):
                 np.testing.assert_array_equal((codes.reshape(n_pages, -1) != MARK_CODE).any(1), used)
     assert not any(np.array_equal(a, b) for a, b in zip(many.layer(0), many.layer(1)))
     m.close()
+
+
+def test_graph_and_new_weights(gpu):
+    """A captured layer goes on with the codes there are when weights are loaded, and takes the new ones where they are
+    quantized again; calls take the loaded weights at once."""
+    H, nh, nkv, hd, T = 256, 8, 2, 64, 6
+    rng = np.random.default_rng(92)
+    att = gpu.Attn(H, nh, nkv, hd, 16)
+
+    def load():
+        att.upload(*[(rng.standard_normal(s) * 0.1).astype(np.float32) for s in (((nh + 2 * nkv) * hd, H), (H, nh * hd))],
+                   np.ones(hd, np.float32), np.ones(hd, np.float32))
+    i32 = lambda *v: dev(gpu, np.array(v, np.int32))  # noqa: E731
+    pool = PoolI8(1, 16, nkv, hd, 16)
+    cache = cache_of(gpu, pool, upload(gpu, pool))
+    batch = gpu.PagedBatch(1, T, 1, T, i32(0, T), i32(T), i32(0), i32(*range(T)), i32(*range(T)))
+    x, out, ws = dev(gpu, rng.standard_normal((T, H)).astype(np.float32)), gpu.Buf.empty((T, H)), Ws(gpu, nh, cache, batch)
+    st = gpu.Stream()
+
+    def call(run):
+        out.zero()
+        gpu.sync()
+        run()
+        st.synchronize()
+        return out.numpy()
+    eager = lambda: call(lambda: att.forward_paged_i8(x, cache, batch, out, ws.b, ws.n, stream=st.h))  # noqa: E731
+    load()
+    att.quantize_i8()
+    old = eager()
+    g = gpu.Graph(st, lambda: att.forward_paged_i8(x, cache, batch, out, ws.b, ws.n, stream=st.h))
+    same_bits(call(g.launch), old)
+    load()
+    plain = eager()
+    assert (plain != old).any()
+    same_bits(call(g.launch), old)
+    att.quantize_i8()
+    new = eager()
+    assert (new != old).any() and (new != plain).any()
+    for _ in range(3):
+        same_bits(call(g.launch), new)
+        same_bits(eager(), new)
+    g.close()
+    st.close()
+    att.close()
