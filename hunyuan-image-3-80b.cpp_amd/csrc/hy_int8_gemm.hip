@@ -74,7 +74,8 @@ hipError_t launch_quantize_rows(const float* x, int rows, int cols, int8_t* code
 // GS_DEPTH steps of 64 ahead.  The waves' sums meet in LDS: whole numbers, so in any order.
 // FUSED: the tokens are f32, up to GF_TOKENS of them, and every work group quantizes them for itself while its
 // first weights are on their way, which spares a launch (one token, 4096 x 6144: 10.0 us, in two launches 9.9 + 2.6).
-// Bound by latency: 25 MB of weights would take 5 us at a copy's rate.
+// Bound by a chain: GS_DEPTH of a wave's 16 steps of weights (4096 wide) are asked for before the tokens are read twice,
+// with two barriers, the others only behind that; 25 MB of weights would take 5 us at a copy's rate.
 constexpr int GS_WAVES = 4, GS_THREADS = WAVE * GS_WAVES, GS_DEPTH = 8;
 constexpr int GF_TOKENS = 4, GF_WIDTH = 8192;
 
@@ -179,10 +180,11 @@ __global__ __launch_bounds__(GS_THREADS) void gemm_i8_stream_kernel(GemmI8Args a
 // every bank once.  The copies' places are fixed, so they fetch the pieces swapped.
 // Rows of 128 bytes: with 64 the copies are half as fast (a request of the L2 is 64 bytes of a line of
 // 128).
-// Bounds.  Tiles of 256 x 256 (4096 tokens x 4096 x 6144: 112 us, 1.8 PO/s; 8192^3 reaches 2.17, a library
+// Bounds.  Tiles of 256 x 256 (4096 tokens x 4096 x 6144: 103 us, 2.0 PO/s; 8192^3 reaches 2.17, a library
 // product 2.09): the matrix pipe and the power it draws, the copies from the L2 and, at 6144 channels, one
-// and a half rounds of 256 work groups.  Small tiles (300 tokens x 4096 x 4096: 17 us, 0.6 PO/s): the copies, 168
-// MB from the L2 at 10 TB/s.  One row of tiles (16 tokens x 4096 x 133120: 111 us): the weights at 5.0 TB/s.
+// and a half rounds of 256 work groups.  Small tiles (300 tokens x 4096 x 4096: 16.5 us, 0.6 PO/s): 32 stages that wait
+// for one another, 0.5 us each, in 320 work groups on 256 CUs; their copies, 168 MB, come at 10 TB/s where the L2
+// gives three times that.  One row of tiles (16 tokens x 4096 x 133120: 112 us): the weights at 4.9 TB/s.
 template <int BT_, int BN_, int WT_, int WN_, int RING_, int KB_>
 struct GtShape {
     static constexpr int BT = BT_, BN = BN_, WT = WT_, WN = WN_, RING = RING_, KB = KB_;

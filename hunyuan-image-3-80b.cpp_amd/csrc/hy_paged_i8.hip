@@ -4,8 +4,8 @@
 //
 // A scale belongs to all rows that a call brings into its block, so the unit of work is a run (rows
 // whose slots follow one another inside a block) times a kv head, a work group each, which the
-// run's first row names.  HD / 4 lanes share a row, 4 dims each; 4 rows per lane are held (32 or 64 rows), runs
-// that are longer are gone through twice (largest magnitude, then codes).
+// run's first row names.  HD / 4 lanes share a row, 4 dims each; a work group holds 16 rows, or 32
+// where blocks are longer (1 to 4 per lane); longer runs are gone through twice (largest magnitude, then codes).
 // A key is rotated and normed in 64 bits and rounded to f32 once: a value next to the border
 // between two codes would otherwise fall by the order of the sum, and a step is 2^-7 of the largest.
 //

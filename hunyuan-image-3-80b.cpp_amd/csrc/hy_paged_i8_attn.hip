@@ -20,11 +20,11 @@
 // Keys that a row does not see get a score of -inf, and factors that leave them a weight of 0; codes are
 // finite, whatever lies in memory.
 //
-// 32 heads over 8 kv heads of 128.  64 requests of one token behind up to 8000 keys: 125 us, 5.3 TB/s, the memory's
-// rate.  32 of six tokens behind up to 2900 keys (32 rows): 45 us, 3.0 TB/s; about 20 of them are a worker's start
+// 32 heads over 8 kv heads of 128.  64 requests of one token behind up to 8000 keys: 127 us, 5.2 TB/s, the memory's
+// rate.  32 of six tokens behind up to 2900 keys (32 rows): 39 us, 3.4 TB/s; about 20 of them are a worker's start
 // and end (finding its piece, q, the block table, the first keys; partial results), the rest is held up by what a
-// turn does in a row (turning codes into f16, products, maximum, exponentials, pieces): one wave per SIMD, or two
-// with twice the pieces, take the same.  One token behind 1000 keys: 8.4 us of latency, and 3.5 for the join.
+// turn does in a row (turning codes into f16, products, maximum, exponentials, pieces).  One token behind 1000 keys:
+// 8.2 us of latency, and 3.5 for the join.
 #include "hy_device.hpp"
 #include "hy_int8.hpp"
 #include "hy_lds.hpp"
@@ -360,22 +360,32 @@ constexpr int PF_ROWS = 32;
 // Rows of the largest request up to which the streams take a whole batch; past it they take the
 // requests of PF_ROWS rows at most, tiles of 256 rows the others.  Requests x tokens (four rows each) behind keys,
 // streams and tiles, us:
-//  * head_dim 128: 1 x 16 behind 6000 33, 33, 4 x 16 41, 57, 8 x 16 59, 88, 16 x 16 110, 155; 1 x 32 43, 38, 4 x 32
-//    61, 61, 8 x 32 99, 93, behind 1000 38, 40, 16 x 32 behind 2000 78, 74; 8 x 64 behind 1000 58, 46, 16 x 64 81, 64;
-//  * head_dim 64: 16 x 16 behind 4000 38, 56, 8 x 32 39, 41, 16 x 32 60, 60; 2 x 64 29, 38, 4 x 64 42, 40, 8 x 64 63,
-//    50; 1 x 128 31, 37, 2 x 128 43, 42, 4 x 128 67, 52; 1 x 256 44, 40.
+//  * 8 kv heads of 128: 1 x 16 behind 6000 31, 31, 4 x 16 43, 64, 8 x 16 66, 103, 16 x 16 108, 178; 1 x 32 34, 33,
+//    4 x 32 59, 67, 8 x 32 100, 107, behind 1000 37, 46, 16 x 32 behind 2000 75, 77; 8 x 64 behind 1000 51, 54, 16 x 64
+//    73, 73;
+//  * 4 of 64: 16 x 16 behind 4000 39, 58, 8 x 32 40, 39.5, 16 x 32 60, 60; 2 x 64 28, 34, 4 x 64 40, 37, 8 x 64 63, 48;
+//    1 x 128 27, 33, 2 x 128 40, 38, 4 x 128 62, 49; 1 x 256 37, 37;
+//  * one kv head of 128, requests x rows: 1 x 64 behind 6000 24, 28.5, 1 x 128 27, 31, 4 x 128 31, 37, 16 x 128 43, 50;
+//    4 x 96 behind 4000 28, 33, 8 x 128 33, 35, 8 x 256 35, 40; of 64: 1 x 128 behind 6000 20, 22, 8 x 128 behind 4000
+//    24, 27.
+// The border does not look at the kv heads: between 97 and 256 rows of head_dim 128 the streams would be as fast, or up
+// to a fifth faster where there are few.
 static int i8_max_rows(int n_req, int hd) {
     if (hd == 64) return n_req > 6 ? 128 : 768 / n_req;
     return 96;
 }
 
 // Up to HALF_ITEMS items half the workers, one wave per SIMD, take the stream: half the pieces, and twice the work
-// groups for each item's join (launch_paged_join).  head_dim 128, all and half the workers, us:
-//  * 16 rows: one request of a token behind 1000 keys 14, 14, behind 120000 62, 52, of 4 behind 4000 37, 19; 8 of
-//    one behind 4000 25, 23, of 4 41, 27; 32 (256 items) of one behind 2000 35, 33, of 4 43, 35; 64 of one behind up to
-//    8000 (512) 134, not timed with half;
-//  * 32 rows: 32 of 6 behind 2000 (256) 48, 63, behind 6000 112, 117; 16 of 8 behind 8000 (128) 87, 90; 64 of 5
-//    behind 3000 (512) 104, 111; 16 of 32 behind 8000 (512) 215, 220.
+// groups for each item's join (launch_paged_join).  Four rows per token and 8 kv heads of 128, all and half the
+// workers, us:
+//  * 16 rows: one request of a token behind 1000 keys 12.5, 12.6, behind 120000 70, 57, of 4 behind 4000 20, 18; 8 of
+//    one behind 4000 24, 23.5, of 4 39, 30; 32 (256 items) of one behind 2000 38, 39, of 4 49, 43; 64 (512) of one
+//    behind 4000 112, 107, behind 8000 202, 194, 128 (1024) behind 2000 114, 111;
+//  * 32 rows: one request of 6 behind 4000 23.2, 22.8, 4 of 6 31, 28; 32 of 6 (256) behind 2000 59, 53, behind 6000
+//    110, 110; 16 of 8 behind 8000 (128) 101, 83; 64 of 5 behind 3000 (512) 109, 113; 16 of 24 behind 8000 (384)
+//    169, 188.
+// One kv head: 32 requests of 32 rows behind 4000 40, 33, of 128 rows of head_dim 64 38.5, 39; 128 of 8 rows behind
+// 2000 29, 25.
 constexpr int HALF_ITEMS = 256;
 static int64_t i8_items(int64_t rows, int m_shift, int n_req, int nkv) {
     return ((rows + (1 << m_shift) - 1) >> m_shift) * n_req * nkv;

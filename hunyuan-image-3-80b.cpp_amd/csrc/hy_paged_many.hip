@@ -40,9 +40,10 @@
 // Caches of 8-bit integers (E = int8_t): codes are exact in f16 and take one piece; K's scale of a block joins the
 // scores, V's, 2^(e + f) with e whole and 0 <= f < 1, the exponent: a weight is 2^(s + f + (e - R)), R a maximum of
 // s + e, and e - R comes first, so that nothing that counts is rounded at the size of e (2^-19 where that is 50).
-// Scales lie in the lanes of a wave, 64 blocks of the cache at a time, and are read from there.  2048 rows of 32 heads behind 8192 keys: 637 us, 485 TFLOP/s of attention, 970
-// of f16 products, matrix pipe 44 % and vector pipe 37 % of the cycles; five prompts of up to 1500 tokens,
-// head_dim 64: 75 us, a third of it waiting at barriers and for a piece's start.
+// Scales lie in the lanes of a wave, 64 blocks of the cache at a time, and are read from there.  2048 rows of 32
+// heads behind 8192 keys: 581 us, 530 TFLOP/s of attention, 1060 of f16 products, matrix pipe busy in 47 % of the
+// cycles, vector instructions issued in 48 %; five prompts of up to 1500 tokens, head_dim 64: 69 us, waves waiting (at
+// barriers, and for a piece's start) for 36 % of their time.
 #include "hy_device.hpp"
 #include "hy_int8.hpp"
 #include "hy_lds.hpp"
