@@ -207,7 +207,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void paged_many_kernel(PagedAttnArgs
         float v_e = 0.0f, v_f = 0.0f, v_rcp = 0.0f;
         auto of_v = [&](float v) {
             v = v < pow2(PM_ELO) ? pow2(PM_ELO) : fmaf(v, 0.0f, v);
-            const int e = min(exponent(__float_as_uint(v), PM_ELO), PM_EHI);
+            const int e = min(exponent(__float_as_uint(v), PM_ELO), 126);  // 2^-e is normal
             const float m = v * pow2(-e);
             v_e = (float)e;
             v_f = __builtin_amdgcn_logf(m);

@@ -57,3 +57,16 @@ def test_powers_of_two_tiles(gpu, hd, lens, bad_page):
                                   [(2000, 8)]])
 def test_powers_of_two_streams(gpu, hd, lens, bad_page):
     check_powers(gpu, lens, hd, bad_page)
+
+
+@pytest.mark.parametrize("hd,lens", [(128, [(90, 90)]), (64, [(200, 200)])])
+def test_larger_scales_in_tiles(gpu, hd, lens):
+    """Past 2^34 value scales are not defined where small ones stand beside them; tiles take large ones alike, up
+    to f32's range for the sums."""
+    rng = np.random.default_rng(5)
+    p, q, table, q_start, kv_len = level_batch(rng, lens, hd)
+    vs = p.vs
+    for e in (40, 70, 100):
+        p.vs = np.ldexp(vs, e).astype(np.float32)
+        args = (q, p, q_start, kv_len, table, hd ** -0.5)
+        I8.check(I8.attend(gpu, *args), *args)
